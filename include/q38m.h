@@ -584,6 +584,131 @@ int q38m_quantize_expert_weights(const uint16_t* src_bf16,
                                  const q38m_expert_weights_v1* dst,
                                  void* stream, int device);
 
+/* ---- microscaled 4-bit rows (MXFP4) ----------------------------------
+ * No counterpart in the reference, whose formats are integer.  A row of
+ * `columns` values is cut into blocks of Q38M_MX_BLOCK values with one
+ * power-of-two scale each:
+ *   scale byte s: 2^(s - 127); 255: every value of the block is NaN
+ *   4-bit code c: (-1)^(c >> 3) * {0, 0.5, 1, 1.5, 2, 3, 4, 6}[c & 7]
+ * Rows are contiguous and padded to whole 128 values with zero codes (their
+ * scale bytes are 0): q38m_mx_row_bytes(columns) = 64 * ceil(columns / 128)
+ * bytes of codes, the even column in the low nibble, and
+ * q38m_mx_scale_bytes(columns) = 4 * ceil(columns / 128) scale bytes.  A
+ * matrix is [experts][rows] of such rows (experts = 1 where there are none);
+ * codes 16-byte, scales 4-byte aligned.  The products read no padding of
+ * other lengths, and a matrix that another program quantised so (columns a
+ * multiple of 128: plain row-major codes and scales) can be passed as it is;
+ * padding codes that are not zero would count. */
+#define Q38M_MX_BLOCK 32u
+/* element types of the entry points that take several */
+#define Q38M_DTYPE_F32 1u
+#define Q38M_DTYPE_BF16 2u
+
+typedef struct q38m_mx_matrix_v1 {
+    void* codes;
+    void* scales;
+    uint32_t experts;
+    uint32_t rows;
+    uint32_t columns;
+    uint32_t reserved; /* 0 */
+} q38m_mx_matrix_v1;
+
+size_t q38m_mx_row_bytes(uint32_t columns);
+size_t q38m_mx_scale_bytes(uint32_t columns);
+
+/* Quantises experts * rows rows of dst->columns values (x_stride elements
+ * from one to the next) into dst's buffers.  Block of 32 with largest
+ * magnitude m: s = max(floor(log2 m) - 2, -127) + 127 (0 for m = 0), codes
+ * rounded to nearest, ties to even, magnitudes above 6 to 6 (m lies in
+ * [4, 8) scales); a block with a NaN or an infinity gets s = 255 and zero
+ * codes.  The last block of a row may hold fewer than 32 values.  rounded:
+ * NULL, or the values that the codes stand for (exact in either type, NaN
+ * where s = 255), contiguous rows of x's type -- what the products compute
+ * with, for training with the rounding in the loop and for error
+ * measurements. */
+int q38m_mx_quantize_v1(const void* x, uint32_t dtype, uint64_t x_stride,
+                        const q38m_mx_matrix_v1* dst, void* rounded, void* stream,
+                        int device);
+
+/* C[m][n] = sum over k of A[m][k] * B[n][k], fp32 sums, one rounding (bf16:
+ * to nearest even); exactly one of c_f32 / c_bf16, c_stride elements from
+ * row to row.  a and b: experts = 1, equal columns.  Floating-point parity:
+ * products and scales are exact, the order of the sum is the kernels'. */
+int q38m_mx_gemm_v1(const q38m_mx_matrix_v1* a, const q38m_mx_matrix_v1* b,
+                    float* c_f32, uint16_t* c_bf16, uint64_t c_stride,
+                    void* stream, int device);
+
+/* The experts' products over rows sorted by expert (q38m_moe_sort_routes_v1;
+ * the order and offsets of q38m_route_plan_v1 fit too): for p in
+ * [expert_offsets[e], expert_offsets[e + 1]), C[p] = A[src(p)] * W[e]^T.
+ * weights: [experts][rows][columns]; rows: experts = 1, equal columns.
+ * packed_assignment NULL: src(p) = p and rows->rows = routes; else src(p) =
+ * packed_assignment[p] / top_k (the token rows, as q38m_moe_grouped_gate_up_v1
+ * gathers them).  routes: C's rows; offsets past it are taken as routes, and
+ * an expert whose end is not behind its begin has no rows.
+ * epilogue SWIGLU: weights' first half of rows is gate, the second half up;
+ * C has half as many columns, h = g / (1 + exp(-g)) * u in fp32, rounded
+ * once.  C is contiguous.  Rows of C that no expert has (dropped routes) are
+ * left as they were; a src(p) past A's rows reads as a row of zeros. */
+#define Q38M_MX_EPILOGUE_NONE 0u
+#define Q38M_MX_EPILOGUE_SWIGLU 1u
+int q38m_mx_grouped_gemm_v1(const q38m_mx_matrix_v1* weights,
+                            const q38m_mx_matrix_v1* rows,
+                            const uint32_t* expert_offsets,
+                            const uint32_t* packed_assignment, uint32_t top_k,
+                            uint32_t routes, uint32_t epilogue, float* c_f32,
+                            uint16_t* c_bf16, void* stream, int device);
+
+/* ---- tokens sorted by expert and back, with gradients -----------------
+ * The order of cuda_moe_build_route_plan_v1 (include/q38/cuda_moe_prefill.h:
+ * 101-104: expert-major, stable in the route index token * top_k + rank) for
+ * any number of tokens, experts and ranks, in bf16 or fp32, with routes that
+ * no expert takes, and the derivatives that training wants.
+ * 1 <= experts <= 1024, top_k >= 1, tokens * top_k < 2^24.
+ *
+ * expert_ids int32 [tokens][top_k]; an id outside [0, experts) drops its
+ * route.  Writes expert_offsets [experts + 1] (the last: the kept routes),
+ * packed_assignment [routes] (place -> route; behind the kept routes the
+ * dropped ones in their order) and assignment_to_packed [routes] (its
+ * inverse; Q38M_ROUTE_DROPPED for a dropped route).  scratch:
+ * q38m_moe_sort_scratch_bytes bytes, 4-byte aligned (0 bytes: may be NULL). */
+#define Q38M_ROUTE_DROPPED 0xffffffffu
+size_t q38m_moe_sort_scratch_bytes(uint32_t tokens, uint32_t top_k, uint32_t experts);
+int q38m_moe_sort_routes_v1(const int32_t* expert_ids, uint32_t tokens, uint32_t top_k,
+                            uint32_t experts, uint32_t* expert_offsets,
+                            uint32_t* packed_assignment, uint32_t* assignment_to_packed,
+                            void* scratch, size_t scratch_bytes, void* stream, int device);
+
+/* rows[assignment_to_packed[t * top_k + r]] = x[t]: token rows [tokens][width]
+ * (dtype) to the sorted order [routes][width].  Rows behind the kept routes
+ * are left as they were.  An inverse entry that is no place (dropped, or past
+ * the routes) is skipped, here and below.  The gradient of x is
+ * q38m_moe_unpermute_rows_v1 of the rows' gradient with NULL weights. */
+int q38m_moe_permute_rows_v1(const void* x, uint32_t dtype,
+                             const uint32_t* assignment_to_packed, uint32_t tokens,
+                             uint32_t top_k, uint32_t width, void* rows, void* stream,
+                             int device);
+
+/* y[t] = sum over r of route_weights[t][r] * rows[assignment_to_packed[t *
+ * top_k + r]], in rank order, fp32 fused multiply-adds, one rounding; NULL
+ * weights are ones.  A token without kept routes gets zeros; what a dropped
+ * route's weight holds does not matter. */
+int q38m_moe_unpermute_rows_v1(const void* rows, uint32_t dtype,
+                               const uint32_t* assignment_to_packed,
+                               const float* route_weights, uint32_t tokens, uint32_t top_k,
+                               uint32_t width, void* y, void* stream, int device);
+
+/* The gradients of q38m_moe_unpermute_rows_v1 for dy [tokens][width]:
+ * d_rows[p] = route_weights[t][r] * dy[t] (rows behind the kept routes are
+ * left as they were) and d_weights[t][r] = sum over the columns of dy[t] *
+ * rows[p] (fp32, a fixed order; 0 for a dropped route).  Either may be NULL,
+ * rows too where d_weights is. */
+int q38m_moe_unpermute_backward_v1(const void* dy, const void* rows, uint32_t dtype,
+                                   const uint32_t* assignment_to_packed,
+                                   const float* route_weights, uint32_t tokens,
+                                   uint32_t top_k, uint32_t width, void* d_rows,
+                                   float* d_weights, void* stream, int device);
+
 /* ---- deterministic synthetic data (counter-based SplitMix64) --------- */
 #define Q38M_SYNTH_NORMAL_F32 1u     /* sigma*N(0,1) (+ bias[i % bias_len]) */
 #define Q38M_SYNTH_NORMAL_BF16 2u    /* bf16(sigma*N(0,1)) */

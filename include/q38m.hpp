@@ -269,6 +269,75 @@ inline void moe_shared_expert(const std::uint16_t* hidden, const std::uint16_t* 
                                     stream, device));
 }
 
+// ---- microscaled 4-bit rows and sorted tokens: no reference counterpart; the
+// entry points of the same names in q38m.h, whose comments say what they do.
+using MxMatrixV1 = q38m_mx_matrix_v1;
+
+enum class DtypeV1 : std::uint32_t { kF32 = Q38M_DTYPE_F32, kBf16 = Q38M_DTYPE_BF16 };
+enum class MxEpilogueV1 : std::uint32_t {
+    kNone = Q38M_MX_EPILOGUE_NONE,
+    kSwiglu = Q38M_MX_EPILOGUE_SWIGLU,
+};
+
+inline void mx_quantize(const void* x, DtypeV1 dtype, std::uint64_t x_stride,
+                        const MxMatrixV1& dst, void* rounded, void* stream, int device) {
+    check(q38m_mx_quantize_v1(x, static_cast<std::uint32_t>(dtype), x_stride, &dst, rounded,
+                              stream, device));
+}
+
+inline void mx_gemm(const MxMatrixV1& a, const MxMatrixV1& b, float* c_f32,
+                    std::uint16_t* c_bf16, std::uint64_t c_stride, void* stream, int device) {
+    check(q38m_mx_gemm_v1(&a, &b, c_f32, c_bf16, c_stride, stream, device));
+}
+
+inline void mx_grouped_gemm(const MxMatrixV1& weights, const MxMatrixV1& rows,
+                            const std::uint32_t* expert_offsets,
+                            const std::uint32_t* packed_assignment, std::uint32_t top_k,
+                            std::uint32_t routes, MxEpilogueV1 epilogue, float* c_f32,
+                            std::uint16_t* c_bf16, void* stream, int device) {
+    check(q38m_mx_grouped_gemm_v1(&weights, &rows, expert_offsets, packed_assignment, top_k,
+                                  routes, static_cast<std::uint32_t>(epilogue), c_f32, c_bf16,
+                                  stream, device));
+}
+
+inline void moe_sort_routes(const std::int32_t* expert_ids, std::uint32_t tokens,
+                            std::uint32_t top_k, std::uint32_t experts,
+                            std::uint32_t* expert_offsets, std::uint32_t* packed_assignment,
+                            std::uint32_t* assignment_to_packed, void* scratch,
+                            std::size_t scratch_bytes, void* stream, int device) {
+    check(q38m_moe_sort_routes_v1(expert_ids, tokens, top_k, experts, expert_offsets,
+                                  packed_assignment, assignment_to_packed, scratch,
+                                  scratch_bytes, stream, device));
+}
+
+inline void moe_permute_rows(const void* x, DtypeV1 dtype,
+                             const std::uint32_t* assignment_to_packed, std::uint32_t tokens,
+                             std::uint32_t top_k, std::uint32_t width, void* rows, void* stream,
+                             int device) {
+    check(q38m_moe_permute_rows_v1(x, static_cast<std::uint32_t>(dtype), assignment_to_packed,
+                                   tokens, top_k, width, rows, stream, device));
+}
+
+inline void moe_unpermute_rows(const void* rows, DtypeV1 dtype,
+                               const std::uint32_t* assignment_to_packed,
+                               const float* route_weights, std::uint32_t tokens,
+                               std::uint32_t top_k, std::uint32_t width, void* y, void* stream,
+                               int device) {
+    check(q38m_moe_unpermute_rows_v1(rows, static_cast<std::uint32_t>(dtype),
+                                     assignment_to_packed, route_weights, tokens, top_k, width,
+                                     y, stream, device));
+}
+
+inline void moe_unpermute_backward(const void* dy, const void* rows, DtypeV1 dtype,
+                                   const std::uint32_t* assignment_to_packed,
+                                   const float* route_weights, std::uint32_t tokens,
+                                   std::uint32_t top_k, std::uint32_t width, void* d_rows,
+                                   float* d_weights, void* stream, int device) {
+    check(q38m_moe_unpermute_backward_v1(dy, rows, static_cast<std::uint32_t>(dtype),
+                                         assignment_to_packed, route_weights, tokens, top_k,
+                                         width, d_rows, d_weights, stream, device));
+}
+
 inline bool cuda_q38_moe_prefill_compiled() { return q38m_moe_compiled() == 1; }
 inline bool cuda_q38_moe_compiled() { return q38m_moe_compiled() == 1; }
 

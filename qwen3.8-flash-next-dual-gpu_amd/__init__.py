@@ -46,6 +46,13 @@ LAYOUT_ROW_MAJOR = 0
 LAYOUT_MFMA16 = 2
 LAYOUT_MFMA16_PAIRED = 3
 
+DTYPE_F32 = 1
+DTYPE_BF16 = 2
+MX_BLOCK = 32
+MX_EPILOGUE_NONE = 0
+MX_EPILOGUE_SWIGLU = 1
+ROUTE_DROPPED = 0xffffffff
+
 SYNTH_NORMAL_F32 = 1
 SYNTH_NORMAL_BF16 = 2
 SYNTH_ABS_NORMAL_F16 = 3
@@ -105,6 +112,12 @@ class PrefillWorkspace(ctypes.Structure):
                 ("weighted_mid", ctypes.c_void_p), ("mid_q", ctypes.c_void_p),
                 ("mid_s", ctypes.c_void_p), ("route_output", ctypes.c_void_p),
                 ("task_flags", ctypes.c_void_p)]
+
+
+class MxMatrix(ctypes.Structure):
+    _fields_ = [("codes", ctypes.c_void_p), ("scales", ctypes.c_void_p),
+                ("experts", ctypes.c_uint32), ("rows", ctypes.c_uint32),
+                ("columns", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
 
 
 class WideWorkspace(ctypes.Structure):
@@ -190,6 +203,19 @@ SIGNATURES = {
     "q38m_hyper_inject_bf16": (_INT, [_P, _P, _P, _P, _U32, _U32, _P, _INT]),
     "q38m_hyper_prepare_scratch_bytes": (_SZ, [_U32, _U32, _U32]),
     "q38m_hyper_prepare_v1": (_INT, [_P, _P, _P, _P, _P, _U32, _U32, _U32, _P, _P, _P, _P, _INT]),
+    "q38m_mx_row_bytes": (_SZ, [_U32]),
+    "q38m_mx_scale_bytes": (_SZ, [_U32]),
+    "q38m_mx_quantize_v1": (_INT, [_P, _U32, _U64, ctypes.POINTER(MxMatrix), _P, _P, _INT]),
+    "q38m_mx_gemm_v1": (_INT, [ctypes.POINTER(MxMatrix), ctypes.POINTER(MxMatrix), _P, _P, _U64,
+                               _P, _INT]),
+    "q38m_mx_grouped_gemm_v1": (_INT, [ctypes.POINTER(MxMatrix), ctypes.POINTER(MxMatrix), _P, _P,
+                                       _U32, _U32, _U32, _P, _P, _P, _INT]),
+    "q38m_moe_sort_scratch_bytes": (_SZ, [_U32, _U32, _U32]),
+    "q38m_moe_sort_routes_v1": (_INT, [_P, _U32, _U32, _U32, _P, _P, _P, _P, _SZ, _P, _INT]),
+    "q38m_moe_permute_rows_v1": (_INT, [_P, _U32, _P, _U32, _U32, _U32, _P, _P, _INT]),
+    "q38m_moe_unpermute_rows_v1": (_INT, [_P, _U32, _P, _P, _U32, _U32, _U32, _P, _P, _INT]),
+    "q38m_moe_unpermute_backward_v1": (_INT, [_P, _P, _U32, _P, _P, _U32, _U32, _U32, _P, _P, _P,
+                                              _INT]),
     "q38m_synth_fill": (_INT, [_U32, _U64, _U64, _U64, _F, _I32, _I32, _P, _U32, _P, _P, _INT]),
     "q38m_moe_compiled": (_INT, []),
     "q38m_last_error": (ctypes.c_char_p, []),
@@ -421,6 +447,48 @@ def repack(weights, paired=False, stream=None):
     call("q38m_repack_expert_weights", ctypes.byref(weights.desc), ctypes.byref(out.desc),
          stream_handle(stream), device_index(data))
     return out
+
+
+class MxRows:
+    """Microscaled 4-bit rows resident in device memory plus their descriptor."""
+
+    def __init__(self, experts, rows, columns, device="cuda"):
+        torch = _torch()
+        row, scale = lib().q38m_mx_row_bytes(columns), lib().q38m_mx_scale_bytes(columns)
+        self.codes = torch.empty(experts * rows, row, dtype=torch.uint8, device=device)
+        self.scales = torch.empty(experts * rows, scale, dtype=torch.uint8, device=device)
+        self.desc = MxMatrix(ptr(self.codes), ptr(self.scales), experts, rows, columns)
+
+
+def mx_quantize(x, experts=1, rounded=None, stream=None):
+    """x [experts * rows][columns] (bf16, raw bf16 words or fp32; any row
+    stride) as MxRows."""
+    torch = _torch()
+    out = MxRows(experts, x.shape[0] // experts, x.shape[1], x.device)
+    dtype = DTYPE_F32 if x.dtype == torch.float32 else DTYPE_BF16
+    call("q38m_mx_quantize_v1", ptr(x), dtype, x.stride(0), ctypes.byref(out.desc), ptr(rounded),
+         stream_handle(stream), device_index(x))
+    return out
+
+
+class SortedRoutes:
+    """Buffers of q38m_moe_sort_routes_v1 for one shape; sort(ids) fills them."""
+
+    def __init__(self, tokens, top_k, experts, device="cuda"):
+        torch = _torch()
+        routes = tokens * top_k
+        self.tokens, self.top_k, self.experts = tokens, top_k, experts
+        self.offsets = torch.empty(experts + 1, dtype=torch.int32, device=device)
+        self.packed = torch.empty(routes, dtype=torch.int32, device=device)
+        self.inverse = torch.empty(routes, dtype=torch.int32, device=device)
+        nbytes = lib().q38m_moe_sort_scratch_bytes(tokens, top_k, experts)
+        self.scratch = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=device)
+
+    def sort(self, ids, stream=None):
+        call("q38m_moe_sort_routes_v1", ptr(ids), self.tokens, self.top_k, self.experts,
+             ptr(self.offsets), ptr(self.packed), ptr(self.inverse), ptr(self.scratch),
+             self.scratch.numel(), stream_handle(stream), device_index(ids))
+        return self
 
 
 class PrefillWorkspace_:

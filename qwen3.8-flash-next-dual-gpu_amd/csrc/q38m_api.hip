@@ -928,6 +928,168 @@ int q38m_quantize_expert_weights(const uint16_t* src_bf16, const q38m_expert_wei
                   "quantize_weights kernels");
 }
 
+namespace {
+
+constexpr uint32_t kMaxWidth = 1u << 24;  // columns and row widths: byte counts of a row below 2^32
+
+bool valid_dtype(uint32_t dtype) { return dtype == Q38M_DTYPE_F32 || dtype == Q38M_DTYPE_BF16; }
+
+bool element_aligned(const void* p, uint32_t dtype) {
+    return aligned(p, dtype == Q38M_DTYPE_F32 ? 4u : 2u);
+}
+
+bool valid_mx(const q38m_mx_matrix_v1* m) {
+    return m && m->codes && m->scales && aligned(m->codes, 16) && aligned(m->scales, 4) &&
+           m->experts != 0u && m->rows != 0u && m->columns != 0u && m->columns <= kMaxWidth &&
+           m->reserved == 0u;
+}
+
+// tokens * top_k, or 0 where a sorted order does not hold so many
+uint32_t sort_routes(uint32_t tokens, uint32_t top_k) {
+    const uint64_t routes = static_cast<uint64_t>(tokens) * top_k;
+    return routes <= q38m::kMaxSortRoutes ? static_cast<uint32_t>(routes) : 0u;
+}
+
+bool valid_rows(uint32_t dtype, uint32_t tokens, uint32_t top_k, uint32_t width) {
+    return valid_dtype(dtype) && sort_routes(tokens, top_k) != 0u && width != 0u &&
+           width <= kMaxWidth;
+}
+
+}  // namespace
+
+size_t q38m_mx_row_bytes(uint32_t columns) {
+    return static_cast<size_t>(q38m::mx_k128(columns)) * 64u;
+}
+
+size_t q38m_mx_scale_bytes(uint32_t columns) {
+    return static_cast<size_t>(q38m::mx_k128(columns)) * 4u;
+}
+
+int q38m_mx_quantize_v1(const void* x, uint32_t dtype, uint64_t x_stride,
+                        const q38m_mx_matrix_v1* dst, void* rounded, void* stream, int device) {
+    if (!x || !valid_dtype(dtype) || !valid_mx(dst) || x_stride < dst->columns ||
+        !element_aligned(x, dtype) || !element_aligned(rounded, dtype))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid microscaled quantisation input");
+    const uint64_t rows = static_cast<uint64_t>(dst->experts) * dst->rows;
+    if (rows > q38m::kMaxMxRows)
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "too many rows for one microscaled quantisation");
+    if (int rc = select_device(device)) return rc;
+    return finish(q38m::launch_mx_quantize(x, dtype, x_stride, static_cast<uint32_t>(rows),
+                                           dst->columns, dst->codes, dst->scales, rounded,
+                                           as_stream(stream)),
+                  "mx_quantize_kernel");
+}
+
+int q38m_mx_gemm_v1(const q38m_mx_matrix_v1* a, const q38m_mx_matrix_v1* b, float* c_f32,
+                    uint16_t* c_bf16, uint64_t c_stride, void* stream, int device) {
+    if (!valid_mx(a) || !valid_mx(b) || a->experts != 1u || b->experts != 1u ||
+        a->columns != b->columns || !c_f32 == !c_bf16 || c_stride < b->rows ||
+        !aligned(c_f32, 4) || !aligned(c_bf16, 2))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid microscaled product");
+    const q38m::MxProduct p{static_cast<const uint8_t*>(a->codes),
+                            static_cast<const uint8_t*>(a->scales),
+                            static_cast<const uint8_t*>(b->codes),
+                            static_cast<const uint8_t*>(b->scales),
+                            nullptr, nullptr, c_f32, c_bf16, c_stride, a->rows, a->rows, b->rows,
+                            q38m::mx_k128(a->columns), 1u, 1u};
+    if (!q38m::mx_product_fits(p, false))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "microscaled product too large for one call");
+    if (int rc = select_device(device)) return rc;
+    return finish(q38m::launch_mx_product(p, false, as_stream(stream)), "mx_product_kernel");
+}
+
+int q38m_mx_grouped_gemm_v1(const q38m_mx_matrix_v1* weights, const q38m_mx_matrix_v1* rows,
+                            const uint32_t* expert_offsets, const uint32_t* packed_assignment,
+                            uint32_t top_k, uint32_t routes, uint32_t epilogue, float* c_f32,
+                            uint16_t* c_bf16, void* stream, int device) {
+    const bool swiglu = epilogue == Q38M_MX_EPILOGUE_SWIGLU;
+    if (!valid_mx(weights) || !valid_mx(rows) || rows->experts != 1u ||
+        weights->columns != rows->columns || weights->experts > q38m::kMaxSortExperts ||
+        !expert_offsets || top_k == 0u || routes == 0u || routes > q38m::kMaxSortRoutes ||
+        (!packed_assignment && rows->rows != routes) ||
+        (!swiglu && epilogue != Q38M_MX_EPILOGUE_NONE) || (swiglu && weights->rows % 2u != 0u) ||
+        !c_f32 == !c_bf16 || !aligned(c_f32, 4) || !aligned(c_bf16, 2))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid microscaled expert product");
+    const q38m::MxProduct p{static_cast<const uint8_t*>(rows->codes),
+                            static_cast<const uint8_t*>(rows->scales),
+                            static_cast<const uint8_t*>(weights->codes),
+                            static_cast<const uint8_t*>(weights->scales),
+                            expert_offsets, packed_assignment, c_f32, c_bf16,
+                            swiglu ? weights->rows / 2u : weights->rows, rows->rows, routes,
+                            weights->rows, q38m::mx_k128(rows->columns), weights->experts, top_k};
+    if (!q38m::mx_product_fits(p, swiglu))
+        return fail(Q38M_ERR_INVALID_ARGUMENT,
+                    "microscaled expert product too large for one call");
+    if (int rc = select_device(device)) return rc;
+    return finish(q38m::launch_mx_product(p, swiglu, as_stream(stream)), "mx_product_kernel");
+}
+
+size_t q38m_moe_sort_scratch_bytes(uint32_t tokens, uint32_t top_k, uint32_t experts) {
+    const uint32_t routes = sort_routes(tokens, top_k);
+    if (routes == 0u || experts == 0u || experts > q38m::kMaxSortExperts) return 0u;
+    return q38m::sort_scratch_words(routes, experts) * sizeof(uint32_t);
+}
+
+int q38m_moe_sort_routes_v1(const int32_t* expert_ids, uint32_t tokens, uint32_t top_k,
+                            uint32_t experts, uint32_t* expert_offsets,
+                            uint32_t* packed_assignment, uint32_t* assignment_to_packed,
+                            void* scratch, size_t scratch_bytes, void* stream, int device) {
+    const uint32_t routes = sort_routes(tokens, top_k);
+    if (!expert_ids || routes == 0u || experts == 0u || experts > q38m::kMaxSortExperts ||
+        !expert_offsets || !packed_assignment || !assignment_to_packed)
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid route sort input");
+    const size_t needed = q38m_moe_sort_scratch_bytes(tokens, top_k, experts);
+    if (needed != 0u && (!scratch || scratch_bytes < needed || !aligned(scratch, 4)))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "route sort scratch is missing, small or unaligned");
+    if (int rc = select_device(device)) return rc;
+    return finish(q38m::launch_sort_routes(expert_ids, routes, experts, expert_offsets,
+                                           packed_assignment, assignment_to_packed,
+                                           static_cast<uint32_t*>(scratch), as_stream(stream)),
+                  "route sort kernels");
+}
+
+int q38m_moe_permute_rows_v1(const void* x, uint32_t dtype, const uint32_t* assignment_to_packed,
+                             uint32_t tokens, uint32_t top_k, uint32_t width, void* rows,
+                             void* stream, int device) {
+    if (!x || !assignment_to_packed || !rows || !valid_rows(dtype, tokens, top_k, width) ||
+        !element_aligned(x, dtype) || !element_aligned(rows, dtype))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid row permutation input");
+    if (int rc = select_device(device)) return rc;
+    return finish(q38m::launch_permute_rows(x, dtype, assignment_to_packed, tokens, top_k, width,
+                                            rows, as_stream(stream)),
+                  "permute_kernel");
+}
+
+int q38m_moe_unpermute_rows_v1(const void* rows, uint32_t dtype,
+                               const uint32_t* assignment_to_packed, const float* route_weights,
+                               uint32_t tokens, uint32_t top_k, uint32_t width, void* y,
+                               void* stream, int device) {
+    if (!rows || !assignment_to_packed || !y || !valid_rows(dtype, tokens, top_k, width) ||
+        !element_aligned(rows, dtype) || !element_aligned(y, dtype) || !aligned(route_weights, 4))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid row return input");
+    if (int rc = select_device(device)) return rc;
+    return finish(q38m::launch_unpermute_rows(rows, dtype, assignment_to_packed, route_weights,
+                                              tokens, top_k, width, y, as_stream(stream)),
+                  "unpermute_kernel");
+}
+
+int q38m_moe_unpermute_backward_v1(const void* dy, const void* rows, uint32_t dtype,
+                                   const uint32_t* assignment_to_packed,
+                                   const float* route_weights, uint32_t tokens, uint32_t top_k,
+                                   uint32_t width, void* d_rows, float* d_weights, void* stream,
+                                   int device) {
+    if (!dy || !assignment_to_packed || !route_weights || (!d_rows && !d_weights) ||
+        (d_weights && !rows) || !valid_rows(dtype, tokens, top_k, width) ||
+        !element_aligned(dy, dtype) || !element_aligned(rows, dtype) ||
+        !element_aligned(d_rows, dtype) || !aligned(route_weights, 4) || !aligned(d_weights, 4))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid row return gradient input");
+    if (int rc = select_device(device)) return rc;
+    return finish(q38m::launch_unpermute_backward(dy, rows, dtype, assignment_to_packed,
+                                                  route_weights, tokens, top_k, width, d_rows,
+                                                  d_weights, as_stream(stream)),
+                  "unpermute_backward_kernel");
+}
+
 int q38m_synth_fill(uint32_t kind, uint64_t seed, uint64_t tag, uint64_t count, float sigma,
                     int32_t lo, int32_t hi, const float* bias, uint32_t bias_len, void* out,
                     void* stream, int device) {

@@ -238,4 +238,61 @@ hipError_t launch_synth(uint32_t kind, uint64_t seed, uint64_t tag, uint64_t cou
                         float sigma, int32_t lo, int32_t hi, const float* bias,
                         uint32_t bias_len, void* out, hipStream_t stream);
 
+// tokens sorted by expert and back (q38m_sort.hip)
+constexpr uint32_t kMaxSortExperts = 1024;
+constexpr uint32_t kMaxSortRoutes = (1u << 24) - 1u;  // a workgroup per token: grids below 2^32 threads
+constexpr uint32_t kSortSmallRoutes = 8192;
+constexpr uint32_t kSortChunk = 1024;
+constexpr uint32_t sort_chunks(uint32_t routes) { return (routes + kSortChunk - 1u) / kSortChunk; }
+// scratch: sort_scratch_words(routes, experts) words
+constexpr size_t sort_scratch_words(uint32_t routes, uint32_t experts) {
+    return routes <= kSortSmallRoutes ? 0u
+                                      : static_cast<size_t>(sort_chunks(routes)) * (experts + 1u);
+}
+hipError_t launch_sort_routes(const int32_t* ids, uint32_t routes, uint32_t experts,
+                              uint32_t* offsets, uint32_t* packed, uint32_t* inverse,
+                              uint32_t* scratch, hipStream_t stream);
+hipError_t launch_permute_rows(const void* x, uint32_t dtype, const uint32_t* inverse,
+                               uint32_t tokens, uint32_t top_k, uint32_t width, void* rows,
+                               hipStream_t stream);
+// weights may be null (ones)
+hipError_t launch_unpermute_rows(const void* rows, uint32_t dtype, const uint32_t* inverse,
+                                 const float* weights, uint32_t tokens, uint32_t top_k,
+                                 uint32_t width, void* y, hipStream_t stream);
+// either of d_rows and d_weights may be null
+hipError_t launch_unpermute_backward(const void* dy, const void* rows, uint32_t dtype,
+                                     const uint32_t* inverse, const float* weights,
+                                     uint32_t tokens, uint32_t top_k, uint32_t width,
+                                     void* d_rows, float* d_weights, hipStream_t stream);
+
+// microscaled 4-bit rows (q38m_mx.hip)
+constexpr uint32_t kMaxMxRows = 1u << 23;  // a workgroup per row: grids below 2^32 threads
+constexpr uint32_t mx_k128(uint32_t columns) { return (columns + 127u) / 128u; }
+// rounded may be null
+hipError_t launch_mx_quantize(const void* x, uint32_t dtype, uint64_t stride, uint32_t rows,
+                              uint32_t columns, void* codes, void* scales, void* rounded,
+                              hipStream_t stream);
+// C = A B^T, or with offsets the experts' products: sorted row p of expert e is
+// A's row p, or packed[p] / top_k, times B's matrix e
+struct MxProduct {
+    const uint8_t* a_codes;
+    const uint8_t* a_scales;
+    const uint8_t* b_codes;
+    const uint8_t* b_scales;
+    const uint32_t* offsets;  // null: the dense product
+    const uint32_t* packed;
+    float* c_f32;      // one of the two
+    uint16_t* c_bf16;
+    uint64_t c_stride;
+    uint32_t a_rows, routes, n, k128, experts, top_k;  // routes: C's rows
+};
+// row tiles that `routes` rows over `experts` experts need at most
+constexpr uint32_t mx_max_tasks(uint32_t routes, uint32_t experts, uint32_t tile) {
+    const uint32_t first = routes < experts ? routes : experts;
+    return first + (routes - first) / tile;
+}
+// whether the launch's grid holds the product
+bool mx_product_fits(const MxProduct& p, bool swiglu);
+hipError_t launch_mx_product(const MxProduct& p, bool swiglu, hipStream_t stream);
+
 }  // namespace q38m
