@@ -5,6 +5,8 @@
 // low nibble; codes past K are zero) and one scale byte for every 32 values.
 // Code c stands for (-1)^(c >> 3) * {0, .5, 1, 1.5, 2, 3, 4, 6}[c & 7], scale
 // byte s for 2^(s - 127), 255 for NaN.
+#include <type_traits>
+
 #include "q38m_device.h"
 #include "q38m_internal.h"
 
@@ -169,121 +171,367 @@ __global__ __launch_bounds__(kQuantThreads) void mx_quantize_kernel(
 // ---- products -----------------------------------------------------------------
 
 typedef int v8i __attribute__((ext_vector_type(8)));
+typedef float v16f __attribute__((ext_vector_type(16)));
 
-// v_mfma_scale_f32_16x16x128_f8f6f4 on 4-bit codes: lane l holds the 32 values
-// k = 32 (l / 16) .. + 31 of row l % 16 of A and of B and their scale byte (the
-// low one); D lane l: rows 4 (l / 16) + i of A, row l % 16 of B.  Products and
-// scales are exact; the sum is rounded in fp32.
-__device__ __forceinline__ v4f mfma_mx_16x16x128(v4i a, uint32_t sa, v4i b, uint32_t sb, v4f c) {
+// The block-scaled matrix instructions on 4-bit codes.  v_mfma_scale_f32_16x16x128:
+// lane l holds the 32 values k = 32 (l / 16) .. + 31 of row l % 16 of A and of B and
+// byte kByteA / kByteB of its scale word is that block's scale; D lane l: rows 4 (l / 16)
+// + i of A, row l % 16 of B.  v_mfma_scale_f32_32x32x64: k = 32 (l / 32) .. + 31 of row
+// l % 32; D lane l: rows 8 (i / 4) + 4 (l / 32) + i % 4 of A, row l % 32 of B.  Products
+// and scales are exact; the sum is rounded in fp32.  In a loop over registers alone
+// the 32x32 form runs at 6.6 PFLOP/s, the 16x16 form at 5.2.
+template <int kByte>
+__device__ __forceinline__ v4f mfma_mx(v4i a, uint32_t sa, v4i b, uint32_t sb, v4f c) {
     const v8i wa = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, wb = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
-    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, wb, c, 4, 4, 0, sa, 0, sb);
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, wb, c, 4, 4, kByte, sa, kByte, sb);
 }
-
-struct MxTask {
-    uint32_t expert, first, count;  // rows first .. first + count of the sorted order
-};
-
-// Row tile `task` of the experts' rows, kRows at a time, found by every wave
-// for itself: lanes hold consecutive experts, a sum over the lanes of their
-// tiles gives the lane that holds the tile.  Offsets past `routes` or falling
-// ones count as no rows.  count = 0: there is no such tile.
-template <uint32_t kRows>
-__device__ MxTask find_task(const uint32_t* __restrict__ offsets, uint32_t experts,
-                            uint32_t routes, uint32_t task) {
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint32_t per = (experts + 63u) / 64u, e0 = lane * per;
-    const uint32_t e1 = min(e0 + per, experts);
-    uint32_t tiles = 0, begin = e0 < experts ? min(offsets[e0], routes) : 0u, next = begin;
-    for (uint32_t e = e0; e < e1; ++e) {
-        const uint32_t end = min(offsets[e + 1u], routes);
-        if (end > next) {
-            tiles += (end - next + kRows - 1u) / kRows;
-        }
-        next = end;
-    }
-    uint32_t sum = tiles;
-#pragma unroll
-    for (uint32_t d = 1; d < 64u; d <<= 1) {
-        const uint32_t up = __shfl_up(sum, d);
-        if (lane >= d) sum += up;
-    }
-    const uint64_t past = __ballot(sum > task);
-    MxTask found{0u, 0u, 0u};
-    if (past == 0u) return found;
-    const uint32_t owner = __builtin_ctzll(past);
-    uint32_t left = task - (sum - tiles), expert = e0;
-    if (lane == owner) {
-        next = begin;
-        for (uint32_t e = e0; e < e1; ++e) {
-            const uint32_t end = min(offsets[e + 1u], routes);
-            const uint32_t n = end > next ? (end - next + kRows - 1u) / kRows : 0u;
-            if (left < n) {
-                expert = e;
-                found.first = next + left * kRows;
-                found.count = min(end - found.first, kRows);
-                break;
-            }
-            left -= n;
-            next = end;
-        }
-    }
-    found.expert = __builtin_amdgcn_readlane(expert, owner);
-    found.first = __builtin_amdgcn_readlane(found.first, owner);
-    found.count = __builtin_amdgcn_readlane(found.count, owner);
-    return found;
+template <int kByte>
+__device__ __forceinline__ v16f mfma_mx(v4i a, uint32_t sa, v4i b, uint32_t sb, v16f c) {
+    const v8i wa = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, wb = {b[0], b[1], b[2], b[3], 0, 0, 0, 0};
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wa, wb, c, 4, 4, kByte, sa, kByte, sb);
 }
 
 // h = silu(g) u
 __device__ __forceinline__ float swiglu(float g, float u) { return g / (1.0f + exp_q(-g)) * u; }
 
-// One wave per 16 x 16 tile of C (with the SwiGLU fold, of its gate half and
-// its up half), operands straight from memory.
-template <bool kSwiglu>
-__global__ __launch_bounds__(64) void mx_product_kernel(MxProduct p) {
-    const uint32_t lane = threadIdx.x, r = lane & 15u, q = lane >> 4;
-    MxTask t;
-    if (p.offsets) {
-        t = find_task<16>(p.offsets, p.experts, p.routes, blockIdx.y);
-        if (t.count == 0u) return;
-    } else {
-        t = MxTask{0u, blockIdx.y * 16u, min(p.routes - blockIdx.y * 16u, 16u)};
-    }
-    const uint32_t n_out = kSwiglu ? p.n / 2u : p.n;
-    const uint32_t n0 = blockIdx.x * 16u;
-    const uint32_t row_bytes = p.k128 * 64u, scale_bytes = p.k128 * 4u;
-    uint32_t source = t.first + min(r, t.count - 1u);
-    if (p.packed) source = p.packed[source] / p.top_k;
-    const bool real = r < t.count && source < p.a_rows;
-    source = min(source, p.a_rows - 1u);
-    const uint8_t* a = p.a_codes + static_cast<uint64_t>(source) * row_bytes + 16u * q;
-    const uint8_t* as = p.a_scales + static_cast<uint64_t>(source) * scale_bytes + q;
-    const uint32_t column = min(n0 + r, n_out - 1u);
-    const uint64_t w_row = static_cast<uint64_t>(t.expert) * p.n + column;
-    const uint8_t* b = p.b_codes + w_row * row_bytes + 16u * q;
-    const uint8_t* bs = p.b_scales + w_row * scale_bytes + q;
-    const uint64_t up = static_cast<uint64_t>(n_out) * row_bytes;
-    const uint64_t up_scale = static_cast<uint64_t>(n_out) * scale_bytes;
-    v4f acc = {0, 0, 0, 0}, acc_up = {0, 0, 0, 0};
-    for (uint32_t k = 0; k < p.k128; ++k) {
-        v4i av = *reinterpret_cast<const v4i*>(a + 64u * k);
-        if (!real) av = v4i{0, 0, 0, 0};
-        const uint32_t sa = real ? as[4u * k] : 127u;
-        acc = mfma_mx_16x16x128(av, sa, *reinterpret_cast<const v4i*>(b + 64u * k), bs[4u * k], acc);
-        if constexpr (kSwiglu)
-            acc_up = mfma_mx_16x16x128(av, sa, *reinterpret_cast<const v4i*>(b + up + 64u * k),
-                                       bs[up_scale + 4u * k], acc_up);
-    }
-    if (n0 + r >= n_out) return;
+struct MxTask {
+    uint32_t expert, first, count;  // rows first .. first + count of the sorted order
+};
+
+// The row tiles of the experts' rows, kRows at a time, held by a wave: lane l holds
+// the experts kPer l .. kPer l + kPer - 1, their first rows and row tiles, and the sum
+// of tiles up to and with them.  Offsets past `routes` count as routes, an end that is
+// not behind its begin as no rows.
+template <uint32_t kRows, uint32_t kPer>
+struct TileList {
+    uint32_t begin[kPer], end[kPer], sum, total;
+
+    __device__ TileList(const uint32_t* __restrict__ offsets, uint32_t experts, uint32_t routes) {
+        const uint32_t lane = threadIdx.x & 63u, e0 = lane * kPer;
+        uint32_t at[kPer + 1];
 #pragma unroll
-    for (uint32_t i = 0; i < 4u; ++i) {
-        const uint32_t m = 4u * q + i;
-        if (m >= t.count) break;
-        const float v = kSwiglu ? swiglu(acc[i], acc_up[i]) : acc[i];
-        const uint64_t at = static_cast<uint64_t>(t.first + m) * p.c_stride + n0 + r;
-        if (p.c_f32) p.c_f32[at] = v;
-        else p.c_bf16[at] = static_cast<uint16_t>(f32_to_bf16(v));
+        for (uint32_t i = 0; i <= kPer; ++i) at[i] = offsets[min(e0 + i, experts)];
+        uint32_t tiles = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; ++i) {
+            begin[i] = min(at[i], routes);
+            end[i] = max(min(at[i + 1u], routes), begin[i]);
+            tiles += (end[i] - begin[i] + kRows - 1u) / kRows;
+        }
+        sum = tiles;
+#pragma unroll
+        for (uint32_t d = 1; d < 64u; d <<= 1) {
+            const uint32_t up = __shfl_up(sum, d);
+            if (lane >= d) sum += up;
+        }
+        total = __builtin_amdgcn_readlane(sum, 63);
+    }
+
+    // task < total
+    __device__ MxTask find(uint32_t task) const {
+        const uint32_t owner = __builtin_ctzll(__ballot(sum > task));
+        uint32_t tiles = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; ++i) tiles += (end[i] - begin[i] + kRows - 1u) / kRows;
+        uint32_t left = task - (sum - tiles), expert = 0, first = 0, count = 0;
+        bool found = false;
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; ++i) {
+            const uint32_t n = (end[i] - begin[i] + kRows - 1u) / kRows;
+            if (!found && left < n) {
+                found = true;
+                expert = (threadIdx.x & 63u) * kPer + i;
+                first = begin[i] + left * kRows;
+                count = min(end[i] - first, kRows);
+            }
+            left -= n;
+        }
+        return MxTask{static_cast<uint32_t>(__builtin_amdgcn_readlane(expert, owner)),
+                      static_cast<uint32_t>(__builtin_amdgcn_readlane(first, owner)),
+                      static_cast<uint32_t>(__builtin_amdgcn_readlane(count, owner))};
+    }
+};
+
+// A workgroup computes kBM rows of C by kBN rows of B (with the SwiGLU fold half of
+// them gate, half up rows).  kWM x kWN waves, each kTM x kTN matrix-instruction tiles
+// of kMF rows.  K goes through LDS 256 values (128 bytes a row) at a time in a ring of
+// kStages slots, loaded straight from memory (no registers between, so the ring's depth
+// costs none).  A slot holds kBM rows of A, kBN rows of B, 128 bytes each, then their
+// scales, 8 bytes each.
+//
+// The eight 16-byte pieces of row r lie at positions p ^ (r / 2 % 8): the lanes of a
+// read take one piece of 16 or 32 consecutive rows, which then spread over all 64
+// banks.  A load instruction fills 1 KB of consecutive LDS, eight rows; the swizzle is
+// in the addresses that its lanes read.
+template <uint32_t kMF_, uint32_t kWM_, uint32_t kWN_, uint32_t kTM_, uint32_t kTN_, uint32_t kStages_>
+struct MxShape {
+    static constexpr uint32_t kMF = kMF_, kWM = kWM_, kWN = kWN_, kTM = kTM_, kTN = kTN_;
+    static constexpr uint32_t kStages = kStages_, kWaves = kWM * kWN;
+    static constexpr uint32_t kBM = kWM * kTM * kMF, kBN = kWN * kTN * kMF, kRows = kBM + kBN;
+    static constexpr uint32_t kData = kRows / 8u;                 // load instructions of 1 KB
+    static constexpr uint32_t kScale = (kRows + 31u) / 32u;       // of 256 bytes
+    static constexpr uint32_t kLoads = kData + kScale;
+    static constexpr uint32_t kMine = (kLoads + kWaves - 1u) / kWaves;  // a wave's, at most
+    static constexpr uint32_t kSlot = kRows * 8u + kScale * 16u;  // 16-byte words
+    static constexpr uint32_t kSteps = 256u * kMF / 2048u;        // matrix instructions deep: 2 or 4
+};
+
+__device__ __forceinline__ void mx_load16(const uint8_t* src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src),
+                 "s"(lds)
+                 : "memory");
+}
+__device__ __forceinline__ void mx_load4(const uint8_t* src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src),
+                 "s"(lds)
+                 : "memory");
+}
+
+// until at most kOutstanding of the wave's loads are in flight and its LDS reads are
+// complete, then for the workgroup's waves to get there
+template <uint32_t kOutstanding>
+__device__ __forceinline__ void mx_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(kOutstanding) : "memory");
+}
+
+// Order of the tiles: groups of kGroup row tiles, in a group column by column, so that
+// tiles at work at the same time share rows of A and of B.  The dispatcher hands
+// workgroups to the eight XCDs in turn, each with an L2 of its own: XCD x takes one
+// contiguous eighth of the order.
+constexpr uint32_t kXcds = 8, kGroup = 4;
+struct MxTile {
+    uint32_t row, column;
+    bool some;
+};
+__device__ __forceinline__ MxTile mx_tile_at(uint32_t workgroup, uint32_t rows, uint32_t columns) {
+    const uint32_t all = rows * columns, per = (all + kXcds - 1u) / kXcds;
+    const uint32_t j = workgroup / kXcds, at = workgroup % kXcds * per + j;
+    if (j >= per || at >= all) return MxTile{0u, 0u, false};
+    const uint32_t group = at / (kGroup * columns), in = at % (kGroup * columns);
+    const uint32_t height = min(kGroup, rows - group * kGroup);
+    return MxTile{group * kGroup + in % height, in / height, true};
+}
+
+template <typename S, bool kSwiglu, uint32_t kPer>
+__global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
+    constexpr uint32_t kMF = S::kMF, kTM = S::kTM, kTN = S::kTN, kBM = S::kBM, kBN = S::kBN;
+    using Acc = std::conditional_t<kMF == 32u, v16f, v4f>;
+    constexpr uint32_t kAcc = kMF == 32u ? 16u : 4u;
+    __shared__ v4i ring[S::kStages * S::kSlot];
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t n_out = kSwiglu ? p.n / 2u : p.n;
+    constexpr uint32_t kColumns = kSwiglu ? kBN / 2u : kBN;
+    const uint32_t columns = (n_out + kColumns - 1u) / kColumns;
+
+    MxTask task;
+    uint32_t n0;
+    if constexpr (kPer != 0u) {
+        const TileList<kBM, kPer> list(p.offsets, p.experts, p.routes);
+        const MxTile tile = mx_tile_at(blockIdx.x, list.total, columns);
+        if (!tile.some) return;
+        task = list.find(tile.row);
+        n0 = tile.column * kColumns;
+    } else {
+        const MxTile tile = mx_tile_at(blockIdx.x, (p.routes + kBM - 1u) / kBM, columns);
+        if (!tile.some) return;
+        task = MxTask{0u, tile.row * kBM, min(p.routes - tile.row * kBM, kBM)};
+        n0 = tile.column * kColumns;
+    }
+
+    // ---- the rows that this lane loads a piece of ----
+    const uint32_t row_bytes = p.k128 * 64u, scale_bytes = p.k128 * 4u;
+    const auto a_row = [&](uint32_t j) {
+        uint32_t source = task.first + min(j, task.count - 1u);
+        if (kPer != 0u && p.packed) source = p.packed[source] / p.top_k;
+        return static_cast<uint64_t>(min(source, p.a_rows - 1u));
+    };
+    const auto b_row = [&](uint32_t j) {
+        uint32_t column = n0 + j, row = 0;
+        if constexpr (kSwiglu) {  // a wave's tiles: half of them gate, half up
+            const uint32_t t = j / kMF % kTN;
+            column = n0 + j / (kTN * kMF) * (kTN / 2u * kMF) + t % (kTN / 2u) * kMF + j % kMF;
+            if (t >= kTN / 2u) row = n_out;
+        }
+        return static_cast<uint64_t>(task.expert) * p.n + row + min(column, n_out - 1u);
+    };
+    const uint8_t* src[S::kMine];
+#pragma unroll
+    for (uint32_t t = 0; t < S::kMine; ++t) {
+        const uint32_t i = wave + t * S::kWaves;
+        if (i < S::kData) {
+            const uint32_t r = 8u * i + (lane >> 3), piece = (lane & 7u) ^ (r >> 1 & 7u);
+            src[t] = (r < kBM ? p.a_codes + a_row(r) * row_bytes
+                              : p.b_codes + b_row(r - kBM) * row_bytes) + 16u * piece;
+        } else {
+            const uint32_t r = min(32u * (i - S::kData) + (lane >> 1), S::kRows - 1u);
+            src[t] = (r < kBM ? p.a_scales + a_row(r) * scale_bytes
+                              : p.b_scales + b_row(r - kBM) * scale_bytes) + 4u * (lane & 1u);
+        }
+    }
+    const uint32_t stages = (p.k128 + 1u) / 2u;
+    const bool odd = (p.k128 & 1u) != 0u;  // the last stage is 128 values
+    const uint32_t ring_at = static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) v4i*)ring));
+    const auto issue = [&](uint32_t stage) {
+        const uint32_t slot = ring_at + stage % S::kStages * (S::kSlot * 16u);
+        const bool half = odd && stage + 1u == stages;  // pieces past the row's end: any of the row's
+#pragma unroll
+        for (uint32_t t = 0; t < S::kMine; ++t) {
+            const uint32_t i = wave + t * S::kWaves;
+            if (i >= S::kLoads) break;
+            if (i < S::kData) {
+                const uint32_t piece = (lane & 7u) ^ (4u * i + (lane >> 4) & 7u);
+                mx_load16(src[t] + stage * 128ull - (half && piece >= 4u ? 64u : 0u),
+                          __builtin_amdgcn_readfirstlane(slot + i * 1024u));
+            } else {
+                mx_load4(src[t] + stage * 8ull - (half && (lane & 1u) ? 4u : 0u),
+                         __builtin_amdgcn_readfirstlane(slot + S::kRows * 128u + (i - S::kData) * 256u));
+            }
+        }
+    };
+
+    // ---- products ----
+    const uint32_t wm = wave / S::kWN, wn = wave % S::kWN;
+    const uint32_t n = lane % kMF, q = lane / kMF;
+    Acc acc[kTN][kTM];
+#pragma unroll
+    for (uint32_t j = 0; j < kTN; ++j)
+#pragma unroll
+        for (uint32_t i = 0; i < kTM; ++i) acc[j][i] = Acc{};
+    const uint32_t a_at = (wm * kTM * kMF + n) * 8u, b_at = (kBM + wn * kTN * kMF + n) * 8u;
+    const uint32_t swizzle = n >> 1 & 7u;
+
+    constexpr uint32_t kAhead = S::kStages - 1u;
+    const bool more = wave < S::kLoads % S::kWaves || S::kLoads % S::kWaves == 0u;  // kMine loads, not one less
+    for (uint32_t s = 0; s < kAhead && s < stages; ++s) issue(s);
+    // waits for stage s, starts the one that takes the place of the stage before
+    const auto advance = [&](uint32_t s) {
+        if (S::kStages > 2u && s + kAhead <= stages) {
+            if (more) mx_barrier<S::kMine * (kAhead - 1u)>();
+            else mx_barrier<(S::kMine - 1u) * (kAhead - 1u)>();
+        } else {
+            mx_barrier<0>();
+        }
+        if (s + kAhead < stages) issue(s + kAhead);
+    };
+    const auto multiply = [&](uint32_t s, auto steps) {
+        const v4i* slot = ring + s % S::kStages * S::kSlot;
+        const uint2* scales = reinterpret_cast<const uint2*>(slot + S::kRows * 8u);
+        uint32_t sa[kTM][2], sb[kTN][2];
+#pragma unroll
+        for (uint32_t i = 0; i < kTM; ++i) {
+            const uint2 w = scales[a_at / 8u + i * kMF];
+            sa[i][0] = w.x >> 8u * q;
+            sa[i][1] = w.y >> 8u * q;
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < kTN; ++j) {
+            const uint2 w = scales[b_at / 8u + j * kMF];
+            sb[j][0] = w.x >> 8u * q;
+            sb[j][1] = w.y >> 8u * q;
+        }
+        const auto step = [&](auto at) {
+            constexpr uint32_t kC = decltype(at)::value;
+            constexpr uint32_t kWord = 2u * kC / S::kSteps;  // of the row's two scale words
+            constexpr int kByte = kMF == 32u ? 2 * (kC & 1u) : 0;
+            const uint32_t piece = (64u / kMF * kC + q) ^ swizzle;
+            v4i av[kTM], bv[kTN];
+#pragma unroll
+            for (uint32_t i = 0; i < kTM; ++i) av[i] = slot[a_at + i * kMF * 8u + piece];
+#pragma unroll
+            for (uint32_t j = 0; j < kTN; ++j) bv[j] = slot[b_at + j * kMF * 8u + piece];
+#pragma unroll
+            for (uint32_t j = 0; j < kTN; ++j)
+#pragma unroll
+                for (uint32_t i = 0; i < kTM; ++i)
+                    acc[j][i] = mfma_mx<kByte>(bv[j], sb[j][kWord], av[i], sa[i][kWord], acc[j][i]);
+        };
+        step(std::integral_constant<uint32_t, 0>{});
+        if constexpr (decltype(steps)::value > 1u) step(std::integral_constant<uint32_t, 1>{});
+        if constexpr (decltype(steps)::value > 2u) {
+            step(std::integral_constant<uint32_t, 2>{});
+            step(std::integral_constant<uint32_t, 3>{});
+        }
+    };
+    const uint32_t full = p.k128 / 2u;
+    for (uint32_t s = 0; s < full; ++s) {
+        advance(s);
+        multiply(s, std::integral_constant<uint32_t, S::kSteps>{});
+    }
+    if (odd) {
+        advance(full);
+        multiply(full, std::integral_constant<uint32_t, S::kSteps / 2u>{});
+    }
+    __syncthreads();
+
+    // ---- C: a wave's rows, kMF at a time, through LDS of its own, so that 16-byte
+    // stores of consecutive lanes are consecutive in a row ----
+    constexpr uint32_t kOut = kSwiglu ? kTN / 2u : kTN;          // tiles across
+    constexpr uint32_t kPitch = (kOut * kMF * 4u + 16u) / 16u;   // 16-byte words a row, of fp32
+    static_assert(S::kWaves * kMF * kPitch <= S::kStages * S::kSlot, "the ring holds the strips");
+    v4i* strip = ring + wave * kMF * kPitch;
+    const uint32_t size = p.c_f32 ? 4u : 2u;
+    uint8_t* c = p.c_f32 ? reinterpret_cast<uint8_t*>(p.c_f32) : reinterpret_cast<uint8_t*>(p.c_bf16);
+    const bool whole = reinterpret_cast<uintptr_t>(c) % 16u == 0u && p.c_stride * size % 16u == 0u;
+    const uint32_t first_column = n0 + wn * kOut * kMF;
+#pragma unroll
+    for (uint32_t i = 0; i < kTM; ++i) {
+        const uint32_t m0 = (wm * kTM + i) * kMF;
+        if (m0 >= task.count) break;
+        bool real = true;
+        if (kPer != 0u && p.packed)
+            real = p.packed[task.first + min(m0 + n, task.count - 1u)] / p.top_k < p.a_rows;
+#pragma unroll
+        for (uint32_t j = 0; j < kOut; ++j)
+#pragma unroll
+            for (uint32_t g = 0; g < kAcc / 4u; ++g) {
+                float v[4];
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) {
+                    v[e] = acc[j][i][4u * g + e];
+                    if constexpr (kSwiglu) v[e] = swiglu(v[e], acc[j + kOut][i][4u * g + e]);
+                    if (!real) v[e] = 0.0f;
+                }
+                const uint32_t column = j * kMF + 64u / kMF * 4u * g + 4u * q;  // four consecutive
+                if (p.c_f32) {
+                    reinterpret_cast<float4*>(strip)[n * kPitch + column / 4u] =
+                        make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+                    uint2 d;
+                    d.x = f32_to_bf16(v[0]) | f32_to_bf16(v[1]) << 16;
+                    d.y = f32_to_bf16(v[2]) | f32_to_bf16(v[3]) << 16;
+                    reinterpret_cast<uint2*>(strip)[n * kPitch * 2u + column / 4u] = d;
+                }
+            }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const uint32_t pieces = kOut * kMF * size / 16u, each = 16u / size;
+        for (uint32_t at = lane; at < kMF * pieces; at += 64u) {
+            const uint32_t r = at / pieces, piece = at % pieces, column = first_column + piece * each;
+            if (m0 + r >= task.count || column >= n_out) continue;
+            const v4i w = strip[r * kPitch + piece];
+            uint8_t* to = c + ((static_cast<uint64_t>(task.first) + m0 + r) * p.c_stride + column) * size;
+            if (whole && column + each <= n_out) {
+                *reinterpret_cast<v4i*>(to) = w;
+            } else if (p.c_f32) {
+                for (uint32_t e = 0; e < 4u && column + e < n_out; ++e)
+                    reinterpret_cast<int*>(to)[e] = w[e];
+            } else {
+                for (uint32_t e = 0; e < 8u && column + e < n_out; ++e)
+                    reinterpret_cast<uint16_t*>(to)[e] =
+                        static_cast<uint16_t>(static_cast<uint32_t>(w[e / 2u]) >> (e % 2u * 16u));
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
     }
 }
+
+using MxLarge = MxShape<32, 2, 2, 4, 4, 2>;   // 256 x 256
+using MxMiddle = MxShape<32, 2, 2, 2, 2, 2>;  // 128 x 128
+using MxSmall = MxShape<16, 2, 2, 2, 2, 3>;   // 64 x 64
+using MxFew = MxShape<16, 1, 4, 1, 2, 4>;     // 16 x 128
 
 }  // namespace
 
@@ -311,25 +559,63 @@ hipError_t launch_mx_quantize(const void* x, uint32_t dtype, uint64_t stride, ui
 }
 
 namespace {
-dim3 product_grid(const MxProduct& p, bool swiglu) {
-    const uint32_t n_out = swiglu ? p.n / 2u : p.n;
-    const uint32_t tasks = p.offsets ? mx_max_tasks(p.routes, p.experts, 16u)
-                                     : (p.routes + 15u) / 16u;
-    return dim3((n_out + 15u) / 16u, tasks);
+
+// workgroups: a bound where the experts' rows are known to the device alone
+template <typename S>
+uint64_t mx_grid(const MxProduct& p, bool swiglu) {
+    const uint64_t across = swiglu ? S::kBN / 2u : S::kBN, n_out = swiglu ? p.n / 2u : p.n;
+    const uint64_t rows = p.offsets ? mx_max_tasks(p.routes, p.experts, S::kBM)
+                                    : (static_cast<uint64_t>(p.routes) + S::kBM - 1u) / S::kBM;
+    const uint64_t all = rows * ((n_out + across - 1u) / across);
+    return (all + kXcds - 1u) / kXcds * kXcds;
 }
+
+template <typename S, bool kSwiglu>
+hipError_t launch_tiles(const MxProduct& p, hipStream_t stream) {
+    const uint32_t grid = static_cast<uint32_t>(mx_grid<S>(p, kSwiglu));
+    if (!p.offsets) {
+        if constexpr (!kSwiglu) mx_tile_kernel<S, false, 0><<<grid, 64u * S::kWaves, 0, stream>>>(p);
+    } else if (p.experts <= 512u) {
+        mx_tile_kernel<S, kSwiglu, 8><<<grid, 64u * S::kWaves, 0, stream>>>(p);
+    } else {
+        mx_tile_kernel<S, kSwiglu, 16><<<grid, 64u * S::kWaves, 0, stream>>>(p);
+    }
+    return hipGetLastError();
+}
+
+// the tile of a product: rows of an expert on average (of C without experts)
+enum class MxTiles { kLarge, kMiddle, kSmall, kFew };
+MxTiles choose_tiles(const MxProduct& p, bool swiglu) {
+    const uint32_t rows = p.offsets ? p.routes / (p.routes < p.experts ? p.routes : p.experts) : p.routes;
+    if (rows <= 16u) return MxTiles::kFew;
+    if (mx_grid<MxLarge>(p, swiglu) >= 256u && rows >= 512u && !p.offsets) return MxTiles::kLarge;
+    if (mx_grid<MxMiddle>(p, swiglu) >= 256u && rows >= 96u) return MxTiles::kMiddle;
+    return MxTiles::kSmall;
+}
+
+template <typename F>
+auto with_tiles(MxTiles tiles, F f) {
+    switch (tiles) {
+        case MxTiles::kLarge: return f(MxLarge{});
+        case MxTiles::kMiddle: return f(MxMiddle{});
+        case MxTiles::kSmall: return f(MxSmall{});
+        default: return f(MxFew{});
+    }
+}
+
 }  // namespace
 
 bool mx_product_fits(const MxProduct& p, bool swiglu) {
-    if (p.n > (1u << 28) || p.routes > (1u << 28)) return false;
-    const dim3 grid = product_grid(p, swiglu);
-    return grid.x < (1u << 25) && grid.y < (1u << 16);
+    // a grid of 256-thread workgroups holds less than 2^32 threads
+    return with_tiles(choose_tiles(p, swiglu),
+                      [&](auto s) { return mx_grid<decltype(s)>(p, swiglu) < (1ull << 24); });
 }
 
 hipError_t launch_mx_product(const MxProduct& p, bool swiglu, hipStream_t stream) {
-    const dim3 grid = product_grid(p, swiglu);
-    if (swiglu) mx_product_kernel<true><<<grid, 64, 0, stream>>>(p);
-    else mx_product_kernel<false><<<grid, 64, 0, stream>>>(p);
-    return hipGetLastError();
+    return with_tiles(choose_tiles(p, swiglu), [&](auto s) {
+        using S = decltype(s);
+        return swiglu ? launch_tiles<S, true>(p, stream) : launch_tiles<S, false>(p, stream);
+    });
 }
 
 }  // namespace q38m
