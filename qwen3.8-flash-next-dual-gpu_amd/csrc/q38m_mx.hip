@@ -270,8 +270,12 @@ struct MxShape {
     static constexpr uint32_t kBM = kWM * kTM * kMF, kBN = kWN * kTN * kMF, kRows = kBM + kBN;
     static constexpr uint32_t kData = kRows / 8u;                 // load instructions of 1 KB
     static constexpr uint32_t kScale = (kRows + 31u) / 32u;       // of 256 bytes
-    static constexpr uint32_t kLoads = kData + kScale;
-    static constexpr uint32_t kMine = (kLoads + kWaves - 1u) / kWaves;  // a wave's, at most
+    // dealt to the waves: what is left over of the first to the first waves, of the
+    // second to the last, so that a wave has at most one more than another
+    static constexpr uint32_t kDataEach = kData / kWaves, kDataRest = kData % kWaves;
+    static constexpr uint32_t kScaleEach = kScale / kWaves, kScaleRest = kScale % kWaves;
+    static constexpr uint32_t kEach = kDataEach + kScaleEach;
+    static_assert(kDataRest + kScaleRest <= kWaves, "one more at most");
     static constexpr uint32_t kSlot = kRows * 8u + kScale * 16u;  // 16-byte words
     static constexpr uint32_t kSteps = 256u * kMF / 2048u;        // matrix instructions deep: 2 or 4
 };
@@ -355,40 +359,50 @@ __global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
         }
         return static_cast<uint64_t>(task.expert) * p.n + row + min(column, n_out - 1u);
     };
-    const uint8_t* src[S::kMine];
+    const auto data_source = [&](uint32_t i) {
+        const uint32_t r = 8u * i + (lane >> 3), piece = (lane & 7u) ^ (r >> 1 & 7u);
+        return (r < kBM ? p.a_codes + a_row(r) * row_bytes
+                        : p.b_codes + b_row(r - kBM) * row_bytes) + 16u * piece;
+    };
+    const auto scale_source = [&](uint32_t i) {
+        const uint32_t r = min(32u * i + (lane >> 1), S::kRows - 1u);
+        return (r < kBM ? p.a_scales + a_row(r) * scale_bytes
+                        : p.b_scales + b_row(r - kBM) * scale_bytes) + 4u * (lane & 1u);
+    };
+    const bool data_rest = S::kDataRest != 0u && wave < S::kDataRest;
+    const bool scale_rest = S::kScaleRest != 0u && wave >= S::kWaves - S::kScaleRest;
+    const uint8_t *data[S::kDataEach], *scale[S::kScaleEach], *last_data = nullptr, *last_scale = nullptr;
 #pragma unroll
-    for (uint32_t t = 0; t < S::kMine; ++t) {
-        const uint32_t i = wave + t * S::kWaves;
-        if (i < S::kData) {
-            const uint32_t r = 8u * i + (lane >> 3), piece = (lane & 7u) ^ (r >> 1 & 7u);
-            src[t] = (r < kBM ? p.a_codes + a_row(r) * row_bytes
-                              : p.b_codes + b_row(r - kBM) * row_bytes) + 16u * piece;
-        } else {
-            const uint32_t r = min(32u * (i - S::kData) + (lane >> 1), S::kRows - 1u);
-            src[t] = (r < kBM ? p.a_scales + a_row(r) * scale_bytes
-                              : p.b_scales + b_row(r - kBM) * scale_bytes) + 4u * (lane & 1u);
-        }
-    }
+    for (uint32_t t = 0; t < S::kDataEach; ++t) data[t] = data_source(wave + t * S::kWaves);
+#pragma unroll
+    for (uint32_t t = 0; t < S::kScaleEach; ++t) scale[t] = scale_source(wave + t * S::kWaves);
+    constexpr uint32_t kLastData = S::kDataEach * S::kWaves, kLastScale = S::kScale - S::kWaves;
+    if (data_rest) last_data = data_source(kLastData + wave);
+    if (scale_rest) last_scale = scale_source(kLastScale + wave);
+
     const uint32_t stages = (p.k128 + 1u) / 2u;
     const bool odd = (p.k128 & 1u) != 0u;  // the last stage is 128 values
     const uint32_t ring_at = static_cast<uint32_t>(
         reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) v4i*)ring));
     const auto issue = [&](uint32_t stage) {
         const uint32_t slot = ring_at + stage % S::kStages * (S::kSlot * 16u);
-        const bool half = odd && stage + 1u == stages;  // pieces past the row's end: any of the row's
+        const uint32_t scales = slot + S::kRows * 128u;
+        const bool half = odd && stage + 1u == stages;  // pieces past the row's end: others of the row
+        const auto load_data = [&](const uint8_t* from, uint32_t i) {
+            const uint32_t piece = (lane & 7u) ^ ((4u * i + (lane >> 4)) & 7u);
+            mx_load16(from + stage * 128ull - (half && piece >= 4u ? 64u : 0u),
+                      __builtin_amdgcn_readfirstlane(slot + i * 1024u));
+        };
+        const auto load_scale = [&](const uint8_t* from, uint32_t i) {
+            mx_load4(from + stage * 8ull - (half && (lane & 1u) ? 4u : 0u),
+                     __builtin_amdgcn_readfirstlane(scales + i * 256u));
+        };
 #pragma unroll
-        for (uint32_t t = 0; t < S::kMine; ++t) {
-            const uint32_t i = wave + t * S::kWaves;
-            if (i >= S::kLoads) break;
-            if (i < S::kData) {
-                const uint32_t piece = (lane & 7u) ^ (4u * i + (lane >> 4) & 7u);
-                mx_load16(src[t] + stage * 128ull - (half && piece >= 4u ? 64u : 0u),
-                          __builtin_amdgcn_readfirstlane(slot + i * 1024u));
-            } else {
-                mx_load4(src[t] + stage * 8ull - (half && (lane & 1u) ? 4u : 0u),
-                         __builtin_amdgcn_readfirstlane(slot + S::kRows * 128u + (i - S::kData) * 256u));
-            }
-        }
+        for (uint32_t t = 0; t < S::kDataEach; ++t) load_data(data[t], wave + t * S::kWaves);
+#pragma unroll
+        for (uint32_t t = 0; t < S::kScaleEach; ++t) load_scale(scale[t], wave + t * S::kWaves);
+        if (data_rest) load_data(last_data, kLastData + wave);
+        if (scale_rest) load_scale(last_scale, kLastScale + wave);
     };
 
     // ---- products ----
@@ -403,13 +417,13 @@ __global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
     const uint32_t swizzle = n >> 1 & 7u;
 
     constexpr uint32_t kAhead = S::kStages - 1u;
-    const bool more = wave < S::kLoads % S::kWaves || S::kLoads % S::kWaves == 0u;  // kMine loads, not one less
+    const bool more = data_rest || scale_rest;  // one load more than kEach
     for (uint32_t s = 0; s < kAhead && s < stages; ++s) issue(s);
     // waits for stage s, starts the one that takes the place of the stage before
     const auto advance = [&](uint32_t s) {
         if (S::kStages > 2u && s + kAhead <= stages) {
-            if (more) mx_barrier<S::kMine * (kAhead - 1u)>();
-            else mx_barrier<(S::kMine - 1u) * (kAhead - 1u)>();
+            if (more) mx_barrier<(S::kEach + 1u) * (kAhead - 1u)>();
+            else mx_barrier<S::kEach * (kAhead - 1u)>();
         } else {
             mx_barrier<0>();
         }
