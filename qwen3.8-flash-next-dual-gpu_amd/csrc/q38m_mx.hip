@@ -202,8 +202,9 @@ struct MxTask {
 // the experts kPer l .. kPer l + kPer - 1, their first rows and row tiles, and the sum
 // of tiles up to and with them.  Offsets past `routes` count as routes, an end that is
 // not behind its begin as no rows.
-template <uint32_t kRows, uint32_t kPer>
+template <uint32_t kRows>
 struct TileList {
+    static constexpr uint32_t kPer = kMaxSortExperts / 64u;
     uint32_t begin[kPer], end[kPer], sum, total;
 
     __device__ TileList(const uint32_t* __restrict__ offsets, uint32_t experts, uint32_t routes) {
@@ -254,10 +255,12 @@ struct TileList {
 
 // A workgroup computes kBM rows of C by kBN rows of B (with the SwiGLU fold half of
 // them gate, half up rows).  kWM x kWN waves, each kTM x kTN matrix-instruction tiles
-// of kMF rows.  K goes through LDS 256 values (128 bytes a row) at a time in a ring of
-// kStages slots, loaded straight from memory (no registers between, so the ring's depth
-// costs none).  A slot holds kBM rows of A, kBN rows of B, 128 bytes each, then their
-// scales, 8 bytes each.
+// of kMF rows.  K goes through LDS in stages of 256 values, a 128-byte line a row, in a
+// ring of kStages slots, loaded straight from memory (no registers between, so the
+// ring's depth costs none).  (Stages of 64 bytes a row, twice as many slots: 8,192^3
+// 352 -> 376 us, the loads' line look-ups double.)  A slot holds kBM rows of A, then kBN
+// rows of B.  The scales of two stages, 16 bytes a row, come with the even one into a
+// ring of their own.
 //
 // The eight 16-byte pieces of row r lie at positions p ^ (r / 2 % 8): the lanes of a
 // read take one piece of 16 or 32 consecutive rows, which then spread over all 64
@@ -268,16 +271,11 @@ struct MxShape {
     static constexpr uint32_t kMF = kMF_, kWM = kWM_, kWN = kWN_, kTM = kTM_, kTN = kTN_;
     static constexpr uint32_t kStages = kStages_, kWaves = kWM * kWN;
     static constexpr uint32_t kBM = kWM * kTM * kMF, kBN = kWN * kTN * kMF, kRows = kBM + kBN;
-    static constexpr uint32_t kData = kRows / 8u;                 // load instructions of 1 KB
-    static constexpr uint32_t kScale = (kRows + 31u) / 32u;       // of 256 bytes
-    // dealt to the waves: what is left over of the first to the first waves, of the
-    // second to the last, so that a wave has at most one more than another
-    static constexpr uint32_t kDataEach = kData / kWaves, kDataRest = kData % kWaves;
-    static constexpr uint32_t kScaleEach = kScale / kWaves, kScaleRest = kScale % kWaves;
-    static constexpr uint32_t kEach = kDataEach + kScaleEach;
-    static_assert(kDataRest + kScaleRest <= kWaves, "one more at most");
-    static constexpr uint32_t kSlot = kRows * 8u + kScale * 16u;  // 16-byte words
-    static constexpr uint32_t kSteps = 256u * kMF / 2048u;        // matrix instructions deep: 2 or 4
+    static constexpr uint32_t kSteps = kMF / 8u;                  // matrix instructions deep: 2 or 4
+    static constexpr uint32_t kSlot = kRows * 8u;                 // 16-byte words
+    static constexpr uint32_t kScaleSlots = kStages / 2u + 1u;    // pairs of stages under way
+    static constexpr uint32_t kScaleSlot = kRows;
+    static constexpr uint32_t kLds = kStages * kSlot + kScaleSlots * kScaleSlot;
 };
 
 __device__ __forceinline__ void mx_load16(const uint8_t* src, uint32_t lds) {
@@ -316,12 +314,14 @@ __device__ __forceinline__ MxTile mx_tile_at(uint32_t workgroup, uint32_t rows, 
     return MxTile{group * kGroup + in % height, in / height, true};
 }
 
-template <typename S, bool kSwiglu, uint32_t kPer>
+// kExperts: rows of experts.  kWide: K is a multiple of 512 and the scales are 16-byte
+// aligned, so that a row's scales of two stages are one 16-byte piece.
+template <typename S, bool kExperts, bool kSwiglu, bool kWide>
 __global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
     constexpr uint32_t kMF = S::kMF, kTM = S::kTM, kTN = S::kTN, kBM = S::kBM, kBN = S::kBN;
     using Acc = std::conditional_t<kMF == 32u, v16f, v4f>;
     constexpr uint32_t kAcc = kMF == 32u ? 16u : 4u;
-    __shared__ v4i ring[S::kStages * S::kSlot];
+    __shared__ v4i ring[S::kLds];
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t n_out = kSwiglu ? p.n / 2u : p.n;
@@ -330,8 +330,8 @@ __global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
 
     MxTask task;
     uint32_t n0;
-    if constexpr (kPer != 0u) {
-        const TileList<kBM, kPer> list(p.offsets, p.experts, p.routes);
+    if constexpr (kExperts) {
+        const TileList<kBM> list(p.offsets, p.experts, p.routes);
         const MxTile tile = mx_tile_at(blockIdx.x, list.total, columns);
         if (!tile.some) return;
         task = list.find(tile.row);
@@ -347,7 +347,7 @@ __global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
     const uint32_t row_bytes = p.k128 * 64u, scale_bytes = p.k128 * 4u;
     const auto a_row = [&](uint32_t j) {
         uint32_t source = task.first + min(j, task.count - 1u);
-        if (kPer != 0u && p.packed) source = p.packed[source] / p.top_k;
+        if (kExperts && p.packed) source = p.packed[source] / p.top_k;
         return static_cast<uint64_t>(min(source, p.a_rows - 1u));
     };
     const auto b_row = [&](uint32_t j) {
@@ -359,50 +359,61 @@ __global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
         }
         return static_cast<uint64_t>(task.expert) * p.n + row + min(column, n_out - 1u);
     };
+    // load instructions, dealt to the waves, the left over ones to the first: 1 KB of
+    // data each; of scales 1 KB where rows of them are whole 16-byte pieces, else 256 bytes
+    constexpr uint32_t kData = S::kRows / 8u, kDataEach = kData / S::kWaves, kDataRest = kData % S::kWaves;
+    constexpr uint32_t kScaleRows = kWide ? 64u : 16u;
+    constexpr uint32_t kScale = (S::kRows + kScaleRows - 1u) / kScaleRows;
+    constexpr uint32_t kScaleEach = kScale / S::kWaves, kScaleRest = kScale % S::kWaves;
+    const bool data_rest = kDataRest != 0u && wave < kDataRest;
+    const bool scale_rest = kScaleRest != 0u && wave < kScaleRest;
     const auto data_source = [&](uint32_t i) {
         const uint32_t r = 8u * i + (lane >> 3), piece = (lane & 7u) ^ (r >> 1 & 7u);
         return (r < kBM ? p.a_codes + a_row(r) * row_bytes
                         : p.b_codes + b_row(r - kBM) * row_bytes) + 16u * piece;
     };
     const auto scale_source = [&](uint32_t i) {
-        const uint32_t r = min(32u * i + (lane >> 1), S::kRows - 1u);
-        return (r < kBM ? p.a_scales + a_row(r) * scale_bytes
-                        : p.b_scales + b_row(r - kBM) * scale_bytes) + 4u * (lane & 1u);
+        const uint32_t r = min(kScaleRows * i + (kWide ? lane : lane >> 2), S::kRows - 1u);
+        return r < kBM ? p.a_scales + a_row(r) * scale_bytes
+                       : p.b_scales + b_row(r - kBM) * scale_bytes;
     };
-    const bool data_rest = S::kDataRest != 0u && wave < S::kDataRest;
-    const bool scale_rest = S::kScaleRest != 0u && wave >= S::kWaves - S::kScaleRest;
-    const uint8_t *data[S::kDataEach], *scale[S::kScaleEach], *last_data = nullptr, *last_scale = nullptr;
+    const uint8_t *data[kDataEach + 1u], *scale[kScaleEach + 1u];
 #pragma unroll
-    for (uint32_t t = 0; t < S::kDataEach; ++t) data[t] = data_source(wave + t * S::kWaves);
+    for (uint32_t t = 0; t < kDataEach; ++t) data[t] = data_source(wave + t * S::kWaves);
 #pragma unroll
-    for (uint32_t t = 0; t < S::kScaleEach; ++t) scale[t] = scale_source(wave + t * S::kWaves);
-    constexpr uint32_t kLastData = S::kDataEach * S::kWaves, kLastScale = S::kScale - S::kWaves;
-    if (data_rest) last_data = data_source(kLastData + wave);
-    if (scale_rest) last_scale = scale_source(kLastScale + wave);
+    for (uint32_t t = 0; t < kScaleEach; ++t) scale[t] = scale_source(wave + t * S::kWaves);
+    if (data_rest) data[kDataEach] = data_source(wave + kDataEach * S::kWaves);
+    if (scale_rest) scale[kScaleEach] = scale_source(wave + kScaleEach * S::kWaves);
 
     const uint32_t stages = (p.k128 + 1u) / 2u;
     const bool odd = (p.k128 & 1u) != 0u;  // the last stage is 128 values
     const uint32_t ring_at = static_cast<uint32_t>(
         reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) v4i*)ring));
-    const auto issue = [&](uint32_t stage) {
-        const uint32_t slot = ring_at + stage % S::kStages * (S::kSlot * 16u);
-        const uint32_t scales = slot + S::kRows * 128u;
-        const bool half = odd && stage + 1u == stages;  // pieces past the row's end: others of the row
-        const auto load_data = [&](const uint8_t* from, uint32_t i) {
+    constexpr uint32_t kScaleLoads = kScaleEach + (kScaleRest != 0u ? 1u : 0u);
+    constexpr uint32_t kDataLoads = kDataEach + (kDataRest != 0u ? 1u : 0u);
+    // load t of a stage's scales or data; past the last stage the last one again, into a
+    // slot that nobody reads any more: the count of loads is the same everywhere
+    const auto load_scale = [&](uint32_t stage, uint32_t t) {
+        const uint32_t i = wave + t * S::kWaves, from = min(stage, (stages - 1u) & ~1u);
+        if (kScaleRest != 0u && t == kScaleEach && !scale_rest) return;
+        // some lane of a load is within the rows
+        if (S::kRows % kScaleRows != 0u && kScaleRows * i + (kWide ? lane : lane >> 2) >= S::kRows) return;
+        const uint32_t at = __builtin_amdgcn_readfirstlane(
+            ring_at + (S::kStages * S::kSlot + stage / 2u % S::kScaleSlots * S::kScaleSlot) * 16u +
+            i * (kScaleRows * 16u));
+        if constexpr (kWide) mx_load16(scale[t] + from * 8ull, at);
+        else mx_load4(scale[t] + 4ull * min(from * 2u + (lane & 3u), p.k128 - 1u), at);
+    };
+    const auto load_data = [&](uint32_t stage, uint32_t t) {
+        const uint32_t i = wave + t * S::kWaves, from = min(stage, stages - 1u);
+        if (kDataRest != 0u && t == kDataEach && !data_rest) return;
+        uint32_t back = 0;  // a piece past the end of its row: another of the row
+        if constexpr (!kWide) {
             const uint32_t piece = (lane & 7u) ^ ((4u * i + (lane >> 4)) & 7u);
-            mx_load16(from + stage * 128ull - (half && piece >= 4u ? 64u : 0u),
-                      __builtin_amdgcn_readfirstlane(slot + i * 1024u));
-        };
-        const auto load_scale = [&](const uint8_t* from, uint32_t i) {
-            mx_load4(from + stage * 8ull - (half && (lane & 1u) ? 4u : 0u),
-                     __builtin_amdgcn_readfirstlane(scales + i * 256u));
-        };
-#pragma unroll
-        for (uint32_t t = 0; t < S::kDataEach; ++t) load_data(data[t], wave + t * S::kWaves);
-#pragma unroll
-        for (uint32_t t = 0; t < S::kScaleEach; ++t) load_scale(scale[t], wave + t * S::kWaves);
-        if (data_rest) load_data(last_data, kLastData + wave);
-        if (scale_rest) load_scale(last_scale, kLastScale + wave);
+            back = odd && from + 1u == stages && piece >= 4u ? 64u : 0u;
+        }
+        mx_load16(data[t] + (from * 128ull - back),
+                  __builtin_amdgcn_readfirstlane(ring_at + stage % S::kStages * (S::kSlot * 16u) + i * 1024u));
     };
 
     // ---- products ----
@@ -413,77 +424,123 @@ __global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
     for (uint32_t j = 0; j < kTN; ++j)
 #pragma unroll
         for (uint32_t i = 0; i < kTM; ++i) acc[j][i] = Acc{};
-    const uint32_t a_at = (wm * kTM * kMF + n) * 8u, b_at = (kBM + wn * kTN * kMF + n) * 8u;
-    const uint32_t swizzle = n >> 1 & 7u;
+    const uint32_t a_at = wm * kTM * kMF + n, b_at = kBM + wn * kTN * kMF + n;  // rows of the slot
+    const uint32_t swizzle = n >> 1 & 7u;  // as of every kMF-th row after it
+    constexpr uint32_t kReads = kTM + kTN;
+    v4i part[2][kReads];       // a step's fragments of A, then of B, and the next step's
+    uint2 factor[2][kReads];   // a stage's scales, and the next stage's
+    const auto read = [&](uint32_t s, uint32_t c, uint32_t i) {
+        const uint32_t row = i < kTM ? a_at + i * kMF : b_at + (i - kTM) * kMF;
+        part[c % 2u][i] = ring[s % S::kStages * S::kSlot + row * 8u + ((64u / kMF * c + q) ^ swizzle)];
+    };
+    const auto read_factor = [&](uint32_t s, uint32_t parity, uint32_t i) {
+        const uint32_t row = i < kTM ? a_at + i * kMF : b_at + (i - kTM) * kMF;
+        factor[parity][i] = reinterpret_cast<const uint2*>(
+            ring + S::kStages * S::kSlot + s / 2u % S::kScaleSlots * S::kScaleSlot)[2u * row + parity];
+    };
+    const auto shift_factor = [&](uint32_t parity, uint32_t i) {  // this lane's bytes to where the instruction takes them
+        factor[parity][i] = make_uint2(factor[parity][i].x >> 8u * q, factor[parity][i].y >> 8u * q);
+    };
+    // The matrix instructions of step c, `ops` other operations among them from the first on
+    const auto multiply = [&](auto step, uint32_t parity, auto ops, auto op) {
+        constexpr uint32_t kC = decltype(step)::value, kOps = decltype(ops)::value, kAll = kTM * kTN;
+        constexpr uint32_t kPer = (kOps + kAll - 1u) / kAll;
+        constexpr int kByte = kMF == 32u ? 2 * (kC & 1u) : 0;
+#pragma unroll
+        for (uint32_t m = 0; m < kAll; ++m) {
+            const uint32_t j = m / kTM, i = m % kTM;
+            const uint2 fa = factor[parity][i], fb = factor[parity][kTM + j];
+            constexpr bool kSecond = 2u * kC >= S::kSteps;  // of the stage's two scale words
+            acc[j][i] = mfma_mx<kByte>(part[kC % 2u][kTM + j], kSecond ? fb.y : fb.x, part[kC % 2u][i],
+                                       kSecond ? fa.y : fa.x, acc[j][i]);
+#pragma unroll
+            for (uint32_t o = m * kPer; o < (m + 1u) * kPer && o < kOps; ++o) op(o);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    constexpr uint32_t kEarly = (kDataLoads + 1u) / 2u;  // data loads behind the barrier's step, the rest a step later
 
-    constexpr uint32_t kAhead = S::kStages - 1u;
-    const bool more = data_rest || scale_rest;  // one load more than kEach
-    for (uint32_t s = 0; s < kAhead && s < stages; ++s) issue(s);
-    // waits for stage s, starts the one that takes the place of the stage before
-    const auto advance = [&](uint32_t s) {
-        if (S::kStages > 2u && s + kAhead <= stages) {
-            if (more) mx_barrier<(S::kEach + 1u) * (kAhead - 1u)>();
-            else mx_barrier<S::kEach * (kAhead - 1u)>();
-        } else {
-            mx_barrier<0>();
-        }
-        if (s + kAhead < stages) issue(s + kAhead);
-    };
-    const auto multiply = [&](uint32_t s, auto steps) {
-        const v4i* slot = ring + s % S::kStages * S::kSlot;
-        const uint2* scales = reinterpret_cast<const uint2*>(slot + S::kRows * 8u);
-        uint32_t sa[kTM][2], sb[kTN][2];
-#pragma unroll
-        for (uint32_t i = 0; i < kTM; ++i) {
-            const uint2 w = scales[a_at / 8u + i * kMF];
-            sa[i][0] = w.x >> 8u * q;
-            sa[i][1] = w.y >> 8u * q;
-        }
-#pragma unroll
-        for (uint32_t j = 0; j < kTN; ++j) {
-            const uint2 w = scales[b_at / 8u + j * kMF];
-            sb[j][0] = w.x >> 8u * q;
-            sb[j][1] = w.y >> 8u * q;
-        }
-        const auto step = [&](auto at) {
-            constexpr uint32_t kC = decltype(at)::value;
-            constexpr uint32_t kWord = 2u * kC / S::kSteps;  // of the row's two scale words
-            constexpr int kByte = kMF == 32u ? 2 * (kC & 1u) : 0;
-            const uint32_t piece = (64u / kMF * kC + q) ^ swizzle;
-            v4i av[kTM], bv[kTN];
-#pragma unroll
-            for (uint32_t i = 0; i < kTM; ++i) av[i] = slot[a_at + i * kMF * 8u + piece];
-#pragma unroll
-            for (uint32_t j = 0; j < kTN; ++j) bv[j] = slot[b_at + j * kMF * 8u + piece];
-#pragma unroll
-            for (uint32_t j = 0; j < kTN; ++j)
-#pragma unroll
-                for (uint32_t i = 0; i < kTM; ++i)
-                    acc[j][i] = mfma_mx<kByte>(bv[j], sb[j][kWord], av[i], sa[i][kWord], acc[j][i]);
+    // Stage s in kSteps steps, software pipelined: a step's fragments are read while the
+    // step in front of it is multiplied.  In front of the last step the workgroup meets:
+    // stage s + 1 has come and stage s is read, so its slot takes stage s + kStages.
+    const auto stage = [&](uint32_t s, auto odd_stage) {
+        constexpr uint32_t kParity = decltype(odd_stage)::value;
+        // of the kStages - 2 stages after s + 1 at least half, rounded down, bring scales
+        constexpr uint32_t kLater = S::kStages - 2u, kBusy = kDataEach * kLater + kLater / 2u * kScaleEach;
+        constexpr uint32_t kNow = (kParity + S::kStages) % 2u == 0u ? kScaleLoads : 0u;
+        const auto next_step = [&](auto c) {
+            constexpr uint32_t kC = decltype(c)::value;
+            constexpr uint32_t kLoads = kC == 0u ? kDataLoads - kEarly : 0u;
+            multiply(c, kParity, std::integral_constant<uint32_t, kReads + kLoads>{}, [&](uint32_t o) {
+                if (o < kReads) read(s, kC + 1u, o);
+                else load_data(s + S::kStages - 1u, kEarly + o - kReads);
+            });
         };
-        step(std::integral_constant<uint32_t, 0>{});
-        if constexpr (decltype(steps)::value > 1u) step(std::integral_constant<uint32_t, 1>{});
-        if constexpr (decltype(steps)::value > 2u) {
-            step(std::integral_constant<uint32_t, 2>{});
-            step(std::integral_constant<uint32_t, 3>{});
+        next_step(std::integral_constant<uint32_t, 0>{});
+        if constexpr (S::kSteps > 2u) {
+            next_step(std::integral_constant<uint32_t, 1>{});
+            next_step(std::integral_constant<uint32_t, 2>{});
         }
+        if (data_rest) mx_barrier<kBusy + (kDataRest != 0u ? kLater : 0u)>();
+        else mx_barrier<kBusy>();
+        multiply(std::integral_constant<uint32_t, S::kSteps - 1u>{}, kParity,
+                 std::integral_constant<uint32_t, 3u * kReads + kNow + kEarly>{}, [&](uint32_t o) {
+                     constexpr uint32_t kLoads = kNow + kEarly;
+                     if (o < kReads) read_factor(s + 1u, 1u - kParity, o);
+                     else if (o < 2u * kReads) read(s + 1u, 0u, o - kReads);
+                     else if (o < 2u * kReads + kNow) load_scale(s + S::kStages, o - 2u * kReads);
+                     else if (o < 2u * kReads + kLoads) load_data(s + S::kStages, o - 2u * kReads - kNow);
+                     else shift_factor(1u - kParity, o - 2u * kReads - kLoads);
+                 });
     };
-    const uint32_t full = p.k128 / 2u;
-    for (uint32_t s = 0; s < full; ++s) {
-        advance(s);
-        multiply(s, std::integral_constant<uint32_t, S::kSteps>{});
+#pragma unroll
+    for (uint32_t s = 0; s < S::kStages; ++s) {
+        if (s % 2u == 0u)
+#pragma unroll
+            for (uint32_t t = 0; t < kScaleLoads; ++t) load_scale(s, t);
+#pragma unroll
+        for (uint32_t t = 0; t < (s + 1u < S::kStages ? kDataLoads : kEarly); ++t) load_data(s, t);
     }
-    if (odd) {
-        advance(full);
-        multiply(full, std::integral_constant<uint32_t, S::kSteps / 2u>{});
+    // stage 0 has come; of the later ones all data loads but the last's second part are under way
+    constexpr uint32_t kFirst = kDataEach * (S::kStages - 2u) + (S::kStages - 1u) / 2u * kScaleEach +
+                                (kEarly < kDataEach ? kEarly : kDataEach);
+    mx_barrier<kFirst>();
+#pragma unroll
+    for (uint32_t i = 0; i < kReads; ++i) {
+        read(0u, 0u, i);
+        read_factor(0u, 0u, i);
     }
-    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < kReads; ++i) shift_factor(0u, i);
+    uint32_t s = 0;
+    for (; s + 2u < stages; s += 2u) {
+        stage(s, std::integral_constant<uint32_t, 0>{});
+        stage(s + 1u, std::integral_constant<uint32_t, 1>{});
+    }
+    if (s + 1u < stages) {
+        stage(s, std::integral_constant<uint32_t, 0>{});
+        ++s;
+#pragma unroll
+        for (uint32_t i = 0; i < kReads; ++i) factor[0][i] = factor[1][i];
+    }
+    const auto last_step = [&](auto c) {
+        constexpr uint32_t kC = decltype(c)::value;
+        multiply(c, 0u, std::integral_constant<uint32_t, kC + 1u < S::kSteps ? kReads : 0u>{},
+                 [&](uint32_t o) { read(s, kC + 1u, o); });
+    };
+    last_step(std::integral_constant<uint32_t, 0>{});
+    if constexpr (S::kSteps > 2u) last_step(std::integral_constant<uint32_t, 1>{});
+    if (kWide || !odd) {
+        if constexpr (S::kSteps > 2u) last_step(std::integral_constant<uint32_t, 2>{});
+        last_step(std::integral_constant<uint32_t, S::kSteps - 1u>{});
+    }
+    mx_barrier<0>();  // no load is under way to what follows in the ring
 
     // ---- C: a wave's rows, kMF at a time, through LDS of its own, so that 16-byte
     // stores of consecutive lanes are consecutive in a row ----
     constexpr uint32_t kOut = kSwiglu ? kTN / 2u : kTN;          // tiles across
     constexpr uint32_t kPitch = (kOut * kMF * 4u + 16u) / 16u;   // 16-byte words a row, of fp32
-    static_assert(S::kWaves * kMF * kPitch <= S::kStages * S::kSlot, "the ring holds the strips");
+    static_assert(S::kWaves * kMF * kPitch <= S::kLds, "the ring holds the strips");
     v4i* strip = ring + wave * kMF * kPitch;
     const uint32_t size = p.c_f32 ? 4u : 2u;
     uint8_t* c = p.c_f32 ? reinterpret_cast<uint8_t*>(p.c_f32) : reinterpret_cast<uint8_t*>(p.c_bf16);
@@ -494,7 +551,7 @@ __global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
         const uint32_t m0 = (wm * kTM + i) * kMF;
         if (m0 >= task.count) break;
         bool real = true;
-        if (kPer != 0u && p.packed)
+        if (kExperts && p.packed)
             real = p.packed[task.first + min(m0 + n, task.count - 1u)] / p.top_k < p.a_rows;
 #pragma unroll
         for (uint32_t j = 0; j < kOut; ++j)
@@ -542,7 +599,7 @@ __global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
     }
 }
 
-using MxLarge = MxShape<32, 2, 2, 4, 4, 2>;   // 256 x 256
+using MxLarge = MxShape<32, 2, 4, 4, 2, 2>;   // 256 x 256
 using MxMiddle = MxShape<32, 2, 2, 2, 2, 2>;  // 128 x 128
 using MxSmall = MxShape<16, 2, 2, 2, 2, 3>;   // 64 x 64
 using MxFew = MxShape<16, 1, 4, 1, 2, 4>;     // 16 x 128
@@ -584,16 +641,13 @@ uint64_t mx_grid(const MxProduct& p, bool swiglu) {
     return (all + kXcds - 1u) / kXcds * kXcds;
 }
 
-template <typename S, bool kSwiglu>
+template <typename S, bool kExperts, bool kSwiglu>
 hipError_t launch_tiles(const MxProduct& p, hipStream_t stream) {
     const uint32_t grid = static_cast<uint32_t>(mx_grid<S>(p, kSwiglu));
-    if (!p.offsets) {
-        if constexpr (!kSwiglu) mx_tile_kernel<S, false, 0><<<grid, 64u * S::kWaves, 0, stream>>>(p);
-    } else if (p.experts <= 512u) {
-        mx_tile_kernel<S, kSwiglu, 8><<<grid, 64u * S::kWaves, 0, stream>>>(p);
-    } else {
-        mx_tile_kernel<S, kSwiglu, 16><<<grid, 64u * S::kWaves, 0, stream>>>(p);
-    }
+    const bool wide = p.k128 % 4u == 0u && reinterpret_cast<uintptr_t>(p.a_scales) % 16u == 0u &&
+                      reinterpret_cast<uintptr_t>(p.b_scales) % 16u == 0u;
+    if (wide) mx_tile_kernel<S, kExperts, kSwiglu, true><<<grid, 64u * S::kWaves, 0, stream>>>(p);
+    else mx_tile_kernel<S, kExperts, kSwiglu, false><<<grid, 64u * S::kWaves, 0, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -628,7 +682,8 @@ bool mx_product_fits(const MxProduct& p, bool swiglu) {
 hipError_t launch_mx_product(const MxProduct& p, bool swiglu, hipStream_t stream) {
     return with_tiles(choose_tiles(p, swiglu), [&](auto s) {
         using S = decltype(s);
-        return swiglu ? launch_tiles<S, true>(p, stream) : launch_tiles<S, false>(p, stream);
+        if (!p.offsets) return launch_tiles<S, false, false>(p, stream);
+        return swiglu ? launch_tiles<S, true, true>(p, stream) : launch_tiles<S, true, false>(p, stream);
     });
 }
 
