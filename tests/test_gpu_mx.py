@@ -255,7 +255,7 @@ def want_experts(w_values, rows, offsets, packed, top_k, experts, k, swiglu):
             g, u, bg, bu = y[:, :columns], y[:, columns:], b[:, :columns], b[:, columns:]
             y = mx.swiglu(g, u)
             b = 1.1 * bg * (np.abs(u) + bu) + np.abs(mx.swiglu(g, 1.0)) * bu + 8 * F32_HALF * np.abs(y)
-            b += 1e-35 * np.abs(u)  # exp beyond its range: silu(g) is 0, not g e^g
+            b += 2.0 ** -126 * np.abs(g * u)  # below g = -88 the exponential is held
         want[p], bound[p] = y, b
     return want, bound
 
@@ -281,6 +281,20 @@ def test_experts(q38m, swiglu, dtype, tokens, top_k, experts, n, k, kind):
         kept = int(offsets[-1])
         assert (words[kept:] == 0x4a4a).all(), "a dropped route's row was written"
         close(got[:kept], want[:kept], bound[:kept], dtype, (tokens, kind, gather))
+
+
+def test_swiglu_far_ends(q38m):
+    """Gates from -1500 to 1500: the exponential at and beyond the ends of its range."""
+    rng = np.random.default_rng(11)
+    experts, n, k, routes = 2, 64, 128, 40
+    offsets, packed = np.array([0, 17, 40], np.uint32), np.arange(40, dtype=np.uint32)
+    w = Encoded(q38m, *encoded(rng, experts * n, k, 126, 131), k, experts)
+    rows = Encoded(q38m, *encoded(rng, routes, k, 120, 128), k)
+    words, got = run_experts(q38m, w, rows, device(offsets), None, 1, routes, True, "f32")
+    want, bound = want_experts(w.values, rows.values, offsets, packed, 0, experts, k, True)
+    gate = np.concatenate([mx.product(rows.values[:17], w.values[:32])[0], mx.product(rows.values[17:], w.values[64:96])[0]])
+    assert gate.min() < -150 and gate.max() > 150 and (np.abs(gate) < 5).any()
+    close(got, want, bound, "f32", "far ends")
 
 
 def test_experts_bad_plan(q38m):
