@@ -649,7 +649,8 @@ int q38m_mx_gemm_v1(const q38m_mx_matrix_v1* a, const q38m_mx_matrix_v1* b,
  * epilogue SWIGLU: weights' first half of rows is gate, the second half up;
  * C has half as many columns, h = g / (1 + exp(-g)) * u in fp32, rounded
  * once.  C is contiguous.  Rows of C that no expert has (dropped routes) are
- * left as they were; a src(p) past A's rows reads as a row of zeros. */
+ * left as they were; a src(p) past A's rows reads A's last row.  One expert's
+ * codes, and those of gathered rows, are below 4 GB. */
 #define Q38M_MX_EPILOGUE_NONE 0u
 #define Q38M_MX_EPILOGUE_SWIGLU 1u
 int q38m_mx_grouped_gemm_v1(const q38m_mx_matrix_v1* weights,

@@ -207,14 +207,15 @@ __device__ __forceinline__ float swiglu(float g, float u) {
     return g * __builtin_amdgcn_rcpf(1.0f + exp) * u;
 }
 
-struct MxTask {
-    uint32_t expert, first, count;  // rows first .. first + count of the sorted order
+// A row tile of the experts' rows: `first` up to kRows rows on or to the expert's end.
+struct RowTile {
+    uint32_t expert, first, end;
 };
 
 // The row tiles of the experts' rows, kRows at a time, held by a wave: lane l holds
-// the experts kPer l .. kPer l + kPer - 1, their first rows and row tiles, and the sum
-// of tiles up to and with them.  Offsets past `routes` count as routes, an end that is
-// not behind its begin as no rows.
+// the experts kPer l .. kPer l + kPer - 1, their rows and the sum of row tiles up to
+// and with them.  Offsets past `routes` count as routes, an end that is not behind its
+// begin as no rows.
 template <uint32_t kRows>
 struct TileList {
     static constexpr uint32_t kPer = kMaxSortExperts / 64u;
@@ -225,14 +226,13 @@ struct TileList {
         uint32_t at[kPer + 1];
 #pragma unroll
         for (uint32_t i = 0; i <= kPer; ++i) at[i] = offsets[min(e0 + i, experts)];
-        uint32_t tiles = 0;
+        sum = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kPer; ++i) {
             begin[i] = min(at[i], routes);
             end[i] = max(min(at[i + 1u], routes), begin[i]);
-            tiles += (end[i] - begin[i] + kRows - 1u) / kRows;
+            sum += tiles(i);
         }
-        sum = tiles;
 #pragma unroll
         for (uint32_t d = 1; d < 64u; d <<= 1) {
             const uint32_t up = __shfl_up(sum, d);
@@ -241,39 +241,67 @@ struct TileList {
         total = __builtin_amdgcn_readlane(sum, 63);
     }
 
-    // task < total
-    __device__ MxTask find(uint32_t task) const {
-        const uint32_t owner = __builtin_ctzll(__ballot(sum > task));
-        uint32_t tiles = 0;
+    __device__ uint32_t tiles(uint32_t i) const { return (end[i] - begin[i] + kRows - 1u) / kRows; }
+
+    // tile < total
+    __device__ RowTile find(uint32_t tile) const {
+        const uint32_t owner = __builtin_ctzll(__ballot(sum > tile));
+        uint32_t before = sum;
 #pragma unroll
-        for (uint32_t i = 0; i < kPer; ++i) tiles += (end[i] - begin[i] + kRows - 1u) / kRows;
-        uint32_t left = task - (sum - tiles), expert = 0, first = 0, count = 0;
+        for (uint32_t i = 0; i < kPer; ++i) before -= tiles(i);
+        uint32_t left = tile - before, expert = 0, first = 0, last = 0;
         bool found = false;
 #pragma unroll
         for (uint32_t i = 0; i < kPer; ++i) {
-            const uint32_t n = (end[i] - begin[i] + kRows - 1u) / kRows;
-            if (!found && left < n) {
+            if (!found && left < tiles(i)) {
                 found = true;
                 expert = (threadIdx.x & 63u) * kPer + i;
                 first = begin[i] + left * kRows;
-                count = min(end[i] - first, kRows);
+                last = end[i];
             }
-            left -= n;
+            left -= tiles(i);
         }
-        return MxTask{static_cast<uint32_t>(__builtin_amdgcn_readlane(expert, owner)),
-                      static_cast<uint32_t>(__builtin_amdgcn_readlane(first, owner)),
-                      static_cast<uint32_t>(__builtin_amdgcn_readlane(count, owner))};
+        return RowTile{static_cast<uint32_t>(__builtin_amdgcn_readlane(expert, owner)),
+                       static_cast<uint32_t>(__builtin_amdgcn_readlane(first, owner)),
+                       static_cast<uint32_t>(__builtin_amdgcn_readlane(last, owner))};
     }
 };
 
-// A workgroup computes kBM rows of C by kBN rows of B (with the SwiGLU fold half of
-// them gate, half up rows).  kWM x kWN waves, each kTM x kTN matrix-instruction tiles
-// of kMF rows.  K goes through LDS in stages of 256 values, a 128-byte line a row, in a
-// ring of kStages slots, loaded straight from memory (no registers between, so the
-// ring's depth costs none).  (Stages of 64 bytes a row, twice as many slots: 8,192^3
-// 352 -> 376 us, the loads' line look-ups double.)  A slot holds kBM rows of A, then kBN
-// rows of B.  The scales of two stages, 16 bytes a row, come with the even one into a
-// ring of their own.
+// Where a workgroup is in its tiles: row tile by row tile, the column tiles of one
+// after the other, so that its rows of A stay the same for as long as can be.
+template <uint32_t kRows>
+struct MxWalk {
+    RowTile row;
+    uint32_t column, left;  // tiles from this one on
+
+    __device__ uint32_t count() const { return min(row.end - row.first, kRows); }
+    // to the next tile; whether it has other rows
+    __device__ bool next(const MxProduct& p, uint32_t columns) {
+        --left;
+        if (++column < columns) return false;
+        column = 0;
+        row.first += kRows;
+        if (row.first < row.end || !p.offsets) return true;
+        while (row.expert + 1u < p.experts) {
+            ++row.expert;
+            row.first = min(p.offsets[row.expert], p.routes);
+            row.end = min(p.offsets[row.expert + 1u], p.routes);
+            if (row.first < row.end) break;
+        }
+        return true;
+    }
+};
+
+// Workgroups stay and compute tile after tile of kBM rows of C by kBN rows of B (with
+// the SwiGLU fold half of them gate, half up rows), kWM x kWN waves, each kTM x kTN
+// matrix-instruction tiles of kMF rows.  K goes through LDS in stages of 256 values, a
+// 128-byte line a row, in a ring of kStages slots, loaded straight from memory (no
+// registers between, so the ring's depth costs none); the stages of a tile follow those
+// of the tile before without a gap.  (Stages of 64 bytes a row, twice as many slots:
+// 8,192^3 352 -> 376 us, the loads' line look-ups double.)  A slot holds kBM rows of A,
+// then kBN rows of B.  Scales have a ring of their own: kWide (K a multiple of 512 and
+// the scales 16-byte aligned) 16 bytes a row with every second stage, else 8 bytes a
+// row and stage.
 //
 // The eight 16-byte pieces of row r lie at positions p ^ (r / 2 % 8): the lanes of a
 // read take one piece of 16 or 32 consecutive rows, which then spread over all 64
@@ -284,21 +312,33 @@ struct MxShape {
     static constexpr uint32_t kMF = kMF_, kWM = kWM_, kWN = kWN_, kTM = kTM_, kTN = kTN_;
     static constexpr uint32_t kStages = kStages_, kWaves = kWM * kWN;
     static constexpr uint32_t kBM = kWM * kTM * kMF, kBN = kWN * kTN * kMF, kRows = kBM + kBN;
-    static constexpr uint32_t kSteps = kMF / 8u;                  // matrix instructions deep: 2 or 4
-    static constexpr uint32_t kSlot = kRows * 8u;                 // 16-byte words
-    static constexpr uint32_t kScaleSlots = kStages / 2u + 1u;    // pairs of stages under way
-    static constexpr uint32_t kScaleSlot = kRows;
-    static constexpr uint32_t kLds = kStages * kSlot + kScaleSlots * kScaleSlot;
+    static constexpr uint32_t kSteps = kMF / 8u;  // matrix instructions deep: 2 or 4
+    // 16-byte words of LDS: the ring, the scales' and a strip of C for each wave.  The
+    // scales of kStages stages may be under way: half as many pairs, begun and ended ones
+    static constexpr uint32_t kSlot = kRows * 8u, kScaleAt = kStages * kSlot;
+    static constexpr uint32_t kScaleWords = (kStages / 2u + 1u) * kRows;
+    static constexpr uint32_t kStrip = kMF * 4u, kStripAt = kScaleAt + kScaleWords;
+    static constexpr uint32_t kLds = kStripAt + kWaves * kStrip;
+    static constexpr uint32_t kResident = 160u * 64u / kLds;  // workgroups a CU
+    static_assert(kResident != 0u, "160 KB of LDS");
 };
 
-__device__ __forceinline__ void mx_load16(const uint8_t* src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src),
-                 "s"(lds)
+__device__ __forceinline__ const uint8_t* mx_uniform(const uint8_t* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+    const uint32_t high = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+    return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(high) << 32 | low);
+}
+
+// 16 bytes (4 bytes) a lane from base + offset to consecutive LDS from byte `lds` on
+__device__ __forceinline__ void mx_load16(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset),
+                 "s"(mx_uniform(base)), "s"(lds)
                  : "memory");
 }
-__device__ __forceinline__ void mx_load4(const uint8_t* src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src),
-                 "s"(lds)
+__device__ __forceinline__ void mx_load4(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset),
+                 "s"(mx_uniform(base)), "s"(lds)
                  : "memory");
 }
 
@@ -309,28 +349,12 @@ __device__ __forceinline__ void mx_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(kOutstanding) : "memory");
 }
 
-// Order of the tiles: groups of kGroup row tiles, in a group column by column, so that
-// tiles at work at the same time share rows of A and of B.  The dispatcher hands
-// workgroups to the eight XCDs in turn, each with an L2 of its own: XCD x takes one
-// contiguous eighth of the order.
-constexpr uint32_t kXcds = 8, kGroup = 4;
-struct MxTile {
-    uint32_t row, column;
-    bool some;
-};
-__device__ __forceinline__ MxTile mx_tile_at(uint32_t workgroup, uint32_t rows, uint32_t columns) {
-    const uint32_t all = rows * columns, per = (all + kXcds - 1u) / kXcds;
-    const uint32_t j = workgroup / kXcds, at = workgroup % kXcds * per + j;
-    if (j >= per || at >= all) return MxTile{0u, 0u, false};
-    const uint32_t group = at / (kGroup * columns), in = at % (kGroup * columns);
-    const uint32_t height = min(kGroup, rows - group * kGroup);
-    return MxTile{group * kGroup + in % height, in / height, true};
-}
+// The dispatcher hands workgroups to the eight XCDs in turn, each with an L2 of its
+// own: the workgroups of an XCD take neighbouring tiles, which share rows of A and of B.
+constexpr uint32_t kXcds = 8, kCus = 256;
 
-// kExperts: rows of experts.  kWide: K is a multiple of 512 and the scales are 16-byte
-// aligned, so that a row's scales of two stages are one 16-byte piece.
 template <typename S, bool kExperts, bool kSwiglu, bool kWide>
-__global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
+__global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 4u) void mx_tile_kernel(MxProduct p) {
     constexpr uint32_t kMF = S::kMF, kTM = S::kTM, kTN = S::kTN, kBM = S::kBM, kBN = S::kBN;
     using Acc = std::conditional_t<kMF == 32u, v16f, v4f>;
     constexpr uint32_t kAcc = kMF == 32u ? 16u : 4u;
@@ -341,92 +365,132 @@ __global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
     constexpr uint32_t kColumns = kSwiglu ? kBN / 2u : kBN;
     const uint32_t columns = (n_out + kColumns - 1u) / kColumns;
 
-    MxTask task;
-    uint32_t n0;
-    if constexpr (kExperts) {
-        const TileList<kBM> list(p.offsets, p.experts, p.routes);
-        const MxTile tile = mx_tile_at(blockIdx.x, list.total, columns);
-        if (!tile.some) return;
-        task = list.find(tile.row);
-        n0 = tile.column * kColumns;
-    } else {
-        const MxTile tile = mx_tile_at(blockIdx.x, (p.routes + kBM - 1u) / kBM, columns);
-        if (!tile.some) return;
-        task = MxTask{0u, tile.row * kBM, min(p.routes - tile.row * kBM, kBM)};
-        n0 = tile.column * kColumns;
-    }
-
-    // ---- the rows that this lane loads a piece of ----
-    const uint32_t row_bytes = p.k128 * 64u, scale_bytes = p.k128 * 4u;
-    const auto a_row = [&](uint32_t j) {
-        uint32_t source = task.first + min(j, task.count - 1u);
-        if (kExperts && p.packed) source = p.packed[source] / p.top_k;
-        return static_cast<uint64_t>(min(source, p.a_rows - 1u));
-    };
-    const auto b_row = [&](uint32_t j) {
-        uint32_t column = n0 + j, row = 0;
-        if constexpr (kSwiglu) {  // a wave's tiles: half of them gate, half up
-            const uint32_t t = j / kMF % kTN;
-            column = n0 + j / (kTN * kMF) * (kTN / 2u * kMF) + t % (kTN / 2u) * kMF + j % kMF;
-            if (t >= kTN / 2u) row = n_out;
+    // ---- this workgroup's tiles ----
+    MxWalk<kBM> ahead;  // the tile whose stages are being loaded
+    {
+        const uint32_t index = blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds;
+        const auto range = [&](uint64_t rows) {
+            const uint64_t all = rows * columns, at = index * all / gridDim.x;
+            ahead.left = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>((index + 1u) * all / gridDim.x - at));
+            ahead.column = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at % columns));
+            return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at / columns)));
+        };
+        if constexpr (kExperts) {
+            const TileList<kBM> list(p.offsets, p.experts, p.routes);
+            const uint32_t row = range(list.total);
+            if (ahead.left == 0u) return;
+            ahead.row = list.find(row);
+        } else {
+            const uint32_t row = range((p.routes + kBM - 1u) / kBM);
+            if (ahead.left == 0u) return;
+            ahead.row = RowTile{0u, row * kBM, p.routes};
         }
-        return static_cast<uint64_t>(task.expert) * p.n + row + min(column, n_out - 1u);
-    };
-    // load instructions, dealt to the waves, the left over ones to the first: 1 KB of
-    // data each; of scales 1 KB where rows of them are whole 16-byte pieces, else 256 bytes
-    constexpr uint32_t kData = S::kRows / 8u, kDataEach = kData / S::kWaves, kDataRest = kData % S::kWaves;
-    constexpr uint32_t kScaleRows = kWide ? 64u : 16u;
-    constexpr uint32_t kScale = (S::kRows + kScaleRows - 1u) / kScaleRows;
+    }
+    MxWalk<kBM> now = ahead;  // the tile being multiplied
+
+    // ---- loads: instructions dealt to the waves, the left over ones to the first: 1 KB
+    // of data each, eight rows; of scales 64 rows where they are 16-byte pieces, else 32.
+    // Rows of A first, then of B, each instruction of one of them: a base of its tile for
+    // all lanes and an offset below 4 GB for each ----
+    constexpr uint32_t kDataA = kBM / 8u, kData = S::kRows / 8u;
+    constexpr uint32_t kDataEach = kData / S::kWaves, kDataRest = kData % S::kWaves;
+    constexpr uint32_t kDataLoads = kDataEach + (kDataRest != 0u ? 1u : 0u);
+    constexpr uint32_t kScaleRows = kWide ? 64u : 32u;
+    constexpr uint32_t kScaleA = (kBM + kScaleRows - 1u) / kScaleRows, kScale = kScaleA + (kBN + kScaleRows - 1u) / kScaleRows;
     constexpr uint32_t kScaleEach = kScale / S::kWaves, kScaleRest = kScale % S::kWaves;
+    constexpr uint32_t kScaleLoads = kScaleEach + (kScaleRest != 0u ? 1u : 0u);
     const bool data_rest = kDataRest != 0u && wave < kDataRest;
     const bool scale_rest = kScaleRest != 0u && wave < kScaleRest;
-    const auto data_source = [&](uint32_t i) {
-        const uint32_t r = 8u * i + (lane >> 3), piece = (lane & 7u) ^ (r >> 1 & 7u);
-        return (r < kBM ? p.a_codes + a_row(r) * row_bytes
-                        : p.b_codes + b_row(r - kBM) * row_bytes) + 16u * piece;
-    };
-    const auto scale_source = [&](uint32_t i) {
-        const uint32_t r = min(kScaleRows * i + (kWide ? lane : lane >> 2), S::kRows - 1u);
-        return r < kBM ? p.a_scales + a_row(r) * scale_bytes
-                       : p.b_scales + b_row(r - kBM) * scale_bytes;
-    };
-    const uint8_t *data[kDataEach + 1u], *scale[kScaleEach + 1u];
-#pragma unroll
-    for (uint32_t t = 0; t < kDataEach; ++t) data[t] = data_source(wave + t * S::kWaves);
-#pragma unroll
-    for (uint32_t t = 0; t < kScaleEach; ++t) scale[t] = scale_source(wave + t * S::kWaves);
-    if (data_rest) data[kDataEach] = data_source(wave + kDataEach * S::kWaves);
-    if (scale_rest) scale[kScaleEach] = scale_source(wave + kScaleEach * S::kWaves);
-
+    const auto data_live = [&](uint32_t t) { return kDataRest == 0u || t < kDataEach || data_rest; };
+    const auto scale_live = [&](uint32_t t) { return kScaleRest == 0u || t < kScaleEach || scale_rest; };
+    const uint32_t row_bytes = p.k128 * 64u, scale_bytes = p.k128 * 4u;
     const uint32_t stages = (p.k128 + 1u) / 2u;
-    const bool odd = (p.k128 & 1u) != 0u;  // the last stage is 128 values
+    const bool odd = !kWide && (p.k128 & 1u) != 0u;  // a tile's last stage is 128 values
+    const uint8_t *a_base, *b_base, *a_scale_base, *b_scale_base;
+    uint32_t data[kDataLoads], scale[kScaleLoads];
+    // points the loads at the tile `ahead`; the rows of A stay where it has the same
+    const auto point = [&](bool other_rows) {
+        uint32_t own_lane = lane;  // the offsets are computed here, not kept from one tile to the next
+        asm volatile("" : "+v"(own_lane));
+        const uint64_t a_first = kExperts && p.packed ? 0u : ahead.row.first;
+        const uint64_t b_first = static_cast<uint64_t>(ahead.row.expert) * p.n + ahead.column * kColumns;
+        a_base = mx_uniform(p.a_codes + a_first * row_bytes);
+        a_scale_base = mx_uniform(p.a_scales + a_first * scale_bytes);
+        b_base = mx_uniform(p.b_codes + b_first * row_bytes);
+        b_scale_base = mx_uniform(p.b_scales + b_first * scale_bytes);
+        const auto a_row = [&](uint32_t j) -> uint32_t {
+            const uint32_t at = min(j, ahead.count() - 1u);
+            if (kExperts && p.packed) return min(p.packed[ahead.row.first + at] / p.top_k, p.a_rows - 1u);
+            return at;
+        };
+        const auto b_row = [&](uint32_t j) -> uint32_t {
+            uint32_t column = j, up = 0;
+            if constexpr (kSwiglu) {  // a wave's tiles: half of them gate, half up
+                const uint32_t t = j / kMF % kTN;
+                column = j / (kTN * kMF) * (kTN / 2u * kMF) + t % (kTN / 2u) * kMF + j % kMF;
+                up = t >= kTN / 2u ? n_out : 0u;
+            }
+            return min(column, n_out - 1u - ahead.column * kColumns) + up;
+        };
+#pragma unroll
+        for (uint32_t t = 0; t < kDataLoads; ++t) {
+            if (!data_live(t)) continue;
+            const uint32_t i = wave + t * S::kWaves;
+            const uint32_t r = 8u * i + (own_lane >> 3), piece = (own_lane & 7u) ^ (r >> 1 & 7u);
+            if (i >= kDataA) data[t] = b_row(r - kBM) * row_bytes + 16u * piece;
+            else if (other_rows) data[t] = a_row(r) * row_bytes + 16u * piece;
+        }
+#pragma unroll
+        for (uint32_t t = 0; t < kScaleLoads; ++t) {
+            if (!scale_live(t)) continue;
+            const uint32_t i = wave + t * S::kWaves, r = kWide ? own_lane : own_lane >> 1;
+            if (i >= kScaleA) scale[t] = b_row(min(r + kScaleRows * (i - kScaleA), kBN - 1u)) * scale_bytes;
+            else if (other_rows) scale[t] = a_row(r + kScaleRows * i) * scale_bytes;
+        }
+    };
+    point(true);
+    uint32_t from = 0, to = 0, scales_to = 0;  // the stage of `ahead` and the slots it is loaded to
     const uint32_t ring_at = static_cast<uint32_t>(
         reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) v4i*)ring));
-    constexpr uint32_t kScaleLoads = kScaleEach + (kScaleRest != 0u ? 1u : 0u);
-    constexpr uint32_t kDataLoads = kDataEach + (kDataRest != 0u ? 1u : 0u);
-    // load t of a stage's scales or data; past the last stage the last one again, into a
-    // slot that nobody reads any more: the count of loads is the same everywhere
-    const auto load_scale = [&](uint32_t stage, uint32_t t) {
-        const uint32_t i = wave + t * S::kWaves, from = min(stage, (stages - 1u) & ~1u);
-        if (kScaleRest != 0u && t == kScaleEach && !scale_rest) return;
-        // some lane of a load is within the rows
-        if (S::kRows % kScaleRows != 0u && kScaleRows * i + (kWide ? lane : lane >> 2) >= S::kRows) return;
+    constexpr uint32_t kScaleSlot = kWide ? S::kRows : S::kRows / 2u;  // words
+    constexpr uint32_t kScaleSlots = S::kScaleWords / kScaleSlot;
+    static_assert(kScaleSlots >= (kWide ? S::kStages / 2u + 1u : S::kStages), "scales under way");
+    const auto load_scale = [&](uint32_t t) {
+        if (!scale_live(t)) return;
+        const uint32_t i = wave + t * S::kWaves, r = kWide ? lane : lane >> 1;
+        const bool of_b = i >= kScaleA;
+        const uint32_t first = of_b ? kScaleRows * (i - kScaleA) : kScaleRows * i;
+        // some lane of a load is within the rows: its count is the same everywhere
+        if ((kBM % kScaleRows != 0u || kBN % kScaleRows != 0u) && first + r >= (of_b ? kBN : kBM)) return;
         const uint32_t at = __builtin_amdgcn_readfirstlane(
-            ring_at + (S::kStages * S::kSlot + stage / 2u % S::kScaleSlots * S::kScaleSlot) * 16u +
-            i * (kScaleRows * 16u));
-        if constexpr (kWide) mx_load16(scale[t] + from * 8ull, at);
-        else mx_load4(scale[t] + 4ull * min(from * 2u + (lane & 3u), p.k128 - 1u), at);
+            ring_at + (S::kScaleAt + scales_to * kScaleSlot) * 16u + (first + (of_b ? kBM : 0u)) * (kWide ? 16u : 8u));
+        const uint8_t* base = of_b ? b_scale_base : a_scale_base;
+        if constexpr (kWide) mx_load16(base + (from & ~1u) * 8ull, scale[t], at);
+        else mx_load4(base, scale[t] + 4u * min(from * 2u + (lane & 1u), p.k128 - 1u), at);
     };
-    const auto load_data = [&](uint32_t stage, uint32_t t) {
-        const uint32_t i = wave + t * S::kWaves, from = min(stage, stages - 1u);
-        if (kDataRest != 0u && t == kDataEach && !data_rest) return;
+    const auto load_data = [&](uint32_t t) {
+        if (!data_live(t)) return;
+        const uint32_t i = wave + t * S::kWaves;
         uint32_t back = 0;  // a piece past the end of its row: another of the row
         if constexpr (!kWide) {
             const uint32_t piece = (lane & 7u) ^ ((4u * i + (lane >> 4)) & 7u);
             back = odd && from + 1u == stages && piece >= 4u ? 64u : 0u;
         }
-        mx_load16(data[t] + (from * 128ull - back),
-                  __builtin_amdgcn_readfirstlane(ring_at + stage % S::kStages * (S::kSlot * 16u) + i * 1024u));
+        mx_load16((i >= kDataA ? b_base : a_base) + (from * 128ull), data[t] - back,
+                  __builtin_amdgcn_readfirstlane(ring_at + to * (S::kSlot * 16u) + i * 1024u));
+    };
+    // to the next stage to load; past the last tile the last stage again, into slots that
+    // nobody reads any more, so that the count of loads under way is always the same
+    const auto load_next = [&](bool scales_too) {
+        to = to + 1u == S::kStages ? 0u : to + 1u;
+        if (scales_too) scales_to = scales_to + 1u == kScaleSlots ? 0u : scales_to + 1u;
+        if (++from < stages) return;
+        if (ahead.left > 1u) {
+            from = 0;
+            point(ahead.next(p, columns));
+        } else {
+            --from;
+        }
     };
 
     // ---- products ----
@@ -440,30 +504,37 @@ __global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
     const uint32_t a_at = wm * kTM * kMF + n, b_at = kBM + wn * kTN * kMF + n;  // rows of the slot
     const uint32_t swizzle = n >> 1 & 7u;  // as of every kMF-th row after it
     constexpr uint32_t kReads = kTM + kTN;
-    v4i part[2][kReads];       // a step's fragments of A, then of B, and the next step's
-    uint2 factor[2][kReads];   // a stage's scales, and the next stage's
-    const auto read = [&](uint32_t s, uint32_t c, uint32_t i) {
+    v4i part[2][kReads];      // a step's fragments of A, then of B, and the next step's
+    uint2 factor[2][kReads];  // a stage's scales, and the next stage's
+    uint32_t slot = 0, scales = 0;  // of the stage whose fragments are read
+    const auto read = [&](uint32_t c, uint32_t i) {
         const uint32_t row = i < kTM ? a_at + i * kMF : b_at + (i - kTM) * kMF;
-        part[c % 2u][i] = ring[s % S::kStages * S::kSlot + row * 8u + ((64u / kMF * c + q) ^ swizzle)];
+        part[c % 2u][i] = ring[slot * S::kSlot + row * 8u + ((64u / kMF * c + q) ^ swizzle)];
     };
-    const auto read_factor = [&](uint32_t s, uint32_t parity, uint32_t i) {
+    const auto read_factor = [&](uint32_t parity, uint32_t buffer, uint32_t i) {
         const uint32_t row = i < kTM ? a_at + i * kMF : b_at + (i - kTM) * kMF;
-        factor[parity][i] = reinterpret_cast<const uint2*>(
-            ring + S::kStages * S::kSlot + s / 2u % S::kScaleSlots * S::kScaleSlot)[2u * row + parity];
+        const uint2* base = reinterpret_cast<const uint2*>(ring + S::kScaleAt + scales * kScaleSlot);
+        factor[buffer][i] = kWide ? base[2u * row + parity] : base[row];
     };
-    const auto shift_factor = [&](uint32_t parity, uint32_t i) {  // this lane's bytes to where the instruction takes them
-        factor[parity][i] = make_uint2(factor[parity][i].x >> 8u * q, factor[parity][i].y >> 8u * q);
+    const auto shift_factor = [&](uint32_t buffer, uint32_t i) {  // this lane's bytes to where the instruction takes them
+        factor[buffer][i] = make_uint2(factor[buffer][i].x >> 8u * q, factor[buffer][i].y >> 8u * q);
     };
-    // The matrix instructions of step c, `ops` other operations among them from the first on
-    const auto multiply = [&](auto step, uint32_t parity, auto ops, auto op) {
+    // The matrix instructions of step c (none where the stage ends in front of it), `ops`
+    // other operations among them from the first on
+    const auto multiply = [&](auto step, uint32_t buffer, bool live, auto ops, auto op) {
         constexpr uint32_t kC = decltype(step)::value, kOps = decltype(ops)::value, kAll = kTM * kTN;
         constexpr uint32_t kPer = (kOps + kAll - 1u) / kAll;
         constexpr int kByte = kMF == 32u ? 2 * (kC & 1u) : 0;
+        constexpr bool kSecond = 2u * kC >= S::kSteps;  // of the stage's two scale words
+        if (!live) {
+#pragma unroll
+            for (uint32_t o = 0; o < kOps; ++o) op(o);
+            return;
+        }
 #pragma unroll
         for (uint32_t m = 0; m < kAll; ++m) {
             const uint32_t j = m / kTM, i = m % kTM;
-            const uint2 fa = factor[parity][i], fb = factor[parity][kTM + j];
-            constexpr bool kSecond = 2u * kC >= S::kSteps;  // of the stage's two scale words
+            const uint2 fa = factor[buffer][i], fb = factor[buffer][kTM + j];
             acc[j][i] = mfma_mx<kByte>(part[kC % 2u][kTM + j], kSecond ? fb.y : fb.x, part[kC % 2u][i],
                                        kSecond ? fa.y : fa.x, acc[j][i]);
 #pragma unroll
@@ -471,151 +542,162 @@ __global__ __launch_bounds__(64u * S::kWaves) void mx_tile_kernel(MxProduct p) {
             __builtin_amdgcn_sched_barrier(0);
         }
     };
-    constexpr uint32_t kEarly = (kDataLoads + 1u) / 2u;  // data loads behind the barrier's step, the rest a step later
+    constexpr uint32_t kEarly = (kDataLoads + 1u) / 2u;  // data loads in the step behind the barrier, the rest a step later
 
-    // Stage s in kSteps steps, software pipelined: a step's fragments are read while the
+    // A stage in kSteps steps, software pipelined: a step's fragments are read while the
     // step in front of it is multiplied.  In front of the last step the workgroup meets:
-    // stage s + 1 has come and stage s is read, so its slot takes stage s + kStages.
-    const auto stage = [&](uint32_t s, auto odd_stage) {
-        constexpr uint32_t kParity = decltype(odd_stage)::value;
-        // of the kStages - 2 stages after s + 1 at least half, rounded down, bring scales
-        constexpr uint32_t kLater = S::kStages - 2u, kBusy = kDataEach * kLater + kLater / 2u * kScaleEach;
-        constexpr uint32_t kNow = (kParity + S::kStages) % 2u == 0u ? kScaleLoads : 0u;
-        const auto next_step = [&](auto c) {
+    // the next stage has come and this one is read, so its slot takes the kStages-th
+    // after it.  kWide: even and odd stages take turns, their scales in two buffers.
+    const auto stage = [&](auto odd_stage, bool half) {
+        constexpr uint32_t kParity = kWide ? decltype(odd_stage)::value : 0u;
+        constexpr bool kScalesNow = !kWide || (kParity + S::kStages) % 2u == 0u;
+        // loads of the kStages - 2 stages behind the next; kWide: at least half of them, rounded down, bring scales
+        constexpr uint32_t kLater = S::kStages - 2u;
+        constexpr uint32_t kBusy = kDataEach * kLater + (kWide ? kLater / 2u : kLater) * kScaleEach;
+        const auto step = [&](auto c) {
             constexpr uint32_t kC = decltype(c)::value;
             constexpr uint32_t kLoads = kC == 0u ? kDataLoads - kEarly : 0u;
-            multiply(c, kParity, std::integral_constant<uint32_t, kReads + kLoads>{}, [&](uint32_t o) {
-                if (o < kReads) read(s, kC + 1u, o);
-                else load_data(s + S::kStages - 1u, kEarly + o - kReads);
-            });
+            multiply(c, kParity, kWide || 2u * kC < S::kSteps || !half,
+                     std::integral_constant<uint32_t, kReads + kLoads>{}, [&](uint32_t o) {
+                         if (o < kReads) read(kC + 1u, o);
+                         else load_data(kEarly + o - kReads);
+                     });
+            if constexpr (kC == 0u) load_next(!kWide || (kParity + S::kStages) % 2u == 0u);
         };
-        next_step(std::integral_constant<uint32_t, 0>{});
+        step(std::integral_constant<uint32_t, 0>{});
         if constexpr (S::kSteps > 2u) {
-            next_step(std::integral_constant<uint32_t, 1>{});
-            next_step(std::integral_constant<uint32_t, 2>{});
+            step(std::integral_constant<uint32_t, 1>{});
+            step(std::integral_constant<uint32_t, 2>{});
         }
         if (data_rest) mx_barrier<kBusy + (kDataRest != 0u ? kLater : 0u)>();
         else mx_barrier<kBusy>();
-        multiply(std::integral_constant<uint32_t, S::kSteps - 1u>{}, kParity,
-                 std::integral_constant<uint32_t, 3u * kReads + kNow + kEarly>{}, [&](uint32_t o) {
-                     constexpr uint32_t kLoads = kNow + kEarly;
-                     if (o < kReads) read_factor(s + 1u, 1u - kParity, o);
-                     else if (o < 2u * kReads) read(s + 1u, 0u, o - kReads);
-                     else if (o < 2u * kReads + kNow) load_scale(s + S::kStages, o - 2u * kReads);
-                     else if (o < 2u * kReads + kLoads) load_data(s + S::kStages, o - 2u * kReads - kNow);
+        slot = slot + 1u == S::kStages ? 0u : slot + 1u;
+        if (!kWide || kParity == 1u) scales = scales + 1u == kScaleSlots ? 0u : scales + 1u;
+        constexpr uint32_t kScaleOps = kScalesNow ? kScaleLoads : 0u, kLoads = kScaleOps + kEarly;
+        multiply(std::integral_constant<uint32_t, S::kSteps - 1u>{}, kParity, kWide || !half,
+                 std::integral_constant<uint32_t, 3u * kReads + kLoads>{}, [&](uint32_t o) {
+                     if (o < kReads) read_factor(1u - kParity, 1u - kParity, o);
+                     else if (o < 2u * kReads) read(0u, o - kReads);
+                     else if (o < 2u * kReads + kScaleOps) load_scale(o - 2u * kReads);
+                     else if (o < 2u * kReads + kLoads) load_data(o - 2u * kReads - kScaleOps);
                      else shift_factor(1u - kParity, o - 2u * kReads - kLoads);
                  });
+        if constexpr (!kWide) {
+#pragma unroll
+            for (uint32_t i = 0; i < kReads; ++i) factor[0][i] = factor[1][i];
+        }
     };
+
+    // ---- C: 64 bytes of a wave's rows at a time through LDS of its own, so that the
+    // 16-byte stores of four consecutive lanes are consecutive in a row ----
+    const auto store = [&](auto* c) {
+        using T = std::remove_pointer_t<decltype(c)>;
+        constexpr uint32_t kSize = sizeof(T), kOut = kSwiglu ? kTN / 2u : kTN;  // tiles across
+        constexpr uint32_t kGap = 64u / kMF * 4u;                               // columns from group to group
+        constexpr uint32_t kPasses = (kOut * kMF * kSize + 63u) / 64u, kEach = 16u / kSize;
+        v4i* strip = ring + S::kStripAt + wave * S::kStrip;
+        const bool whole = reinterpret_cast<uintptr_t>(c) % 16u == 0u && p.c_stride * kSize % 16u == 0u;
+        const uint32_t count = now.count(), first_column = now.column * kColumns + wn * kOut * kMF;
+#pragma unroll
+        for (uint32_t i = 0; i < kTM; ++i) {
+            const uint32_t m0 = (wm * kTM + i) * kMF;
+            if (m0 >= count) break;
+#pragma unroll
+            for (uint32_t pass = 0; pass < kPasses; ++pass) {
+#pragma unroll
+                for (uint32_t j = 0; j < kOut; ++j)
+#pragma unroll
+                    for (uint32_t g = 0; g < kAcc / 4u; ++g) {
+                        if ((j * kMF + kGap * g) * kSize / 64u != pass) continue;
+                        float v[4];  // four consecutive columns
+#pragma unroll
+                        for (uint32_t e = 0; e < 4u; ++e) {
+                            v[e] = acc[j][i][4u * g + e];
+                            if constexpr (kSwiglu) v[e] = swiglu(v[e], acc[j + kOut][i][4u * g + e]);
+                        }
+                        const uint32_t byte = ((j * kMF + kGap * g) * kSize) % 64u + 4u * q * kSize;
+                        const uint32_t at = n * 4u + (byte / 16u ^ (n >> 2 & 3u));
+                        if constexpr (kSize == 4u) {
+                            reinterpret_cast<float4*>(strip)[at] = make_float4(v[0], v[1], v[2], v[3]);
+                        } else {
+                            uint2 d;
+                            d.x = f32_to_bf16(v[0]) | f32_to_bf16(v[1]) << 16;
+                            d.y = f32_to_bf16(v[2]) | f32_to_bf16(v[3]) << 16;
+                            reinterpret_cast<uint2*>(strip)[at * 2u + (q & 1u)] = d;
+                        }
+                    }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (uint32_t h = 0; h < kMF / 16u; ++h) {
+                    const uint32_t r = 16u * h + (lane >> 2), piece = lane & 3u;
+                    const uint32_t within = pass * (64u / kSize) + piece * kEach, column = first_column + within;
+                    if (m0 + r >= count || within >= kOut * kMF || column >= n_out) continue;
+                    const v4i w = strip[r * 4u + (piece ^ (r >> 2 & 3u))];
+                    T* to = c + (static_cast<uint64_t>(now.row.first) + m0 + r) * p.c_stride + column;
+                    if (whole && column + kEach <= n_out) {
+                        *reinterpret_cast<v4i*>(to) = w;
+                    } else {
+                        for (uint32_t e = 0; e < kEach && column + e < n_out; ++e) {
+                            const uint32_t word = w[e * kSize / 4u];
+                            to[e] = __builtin_bit_cast(T, static_cast<std::conditional_t<kSize == 4u, uint32_t, uint16_t>>(
+                                                              kSize == 4u ? word : word >> (e % 2u * 16u)));
+                        }
+                    }
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+    };
+
+    // all stages that the ring holds under way, but for the last one's later loads
 #pragma unroll
     for (uint32_t s = 0; s < S::kStages; ++s) {
-        if (s % 2u == 0u)
+        if (!kWide || s % 2u == 0u)
 #pragma unroll
-            for (uint32_t t = 0; t < kScaleLoads; ++t) load_scale(s, t);
+            for (uint32_t t = 0; t < kScaleLoads; ++t) load_scale(t);
 #pragma unroll
-        for (uint32_t t = 0; t < (s + 1u < S::kStages ? kDataLoads : kEarly); ++t) load_data(s, t);
+        for (uint32_t t = 0; t < (s + 1u < S::kStages ? kDataLoads : kEarly); ++t) load_data(t);
+        // the ring of pairs moves on behind a pair's second stage
+        if (s + 1u < S::kStages) load_next(!kWide || s % 2u == 1u);
     }
-    // stage 0 has come; of the later ones all data loads but the last's second part are under way
-    constexpr uint32_t kFirst = kDataEach * (S::kStages - 2u) + (S::kStages - 1u) / 2u * kScaleEach +
-                                (kEarly < kDataEach ? kEarly : kDataEach);
+    constexpr uint32_t kFirst = kDataEach * (S::kStages - 2u) + (kEarly < kDataEach ? kEarly : kDataEach) +
+                                (kWide ? (S::kStages - 1u) / 2u : S::kStages - 1u) * kScaleEach;
     mx_barrier<kFirst>();
 #pragma unroll
     for (uint32_t i = 0; i < kReads; ++i) {
-        read(0u, 0u, i);
+        read(0u, i);
         read_factor(0u, 0u, i);
     }
 #pragma unroll
     for (uint32_t i = 0; i < kReads; ++i) shift_factor(0u, i);
-    uint32_t s = 0;
-    for (; s + 2u < stages; s += 2u) {
-        stage(s, std::integral_constant<uint32_t, 0>{});
-        stage(s + 1u, std::integral_constant<uint32_t, 1>{});
-    }
-    if (s + 1u < stages) {
-        stage(s, std::integral_constant<uint32_t, 0>{});
-        ++s;
-#pragma unroll
-        for (uint32_t i = 0; i < kReads; ++i) factor[0][i] = factor[1][i];
-    }
-    const auto last_step = [&](auto c) {
-        constexpr uint32_t kC = decltype(c)::value;
-        multiply(c, 0u, std::integral_constant<uint32_t, kC + 1u < S::kSteps ? kReads : 0u>{},
-                 [&](uint32_t o) { read(s, kC + 1u, o); });
-    };
-    last_step(std::integral_constant<uint32_t, 0>{});
-    if constexpr (S::kSteps > 2u) last_step(std::integral_constant<uint32_t, 1>{});
-    if (kWide || !odd) {
-        if constexpr (S::kSteps > 2u) last_step(std::integral_constant<uint32_t, 2>{});
-        last_step(std::integral_constant<uint32_t, S::kSteps - 1u>{});
-    }
-    mx_barrier<0>();  // no load is under way to what follows in the ring
-
-    // ---- C: a wave's rows, kMF at a time, through LDS of its own, so that 16-byte
-    // stores of consecutive lanes are consecutive in a row ----
-    constexpr uint32_t kOut = kSwiglu ? kTN / 2u : kTN;          // tiles across
-    constexpr uint32_t kPitch = (kOut * kMF * 4u + 16u) / 16u;   // 16-byte words a row, of fp32
-    static_assert(S::kWaves * kMF * kPitch <= S::kLds, "the ring holds the strips");
-    v4i* strip = ring + wave * kMF * kPitch;
-    const uint32_t size = p.c_f32 ? 4u : 2u;
-    uint8_t* c = p.c_f32 ? reinterpret_cast<uint8_t*>(p.c_f32) : reinterpret_cast<uint8_t*>(p.c_bf16);
-    const bool whole = reinterpret_cast<uintptr_t>(c) % 16u == 0u && p.c_stride * size % 16u == 0u;
-    const uint32_t first_column = n0 + wn * kOut * kMF;
-#pragma unroll
-    for (uint32_t i = 0; i < kTM; ++i) {
-        const uint32_t m0 = (wm * kTM + i) * kMF;
-        if (m0 >= task.count) break;
-        bool real = true;
-        if (kExperts && p.packed)
-            real = p.packed[task.first + min(m0 + n, task.count - 1u)] / p.top_k < p.a_rows;
-#pragma unroll
-        for (uint32_t j = 0; j < kOut; ++j)
-#pragma unroll
-            for (uint32_t g = 0; g < kAcc / 4u; ++g) {
-                float v[4];
-#pragma unroll
-                for (uint32_t e = 0; e < 4u; ++e) {
-                    v[e] = acc[j][i][4u * g + e];
-                    if constexpr (kSwiglu) v[e] = swiglu(v[e], acc[j + kOut][i][4u * g + e]);
-                    if (!real) v[e] = 0.0f;
-                }
-                const uint32_t column = j * kMF + 64u / kMF * 4u * g + 4u * q;  // four consecutive
-                if (p.c_f32) {
-                    reinterpret_cast<float4*>(strip)[n * kPitch + column / 4u] =
-                        make_float4(v[0], v[1], v[2], v[3]);
-                } else {
-                    uint2 d;
-                    d.x = f32_to_bf16(v[0]) | f32_to_bf16(v[1]) << 16;
-                    d.y = f32_to_bf16(v[2]) | f32_to_bf16(v[3]) << 16;
-                    reinterpret_cast<uint2*>(strip)[n * kPitch * 2u + column / 4u] = d;
-                }
+    for (;;) {
+        if constexpr (kWide) {
+            for (uint32_t s = 0; s < stages; s += 2u) {
+                stage(std::integral_constant<uint32_t, 0>{}, false);
+                stage(std::integral_constant<uint32_t, 1>{}, false);
             }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const uint32_t pieces = kOut * kMF * size / 16u, each = 16u / size;
-        for (uint32_t at = lane; at < kMF * pieces; at += 64u) {
-            const uint32_t r = at / pieces, piece = at % pieces, column = first_column + piece * each;
-            if (m0 + r >= task.count || column >= n_out) continue;
-            const v4i w = strip[r * kPitch + piece];
-            uint8_t* to = c + ((static_cast<uint64_t>(task.first) + m0 + r) * p.c_stride + column) * size;
-            if (whole && column + each <= n_out) {
-                *reinterpret_cast<v4i*>(to) = w;
-            } else if (p.c_f32) {
-                for (uint32_t e = 0; e < 4u && column + e < n_out; ++e)
-                    reinterpret_cast<int*>(to)[e] = w[e];
-            } else {
-                for (uint32_t e = 0; e < 8u && column + e < n_out; ++e)
-                    reinterpret_cast<uint16_t*>(to)[e] =
-                        static_cast<uint16_t>(static_cast<uint32_t>(w[e / 2u]) >> (e % 2u * 16u));
-            }
+        } else {
+            for (uint32_t s = 0; s < stages; ++s)
+                stage(std::integral_constant<uint32_t, 0>{}, odd && s + 1u == stages);
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
+        if (p.c_f32) store(p.c_f32);
+        else store(p.c_bf16);
+        if (now.left == 1u) break;
+        now.next(p, columns);
+#pragma unroll
+        for (uint32_t j = 0; j < kTN; ++j)
+#pragma unroll
+            for (uint32_t i = 0; i < kTM; ++i) acc[j][i] = Acc{};
     }
+    mx_barrier<0>();  // no load is under way to LDS that the next workgroup gets
 }
 
-using MxLarge = MxShape<32, 2, 4, 4, 2, 2>;   // 256 x 256
+using MxLarge = MxShape<32, 4, 2, 2, 4, 2>;   // 256 x 256
 using MxMiddle = MxShape<32, 2, 2, 2, 2, 2>;  // 128 x 128
 using MxSmall = MxShape<16, 2, 2, 2, 2, 3>;   // 64 x 64
-using MxFew = MxShape<16, 1, 4, 1, 2, 4>;     // 16 x 128
+using MxFew = MxShape<16, 1, 4, 1, 2, 3>;     // 16 x 128
 
 }  // namespace
 
@@ -644,19 +726,19 @@ hipError_t launch_mx_quantize(const void* x, uint32_t dtype, uint64_t stride, ui
 
 namespace {
 
-// workgroups: a bound where the experts' rows are known to the device alone
+// tiles: a bound where the experts' rows are known to the device alone
 template <typename S>
-uint64_t mx_grid(const MxProduct& p, bool swiglu) {
+uint64_t mx_tiles(const MxProduct& p, bool swiglu) {
     const uint64_t across = swiglu ? S::kBN / 2u : S::kBN, n_out = swiglu ? p.n / 2u : p.n;
     const uint64_t rows = p.offsets ? mx_max_tasks(p.routes, p.experts, S::kBM)
                                     : (static_cast<uint64_t>(p.routes) + S::kBM - 1u) / S::kBM;
-    const uint64_t all = rows * ((n_out + across - 1u) / across);
-    return (all + kXcds - 1u) / kXcds * kXcds;
+    return rows * ((n_out + across - 1u) / across);
 }
 
 template <typename S, bool kExperts, bool kSwiglu>
 hipError_t launch_tiles(const MxProduct& p, hipStream_t stream) {
-    const uint32_t grid = static_cast<uint32_t>(mx_grid<S>(p, kSwiglu));
+    const uint64_t tiles = (mx_tiles<S>(p, kSwiglu) + kXcds - 1u) / kXcds * kXcds;
+    const uint32_t grid = tiles < S::kResident * kCus ? static_cast<uint32_t>(tiles) : S::kResident * kCus;
     const bool wide = p.k128 % 4u == 0u && reinterpret_cast<uintptr_t>(p.a_scales) % 16u == 0u &&
                       reinterpret_cast<uintptr_t>(p.b_scales) % 16u == 0u;
     if (wide) mx_tile_kernel<S, kExperts, kSwiglu, true><<<grid, 64u * S::kWaves, 0, stream>>>(p);
@@ -669,8 +751,8 @@ enum class MxTiles { kLarge, kMiddle, kSmall, kFew };
 MxTiles choose_tiles(const MxProduct& p, bool swiglu) {
     const uint32_t rows = p.offsets ? p.routes / (p.routes < p.experts ? p.routes : p.experts) : p.routes;
     if (rows <= 16u) return MxTiles::kFew;
-    if (mx_grid<MxLarge>(p, swiglu) >= 256u && rows >= 512u && !p.offsets) return MxTiles::kLarge;
-    if (mx_grid<MxMiddle>(p, swiglu) >= 256u && rows >= 96u) return MxTiles::kMiddle;
+    if (mx_tiles<MxLarge>(p, swiglu) >= 256u && rows >= 512u && !p.offsets) return MxTiles::kLarge;
+    if (mx_tiles<MxMiddle>(p, swiglu) >= 256u && rows >= 96u) return MxTiles::kMiddle;
     return MxTiles::kSmall;
 }
 
@@ -687,9 +769,8 @@ auto with_tiles(MxTiles tiles, F f) {
 }  // namespace
 
 bool mx_product_fits(const MxProduct& p, bool swiglu) {
-    // a grid of 256-thread workgroups holds less than 2^32 threads
     return with_tiles(choose_tiles(p, swiglu),
-                      [&](auto s) { return mx_grid<decltype(s)>(p, swiglu) < (1ull << 24); });
+                      [&](auto s) { return mx_tiles<decltype(s)>(p, swiglu) < (1ull << 32); });
 }
 
 hipError_t launch_mx_product(const MxProduct& p, bool swiglu, hipStream_t stream) {
