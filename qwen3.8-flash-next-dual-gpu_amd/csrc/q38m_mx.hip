@@ -191,48 +191,57 @@ __device__ __forceinline__ v16f mfma_mx(v4i a, uint32_t sa, v4i b, uint32_t sb, 
     return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wa, wb, c, 4, 4, kByte, sa, kByte, sb);
 }
 
-// h = g / (1 + exp(-g)) u on the base-2 exponential and reciprocal instructions
-// (one unit in the last place each): with the rounding of -g log2 e put back, within 8
-// roundings of h.  The exponential's argument is held to 88, where it is still finite:
-// below g = -88 h is within 2^-126 |g u| of the formula's.  (The contract's exp and an
-// IEEE division take three times the instructions: 32,768-token gate/up 750 -> 640 us.)
+// h = g / (1 + exp(-g)) u on the base-2 exponential and reciprocal instructions (one
+// unit in the last place each).  The exponential's argument is held to 88, where it is
+// still finite: below g = -88 h is within 2^-126 |g u| of the formula's.  kExact puts the
+// rounding of -g log2 e back: within 8 roundings of h; without it, |g| roundings more,
+// 2^-17 of h at most, far below half a step of bf16.  (The contract's exp and an IEEE
+// division take three times the instructions: 32,768-token gate/up 750 -> 640 us.)
+template <bool kExact>
 __device__ __forceinline__ float swiglu(float g, float u) {
-    constexpr float kLog2e = 1.44269502162933349609375f;      // and what it lacks of log2 e
+    constexpr float kLog2e = 1.44269502162933349609375f;  // and what it lacks of log2 e
     constexpr float kLog2eLow = 1.92596299112661746887e-8f;
     const float x = -__builtin_amdgcn_fmed3f(g, -88.0f, 88.0f);
     const float a = x * kLog2e;
-    const float low = __builtin_fmaf(x, kLog2eLow, __builtin_fmaf(x, kLog2e, -a));
-    const float e = __builtin_amdgcn_exp2f(a);
-    const float exp = __builtin_fmaf(e * low, 0.693147180559945309f, e);
-    return g * __builtin_amdgcn_rcpf(1.0f + exp) * u;
+    float e = __builtin_amdgcn_exp2f(a);
+    if constexpr (kExact) {
+        const float low = __builtin_fmaf(x, kLog2eLow, __builtin_fmaf(x, kLog2e, -a));
+        e = __builtin_fmaf(e * low, 0.693147180559945309f, e);
+    }
+    return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
 }
 
-// A row tile of the experts' rows: `first` up to kRows rows on or to the expert's end.
+// the kernel's steps, which share its registers
+#define MX_INLINE __attribute__((always_inline))
+
 struct RowTile {
-    uint32_t expert, first, end;
+    uint32_t expert, first, count;  // rows first .. first + count of the sorted order
 };
 
-// The row tiles of the experts' rows, kRows at a time, held by a wave: lane l holds
-// the experts kPer l .. kPer l + kPer - 1, their rows and the sum of row tiles up to
-// and with them.  Offsets past `routes` count as routes, an end that is not behind its
-// begin as no rows.
+// The row tiles of the experts' rows, kRows at a time, found by a wave from the offsets
+// (LDS, all of kMaxSortExperts; those past the experts are the last one, `last`).  Lane l
+// keeps the row tiles of the first 16 (l + 1) experts.  Offsets past `routes` count as
+// routes, an end that is not behind its begin as no rows.
 template <uint32_t kRows>
 struct TileList {
     static constexpr uint32_t kPer = kMaxSortExperts / 64u;
-    uint32_t begin[kPer], end[kPer], sum, total;
+    static_assert(kPer == 16u, "a row of lanes looks at a lane's experts");
+    const uint32_t* offsets;
+    uint32_t last, routes, sum, total;
 
-    __device__ TileList(const uint32_t* __restrict__ offsets, uint32_t experts, uint32_t routes) {
-        const uint32_t lane = threadIdx.x & 63u, e0 = lane * kPer;
+    __device__ MX_INLINE TileList(const uint32_t* offsets_, uint32_t last_, uint32_t routes_)
+        : offsets(offsets_), last(last_), routes(routes_), sum(0) {
+        const uint32_t lane = threadIdx.x & 63u;
         uint32_t at[kPer + 1];
 #pragma unroll
-        for (uint32_t i = 0; i <= kPer; ++i) at[i] = offsets[min(e0 + i, experts)];
-        sum = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < kPer; ++i) {
-            begin[i] = min(at[i], routes);
-            end[i] = max(min(at[i + 1u], routes), begin[i]);
-            sum += tiles(i);
+        for (uint32_t i = 0; i < kPer; i += 4u) {
+            const v4i w = reinterpret_cast<const v4i*>(offsets)[(lane * kPer + i) / 4u];
+            at[i] = w[0], at[i + 1u] = w[1], at[i + 2u] = w[2], at[i + 3u] = w[3];
         }
+        at[kPer] = __shfl_down(at[0], 1);
+        if (lane == 63u) at[kPer] = last;
+#pragma unroll
+        for (uint32_t i = 0; i < kPer; ++i) sum += tiles(at[i], at[i + 1u]);
 #pragma unroll
         for (uint32_t d = 1; d < 64u; d <<= 1) {
             const uint32_t up = __shfl_up(sum, d);
@@ -241,55 +250,56 @@ struct TileList {
         total = __builtin_amdgcn_readlane(sum, 63);
     }
 
-    __device__ uint32_t tiles(uint32_t i) const { return (end[i] - begin[i] + kRows - 1u) / kRows; }
+    __device__ MX_INLINE uint32_t tiles(uint32_t begin, uint32_t end) const {
+        begin = min(begin, routes);
+        return (max(min(end, routes), begin) - begin + kRows - 1u) / kRows;
+    }
 
     // tile < total
-    __device__ RowTile find(uint32_t tile) const {
-        const uint32_t owner = __builtin_ctzll(__ballot(sum > tile));
-        uint32_t before = sum;
-#pragma unroll
-        for (uint32_t i = 0; i < kPer; ++i) before -= tiles(i);
-        uint32_t left = tile - before, expert = 0, first = 0, last = 0;
-        bool found = false;
-#pragma unroll
-        for (uint32_t i = 0; i < kPer; ++i) {
-            if (!found && left < tiles(i)) {
-                found = true;
-                expert = (threadIdx.x & 63u) * kPer + i;
-                first = begin[i] + left * kRows;
-                last = end[i];
-            }
-            left -= tiles(i);
-        }
-        return RowTile{static_cast<uint32_t>(__builtin_amdgcn_readlane(expert, owner)),
-                       static_cast<uint32_t>(__builtin_amdgcn_readlane(first, owner)),
-                       static_cast<uint32_t>(__builtin_amdgcn_readlane(last, owner))};
+    __device__ MX_INLINE RowTile find(uint32_t tile) const {
+        const uint32_t group = __builtin_ctzll(__ballot(sum > tile));
+        const uint32_t left = tile - (group != 0u ? __builtin_amdgcn_readlane(sum, group - 1u) : 0u);
+        const uint32_t e = group * kPer + threadIdx.x % kPer;
+        const uint32_t begin = min(offsets[e], routes);
+        const uint32_t end = min(e + 1u < kMaxSortExperts ? offsets[min(e + 1u, kMaxSortExperts - 1u)] : last, routes);
+        uint32_t upto = tiles(begin, end);
+        upto += __builtin_amdgcn_update_dpp(0, upto, 0x111, 0xf, 0xf, true);  // from 1, 2, 4, 8 lanes below
+        upto += __builtin_amdgcn_update_dpp(0, upto, 0x112, 0xf, 0xf, true);
+        upto += __builtin_amdgcn_update_dpp(0, upto, 0x114, 0xf, 0xf, true);
+        upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xf, 0xf, true);
+        const uint32_t at = __builtin_ctzll(__ballot(upto > left));
+        const uint32_t before = at != 0u ? __builtin_amdgcn_readlane(upto, at - 1u) : 0u;
+        const uint32_t first = __builtin_amdgcn_readlane(begin, at) + (left - before) * kRows;
+        const uint32_t count = min(__builtin_amdgcn_readlane(end, at) - first, kRows);
+        return RowTile{group * kPer + at, first, count};
     }
 };
 
-// Where a workgroup is in its tiles: row tile by row tile, the column tiles of one
-// after the other, so that its rows of A stay the same for as long as can be.
-template <uint32_t kRows>
-struct MxWalk {
-    RowTile row;
-    uint32_t column, left;  // tiles from this one on
+// The order of the tiles, and each workgroup's part of it: groups of kGroup row tiles,
+// column by column.  The dispatcher hands workgroups to the eight XCDs in turn, each
+// with an L2 of its own: an XCD has one contiguous eighth of the order, and its
+// workgroups take turns, so that those at work at the same time share rows of A and of
+// B.  (Each a run of consecutive tiles, with the same rows of A: gate/up of 512 experts
+// 112 instead of 108 us for 512 tokens, 316 instead of 182 for 2,048, 968 instead of 608
+// for 32,768: the workgroups stream B at different places.)
+constexpr uint32_t kXcds = 8, kCus = 256, kGroup = 4;
+struct MxOrder {
+    uint32_t rows, columns;   // of tiles
+    uint32_t at, step, count;  // this workgroup's tiles
 
-    __device__ uint32_t count() const { return min(row.end - row.first, kRows); }
-    // to the next tile; whether it has other rows
-    __device__ bool next(const MxProduct& p, uint32_t columns) {
-        --left;
-        if (++column < columns) return false;
-        column = 0;
-        row.first += kRows;
-        if (row.first < row.end || !p.offsets) return true;
-        while (row.expert + 1u < p.experts) {
-            ++row.expert;
-            row.first = min(p.offsets[row.expert], p.routes);
-            row.end = min(p.offsets[row.expert + 1u], p.routes);
-            if (row.first < row.end) break;
-        }
-        return true;
+    __device__ MX_INLINE MxOrder(uint32_t rows_, uint32_t columns_) : rows(rows_), columns(columns_) {
+        const uint64_t all = static_cast<uint64_t>(rows) * columns;
+        const uint32_t xcd = blockIdx.x % kXcds;
+        step = gridDim.x / kXcds;
+        at = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(xcd * all / kXcds)) + blockIdx.x / kXcds;
+        const uint32_t end = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>((xcd + 1u) * all / kXcds));
+        count = at < end ? (end - at + step - 1u) / step : 0u;
     }
+    __device__ MX_INLINE uint32_t height() const { return min(kGroup, rows - at / (kGroup * columns) * kGroup); }
+    __device__ MX_INLINE uint32_t row() const {
+        return at / (kGroup * columns) * kGroup + at % (kGroup * columns) % height();
+    }
+    __device__ MX_INLINE uint32_t column() const { return at % (kGroup * columns) / height(); }
 };
 
 // Workgroups stay and compute tile after tile of kBM rows of C by kBN rows of B (with
@@ -313,12 +323,14 @@ struct MxShape {
     static constexpr uint32_t kStages = kStages_, kWaves = kWM * kWN;
     static constexpr uint32_t kBM = kWM * kTM * kMF, kBN = kWN * kTN * kMF, kRows = kBM + kBN;
     static constexpr uint32_t kSteps = kMF / 8u;  // matrix instructions deep: 2 or 4
-    // 16-byte words of LDS: the ring, the scales' and a strip of C for each wave.  The
-    // scales of kStages stages may be under way: half as many pairs, begun and ended ones
+    // 16-byte words of LDS: the ring, the scales', a strip of C for each wave and the
+    // experts' offsets.  The scales of kStages stages may be under way: half as many
+    // pairs, begun and ended ones
     static constexpr uint32_t kSlot = kRows * 8u, kScaleAt = kStages * kSlot;
     static constexpr uint32_t kScaleWords = (kStages / 2u + 1u) * kRows;
-    static constexpr uint32_t kStrip = kMF * 4u, kStripAt = kScaleAt + kScaleWords;
-    static constexpr uint32_t kLds = kStripAt + kWaves * kStrip;
+    static constexpr uint32_t kStrip = 64u, kStripAt = kScaleAt + kScaleWords;
+    static constexpr uint32_t kOffsetsAt = kStripAt + kWaves * kStrip;
+    static constexpr uint32_t kLds = kOffsetsAt + kMaxSortExperts / 4u;
     static constexpr uint32_t kResident = 160u * 64u / kLds;  // workgroups a CU
     static_assert(kResident != 0u, "160 KB of LDS");
 };
@@ -349,10 +361,6 @@ __device__ __forceinline__ void mx_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(kOutstanding) : "memory");
 }
 
-// The dispatcher hands workgroups to the eight XCDs in turn, each with an L2 of its
-// own: the workgroups of an XCD take neighbouring tiles, which share rows of A and of B.
-constexpr uint32_t kXcds = 8, kCus = 256;
-
 template <typename S, bool kExperts, bool kSwiglu, bool kWide>
 __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 4u) void mx_tile_kernel(MxProduct p) {
     constexpr uint32_t kMF = S::kMF, kTM = S::kTM, kTN = S::kTN, kBM = S::kBM, kBN = S::kBN;
@@ -365,28 +373,27 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     constexpr uint32_t kColumns = kSwiglu ? kBN / 2u : kBN;
     const uint32_t columns = (n_out + kColumns - 1u) / kColumns;
 
-    // ---- this workgroup's tiles ----
-    MxWalk<kBM> ahead;  // the tile whose stages are being loaded
-    {
-        const uint32_t index = blockIdx.x % kXcds * (gridDim.x / kXcds) + blockIdx.x / kXcds;
-        const auto range = [&](uint64_t rows) {
-            const uint64_t all = rows * columns, at = index * all / gridDim.x;
-            ahead.left = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>((index + 1u) * all / gridDim.x - at));
-            ahead.column = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at % columns));
-            return static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(at / columns)));
-        };
-        if constexpr (kExperts) {
-            const TileList<kBM> list(p.offsets, p.experts, p.routes);
-            const uint32_t row = range(list.total);
-            if (ahead.left == 0u) return;
-            ahead.row = list.find(row);
-        } else {
-            const uint32_t row = range((p.routes + kBM - 1u) / kBM);
-            if (ahead.left == 0u) return;
-            ahead.row = RowTile{0u, row * kBM, p.routes};
-        }
+    // ---- this workgroup's tiles, and what is known of those being loaded: lane t % 64
+    // holds the t-th ----
+    uint32_t* offsets = reinterpret_cast<uint32_t*>(ring + S::kOffsetsAt);
+    const uint32_t last_offset = kExperts ? p.offsets[p.experts] : 0u;
+    if constexpr (kExperts) {
+        for (uint32_t e = threadIdx.x; e < kMaxSortExperts; e += 64u * S::kWaves)
+            offsets[e] = e < p.experts ? p.offsets[e] : last_offset;
+        __syncthreads();
     }
-    MxWalk<kBM> now = ahead;  // the tile being multiplied
+    const auto make_list = [&]() MX_INLINE {
+        if constexpr (kExperts) return TileList<kBM>(offsets, last_offset, p.routes);
+        else return 0;
+    };
+    const auto list = make_list();
+    const auto row_tiles = [&]() MX_INLINE {
+        if constexpr (kExperts) return list.total;
+        else return (p.routes + kBM - 1u) / kBM;
+    };
+    MxOrder order(row_tiles(), columns);
+    if (order.count == 0u) return;
+    uint32_t known_first = 0, known_count = 0, known_column = 0;
 
     // ---- loads: instructions dealt to the waves, the left over ones to the first: 1 KB
     // of data each, eight rows; of scales 64 rows where they are 16-byte pieces, else 32.
@@ -401,61 +408,96 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     constexpr uint32_t kScaleLoads = kScaleEach + (kScaleRest != 0u ? 1u : 0u);
     const bool data_rest = kDataRest != 0u && wave < kDataRest;
     const bool scale_rest = kScaleRest != 0u && wave < kScaleRest;
-    const auto data_live = [&](uint32_t t) { return kDataRest == 0u || t < kDataEach || data_rest; };
-    const auto scale_live = [&](uint32_t t) { return kScaleRest == 0u || t < kScaleEach || scale_rest; };
+    const auto data_live = [&](uint32_t t) MX_INLINE { return kDataRest == 0u || t < kDataEach || data_rest; };
+    const auto scale_live = [&](uint32_t t) MX_INLINE { return kScaleRest == 0u || t < kScaleEach || scale_rest; };
     const uint32_t row_bytes = p.k128 * 64u, scale_bytes = p.k128 * 4u;
     const uint32_t stages = (p.k128 + 1u) / 2u;
     const bool odd = !kWide && (p.k128 & 1u) != 0u;  // a tile's last stage is 128 values
     const uint8_t *a_base, *b_base, *a_scale_base, *b_scale_base;
     uint32_t data[kDataLoads], scale[kScaleLoads];
-    // points the loads at the tile `ahead`; the rows of A stay where it has the same
-    const auto point = [&](bool other_rows) {
+    // the next tile to load, the `found`-th from one on, and the sources of its rows of A
+    // where they are gathered: looked up a tile ahead, so that nobody waits for them
+    uint32_t found = 0, next_column = 0;
+    RowTile next{0u, 0u, 0u};
+    uint32_t data_source[kDataLoads], scale_source[kScaleLoads];
+    const auto look_up = [&]() MX_INLINE {
+        if (found == order.count) return;
+        if (found != 0u) order.at += order.step;
+        const uint32_t row = order.row();
+        next_column = order.column();
+        if constexpr (kExperts) next = list.find(row);
+        else next = RowTile{0u, row * kBM, static_cast<uint32_t>(min(p.routes - row * kBM, kBM))};
+        if (lane == found % 64u) {
+            known_first = next.first;
+            known_count = next.count;
+            known_column = next_column;
+        }
+        ++found;
+        if (!kExperts || !p.packed) return;
+#pragma unroll
+        for (uint32_t t = 0; t < kDataLoads; ++t) {
+            const uint32_t i = wave + t * S::kWaves;
+            if (data_live(t) && i < kDataA)
+                data_source[t] = p.packed[next.first + min(8u * i + (lane >> 3), next.count - 1u)];
+        }
+#pragma unroll
+        for (uint32_t t = 0; t < kScaleLoads; ++t) {
+            const uint32_t i = wave + t * S::kWaves;
+            if (scale_live(t) && i < kScaleA)
+                scale_source[t] = p.packed[next.first + min(kScaleRows * i + (kWide ? lane : lane >> 1), next.count - 1u)];
+        }
+    };
+    // points the loads at the tile that was looked up, and looks up the one after it
+    const auto point = [&]() MX_INLINE {
         uint32_t own_lane = lane;  // the offsets are computed here, not kept from one tile to the next
         asm volatile("" : "+v"(own_lane));
-        const uint64_t a_first = kExperts && p.packed ? 0u : ahead.row.first;
-        const uint64_t b_first = static_cast<uint64_t>(ahead.row.expert) * p.n + ahead.column * kColumns;
+        const bool gather = kExperts && p.packed;
+        const uint64_t a_first = gather ? 0u : next.first;
+        const uint64_t b_first = static_cast<uint64_t>(next.expert) * p.n + next_column * kColumns;
         a_base = mx_uniform(p.a_codes + a_first * row_bytes);
         a_scale_base = mx_uniform(p.a_scales + a_first * scale_bytes);
         b_base = mx_uniform(p.b_codes + b_first * row_bytes);
         b_scale_base = mx_uniform(p.b_scales + b_first * scale_bytes);
-        const auto a_row = [&](uint32_t j) -> uint32_t {
-            const uint32_t at = min(j, ahead.count() - 1u);
-            if (kExperts && p.packed) return min(p.packed[ahead.row.first + at] / p.top_k, p.a_rows - 1u);
-            return at;
+        const auto a_row = [&](uint32_t j, uint32_t source) MX_INLINE -> uint32_t {
+            if (gather) return min(source / p.top_k, p.a_rows - 1u);
+            return min(j, next.count - 1u);
         };
-        const auto b_row = [&](uint32_t j) -> uint32_t {
+        const auto b_row = [&](uint32_t j) MX_INLINE -> uint32_t {
             uint32_t column = j, up = 0;
             if constexpr (kSwiglu) {  // a wave's tiles: half of them gate, half up
                 const uint32_t t = j / kMF % kTN;
                 column = j / (kTN * kMF) * (kTN / 2u * kMF) + t % (kTN / 2u) * kMF + j % kMF;
                 up = t >= kTN / 2u ? n_out : 0u;
             }
-            return min(column, n_out - 1u - ahead.column * kColumns) + up;
+            return min(column, n_out - 1u - next_column * kColumns) + up;
         };
 #pragma unroll
         for (uint32_t t = 0; t < kDataLoads; ++t) {
             if (!data_live(t)) continue;
             const uint32_t i = wave + t * S::kWaves;
             const uint32_t r = 8u * i + (own_lane >> 3), piece = (own_lane & 7u) ^ (r >> 1 & 7u);
-            if (i >= kDataA) data[t] = b_row(r - kBM) * row_bytes + 16u * piece;
-            else if (other_rows) data[t] = a_row(r) * row_bytes + 16u * piece;
+            data[t] = (i < kDataA ? a_row(r, data_source[t]) : b_row(r - kBM)) * row_bytes + 16u * piece;
         }
 #pragma unroll
         for (uint32_t t = 0; t < kScaleLoads; ++t) {
             if (!scale_live(t)) continue;
             const uint32_t i = wave + t * S::kWaves, r = kWide ? own_lane : own_lane >> 1;
-            if (i >= kScaleA) scale[t] = b_row(min(r + kScaleRows * (i - kScaleA), kBN - 1u)) * scale_bytes;
-            else if (other_rows) scale[t] = a_row(r + kScaleRows * i) * scale_bytes;
+            scale[t] = (i < kScaleA ? a_row(kScaleRows * i + r, scale_source[t])
+                                    : b_row(min(kScaleRows * (i - kScaleA) + r, kBN - 1u))) * scale_bytes;
         }
+        look_up();
     };
-    point(true);
-    uint32_t from = 0, to = 0, scales_to = 0;  // the stage of `ahead` and the slots it is loaded to
+    look_up();
+    uint32_t tiles_left = order.count;  // with the one being loaded
+    bool turn = false;
+    point();
+    uint32_t from = 0, to = 0, scales_to = 0;  // the stage of the tile and the slots it is loaded to
     const uint32_t ring_at = static_cast<uint32_t>(
         reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) v4i*)ring));
     constexpr uint32_t kScaleSlot = kWide ? S::kRows : S::kRows / 2u;  // words
     constexpr uint32_t kScaleSlots = S::kScaleWords / kScaleSlot;
     static_assert(kScaleSlots >= (kWide ? S::kStages / 2u + 1u : S::kStages), "scales under way");
-    const auto load_scale = [&](uint32_t t) {
+    const auto load_scale = [&](uint32_t t) MX_INLINE {
         if (!scale_live(t)) return;
         const uint32_t i = wave + t * S::kWaves, r = kWide ? lane : lane >> 1;
         const bool of_b = i >= kScaleA;
@@ -468,7 +510,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         if constexpr (kWide) mx_load16(base + (from & ~1u) * 8ull, scale[t], at);
         else mx_load4(base, scale[t] + 4u * min(from * 2u + (lane & 1u), p.k128 - 1u), at);
     };
-    const auto load_data = [&](uint32_t t) {
+    const auto load_data = [&](uint32_t t) MX_INLINE {
         if (!data_live(t)) return;
         const uint32_t i = wave + t * S::kWaves;
         uint32_t back = 0;  // a piece past the end of its row: another of the row
@@ -479,18 +521,24 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         mx_load16((i >= kDataA ? b_base : a_base) + (from * 128ull), data[t] - back,
                   __builtin_amdgcn_readfirstlane(ring_at + to * (S::kSlot * 16u) + i * 1024u));
     };
-    // to the next stage to load; past the last tile the last stage again, into slots that
-    // nobody reads any more, so that the count of loads under way is always the same
-    const auto load_next = [&](bool scales_too) {
+    // to the next stage to load, at a tile's first stage with a turn to take before its loads;
+    // past the last tile the last stage again, into slots that nobody reads any more, so
+    // that the count of loads under way is always the same
+    const auto load_next = [&](bool scales_too) MX_INLINE {
         to = to + 1u == S::kStages ? 0u : to + 1u;
         if (scales_too) scales_to = scales_to + 1u == kScaleSlots ? 0u : scales_to + 1u;
-        if (++from < stages) return;
-        if (ahead.left > 1u) {
+        if (from + 1u < stages) {
+            ++from;
+        } else if (tiles_left != 1u) {
             from = 0;
-            point(ahead.next(p, columns));
-        } else {
-            --from;
+            turn = true;
         }
+    };
+    const auto take_turn = [&]() MX_INLINE {
+        if (!turn) return;
+        turn = false;
+        --tiles_left;
+        point();
     };
 
     // ---- products ----
@@ -507,21 +555,21 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     v4i part[2][kReads];      // a step's fragments of A, then of B, and the next step's
     uint2 factor[2][kReads];  // a stage's scales, and the next stage's
     uint32_t slot = 0, scales = 0;  // of the stage whose fragments are read
-    const auto read = [&](uint32_t c, uint32_t i) {
+    const auto read = [&](uint32_t c, uint32_t i) MX_INLINE {
         const uint32_t row = i < kTM ? a_at + i * kMF : b_at + (i - kTM) * kMF;
         part[c % 2u][i] = ring[slot * S::kSlot + row * 8u + ((64u / kMF * c + q) ^ swizzle)];
     };
-    const auto read_factor = [&](uint32_t parity, uint32_t buffer, uint32_t i) {
+    const auto read_factor = [&](uint32_t parity, uint32_t buffer, uint32_t i) MX_INLINE {
         const uint32_t row = i < kTM ? a_at + i * kMF : b_at + (i - kTM) * kMF;
         const uint2* base = reinterpret_cast<const uint2*>(ring + S::kScaleAt + scales * kScaleSlot);
         factor[buffer][i] = kWide ? base[2u * row + parity] : base[row];
     };
-    const auto shift_factor = [&](uint32_t buffer, uint32_t i) {  // this lane's bytes to where the instruction takes them
+    const auto shift_factor = [&](uint32_t buffer, uint32_t i) MX_INLINE {  // this lane's bytes to where the instruction takes them
         factor[buffer][i] = make_uint2(factor[buffer][i].x >> 8u * q, factor[buffer][i].y >> 8u * q);
     };
     // The matrix instructions of step c (none where the stage ends in front of it), `ops`
     // other operations among them from the first on
-    const auto multiply = [&](auto step, uint32_t buffer, bool live, auto ops, auto op) {
+    const auto multiply = [&](auto step, uint32_t buffer, bool live, auto ops, auto op) MX_INLINE {
         constexpr uint32_t kC = decltype(step)::value, kOps = decltype(ops)::value, kAll = kTM * kTN;
         constexpr uint32_t kPer = (kOps + kAll - 1u) / kAll;
         constexpr int kByte = kMF == 32u ? 2 * (kC & 1u) : 0;
@@ -548,13 +596,13 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     // step in front of it is multiplied.  In front of the last step the workgroup meets:
     // the next stage has come and this one is read, so its slot takes the kStages-th
     // after it.  kWide: even and odd stages take turns, their scales in two buffers.
-    const auto stage = [&](auto odd_stage, bool half) {
+    const auto stage = [&](auto odd_stage, bool half) MX_INLINE {
         constexpr uint32_t kParity = kWide ? decltype(odd_stage)::value : 0u;
         constexpr bool kScalesNow = !kWide || (kParity + S::kStages) % 2u == 0u;
         // loads of the kStages - 2 stages behind the next; kWide: at least half of them, rounded down, bring scales
         constexpr uint32_t kLater = S::kStages - 2u;
         constexpr uint32_t kBusy = kDataEach * kLater + (kWide ? kLater / 2u : kLater) * kScaleEach;
-        const auto step = [&](auto c) {
+        const auto step = [&](auto c) MX_INLINE {
             constexpr uint32_t kC = decltype(c)::value;
             constexpr uint32_t kLoads = kC == 0u ? kDataLoads - kEarly : 0u;
             multiply(c, kParity, kWide || 2u * kC < S::kSteps || !half,
@@ -571,6 +619,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         }
         if (data_rest) mx_barrier<kBusy + (kDataRest != 0u ? kLater : 0u)>();
         else mx_barrier<kBusy>();
+        take_turn();
         slot = slot + 1u == S::kStages ? 0u : slot + 1u;
         if (!kWide || kParity == 1u) scales = scales + 1u == kScaleSlots ? 0u : scales + 1u;
         constexpr uint32_t kScaleOps = kScalesNow ? kScaleLoads : 0u, kLoads = kScaleOps + kEarly;
@@ -590,63 +639,70 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
 
     // ---- C: 64 bytes of a wave's rows at a time through LDS of its own, so that the
     // 16-byte stores of four consecutive lanes are consecutive in a row ----
-    const auto store = [&](auto* c) {
+    const auto store = [&](uint32_t t, auto* c) MX_INLINE {
         using T = std::remove_pointer_t<decltype(c)>;
         constexpr uint32_t kSize = sizeof(T), kOut = kSwiglu ? kTN / 2u : kTN;  // tiles across
         constexpr uint32_t kGap = 64u / kMF * 4u;                               // columns from group to group
         constexpr uint32_t kPasses = (kOut * kMF * kSize + 63u) / 64u, kEach = 16u / kSize;
         v4i* strip = ring + S::kStripAt + wave * S::kStrip;
         const bool whole = reinterpret_cast<uintptr_t>(c) % 16u == 0u && p.c_stride * kSize % 16u == 0u;
-        const uint32_t count = now.count(), first_column = now.column * kColumns + wn * kOut * kMF;
+        const uint32_t first_row = __builtin_amdgcn_readlane(known_first, t % 64u);
+        const uint32_t count = __builtin_amdgcn_readlane(known_count, t % 64u);
+        const uint32_t first_column = __builtin_amdgcn_readlane(known_column, t % 64u) * kColumns + wn * kOut * kMF;
 #pragma unroll
         for (uint32_t i = 0; i < kTM; ++i) {
             const uint32_t m0 = (wm * kTM + i) * kMF;
             if (m0 >= count) break;
 #pragma unroll
             for (uint32_t pass = 0; pass < kPasses; ++pass) {
+                using Four = std::conditional_t<kSize == 4u, float4, uint2>;  // consecutive columns
+                constexpr uint32_t kFours = 64u / (kGap * kSize);            // a lane's in 64 bytes of a row
+                Four four[kFours];
 #pragma unroll
-                for (uint32_t j = 0; j < kOut; ++j)
+                for (uint32_t f = 0; f < kFours; ++f) {
+                    const uint32_t j = (pass * kFours + f) / (kAcc / 4u), g = (pass * kFours + f) % (kAcc / 4u);
+                    if (j >= kOut) continue;
+                    float v[4];
 #pragma unroll
-                    for (uint32_t g = 0; g < kAcc / 4u; ++g) {
-                        if ((j * kMF + kGap * g) * kSize / 64u != pass) continue;
-                        float v[4];  // four consecutive columns
-#pragma unroll
-                        for (uint32_t e = 0; e < 4u; ++e) {
-                            v[e] = acc[j][i][4u * g + e];
-                            if constexpr (kSwiglu) v[e] = swiglu(v[e], acc[j + kOut][i][4u * g + e]);
-                        }
-                        const uint32_t byte = ((j * kMF + kGap * g) * kSize) % 64u + 4u * q * kSize;
-                        const uint32_t at = n * 4u + (byte / 16u ^ (n >> 2 & 3u));
-                        if constexpr (kSize == 4u) {
-                            reinterpret_cast<float4*>(strip)[at] = make_float4(v[0], v[1], v[2], v[3]);
-                        } else {
-                            uint2 d;
-                            d.x = f32_to_bf16(v[0]) | f32_to_bf16(v[1]) << 16;
-                            d.y = f32_to_bf16(v[2]) | f32_to_bf16(v[3]) << 16;
-                            reinterpret_cast<uint2*>(strip)[at * 2u + (q & 1u)] = d;
-                        }
+                    for (uint32_t e = 0; e < 4u; ++e) {
+                        v[e] = acc[j][i][4u * g + e];
+                        if constexpr (kSwiglu) v[e] = swiglu<kSize == 4u>(v[e], acc[j + kOut][i][4u * g + e]);
                     }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
-#pragma unroll
-                for (uint32_t h = 0; h < kMF / 16u; ++h) {
-                    const uint32_t r = 16u * h + (lane >> 2), piece = lane & 3u;
-                    const uint32_t within = pass * (64u / kSize) + piece * kEach, column = first_column + within;
-                    if (m0 + r >= count || within >= kOut * kMF || column >= n_out) continue;
-                    const v4i w = strip[r * 4u + (piece ^ (r >> 2 & 3u))];
-                    T* to = c + (static_cast<uint64_t>(now.row.first) + m0 + r) * p.c_stride + column;
-                    if (whole && column + kEach <= n_out) {
-                        *reinterpret_cast<v4i*>(to) = w;
-                    } else {
-                        for (uint32_t e = 0; e < kEach && column + e < n_out; ++e) {
-                            const uint32_t word = w[e * kSize / 4u];
-                            to[e] = __builtin_bit_cast(T, static_cast<std::conditional_t<kSize == 4u, uint32_t, uint16_t>>(
-                                                              kSize == 4u ? word : word >> (e % 2u * 16u)));
-                        }
-                    }
+                    if constexpr (kSize == 4u) four[f] = make_float4(v[0], v[1], v[2], v[3]);
+                    else four[f] = make_uint2(f32_to_bf16(v[0]) | f32_to_bf16(v[1]) << 16,
+                                              f32_to_bf16(v[2]) | f32_to_bf16(v[3]) << 16);
                 }
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (uint32_t half = 0; half < kMF / 16u; ++half) {  // the strip holds 16 rows
+                    if (n / 16u == half) {
+#pragma unroll
+                        for (uint32_t f = 0; f < kFours; ++f) {
+                            const uint32_t byte = f * kGap * kSize + 4u * q * kSize;
+                            const uint32_t at = n % 16u * 4u + (byte / 16u ^ (n >> 2 & 3u));
+                            if constexpr (kSize == 4u) reinterpret_cast<float4*>(strip)[at] = four[f];
+                            else reinterpret_cast<uint2*>(strip)[at * 2u + (q & 1u)] = four[f];
+                        }
+                    }
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                    const uint32_t r = lane >> 2, piece = lane & 3u, m = m0 + 16u * half + r;
+                    const uint32_t within = pass * (64u / kSize) + piece * kEach, column = first_column + within;
+                    if (m < count && within < kOut * kMF && column < n_out) {
+                        const v4i w = strip[r * 4u + (piece ^ (r >> 2 & 3u))];
+                        T* to = c + (static_cast<uint64_t>(first_row) + m) * p.c_stride + column;
+                        if (whole && column + kEach <= n_out) {
+                            *reinterpret_cast<v4i*>(to) = w;
+                        } else {
+                            for (uint32_t e = 0; e < kEach && column + e < n_out; ++e) {
+                                const uint32_t word = w[e * kSize / 4u];
+                                to[e] = __builtin_bit_cast(T, static_cast<std::conditional_t<kSize == 4u, uint32_t, uint16_t>>(
+                                                                  kSize == 4u ? word : word >> (e % 2u * 16u)));
+                            }
+                        }
+                    }
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                }
             }
         }
     };
@@ -660,7 +716,10 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
 #pragma unroll
         for (uint32_t t = 0; t < (s + 1u < S::kStages ? kDataLoads : kEarly); ++t) load_data(t);
         // the ring of pairs moves on behind a pair's second stage
-        if (s + 1u < S::kStages) load_next(!kWide || s % 2u == 1u);
+        if (s + 1u < S::kStages) {
+            load_next(!kWide || s % 2u == 1u);
+            take_turn();
+        }
     }
     constexpr uint32_t kFirst = kDataEach * (S::kStages - 2u) + (kEarly < kDataEach ? kEarly : kDataEach) +
                                 (kWide ? (S::kStages - 1u) / 2u : S::kStages - 1u) * kScaleEach;
@@ -672,7 +731,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     }
 #pragma unroll
     for (uint32_t i = 0; i < kReads; ++i) shift_factor(0u, i);
-    for (;;) {
+    for (uint32_t t = 0;; ++t) {
         if constexpr (kWide) {
             for (uint32_t s = 0; s < stages; s += 2u) {
                 stage(std::integral_constant<uint32_t, 0>{}, false);
@@ -682,10 +741,9 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
             for (uint32_t s = 0; s < stages; ++s)
                 stage(std::integral_constant<uint32_t, 0>{}, odd && s + 1u == stages);
         }
-        if (p.c_f32) store(p.c_f32);
-        else store(p.c_bf16);
-        if (now.left == 1u) break;
-        now.next(p, columns);
+        if (p.c_f32) store(t, p.c_f32);
+        else store(t, p.c_bf16);
+        if (t + 1u == order.count) break;
 #pragma unroll
         for (uint32_t j = 0; j < kTN; ++j)
 #pragma unroll
@@ -697,7 +755,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
 using MxLarge = MxShape<32, 4, 2, 2, 4, 2>;   // 256 x 256
 using MxMiddle = MxShape<32, 2, 2, 2, 2, 2>;  // 128 x 128
 using MxSmall = MxShape<16, 2, 2, 2, 2, 3>;   // 64 x 64
-using MxFew = MxShape<16, 1, 4, 1, 2, 3>;     // 16 x 128
+using MxFew = MxShape<16, 1, 4, 1, 2, 3>;    // 16 x 128
 
 }  // namespace
 
