@@ -172,6 +172,8 @@ __global__ __launch_bounds__(kQuantThreads) void mx_quantize_kernel(
 
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 // The block-scaled matrix instructions on 4-bit codes.  v_mfma_scale_f32_16x16x128:
 // lane l holds the 32 values k = 32 (l / 16) .. + 31 of row l % 16 of A and of B and
@@ -323,13 +325,11 @@ struct MxShape {
     static constexpr uint32_t kStages = kStages_, kWaves = kWM * kWN;
     static constexpr uint32_t kBM = kWM * kTM * kMF, kBN = kWN * kTN * kMF, kRows = kBM + kBN;
     static constexpr uint32_t kSteps = kMF / 8u;  // matrix instructions deep: 2 or 4
-    // 16-byte words of LDS: the ring, the scales', a strip of C for each wave and the
-    // experts' offsets.  The scales of kStages stages may be under way: half as many
-    // pairs, begun and ended ones
+    // 16-byte words of LDS: the ring, the scales' and the experts' offsets.  The scales
+    // of kStages stages may be under way: half as many pairs, begun and ended ones
     static constexpr uint32_t kSlot = kRows * 8u, kScaleAt = kStages * kSlot;
     static constexpr uint32_t kScaleWords = (kStages / 2u + 1u) * kRows;
-    static constexpr uint32_t kStrip = 64u, kStripAt = kScaleAt + kScaleWords;
-    static constexpr uint32_t kOffsetsAt = kStripAt + kWaves * kStrip;
+    static constexpr uint32_t kOffsetsAt = kScaleAt + kScaleWords;
     static constexpr uint32_t kLds = kOffsetsAt + kMaxSortExperts / 4u;
     static constexpr uint32_t kResident = 160u * 64u / kLds;  // workgroups a CU
     static_assert(kResident != 0u, "160 KB of LDS");
@@ -637,71 +637,79 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         }
     };
 
-    // ---- C: 64 bytes of a wave's rows at a time through LDS of its own, so that the
-    // 16-byte stores of four consecutive lanes are consecutive in a row ----
+    // ---- C: a lane has four consecutive columns of a row, 16 bytes of fp32; in bf16 it
+    // trades one of two such groups with the lane that has the columns beside the other's,
+    // which gives both of them 16 bytes.  (Through strips of LDS, 64 bytes of a row at a
+    // time: 8 us a 256 x 256 tile, of 26.) ----
     const auto store = [&](uint32_t t, auto* c) MX_INLINE {
         using T = std::remove_pointer_t<decltype(c)>;
         constexpr uint32_t kSize = sizeof(T), kOut = kSwiglu ? kTN / 2u : kTN;  // tiles across
-        constexpr uint32_t kGap = 64u / kMF * 4u;                               // columns from group to group
-        constexpr uint32_t kPasses = (kOut * kMF * kSize + 63u) / 64u, kEach = 16u / kSize;
-        v4i* strip = ring + S::kStripAt + wave * S::kStrip;
+        constexpr uint32_t kFours = kOut * kAcc / 4u;                           // a lane's groups of four
         const bool whole = reinterpret_cast<uintptr_t>(c) % 16u == 0u && p.c_stride * kSize % 16u == 0u;
         const uint32_t first_row = __builtin_amdgcn_readlane(known_first, t % 64u);
         const uint32_t count = __builtin_amdgcn_readlane(known_count, t % 64u);
         const uint32_t first_column = __builtin_amdgcn_readlane(known_column, t % 64u) * kColumns + wn * kOut * kMF;
 #pragma unroll
         for (uint32_t i = 0; i < kTM; ++i) {
-            const uint32_t m0 = (wm * kTM + i) * kMF;
-            if (m0 >= count) break;
-#pragma unroll
-            for (uint32_t pass = 0; pass < kPasses; ++pass) {
-                using Four = std::conditional_t<kSize == 4u, float4, uint2>;  // consecutive columns
-                constexpr uint32_t kFours = 64u / (kGap * kSize);            // a lane's in 64 bytes of a row
-                Four four[kFours];
-#pragma unroll
-                for (uint32_t f = 0; f < kFours; ++f) {
-                    const uint32_t j = (pass * kFours + f) / (kAcc / 4u), g = (pass * kFours + f) % (kAcc / 4u);
-                    if (j >= kOut) continue;
-                    float v[4];
-#pragma unroll
-                    for (uint32_t e = 0; e < 4u; ++e) {
-                        v[e] = acc[j][i][4u * g + e];
-                        if constexpr (kSwiglu) v[e] = swiglu<kSize == 4u>(v[e], acc[j + kOut][i][4u * g + e]);
-                    }
-                    if constexpr (kSize == 4u) four[f] = make_float4(v[0], v[1], v[2], v[3]);
-                    else four[f] = make_uint2(f32_to_bf16(v[0]) | f32_to_bf16(v[1]) << 16,
-                                              f32_to_bf16(v[2]) | f32_to_bf16(v[3]) << 16);
+            const uint32_t m = (wm * kTM + i) * kMF + n;
+            if ((wm * kTM + i) * kMF >= count) break;
+            T* row = c + (static_cast<uint64_t>(first_row) + m) * p.c_stride;
+            const auto put = [&](const auto& words, uint32_t column) MX_INLINE {
+                constexpr uint32_t kEach = sizeof(words) / kSize;
+                if (m >= count || column >= n_out) return;
+                T* to = row + column;
+                if (whole && column + kEach <= n_out) {
+                    *reinterpret_cast<std::remove_cv_t<std::remove_reference_t<decltype(words)>>*>(to) = words;
+                    return;
                 }
 #pragma unroll
-                for (uint32_t half = 0; half < kMF / 16u; ++half) {  // the strip holds 16 rows
-                    if (n / 16u == half) {
+                for (uint32_t e = 0; e < kEach; ++e) {
+                    if (column + e >= n_out) break;
+                    const uint32_t word = words[e * kSize / 4u];
+                    if constexpr (kSize == 4u) to[e] = __uint_as_float(word);
+                    else to[e] = static_cast<uint16_t>(word >> (e % 2u * 16u));
+                }
+            };
+            const auto four = [&](uint32_t f, float* v) MX_INLINE {
+                const uint32_t j = f / (kAcc / 4u), g = f % (kAcc / 4u);
 #pragma unroll
-                        for (uint32_t f = 0; f < kFours; ++f) {
-                            const uint32_t byte = f * kGap * kSize + 4u * q * kSize;
-                            const uint32_t at = n % 16u * 4u + (byte / 16u ^ (n >> 2 & 3u));
-                            if constexpr (kSize == 4u) reinterpret_cast<float4*>(strip)[at] = four[f];
-                            else reinterpret_cast<uint2*>(strip)[at * 2u + (q & 1u)] = four[f];
-                        }
+                for (uint32_t e = 0; e < 4u; ++e) {
+                    v[e] = acc[j][i][4u * g + e];
+                    if constexpr (kSwiglu) v[e] = swiglu<kSize == 4u>(v[e], acc[j + kOut][i][4u * g + e]);
+                }
+            };
+            // the columns of group f start at kGap f + 4 q of the wave's
+            constexpr uint32_t kGap = kMF == 32u ? 8u : 16u;
+            if constexpr (kSize == 4u) {
+#pragma unroll
+                for (uint32_t f = 0; f < kFours; ++f) {
+                    float v[4];
+                    four(f, v);
+                    put(v4u{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])},
+                        first_column + kGap * f + 4u * q);
+                }
+            } else if constexpr (kFours == 1u) {
+                float v[4];
+                four(0u, v);
+                put(v2u{f32_to_bf16(v[0]) | f32_to_bf16(v[1]) << 16, f32_to_bf16(v[2]) | f32_to_bf16(v[3]) << 16},
+                    first_column + 4u * q);
+            } else {
+#pragma unroll
+                for (uint32_t f = 0; f < kFours; f += 2u) {
+                    float v[4], w[4];
+                    four(f, v);
+                    four(f + 1u, w);
+                    uint32_t d[4] = {f32_to_bf16(v[0]) | f32_to_bf16(v[1]) << 16, f32_to_bf16(v[2]) | f32_to_bf16(v[3]) << 16,
+                                     f32_to_bf16(w[0]) | f32_to_bf16(w[1]) << 16, f32_to_bf16(w[2]) | f32_to_bf16(w[3]) << 16};
+                    if constexpr (kMF == 32u) {  // q = 1 of the first group with q = 0 of the second
+                        const auto low = __builtin_amdgcn_permlane32_swap(d[0], d[2], false, false);
+                        const auto high = __builtin_amdgcn_permlane32_swap(d[1], d[3], false, false);
+                        put(v4u{low[0], high[0], low[1], high[1]}, first_column + kGap * (f + q));
+                    } else {  // odd q of the first group with the q below of the second
+                        const auto low = __builtin_amdgcn_permlane16_swap(d[0], d[2], false, false);
+                        const auto high = __builtin_amdgcn_permlane16_swap(d[1], d[3], false, false);
+                        put(v4u{low[0], high[0], low[1], high[1]}, first_column + kGap * (f + q % 2u) + 4u * (q & 2u));
                     }
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    __builtin_amdgcn_wave_barrier();
-                    const uint32_t r = lane >> 2, piece = lane & 3u, m = m0 + 16u * half + r;
-                    const uint32_t within = pass * (64u / kSize) + piece * kEach, column = first_column + within;
-                    if (m < count && within < kOut * kMF && column < n_out) {
-                        const v4i w = strip[r * 4u + (piece ^ (r >> 2 & 3u))];
-                        T* to = c + (static_cast<uint64_t>(first_row) + m) * p.c_stride + column;
-                        if (whole && column + kEach <= n_out) {
-                            *reinterpret_cast<v4i*>(to) = w;
-                        } else {
-                            for (uint32_t e = 0; e < kEach && column + e < n_out; ++e) {
-                                const uint32_t word = w[e * kSize / 4u];
-                                to[e] = __builtin_bit_cast(T, static_cast<std::conditional_t<kSize == 4u, uint32_t, uint16_t>>(
-                                                                  kSize == 4u ? word : word >> (e % 2u * 16u)));
-                            }
-                        }
-                    }
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    __builtin_amdgcn_wave_barrier();
                 }
             }
         }
