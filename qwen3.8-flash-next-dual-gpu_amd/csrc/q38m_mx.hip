@@ -5,6 +5,9 @@
 // low nibble; codes past K are zero) and one scale byte for every 32 values.
 // Code c stands for (-1)^(c >> 3) * {0, .5, 1, 1.5, 2, 3, 4, 6}[c & 7], scale
 // byte s for 2^(s - 127), 255 for NaN.
+#include <algorithm>
+#include <cmath>
+#include <iterator>
 #include <type_traits>
 
 #include "q38m_device.h"
@@ -437,13 +440,13 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
 #pragma unroll
         for (uint32_t t = 0; t < kDataLoads; ++t) {
             const uint32_t i = wave + t * S::kWaves;
-            if (data_live(t) && i < kDataA)
+            if (t * S::kWaves < kDataA && data_live(t) && i < kDataA)
                 data_source[t] = p.packed[next.first + min(8u * i + (lane >> 3), next.count - 1u)];
         }
 #pragma unroll
         for (uint32_t t = 0; t < kScaleLoads; ++t) {
             const uint32_t i = wave + t * S::kWaves;
-            if (scale_live(t) && i < kScaleA)
+            if (t * S::kWaves < kScaleA && scale_live(t) && i < kScaleA)
                 scale_source[t] = p.packed[next.first + min(kScaleRows * i + (kWide ? lane : lane >> 1), next.count - 1u)];
         }
     };
@@ -476,14 +479,16 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
             if (!data_live(t)) continue;
             const uint32_t i = wave + t * S::kWaves;
             const uint32_t r = 8u * i + (own_lane >> 3), piece = (own_lane & 7u) ^ (r >> 1 & 7u);
-            data[t] = (i < kDataA ? a_row(r, data_source[t]) : b_row(r - kBM)) * row_bytes + 16u * piece;
+            const bool of_a = t * S::kWaves < kDataA && i < kDataA;
+            data[t] = (of_a ? a_row(r, data_source[t]) : b_row(r - kBM)) * row_bytes + 16u * piece;
         }
 #pragma unroll
         for (uint32_t t = 0; t < kScaleLoads; ++t) {
             if (!scale_live(t)) continue;
             const uint32_t i = wave + t * S::kWaves, r = kWide ? own_lane : own_lane >> 1;
-            scale[t] = (i < kScaleA ? a_row(kScaleRows * i + r, scale_source[t])
-                                    : b_row(min(kScaleRows * (i - kScaleA) + r, kBN - 1u))) * scale_bytes;
+            const bool of_a = t * S::kWaves < kScaleA && i < kScaleA;
+            scale[t] = (of_a ? a_row(kScaleRows * i + r, scale_source[t])
+                             : b_row(min(kScaleRows * (i - kScaleA) + r, kBN - 1u))) * scale_bytes;
         }
         look_up();
     };
@@ -500,7 +505,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     const auto load_scale = [&](uint32_t t) MX_INLINE {
         if (!scale_live(t)) return;
         const uint32_t i = wave + t * S::kWaves, r = kWide ? lane : lane >> 1;
-        const bool of_b = i >= kScaleA;
+        const bool of_b = t * S::kWaves >= kScaleA || i >= kScaleA;
         const uint32_t first = of_b ? kScaleRows * (i - kScaleA) : kScaleRows * i;
         // some lane of a load is within the rows: its count is the same everywhere
         if ((kBM % kScaleRows != 0u || kBN % kScaleRows != 0u) && first + r >= (of_b ? kBN : kBM)) return;
@@ -518,7 +523,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
             const uint32_t piece = (lane & 7u) ^ ((4u * i + (lane >> 4)) & 7u);
             back = odd && from + 1u == stages && piece >= 4u ? 64u : 0u;
         }
-        mx_load16((i >= kDataA ? b_base : a_base) + (from * 128ull), data[t] - back,
+        mx_load16((t * S::kWaves >= kDataA || i >= kDataA ? b_base : a_base) + (from * 128ull), data[t] - back,
                   __builtin_amdgcn_readfirstlane(ring_at + to * (S::kSlot * 16u) + i * 1024u));
     };
     // to the next stage to load, at a tile's first stage with a turn to take before its loads;
@@ -555,9 +560,12 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     v4i part[2][kReads];      // a step's fragments of A, then of B, and the next step's
     uint2 factor[2][kReads];  // a stage's scales, and the next stage's
     uint32_t slot = 0, scales = 0;  // of the stage whose fragments are read
-    const auto read = [&](uint32_t c, uint32_t i) MX_INLINE {
+    // a fragment of step c; those of A are zero behind a stage's end, where K ends in it
+    // (and B's are others of the row)
+    const auto read = [&](uint32_t c, uint32_t i, bool behind) MX_INLINE {
         const uint32_t row = i < kTM ? a_at + i * kMF : b_at + (i - kTM) * kMF;
         part[c % 2u][i] = ring[slot * S::kSlot + row * 8u + ((64u / kMF * c + q) ^ swizzle)];
+        if (!kWide && 2u * c >= S::kSteps && i < kTM && behind) part[c % 2u][i] = v4i{0, 0, 0, 0};
     };
     const auto read_factor = [&](uint32_t parity, uint32_t buffer, uint32_t i) MX_INLINE {
         const uint32_t row = i < kTM ? a_at + i * kMF : b_at + (i - kTM) * kMF;
@@ -567,18 +575,12 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     const auto shift_factor = [&](uint32_t buffer, uint32_t i) MX_INLINE {  // this lane's bytes to where the instruction takes them
         factor[buffer][i] = make_uint2(factor[buffer][i].x >> 8u * q, factor[buffer][i].y >> 8u * q);
     };
-    // The matrix instructions of step c (none where the stage ends in front of it), `ops`
-    // other operations among them from the first on
-    const auto multiply = [&](auto step, uint32_t buffer, bool live, auto ops, auto op) MX_INLINE {
+    // the matrix instructions of step c, `ops` other operations among them from the first on
+    const auto multiply = [&](auto step, uint32_t buffer, auto ops, auto op) MX_INLINE {
         constexpr uint32_t kC = decltype(step)::value, kOps = decltype(ops)::value, kAll = kTM * kTN;
         constexpr uint32_t kPer = (kOps + kAll - 1u) / kAll;
         constexpr int kByte = kMF == 32u ? 2 * (kC & 1u) : 0;
         constexpr bool kSecond = 2u * kC >= S::kSteps;  // of the stage's two scale words
-        if (!live) {
-#pragma unroll
-            for (uint32_t o = 0; o < kOps; ++o) op(o);
-            return;
-        }
 #pragma unroll
         for (uint32_t m = 0; m < kAll; ++m) {
             const uint32_t j = m / kTM, i = m % kTM;
@@ -605,11 +607,10 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         const auto step = [&](auto c) MX_INLINE {
             constexpr uint32_t kC = decltype(c)::value;
             constexpr uint32_t kLoads = kC == 0u ? kDataLoads - kEarly : 0u;
-            multiply(c, kParity, kWide || 2u * kC < S::kSteps || !half,
-                     std::integral_constant<uint32_t, kReads + kLoads>{}, [&](uint32_t o) {
-                         if (o < kReads) read(kC + 1u, o);
-                         else load_data(kEarly + o - kReads);
-                     });
+            multiply(c, kParity, std::integral_constant<uint32_t, kReads + kLoads>{}, [&](uint32_t o) MX_INLINE {
+                if (o < kReads) read(kC + 1u, o, half);
+                else load_data(kEarly + o - kReads);
+            });
             if constexpr (kC == 0u) load_next(!kWide || (kParity + S::kStages) % 2u == 0u);
         };
         step(std::integral_constant<uint32_t, 0>{});
@@ -623,10 +624,10 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         slot = slot + 1u == S::kStages ? 0u : slot + 1u;
         if (!kWide || kParity == 1u) scales = scales + 1u == kScaleSlots ? 0u : scales + 1u;
         constexpr uint32_t kScaleOps = kScalesNow ? kScaleLoads : 0u, kLoads = kScaleOps + kEarly;
-        multiply(std::integral_constant<uint32_t, S::kSteps - 1u>{}, kParity, kWide || !half,
-                 std::integral_constant<uint32_t, 3u * kReads + kLoads>{}, [&](uint32_t o) {
+        multiply(std::integral_constant<uint32_t, S::kSteps - 1u>{}, kParity,
+                 std::integral_constant<uint32_t, 3u * kReads + kLoads>{}, [&](uint32_t o) MX_INLINE {
                      if (o < kReads) read_factor(1u - kParity, 1u - kParity, o);
-                     else if (o < 2u * kReads) read(0u, o - kReads);
+                     else if (o < 2u * kReads) read(0u, o - kReads, false);
                      else if (o < 2u * kReads + kScaleOps) load_scale(o - 2u * kReads);
                      else if (o < 2u * kReads + kLoads) load_data(o - 2u * kReads - kScaleOps);
                      else shift_factor(1u - kParity, o - 2u * kReads - kLoads);
@@ -734,7 +735,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     mx_barrier<kFirst>();
 #pragma unroll
     for (uint32_t i = 0; i < kReads; ++i) {
-        read(0u, i);
+        read(0u, i, false);
         read_factor(0u, 0u, i);
     }
 #pragma unroll
@@ -760,10 +761,12 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     mx_barrier<0>();  // no load is under way to LDS that the next workgroup gets
 }
 
-using MxLarge = MxShape<32, 4, 2, 2, 4, 2>;   // 256 x 256
-using MxMiddle = MxShape<32, 2, 2, 2, 2, 2>;  // 128 x 128
-using MxSmall = MxShape<16, 2, 2, 2, 2, 3>;   // 64 x 64
-using MxFew = MxShape<16, 1, 4, 1, 2, 3>;    // 16 x 128
+using Mx256x256 = MxShape<32, 4, 2, 2, 4, 2>;
+using Mx128x128 = MxShape<32, 2, 2, 2, 2, 2>;
+using Mx64x64 = MxShape<16, 2, 2, 2, 2, 3>;
+using Mx32x128 = MxShape<16, 1, 4, 2, 2, 3>;
+using Mx16x128 = MxShape<16, 1, 4, 1, 2, 3>;
+using Mx16x64 = MxShape<16, 1, 2, 1, 2, 4>;
 
 }  // namespace
 
@@ -801,46 +804,93 @@ uint64_t mx_tiles(const MxProduct& p, bool swiglu) {
     return rows * ((n_out + across - 1u) / across);
 }
 
+// What a stage of all tiles takes, us: `each` for every 256 tiles.  An expert's last row
+// tile is taken to be half full.
+template <typename S>
+float stage_us(const MxProduct& p, bool swiglu, float each) {
+    const uint32_t across = swiglu ? S::kBN / 2u : S::kBN, n_out = swiglu ? p.n / 2u : p.n;
+    float rows = static_cast<float>((p.routes + S::kBM - 1u) / S::kBM);
+    if (p.offsets) {
+        const float active = static_cast<float>(p.routes < p.experts ? p.routes : p.experts);
+        const float of_each = static_cast<float>(p.routes) / active / S::kBM + 0.5f;
+        rows = active * (of_each > 1.0f ? of_each : 1.0f);
+    }
+    const float tiles = rows * static_cast<float>((n_out + across - 1u) / across);
+    return each * std::ceil(tiles / 256.0f);
+}
+
+// a row's scales of two stages are one 16-byte piece
+bool mx_wide(const MxProduct& p) {
+    return p.k128 % 4u == 0u && reinterpret_cast<uintptr_t>(p.a_scales) % 16u == 0u &&
+           reinterpret_cast<uintptr_t>(p.b_scales) % 16u == 0u;
+}
+
 template <typename S, bool kExperts, bool kSwiglu>
 hipError_t launch_tiles(const MxProduct& p, hipStream_t stream) {
     const uint64_t tiles = (mx_tiles<S>(p, kSwiglu) + kXcds - 1u) / kXcds * kXcds;
     const uint32_t grid = tiles < S::kResident * kCus ? static_cast<uint32_t>(tiles) : S::kResident * kCus;
-    const bool wide = p.k128 % 4u == 0u && reinterpret_cast<uintptr_t>(p.a_scales) % 16u == 0u &&
-                      reinterpret_cast<uintptr_t>(p.b_scales) % 16u == 0u;
-    if (wide) mx_tile_kernel<S, kExperts, kSwiglu, true><<<grid, 64u * S::kWaves, 0, stream>>>(p);
-    else mx_tile_kernel<S, kExperts, kSwiglu, false><<<grid, 64u * S::kWaves, 0, stream>>>(p);
+    if constexpr (!std::is_same_v<S, Mx256x256>) {
+        if (!mx_wide(p)) {
+            mx_tile_kernel<S, kExperts, kSwiglu, false><<<grid, 64u * S::kWaves, 0, stream>>>(p);
+            return hipGetLastError();
+        }
+    }
+    mx_tile_kernel<S, kExperts, kSwiglu, true><<<grid, 64u * S::kWaves, 0, stream>>>(p);
     return hipGetLastError();
 }
 
-// the tile of a product: rows of an expert on average (of C without experts)
-enum class MxTiles { kLarge, kMiddle, kSmall, kFew };
-MxTiles choose_tiles(const MxProduct& p, bool swiglu) {
-    const uint32_t rows = p.offsets ? p.routes / (p.routes < p.experts ? p.routes : p.experts) : p.routes;
-    if (rows <= 16u) return MxTiles::kFew;
-    if (mx_tiles<MxLarge>(p, swiglu) >= 256u && rows >= 512u && !p.offsets) return MxTiles::kLarge;
-    if (mx_tiles<MxMiddle>(p, swiglu) >= 256u && rows >= 96u) return MxTiles::kMiddle;
-    return MxTiles::kSmall;
-}
-
+// Calls f with the shape that a product runs on, the one with the shortest stage.  The
+// figures of `each` are fitted to these, us on 16 x 64, 16 x 128, 32 x 128, 64 x 64, 128 x
+// 128 and 256 x 256 tiles:
+//   1 x 8,192 x 2,048        4.6   5.2     -   5.4     -     -
+//   32 x 4,096 x 4,096         -   7.4   7.9   7.8    11    22
+//   256 x 4,096 x 4,096        -  13.1   9.4   8.9    13    25
+//   509 x 2,048 x 8,192        -    23    16    14    22    44
+//   1,024 x 4,096 x 4,096      -    41    25    21    17    28
+//   4,096 x 4,096 x 4,096      -     -     -     -    49    42
+//   8,192 x 8,192 x 8,192      -     -     -     -   378   301
+// and gate/up (1,024 x 2,048) of 512 experts, top-10, by tokens:
+//   1                        7.1   8.6     -   7.3     -     -
+//   64                        72    72     -    78     -     -
+//   512                      110   106     -   122     -     -
+//   1,024                      -   131   113   128   125   163
+//   2,048                      -   170   143   137   133   174
+//   4,096                      -   267   191   203   144   179
+//   8,192                      -   447   313   287   223   193
+//   32,768                     -     -     -     -   576   520
+// 256 x 256 tiles are for mx_wide products alone: without it they need registers that
+// their waves do not have.
 template <typename F>
-auto with_tiles(MxTiles tiles, F f) {
-    switch (tiles) {
-        case MxTiles::kLarge: return f(MxLarge{});
-        case MxTiles::kMiddle: return f(MxMiddle{});
-        case MxTiles::kSmall: return f(MxSmall{});
-        default: return f(MxFew{});
+auto with_tiles(const MxProduct& p, bool swiglu, F f) {
+    const float us[] = {stage_us<Mx16x64>(p, swiglu, 0.2f),   stage_us<Mx16x128>(p, swiglu, 0.33f),
+                        stage_us<Mx32x128>(p, swiglu, 0.45f), stage_us<Mx64x64>(p, swiglu, 0.38f),
+                        stage_us<Mx128x128>(p, swiglu, 0.66f),
+                        stage_us<Mx256x256>(p, swiglu, mx_wide(p) ? 2.0f : 1e30f)};
+    switch (std::min_element(std::begin(us), std::end(us)) - us) {
+        case 0: return f(Mx16x64{});
+        case 1: return f(Mx16x128{});
+        case 2: return f(Mx32x128{});
+        case 3: return f(Mx64x64{});
+        case 4: return f(Mx128x128{});
+        default: return f(Mx256x256{});
     }
 }
 
 }  // namespace
 
 bool mx_product_fits(const MxProduct& p, bool swiglu) {
-    return with_tiles(choose_tiles(p, swiglu),
-                      [&](auto s) { return mx_tiles<decltype(s)>(p, swiglu) < (1ull << 32); });
+    // tiles and their places are 32-bit numbers, and so are a tile's offsets: rows of C and
+    // of an expert, a row's bytes (a tile's 256 rows of them below 2^32) and, gathered, all
+    // of A's
+    const uint64_t row_bytes = static_cast<uint64_t>(p.k128) * 64u;
+    const uint64_t b_rows = swiglu ? p.n : 256u, a_rows = p.packed ? p.a_rows : 256u;
+    return p.n <= (1u << 28) && p.routes <= (1u << 28) && b_rows * row_bytes < (1ull << 32) &&
+           a_rows * row_bytes < (1ull << 32) &&
+           with_tiles(p, swiglu, [&](auto s) { return mx_tiles<decltype(s)>(p, swiglu) < (1ull << 31); });
 }
 
 hipError_t launch_mx_product(const MxProduct& p, bool swiglu, hipStream_t stream) {
-    return with_tiles(choose_tiles(p, swiglu), [&](auto s) {
+    return with_tiles(p, swiglu, [&](auto s) {
         using S = decltype(s);
         if (!p.offsets) return launch_tiles<S, false, false>(p, stream);
         return swiglu ? launch_tiles<S, true, true>(p, stream) : launch_tiles<S, true, false>(p, stream);

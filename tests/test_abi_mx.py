@@ -88,6 +88,10 @@ def test_grouped_refusals(q38m):
     call(f32=None)
     call(bf16=P)
     call(f32=P + 1)
+    # gathered rows, or one expert's, of 4 GB and more
+    call(w=matrix(q38m, experts=3, columns=2048), rows=matrix(q38m, rows=1 << 22, columns=2048))
+    call(w=matrix(q38m, experts=3, rows=1 << 22, columns=2048), rows=matrix(q38m, columns=2048),
+         epilogue=q38m.MX_EPILOGUE_SWIGLU)
 
 
 def test_sort_refusals(q38m):

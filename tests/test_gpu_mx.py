@@ -181,7 +181,9 @@ SHAPES = [(1, 1, 1), (1, 16, 128), (1, 17, 33), (2, 100, 64), (3, 5, 2048), (7, 
           (16, 64, 640), (17, 16, 128), (31, 33, 500), (32, 256, 2048), (33, 65, 129),
           (64, 64, 384), (65, 200, 1111), (100, 300, 256), (128, 128, 512), (129, 127, 4096),
           (200, 513, 896), (255, 257, 130), (256, 256, 1024), (300, 520, 768), (513, 1024, 2048),
-          (1, 8192, 256), (700, 1, 384), (1, 512, 8192), (4, 2048, 1920)]
+          (1, 8192, 256), (700, 1, 384), (1, 512, 8192), (4, 2048, 1920),
+          # whole rounds of the larger tiles, with and without an edge
+          (1030, 4090, 300), (1024, 2050, 1024), (4096, 4096, 512), (4100, 4090, 384), (5000, 4444, 130)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -265,7 +267,9 @@ def want_experts(w_values, rows, offsets, packed, top_k, experts, k, swiglu):
     (1, 1, 1, 2, 1, "even"), (1, 10, 512, 64, 256, "even"), (3, 2, 5, 34, 100, "dropped"),
     (17, 4, 8, 96, 640, "skewed"), (40, 10, 60, 130, 129, "dropped"), (33, 3, 7, 64, 512, "one"),
     (64, 10, 512, 32, 128, "even"), (150, 2, 4, 256, 384, "skewed"), (20, 1, 1024, 18, 64, "even"),
-    (300, 8, 16, 192, 256, "dropped"), (9, 2, 3, 48, 96, "none"), (513, 1, 2, 260, 1280, "even")])
+    (300, 8, 16, 192, 256, "dropped"), (9, 2, 3, 48, 96, "none"), (513, 1, 2, 260, 1280, "even"),
+    # many rows an expert: the larger tiles
+    (700, 4, 12, 512, 512, "skewed"), (2400, 8, 8, 2048, 128, "dropped"), (1500, 8, 7, 1030, 640, "even")])
 def test_experts(q38m, swiglu, dtype, tokens, top_k, experts, n, k, kind):
     print(f"experts {tokens} x {top_k} of {experts}, {n} x {k} {kind} swiglu {swiglu} {dtype}", flush=True)
     rng = np.random.default_rng(tokens * 31 + experts)
