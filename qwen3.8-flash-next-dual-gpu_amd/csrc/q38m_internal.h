@@ -247,7 +247,7 @@ constexpr uint32_t sort_chunks(uint32_t routes) { return (routes + kSortChunk - 
 // scratch: sort_scratch_words(routes, experts) words
 constexpr size_t sort_scratch_words(uint32_t routes, uint32_t experts) {
     return routes <= kSortSmallRoutes ? 0u
-                                      : static_cast<size_t>(sort_chunks(routes)) * (experts + 1u);
+                                      : (sort_chunks(routes) + 1u) * static_cast<size_t>(experts + 1u);
 }
 hipError_t launch_sort_routes(const int32_t* ids, uint32_t routes, uint32_t experts,
                               uint32_t* offsets, uint32_t* packed, uint32_t* inverse,

@@ -54,33 +54,54 @@ __device__ uint32_t group_exclusive_sum(uint32_t v, uint32_t* wave_sums) {
     return base + sum - v;
 }
 
-// Scatters one wave's routes [first, last), in order: a route's place is its
-// key's next one in `place` (this wave's row), advanced as the wave goes.
-__device__ __forceinline__ void scatter_routes(const int32_t* __restrict__ ids, uint32_t first,
-                                               uint32_t last, uint32_t experts, uint32_t* place,
-                                               uint32_t* __restrict__ packed,
-                                               uint32_t* __restrict__ inverse) {
-    const uint32_t lane = threadIdx.x & 63u;
-    for (uint32_t r0 = first; r0 < last; r0 += 64u) {
-        const uint32_t r = r0 + lane;
-        const bool live = r < last;
-        const uint32_t key = live ? route_key(ids[r], experts) : experts;
-        const uint64_t same = equal_lanes<kKeyBits>(key, live);
-        const uint32_t below = __popcll(same & ((1ull << lane) - 1u));
-        if (live) {
-            const uint32_t at = place[key] + below;
-            packed[at] = r;
-            inverse[r] = key < experts ? at : Q38M_ROUTE_DROPPED;
-        }
-        // every lane has read its place before the last of each key moves it on
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (live && (same >> lane) == 1u) place[key] += below + 1u;
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    }
-}
+// One wave's routes, kSteps times 64 from `first` up to `last`, in registers.
+template <uint32_t kSteps>
+struct WaveRoutes {
+    uint32_t key[kSteps], first, last;
 
-// One workgroup sorts everything: each wave counts its own contiguous routes,
-// the counts become places by a sum over the waves of a key and over the keys.
+    __device__ WaveRoutes(const int32_t* __restrict__ ids, uint32_t first_, uint32_t last_,
+                          uint32_t experts)
+        : first(first_), last(last_) {
+        int32_t id[kSteps];  // all loads under way at once
+#pragma unroll
+        for (uint32_t s = 0; s < kSteps; ++s) id[s] = live(s) ? ids[route(s)] : -1;
+#pragma unroll
+        for (uint32_t s = 0; s < kSteps; ++s) key[s] = route_key(id[s], experts);
+    }
+    __device__ uint32_t route(uint32_t s) const { return first + 64u * s + (threadIdx.x & 63u); }
+    __device__ bool live(uint32_t s) const { return route(s) < last; }
+
+    __device__ void count(uint32_t* counts) const {
+#pragma unroll
+        for (uint32_t s = 0; s < kSteps; ++s)
+            if (live(s)) atomicAdd(&counts[key[s]], 1u);
+    }
+    // a route's place is its key's next one in `place` (this wave's), advanced as the wave goes
+    __device__ void scatter(uint32_t experts, uint32_t* place, uint32_t* __restrict__ packed,
+                            uint32_t* __restrict__ inverse) const {
+        const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+        for (uint32_t s = 0; s < kSteps; ++s) {
+            if (first + 64u * s >= last) break;
+            const uint64_t same = equal_lanes<kKeyBits>(key[s], live(s));
+            const uint32_t below = __popcll(same & ((1ull << lane) - 1u));
+            if (live(s)) {
+                const uint32_t at = place[key[s]] + below;
+                packed[at] = route(s);
+                inverse[route(s)] = key[s] < experts ? at : Q38M_ROUTE_DROPPED;
+            }
+            // every lane has read its place before the last of each key moves it on
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            if (live(s) && (same >> lane) == 1u) place[key[s]] += below + 1u;
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+    }
+};
+
+// One workgroup sorts everything: each wave counts its own contiguous routes, the counts
+// become places by a sum over the waves of a key and over the keys.  What takes its time
+// is latency: ids read, LDS counters, the sums, writes (512 tokens, top-10: 9.9 us with
+// the ids read again for every step; see the table of cases).
 constexpr uint32_t kSmallWaves = 16;
 __global__ __launch_bounds__(kSmallWaves * 64) void sort_small_kernel(
     const int32_t* __restrict__ ids, uint32_t routes, uint32_t experts,
@@ -90,28 +111,31 @@ __global__ __launch_bounds__(kSmallWaves * 64) void sort_small_kernel(
     __shared__ uint32_t sums[kSmallWaves];
     const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
     const uint32_t per = (routes + kSmallWaves * 64u - 1u) / (kSmallWaves * 64u) * 64u;
-    const uint32_t first = min(wave * per, routes), last = min(first + per, routes);
+    const uint32_t first = min(wave * per, routes);
+    const WaveRoutes<kSortSmallRoutes / (kSmallWaves * 64u)> mine(ids, first, min(first + per, routes), experts);
     for (uint32_t k = lane; k <= experts; k += 64u) place[wave][k] = 0u;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    for (uint32_t r = first + lane; r < last; r += 64u)
-        atomicAdd(&place[wave][route_key(ids[r], experts)], 1u);
+    mine.count(place[wave]);
     __syncthreads();
-    // thread t owns key t; key kMaxSortExperts (dropped, all experts in use)
-    // is placed behind the rest by thread 0 below
-    uint32_t total = 0;
-    if (t <= experts)
-        for (uint32_t w = 0; w < kSmallWaves; ++w) total += place[w][t];
+    // thread t owns key t; where all 1,024 experts are in use the last thread also owns
+    // the key of the dropped routes
+    uint32_t count[kSmallWaves], total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kSmallWaves; ++w) {
+        count[w] = t <= experts ? place[w][t] : 0u;
+        total += count[w];
+    }
     uint32_t base = group_exclusive_sum<kSmallWaves>(total, sums);
     if (t <= experts) {
         offsets[t] = base;
+#pragma unroll
         for (uint32_t w = 0; w < kSmallWaves; ++w) {
-            const uint32_t n = place[w][t];
             place[w][t] = base;
-            base += n;
+            base += count[w];
         }
     }
     if (t == kMaxSortExperts - 1u && experts == kMaxSortExperts) {
-        offsets[experts] = base;  // the last expert's end
+        offsets[experts] = base;
         for (uint32_t w = 0; w < kSmallWaves; ++w) {
             const uint32_t n = place[w][experts];
             place[w][experts] = base;
@@ -119,75 +143,100 @@ __global__ __launch_bounds__(kSmallWaves * 64) void sort_small_kernel(
         }
     }
     __syncthreads();
-    scatter_routes(ids, first, last, experts, place[wave], packed, inverse);
+    mine.scatter(experts, place[wave], packed, inverse);
 }
 
-// The same in three launches over chunks of routes.
-constexpr uint32_t kChunkWaves = 4;
+// The same in three launches over chunks of routes: the chunks' counts; each key's
+// counts summed over the chunks in front; the scatter, which sums the keys' totals.
+constexpr uint32_t kChunkWaves = 4, kChunkSteps = kSortChunk / (kChunkWaves * 64u);
 __global__ __launch_bounds__(kChunkWaves * 64) void sort_count_kernel(
     const int32_t* __restrict__ ids, uint32_t routes, uint32_t experts,
     uint32_t* __restrict__ counts) {
     __shared__ uint32_t count[kKeys];
+    const uint32_t first = blockIdx.x * kSortChunk + (threadIdx.x >> 6) * (kChunkSteps * 64u);
+    const WaveRoutes<kChunkSteps> mine(ids, first, min(first + kChunkSteps * 64u, routes), experts);
     for (uint32_t k = threadIdx.x; k <= experts; k += kChunkWaves * 64u) count[k] = 0u;
     __syncthreads();
-    const uint32_t first = blockIdx.x * kSortChunk, last = min(first + kSortChunk, routes);
-    for (uint32_t r = first + threadIdx.x; r < last; r += kChunkWaves * 64u)
-        atomicAdd(&count[route_key(ids[r], experts)], 1u);
+    mine.count(count);
     __syncthreads();
     uint32_t* out = counts + static_cast<size_t>(blockIdx.x) * (experts + 1u);
     for (uint32_t k = threadIdx.x; k <= experts; k += kChunkWaves * 64u) out[k] = count[k];
 }
 
-// counts[chunk][key] -> the place of the chunk's first route of the key
-__global__ __launch_bounds__(1024) void sort_place_kernel(uint32_t* __restrict__ counts,
-                                                          uint32_t chunks, uint32_t experts,
-                                                          uint32_t* __restrict__ offsets) {
-    __shared__ uint32_t sums[16];
-    const uint32_t t = threadIdx.x, stride = experts + 1u;
-    const bool mine = t <= experts;
+// counts[chunk][key] -> how many of the key lie in the chunks in front; totals[key].  A
+// workgroup has 64 keys, a lane each, and its waves a run of chunks each.  (All keys in one
+// workgroup, one chunk after the other: 110 us for 327,680 routes.)
+constexpr uint32_t kPlaceWaves = 16;
+__global__ __launch_bounds__(kPlaceWaves * 64) void sort_place_kernel(
+    uint32_t* __restrict__ counts, uint32_t chunks, uint32_t experts, uint32_t* __restrict__ totals) {
+    __shared__ uint32_t sums[kPlaceWaves][64];
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+    const uint32_t key = blockIdx.x * 64u + lane, stride = experts + 1u;
+    const bool mine = key <= experts;
+    const uint32_t per = (chunks + kPlaceWaves - 1u) / kPlaceWaves;
+    const uint32_t first = min(wave * per, chunks), last = min(first + per, chunks);
     uint32_t total = 0;
-    if (mine)
-        for (uint32_t c = 0; c < chunks; ++c) total += counts[static_cast<size_t>(c) * stride + t];
-    uint32_t base = group_exclusive_sum<16>(total, sums);
-    // with all 1,024 experts in use the last thread places the dropped ones too
-    const uint32_t keys = t == kMaxSortExperts - 1u && experts == kMaxSortExperts ? 2u : 1u;
+#pragma unroll 8
+    for (uint32_t c = first; c < last; ++c) total += mine ? counts[static_cast<size_t>(c) * stride + key] : 0u;
+    sums[wave][lane] = total;
+    __syncthreads();
+    uint32_t base = 0;
+    for (uint32_t w = 0; w < wave; ++w) base += sums[w][lane];
     if (!mine) return;
-    for (uint32_t k = t; k < t + keys; ++k) {
-        offsets[k] = base;
-        for (uint32_t c = 0; c < chunks; ++c) {
-            uint32_t* at = &counts[static_cast<size_t>(c) * stride + k];
-            const uint32_t n = *at;
-            *at = base;
-            base += n;
+    if (wave == kPlaceWaves - 1u) totals[key] = base + total;
+    for (uint32_t c0 = first; c0 < last; c0 += 8u) {  // eight loads under way at once
+        uint32_t n[8];
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i)
+            n[i] = c0 + i < last ? counts[static_cast<size_t>(c0 + i) * stride + key] : 0u;
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) {
+            if (c0 + i < last) counts[static_cast<size_t>(c0 + i) * stride + key] = base;
+            base += n[i];
         }
     }
 }
 
 __global__ __launch_bounds__(kChunkWaves * 64) void sort_scatter_kernel(
     const int32_t* __restrict__ ids, uint32_t routes, uint32_t experts,
-    const uint32_t* __restrict__ places, uint32_t* __restrict__ packed,
-    uint32_t* __restrict__ inverse) {
+    const uint32_t* __restrict__ counts, const uint32_t* __restrict__ totals,
+    uint32_t* __restrict__ offsets, uint32_t* __restrict__ packed, uint32_t* __restrict__ inverse) {
     __shared__ uint32_t place[kChunkWaves][kKeys];
+    __shared__ uint32_t sums[kChunkWaves];
     const uint32_t t = threadIdx.x, lane = t & 63u, wave = t >> 6;
-    constexpr uint32_t per = kSortChunk / kChunkWaves;
-    const uint32_t begin = blockIdx.x * kSortChunk;
-    const uint32_t first = min(begin + wave * per, routes), last = min(first + per, routes);
+    const uint32_t first = blockIdx.x * kSortChunk + wave * (kChunkSteps * 64u);
+    const WaveRoutes<kChunkSteps> mine(ids, first, min(first + kChunkSteps * 64u, routes), experts);
     for (uint32_t k = lane; k <= experts; k += 64u) place[wave][k] = 0u;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    for (uint32_t r = first + lane; r < last; r += 64u)
-        atomicAdd(&place[wave][route_key(ids[r], experts)], 1u);
-    __syncthreads();
-    const uint32_t* from = places + static_cast<size_t>(blockIdx.x) * (experts + 1u);
-    for (uint32_t k = t; k <= experts; k += kChunkWaves * 64u) {
-        uint32_t base = from[k];
+    mine.count(place[wave]);
+    // thread t owns kOwn consecutive keys, which covers all
+    constexpr uint32_t kThreads = kChunkWaves * 64u, kOwn = (kKeys + kThreads - 1u) / kThreads;
+    const uint32_t* in_front = counts + static_cast<size_t>(blockIdx.x) * (experts + 1u);
+    uint32_t total[kOwn], front[kOwn], all = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < kOwn; ++i) {
+        const uint32_t k = t * kOwn + i;
+        total[i] = k <= experts ? totals[k] : 0u;
+        front[i] = k <= experts ? in_front[k] : 0u;
+        all += total[i];
+    }
+    uint32_t base = group_exclusive_sum<kChunkWaves>(all, sums);  // and the waves' counts are there
+#pragma unroll
+    for (uint32_t i = 0; i < kOwn; ++i) {
+        const uint32_t k = t * kOwn + i;
+        if (k > experts) break;
+        if (blockIdx.x == 0u) offsets[k] = base;
+        uint32_t at = base + front[i];
+#pragma unroll
         for (uint32_t w = 0; w < kChunkWaves; ++w) {
             const uint32_t n = place[w][k];
-            place[w][k] = base;
-            base += n;
+            place[w][k] = at;
+            at += n;
         }
+        base += total[i];
     }
     __syncthreads();
-    scatter_routes(ids, first, last, experts, place[wave], packed, inverse);
+    mine.scatter(experts, place[wave], packed, inverse);
 }
 
 // ---- rows -------------------------------------------------------------------
@@ -199,15 +248,24 @@ struct Piece;
 
 template <uint32_t kN>
 struct Piece<float, kN> {
-    __device__ static void load(const float* p, float* v) {
+    struct Raw {
+        float v[kN];
+    };
+    __device__ static Raw get(const float* p) {
+        Raw r;
         if constexpr (kN == 8u) {
             const float4 a = reinterpret_cast<const float4*>(p)[0];
             const float4 b = reinterpret_cast<const float4*>(p)[1];
-            v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-            v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+            r.v[0] = a.x; r.v[1] = a.y; r.v[2] = a.z; r.v[3] = a.w;
+            r.v[4] = b.x; r.v[5] = b.y; r.v[6] = b.z; r.v[7] = b.w;
         } else {
-            v[0] = *p;
+            r.v[0] = *p;
         }
+        return r;
+    }
+    __device__ static void widen(const Raw& r, float* v) {
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i) v[i] = r.v[i];
     }
     __device__ static void store(float* p, const float* v) {
         if constexpr (kN == 8u) {
@@ -221,18 +279,23 @@ struct Piece<float, kN> {
 
 template <uint32_t kN>
 struct Piece<uint16_t, kN> {
-    __device__ static void load(const uint16_t* p, float* v) {
+    struct Raw {
+        uint32_t d[(kN + 1u) / 2u];
+    };
+    __device__ static Raw get(const uint16_t* p) {
+        Raw r;
         if constexpr (kN == 8u) {
             const uint4 w = *reinterpret_cast<const uint4*>(p);
-            const uint32_t d[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (uint32_t i = 0; i < 4u; ++i) {
-                v[2 * i] = __uint_as_float(d[i] << 16);
-                v[2 * i + 1] = __uint_as_float(d[i] & 0xffff0000u);
-            }
+            r.d[0] = w.x; r.d[1] = w.y; r.d[2] = w.z; r.d[3] = w.w;
         } else {
-            v[0] = bf16_to_f32(*p);
+            r.d[0] = *p;
         }
+        return r;
+    }
+    __device__ static void widen(const Raw& r, float* v) {
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i)
+            v[i] = __uint_as_float(i % 2u ? r.d[i / 2u] & 0xffff0000u : r.d[i / 2u] << 16);
     }
     __device__ static void store(uint16_t* p, const float* v) {
         if constexpr (kN == 8u) {
@@ -246,6 +309,11 @@ struct Piece<uint16_t, kN> {
         }
     }
 };
+
+template <typename T, uint32_t kN>
+__device__ __forceinline__ void load_piece(const T* p, float* v) {
+    Piece<T, kN>::widen(Piece<T, kN>::get(p), v);
+}
 
 constexpr uint32_t kRowThreads = 256;
 
@@ -272,33 +340,53 @@ __global__ __launch_bounds__(kRowThreads) void permute_kernel(
     const uint32_t* at = inverse + static_cast<size_t>(p.token) * top_k;
     for (uint32_t c = p.column; c < width; c += p.step) {
         float v[kN];
-        Piece<T, kN>::load(x + static_cast<size_t>(p.token) * width + c, v);
+        load_piece<T, kN>(x + static_cast<size_t>(p.token) * width + c, v);
         for (uint32_t r = 0; r < top_k; ++r)
             if (at[r] < routes)
                 Piece<T, kN>::store(rows + static_cast<size_t>(at[r]) * width + c, v);
     }
 }
 
-// y[t] = sum over t's kept routes, in rank order, of weight * row
+// y[t] = sum over t's kept routes, in rank order, of weight * row.  The rows of kRanks
+// routes are under way at once.
 template <typename T, uint32_t kN>
 __global__ __launch_bounds__(kRowThreads) void unpermute_kernel(
     const T* __restrict__ rows, const uint32_t* __restrict__ inverse,
     const float* __restrict__ weights, uint32_t tokens, uint32_t top_k, uint32_t width,
     uint32_t lanes_log2, T* __restrict__ y) {
+    constexpr uint32_t kRanks = sizeof(T) == 2u ? 16u : 8u;
     const RowPlace p = row_place<kN>(lanes_log2);
     if (p.token >= tokens) return;
     const uint32_t routes = tokens * top_k;
     const size_t first = static_cast<size_t>(p.token) * top_k;
     for (uint32_t c = p.column; c < width; c += p.step) {
         float sum[kN] = {};
-        for (uint32_t r = 0; r < top_k; ++r) {
-            const uint32_t at = inverse[first + r];
-            if (at >= routes) continue;
-            const float w = weights ? weights[first + r] : 1.0f;
-            float v[kN];
-            Piece<T, kN>::load(rows + static_cast<size_t>(at) * width + c, v);
+        for (uint32_t r0 = 0; r0 < top_k; r0 += kRanks) {
+            uint32_t at[kRanks];
+            float w[kRanks];
 #pragma unroll
-            for (uint32_t i = 0; i < kN; ++i) sum[i] = __builtin_fmaf(w, v[i], sum[i]);
+            for (uint32_t i = 0; i < kRanks; ++i) {
+                at[i] = Q38M_ROUTE_DROPPED;
+                w[i] = 1.0f;
+                if (r0 + i < top_k) {
+                    at[i] = inverse[first + r0 + i];
+                    if (weights) w[i] = weights[first + r0 + i];
+                }
+            }
+            typename Piece<T, kN>::Raw raw[kRanks];
+#pragma unroll
+            for (uint32_t i = 0; i < kRanks; ++i) {
+                raw[i] = typename Piece<T, kN>::Raw{};
+                if (at[i] < routes) raw[i] = Piece<T, kN>::get(rows + static_cast<size_t>(at[i]) * width + c);
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < kRanks; ++i) {
+                if (at[i] >= routes) w[i] = 0.0f;  // of a row of zeros
+                float v[kN];
+                Piece<T, kN>::widen(raw[i], v);
+#pragma unroll
+                for (uint32_t j = 0; j < kN; ++j) sum[j] = __builtin_fmaf(w[i], v[j], sum[j]);
+            }
         }
         Piece<T, kN>::store(y + static_cast<size_t>(p.token) * width + c, sum);
     }
@@ -321,9 +409,9 @@ __global__ __launch_bounds__(kRowThreads) void unpermute_backward_kernel(
         const size_t row = static_cast<size_t>(at) * width;
         for (uint32_t c = lane * kN; c < width; c += 64u * kN) {
             float g[kN], v[kN];
-            Piece<T, kN>::load(from + c, g);
+            load_piece<T, kN>(from + c, g);
             if (d_weights) {
-                Piece<T, kN>::load(rows + row + c, v);
+                load_piece<T, kN>(rows + row + c, v);
 #pragma unroll
                 for (uint32_t i = 0; i < kN; ++i) dot = __builtin_fmaf(g[i], v[i], dot);
             }
@@ -415,10 +503,11 @@ hipError_t launch_sort_routes(const int32_t* ids, uint32_t routes, uint32_t expe
         return hipGetLastError();
     }
     const uint32_t chunks = sort_chunks(routes);
+    uint32_t* totals = scratch + static_cast<size_t>(chunks) * (experts + 1u);
     sort_count_kernel<<<chunks, kChunkWaves * 64u, 0, stream>>>(ids, routes, experts, scratch);
-    sort_place_kernel<<<1, 1024, 0, stream>>>(scratch, chunks, experts, offsets);
-    sort_scatter_kernel<<<chunks, kChunkWaves * 64u, 0, stream>>>(ids, routes, experts, scratch,
-                                                                  packed, inverse);
+    sort_place_kernel<<<(experts + 64u) / 64u, kPlaceWaves * 64u, 0, stream>>>(scratch, chunks, experts, totals);
+    sort_scatter_kernel<<<chunks, kChunkWaves * 64u, 0, stream>>>(ids, routes, experts, scratch, totals,
+                                                                  offsets, packed, inverse);
     return hipGetLastError();
 }
 
