@@ -241,79 +241,75 @@ __global__ __launch_bounds__(kChunkWaves * 64) void sort_scatter_kernel(
 
 // ---- rows -------------------------------------------------------------------
 
-// kN consecutive values of a row as fp32, and back (one rounding).  kN = 8 is
-// 16-byte aligned; kN = 1 takes any row.
+// 16 bytes, kStream: past the caches
+template <bool kStream>
+__device__ __forceinline__ uint4 get16(const void* p) {
+    if constexpr (kStream) return load_stream(static_cast<const uint4*>(p));
+    else return *static_cast<const uint4*>(p);
+}
+template <bool kStream>
+__device__ __forceinline__ void put16(void* p, uint4 w) {
+    if constexpr (kStream) {
+        const v4u_t v = {w.x, w.y, w.z, w.w};
+        __builtin_nontemporal_store(v, static_cast<v4u_t*>(p));
+    } else {
+        *static_cast<uint4*>(p) = w;
+    }
+}
+
+// kN consecutive values of a row, and as fp32 (back: one rounding).  kN = 8 is 16-byte
+// aligned; kN = 1 takes any row.
 template <typename T, uint32_t kN>
-struct Piece;
+struct Piece {
+    static constexpr uint32_t kWords = (kN * sizeof(T) + 3u) / 4u;
+    uint32_t d[kWords];
 
-template <uint32_t kN>
-struct Piece<float, kN> {
-    struct Raw {
-        float v[kN];
-    };
-    __device__ static Raw get(const float* p) {
-        Raw r;
+    template <bool kStream>
+    __device__ static Piece get(const T* p) {
+        Piece r;
         if constexpr (kN == 8u) {
-            const float4 a = reinterpret_cast<const float4*>(p)[0];
-            const float4 b = reinterpret_cast<const float4*>(p)[1];
-            r.v[0] = a.x; r.v[1] = a.y; r.v[2] = a.z; r.v[3] = a.w;
-            r.v[4] = b.x; r.v[5] = b.y; r.v[6] = b.z; r.v[7] = b.w;
-        } else {
-            r.v[0] = *p;
-        }
-        return r;
-    }
-    __device__ static void widen(const Raw& r, float* v) {
 #pragma unroll
-        for (uint32_t i = 0; i < kN; ++i) v[i] = r.v[i];
-    }
-    __device__ static void store(float* p, const float* v) {
-        if constexpr (kN == 8u) {
-            reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-            reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-        } else {
-            *p = v[0];
-        }
-    }
-};
-
-template <uint32_t kN>
-struct Piece<uint16_t, kN> {
-    struct Raw {
-        uint32_t d[(kN + 1u) / 2u];
-    };
-    __device__ static Raw get(const uint16_t* p) {
-        Raw r;
-        if constexpr (kN == 8u) {
-            const uint4 w = *reinterpret_cast<const uint4*>(p);
-            r.d[0] = w.x; r.d[1] = w.y; r.d[2] = w.z; r.d[3] = w.w;
+            for (uint32_t i = 0; i < kWords; i += 4u) {
+                const uint4 w = get16<kStream>(p + i * 4u / sizeof(T));
+                r.d[i] = w.x, r.d[i + 1u] = w.y, r.d[i + 2u] = w.z, r.d[i + 3u] = w.w;
+            }
+        } else if constexpr (sizeof(T) == 4u) {
+            r.d[0] = __float_as_uint(*p);
         } else {
             r.d[0] = *p;
         }
         return r;
     }
-    __device__ static void widen(const Raw& r, float* v) {
-#pragma unroll
-        for (uint32_t i = 0; i < kN; ++i)
-            v[i] = __uint_as_float(i % 2u ? r.d[i / 2u] & 0xffff0000u : r.d[i / 2u] << 16);
-    }
-    __device__ static void store(uint16_t* p, const float* v) {
+    template <bool kStream>
+    __device__ void put(T* p) const {
         if constexpr (kN == 8u) {
-            uint32_t d[4];
 #pragma unroll
-            for (uint32_t i = 0; i < 4u; ++i)
-                d[i] = f32_to_bf16(v[2 * i]) | f32_to_bf16(v[2 * i + 1]) << 16;
-            *reinterpret_cast<uint4*>(p) = make_uint4(d[0], d[1], d[2], d[3]);
+            for (uint32_t i = 0; i < kWords; i += 4u)
+                put16<kStream>(p + i * 4u / sizeof(T), make_uint4(d[i], d[i + 1u], d[i + 2u], d[i + 3u]));
+        } else if constexpr (sizeof(T) == 4u) {
+            *p = __uint_as_float(d[0]);
         } else {
-            *p = static_cast<uint16_t>(f32_to_bf16(v[0]));
+            *p = static_cast<T>(d[0]);
         }
     }
+    __device__ void widen(float* v) const {
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i) {
+            if constexpr (sizeof(T) == 4u) v[i] = __uint_as_float(d[i]);
+            else v[i] = __uint_as_float(i % 2u ? d[i / 2u] & 0xffff0000u : d[i / 2u] << 16);
+        }
+    }
+    __device__ static Piece round(const float* v) {
+        Piece r;
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i) {
+            if constexpr (sizeof(T) == 4u) r.d[i] = __float_as_uint(v[i]);
+            else if (i % 2u) r.d[i / 2u] |= f32_to_bf16(v[i]) << 16;
+            else r.d[i / 2u] = f32_to_bf16(v[i]);
+        }
+        return r;
+    }
 };
-
-template <typename T, uint32_t kN>
-__device__ __forceinline__ void load_piece(const T* p, float* v) {
-    Piece<T, kN>::widen(Piece<T, kN>::get(p), v);
-}
 
 constexpr uint32_t kRowThreads = 256;
 
@@ -339,17 +335,17 @@ __global__ __launch_bounds__(kRowThreads) void permute_kernel(
     const uint32_t routes = tokens * top_k;
     const uint32_t* at = inverse + static_cast<size_t>(p.token) * top_k;
     for (uint32_t c = p.column; c < width; c += p.step) {
-        float v[kN];
-        load_piece<T, kN>(x + static_cast<size_t>(p.token) * width + c, v);
+        const auto v = Piece<T, kN>::template get<false>(x + static_cast<size_t>(p.token) * width + c);
         for (uint32_t r = 0; r < top_k; ++r)
-            if (at[r] < routes)
-                Piece<T, kN>::store(rows + static_cast<size_t>(at[r]) * width + c, v);
+            if (at[r] < routes) v.template put<false>(rows + static_cast<size_t>(at[r]) * width + c);
     }
 }
 
 // y[t] = sum over t's kept routes, in rank order, of weight * row.  The rows of kRanks
-// routes are under way at once.
-template <typename T, uint32_t kN>
+// routes are under way at once.  y goes past the caches, and the rows come past them where
+// they are more than the 256 MB behind the L2s hold: 1.3 GB of them cached / y past the
+// caches / both 325 / 265 / 239 us (6.2 TB/s), 21 MB of them 5.0 / 4.3 / 4.8.
+template <typename T, uint32_t kN, bool kStream>
 __global__ __launch_bounds__(kRowThreads) void unpermute_kernel(
     const T* __restrict__ rows, const uint32_t* __restrict__ inverse,
     const float* __restrict__ weights, uint32_t tokens, uint32_t top_k, uint32_t width,
@@ -373,22 +369,23 @@ __global__ __launch_bounds__(kRowThreads) void unpermute_kernel(
                     if (weights) w[i] = weights[first + r0 + i];
                 }
             }
-            typename Piece<T, kN>::Raw raw[kRanks];
+            Piece<T, kN> row[kRanks];
 #pragma unroll
             for (uint32_t i = 0; i < kRanks; ++i) {
-                raw[i] = typename Piece<T, kN>::Raw{};
-                if (at[i] < routes) raw[i] = Piece<T, kN>::get(rows + static_cast<size_t>(at[i]) * width + c);
+                row[i] = Piece<T, kN>{};
+                if (at[i] < routes)
+                    row[i] = Piece<T, kN>::template get<kStream>(rows + static_cast<size_t>(at[i]) * width + c);
             }
 #pragma unroll
             for (uint32_t i = 0; i < kRanks; ++i) {
                 if (at[i] >= routes) w[i] = 0.0f;  // of a row of zeros
                 float v[kN];
-                Piece<T, kN>::widen(raw[i], v);
+                row[i].widen(v);
 #pragma unroll
                 for (uint32_t j = 0; j < kN; ++j) sum[j] = __builtin_fmaf(w[i], v[j], sum[j]);
             }
         }
-        Piece<T, kN>::store(y + static_cast<size_t>(p.token) * width + c, sum);
+        Piece<T, kN>::round(sum).template put<true>(y + static_cast<size_t>(p.token) * width + c);
     }
 }
 
@@ -409,16 +406,16 @@ __global__ __launch_bounds__(kRowThreads) void unpermute_backward_kernel(
         const size_t row = static_cast<size_t>(at) * width;
         for (uint32_t c = lane * kN; c < width; c += 64u * kN) {
             float g[kN], v[kN];
-            load_piece<T, kN>(from + c, g);
+            Piece<T, kN>::template get<false>(from + c).widen(g);
             if (d_weights) {
-                load_piece<T, kN>(rows + row + c, v);
+                Piece<T, kN>::template get<false>(rows + row + c).widen(v);
 #pragma unroll
                 for (uint32_t i = 0; i < kN; ++i) dot = __builtin_fmaf(g[i], v[i], dot);
             }
             if (d_rows) {
 #pragma unroll
                 for (uint32_t i = 0; i < kN; ++i) g[i] *= w;
-                Piece<T, kN>::store(d_rows + row + c, g);
+                Piece<T, kN>::round(g).template put<false>(d_rows + row + c);
             }
         }
     }
@@ -462,19 +459,27 @@ hipError_t permute(const T* x, const uint32_t* inverse, uint32_t tokens, uint32_
     return hipGetLastError();
 }
 
+constexpr uint64_t kCachedBytes = 256u << 20;
+
+template <typename T, uint32_t kN>
+hipError_t unpermute(const T* rows, const uint32_t* inverse, const float* weights,
+                     uint32_t tokens, uint32_t top_k, uint32_t width, T* y, hipStream_t stream) {
+    const uint32_t lanes = row_lanes_log2(width, kN), grid = row_grid(tokens, lanes);
+    if (static_cast<uint64_t>(tokens) * top_k * width * sizeof(T) > kCachedBytes)
+        unpermute_kernel<T, kN, true><<<grid, kRowThreads, 0, stream>>>(
+            rows, inverse, weights, tokens, top_k, width, lanes, y);
+    else
+        unpermute_kernel<T, kN, false><<<grid, kRowThreads, 0, stream>>>(
+            rows, inverse, weights, tokens, top_k, width, lanes, y);
+    return hipGetLastError();
+}
+
 template <typename T>
 hipError_t unpermute(const T* rows, const uint32_t* inverse, const float* weights,
                      uint32_t tokens, uint32_t top_k, uint32_t width, T* y, hipStream_t stream) {
-    if (whole_pieces(width, {rows, y})) {
-        const uint32_t lanes = row_lanes_log2(width, 8u);
-        unpermute_kernel<T, 8><<<row_grid(tokens, lanes), kRowThreads, 0, stream>>>(
-            rows, inverse, weights, tokens, top_k, width, lanes, y);
-    } else {
-        const uint32_t lanes = row_lanes_log2(width, 1u);
-        unpermute_kernel<T, 1><<<row_grid(tokens, lanes), kRowThreads, 0, stream>>>(
-            rows, inverse, weights, tokens, top_k, width, lanes, y);
-    }
-    return hipGetLastError();
+    return whole_pieces(width, {rows, y})
+               ? unpermute<T, 8>(rows, inverse, weights, tokens, top_k, width, y, stream)
+               : unpermute<T, 1>(rows, inverse, weights, tokens, top_k, width, y, stream);
 }
 
 template <typename T>
