@@ -372,6 +372,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     __shared__ v4i ring[S::kLds];
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __builtin_assume(wave < S::kWaves);  // settles at compile time which loads are of A and which of B
     const uint32_t n_out = kSwiglu ? p.n / 2u : p.n;
     constexpr uint32_t kColumns = kSwiglu ? kBN / 2u : kBN;
     const uint32_t columns = (n_out + kColumns - 1u) / kColumns;
