@@ -598,7 +598,10 @@ int q38m_quantize_expert_weights(const uint16_t* src_bf16,
  * codes 16-byte, scales 4-byte aligned.  The products read no padding of
  * other lengths, and a matrix that another program quantised so (columns a
  * multiple of 128: plain row-major codes and scales) can be passed as it is;
- * padding codes that are not zero would count. */
+ * padding codes that are not zero would count.
+ *
+ * Here and in the sorted-row calls below, outputs overlap no input and no
+ * other output, and index and weight arrays are 4-byte aligned. */
 #define Q38M_MX_BLOCK 32u
 /* element types of the entry points that take several */
 #define Q38M_DTYPE_F32 1u

@@ -449,6 +449,16 @@ def repack(weights, paired=False, stream=None):
     return out
 
 
+def _require(holds, message):
+    if not holds:
+        raise InvalidArgument(message)
+
+
+def _stream_of(tensor, stream):
+    """The given stream, or the current one of the tensor's device."""
+    return stream if stream is not None else _torch().cuda.current_stream(tensor.device)
+
+
 class MxRows:
     """Microscaled 4-bit rows resident in device memory plus their descriptor."""
 
@@ -461,13 +471,25 @@ class MxRows:
 
 
 def mx_quantize(x, experts=1, rounded=None, stream=None):
-    """x [experts * rows][columns] (bf16, raw bf16 words or fp32; any row
-    stride) as MxRows."""
+    """x [experts * rows][columns] on a GPU (bf16, raw bf16 words in 16-bit integers, or fp32;
+    any row stride, columns side by side) as MxRows.  rounded: None, or a contiguous tensor like
+    x that gets the values the codes stand for."""
     torch = _torch()
-    out = MxRows(experts, x.shape[0] // experts, x.shape[1], x.device)
-    dtype = DTYPE_F32 if x.dtype == torch.float32 else DTYPE_BF16
-    call("q38m_mx_quantize_v1", ptr(x), dtype, x.stride(0), ctypes.byref(out.desc), ptr(rounded),
-         stream_handle(stream), device_index(x))
+    words = (torch.bfloat16, torch.int16, torch.uint16)
+    _require(x.dim() == 2 and (x.dtype == torch.float32 or x.dtype in words),
+             "microscaled rows are made of a bf16 or fp32 matrix")
+    _require(x.shape[1] <= 1 or x.stride(1) == 1, "columns to quantise must lie side by side")
+    _require(experts > 0 and x.shape[0] % experts == 0, "the experts' rows must be equally many")
+    _require(rounded is None or (rounded.shape == x.shape and rounded.dtype == x.dtype and
+                                 rounded.device == x.device and rounded.is_contiguous()),
+             "rounded must be a contiguous tensor like x")
+    _require(x.is_cuda, "rows to quantise must be on a GPU")
+    stream = _stream_of(x, stream)
+    with torch.cuda.stream(stream):  # whose memory the rows are
+        out = MxRows(experts, x.shape[0] // experts, x.shape[1], x.device)
+    call("q38m_mx_quantize_v1", ptr(x), DTYPE_F32 if x.dtype == torch.float32 else DTYPE_BF16,
+         x.stride(0) if x.shape[0] > 1 else x.shape[1], ctypes.byref(out.desc), ptr(rounded),
+         stream.cuda_stream, device_index(x))
     return out
 
 
@@ -485,9 +507,15 @@ class SortedRoutes:
         self.scratch = torch.empty(max(nbytes, 4), dtype=torch.uint8, device=device)
 
     def sort(self, ids, stream=None):
+        """ids int32 [tokens][top_k], contiguous, on the buffers' device."""
+        _require(ids.dtype == _torch().int32 and ids.is_contiguous() and
+                 tuple(ids.shape) == (self.tokens, self.top_k),
+                 "expert ids must be a contiguous int32 matrix of the sort's shape")
+        _require(ids.is_cuda and ids.device == self.offsets.device,
+                 "expert ids must be on the GPU of the sort's buffers")
         call("q38m_moe_sort_routes_v1", ptr(ids), self.tokens, self.top_k, self.experts,
              ptr(self.offsets), ptr(self.packed), ptr(self.inverse), ptr(self.scratch),
-             self.scratch.numel(), stream_handle(stream), device_index(ids))
+             self.scratch.numel(), _stream_of(ids, stream).cuda_stream, device_index(ids))
         return self
 
 

@@ -1008,7 +1008,8 @@ int q38m_mx_grouped_gemm_v1(const q38m_mx_matrix_v1* weights, const q38m_mx_matr
         !expert_offsets || top_k == 0u || routes == 0u || routes > q38m::kMaxSortRoutes ||
         (!packed_assignment && rows->rows != routes) ||
         (!swiglu && epilogue != Q38M_MX_EPILOGUE_NONE) || (swiglu && weights->rows % 2u != 0u) ||
-        !c_f32 == !c_bf16 || !aligned(c_f32, 4) || !aligned(c_bf16, 2))
+        !c_f32 == !c_bf16 || !aligned(c_f32, 4) || !aligned(c_bf16, 2) ||
+        !aligned(expert_offsets, 4) || !aligned(packed_assignment, 4))
         return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid microscaled expert product");
     const q38m::MxProduct p{static_cast<const uint8_t*>(rows->codes),
                             static_cast<const uint8_t*>(rows->scales),
@@ -1036,7 +1037,9 @@ int q38m_moe_sort_routes_v1(const int32_t* expert_ids, uint32_t tokens, uint32_t
                             void* scratch, size_t scratch_bytes, void* stream, int device) {
     const uint32_t routes = sort_routes(tokens, top_k);
     if (!expert_ids || routes == 0u || experts == 0u || experts > q38m::kMaxSortExperts ||
-        !expert_offsets || !packed_assignment || !assignment_to_packed)
+        !expert_offsets || !packed_assignment || !assignment_to_packed ||
+        !aligned(expert_ids, 4) || !aligned(expert_offsets, 4) ||
+        !aligned(packed_assignment, 4) || !aligned(assignment_to_packed, 4))
         return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid route sort input");
     const size_t needed = q38m_moe_sort_scratch_bytes(tokens, top_k, experts);
     if (needed != 0u && (!scratch || scratch_bytes < needed || !aligned(scratch, 4)))
@@ -1052,7 +1055,8 @@ int q38m_moe_permute_rows_v1(const void* x, uint32_t dtype, const uint32_t* assi
                              uint32_t tokens, uint32_t top_k, uint32_t width, void* rows,
                              void* stream, int device) {
     if (!x || !assignment_to_packed || !rows || !valid_rows(dtype, tokens, top_k, width) ||
-        !element_aligned(x, dtype) || !element_aligned(rows, dtype))
+        !element_aligned(x, dtype) || !element_aligned(rows, dtype) ||
+        !aligned(assignment_to_packed, 4))
         return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid row permutation input");
     if (int rc = select_device(device)) return rc;
     return finish(q38m::launch_permute_rows(x, dtype, assignment_to_packed, tokens, top_k, width,
@@ -1065,7 +1069,8 @@ int q38m_moe_unpermute_rows_v1(const void* rows, uint32_t dtype,
                                uint32_t tokens, uint32_t top_k, uint32_t width, void* y,
                                void* stream, int device) {
     if (!rows || !assignment_to_packed || !y || !valid_rows(dtype, tokens, top_k, width) ||
-        !element_aligned(rows, dtype) || !element_aligned(y, dtype) || !aligned(route_weights, 4))
+        !element_aligned(rows, dtype) || !element_aligned(y, dtype) || !aligned(route_weights, 4) ||
+        !aligned(assignment_to_packed, 4))
         return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid row return input");
     if (int rc = select_device(device)) return rc;
     return finish(q38m::launch_unpermute_rows(rows, dtype, assignment_to_packed, route_weights,
@@ -1081,7 +1086,8 @@ int q38m_moe_unpermute_backward_v1(const void* dy, const void* rows, uint32_t dt
     if (!dy || !assignment_to_packed || !route_weights || (!d_rows && !d_weights) ||
         (d_weights && !rows) || !valid_rows(dtype, tokens, top_k, width) ||
         !element_aligned(dy, dtype) || !element_aligned(rows, dtype) ||
-        !element_aligned(d_rows, dtype) || !aligned(route_weights, 4) || !aligned(d_weights, 4))
+        !element_aligned(d_rows, dtype) || !aligned(route_weights, 4) || !aligned(d_weights, 4) ||
+        !aligned(assignment_to_packed, 4))
         return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid row return gradient input");
     if (int rc = select_device(device)) return rc;
     return finish(q38m::launch_unpermute_backward(dy, rows, dtype, assignment_to_packed,

@@ -88,6 +88,8 @@ def test_grouped_refusals(q38m):
     call(f32=None)
     call(bf16=P)
     call(f32=P + 1)
+    call(offsets=P + 2)
+    call(packed=P + 1)
     # gathered rows, or one expert's, of 4 GB and more
     call(w=matrix(q38m, experts=3, columns=2048), rows=matrix(q38m, rows=1 << 22, columns=2048))
     call(w=matrix(q38m, experts=3, rows=1 << 22, columns=2048), rows=matrix(q38m, columns=2048),
@@ -117,13 +119,17 @@ def test_sort_refusals(q38m):
     call(experts=1025)
     call(scratch=None)
     call(scratch=P + 2)
+    call(ids=P + 2)
+    call(offsets=P + 1)
+    call(packed=P + 2)
+    call(inverse=P + 3)
     call(nbytes=size(32768, 10, 512) - 1)
 
 
 def test_row_refusals(q38m):
     bf16, f32 = q38m.DTYPE_BF16, q38m.DTYPE_F32
     for bad in (dict(x=None), dict(x=P + 1), dict(x=P + 2, dtype=f32), dict(inverse=None),
-                dict(rows=None), dict(rows=P + 1), dict(dtype=7), dict(tokens=0), dict(top_k=0),
+                dict(inverse=P + 2), dict(rows=None), dict(rows=P + 1), dict(dtype=7), dict(tokens=0), dict(top_k=0),
                 dict(tokens=1 << 24, top_k=1), dict(width=0), dict(width=(1 << 24) + 1)):
         a = dict(x=P, dtype=bf16, inverse=P, tokens=4, top_k=2, width=8, rows=P)
         a.update(bad)
@@ -145,3 +151,20 @@ def test_row_refusals(q38m):
     backward(rows=None)
     backward(rows=P + 1)
     backward(d_weights=P + 2)
+
+
+def test_python_refusals(q38m):
+    """What the conveniences would otherwise pass on as something else: other types, columns
+    apart, unequal experts, host memory."""
+    import torch as t
+
+    x = t.zeros(6, 64, dtype=t.bfloat16)
+    for bad in ((x.half(),), (x.double(),), (x.int(),), (x[0],), (x.T,), (x[:, ::2],), (x, 4),
+                (x, 0), (x, 1, x.float()), (x, 1, x[:3]), (x, 1, x.T.contiguous().T), (x,)):
+        with pytest.raises(q38m.InvalidArgument):
+            q38m.mx_quantize(*bad)
+    routes = q38m.SortedRoutes(6, 4, 8, device="cpu")
+    ids = t.zeros(6, 4, dtype=t.int32)
+    for bad in (ids.long(), ids.short(), ids[:5], ids.T.contiguous().T, ids.reshape(4, 6), ids):
+        with pytest.raises(q38m.InvalidArgument):
+            routes.sort(bad)
