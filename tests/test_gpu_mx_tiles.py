@@ -1,0 +1,60 @@
+"""The microscaled products on every tile shape, with scales in 16-byte pieces
+(K of 450: padded to 512) and without (K of 129 and 300), each with rows and
+columns that end inside a tile and with several tiles a workgroup, against the
+plain 64-bit form.  The comments name the shape that the rule on sizes takes;
+test_gpu_mx.py derives the bounds."""
+import numpy as np
+import pytest
+
+from conftest import load_oracle
+from helpers import device
+from test_gpu_mx import Encoded, check_product, close, encoded, run_experts, want_experts
+
+load_oracle()
+import mx_oracle as mx  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("m,n,k", [
+    (5, 17313, 129), (4, 16493, 450),                # 16 x 128
+    (21, 17444, 129), (17, 17190, 450),              # 32 x 128
+    (4149, 40, 129), (4402, 50, 450),                # 64 x 64
+    (8290, 72, 129), (8340, 66, 450),                # 128 x 128
+    (385, 25762, 450), (4000, 7900, 500)])          # 256 x 256: padded K of 512 and more alone
+def test_product(q38m, m, n, k):
+    print(f"product {m} x {n} x {k}", flush=True)
+    rng = np.random.default_rng(m + n + k)
+    check_product(q38m, Encoded(q38m, *encoded(rng, m, k), k), Encoded(q38m, *encoded(rng, n, k), k), k,
+                  "bf16" if m % 2 else "f32", spare=3)
+
+
+@pytest.mark.parametrize("swiglu,routes,experts,n,k", [
+    (False, 8, 3, 34, 450), (True, 8, 3, 34, 450),               # 16 x 64
+    (False, 200, 130, 66, 129), (False, 162, 130, 72, 450),      # 16 x 128
+    (True, 149, 130, 66, 129), (True, 130, 130, 66, 500),
+    (False, 3318, 130, 67, 129), (False, 3400, 130, 69, 450),    # 32 x 128
+    (True, 3684, 130, 70, 129), (True, 3198, 130, 68, 450),
+    (False, 4072, 7, 33, 300), (False, 4143, 3, 40, 450),        # 64 x 64
+    (True, 4264, 3, 38, 129), (True, 4305, 3, 34, 450),
+    (False, 13187, 130, 33, 129), (False, 17201, 12, 42, 450),   # 128 x 128
+    (True, 16290, 7, 34, 129), (True, 12821, 130, 34, 450),
+    (False, 594, 3, 16417, 450), (False, 15000, 5, 2048, 500),   # 256 x 256
+    (True, 469, 3, 18958, 450), (True, 15000, 5, 2048, 500)])
+def test_experts(q38m, swiglu, routes, experts, n, k):
+    """Routes in part without an expert, experts without rows, gathered rows and rows in place."""
+    print(f"experts {routes} of {experts}, {n} x {k} swiglu {swiglu}", flush=True)
+    rng = np.random.default_rng(routes + n)
+    ids = rng.integers(0, experts, size=(routes, 1)).astype(np.int32)
+    ids[rng.random(ids.shape) < 0.03] = -1
+    ids[ids == 1] = 2
+    offsets, packed, _ = mx.sort_routes(ids, experts)
+    kept = int(offsets[-1])
+    w = Encoded(q38m, *encoded(rng, experts * n, k, 122, 126), k, experts)
+    rows = Encoded(q38m, *encoded(rng, routes, k, 122, 126), k)
+    for gather, dtype in ((True, "bf16"), (False, "f32")):
+        words, got = run_experts(q38m, w, rows, device(offsets), device(packed) if gather else None, 1, routes,
+                                 swiglu, dtype)
+        want, bound = want_experts(w.values, rows.values, offsets, packed, 1 if gather else 0, experts, k, swiglu)
+        assert (words[kept:] == 0x4a4a).all(), "a dropped route's row was written"
+        close(got[:kept], want[:kept], bound[:kept], dtype, (routes, experts, n, k, gather))
