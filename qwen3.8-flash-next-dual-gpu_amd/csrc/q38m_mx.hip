@@ -19,6 +19,7 @@ namespace {
 
 // ---- quantisation -----------------------------------------------------------
 
+typedef uint32_t v4u_any __attribute__((ext_vector_type(4), aligned(2)));  // 16 bytes at any element
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef float v2f __attribute__((ext_vector_type(2)));
 typedef unsigned short v2us __attribute__((ext_vector_type(2)));
@@ -44,16 +45,16 @@ template <>
 struct Eight<uint16_t> {
     uint32_t d[4];  // bf16 pairs
     __device__ void load(const uint16_t* p) {
-        const uint4 w = *reinterpret_cast<const uint4*>(p);
+        const v4u_any w = *reinterpret_cast<const v4u_any*>(p);
         d[0] = w.x; d[1] = w.y; d[2] = w.z; d[3] = w.w;
     }
-    __device__ void gather(const uint16_t* p, uint32_t count) {
+    __device__ void gather(const uint16_t* p, uint32_t count) {  // 1 <= count, zeros behind
+        uint32_t v[8];
 #pragma unroll
-        for (uint32_t i = 0; i < 4u; ++i) {
-            const uint32_t lo = 2u * i < count ? p[2u * i] : 0u;
-            const uint32_t hi = 2u * i + 1u < count ? p[2u * i + 1u] : 0u;
-            d[i] = lo | hi << 16;
-        }
+        for (uint32_t i = 0; i < 8u; ++i) v[i] = p[min(i, count - 1u)];
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i)
+            d[i] = (2u * i < count ? v[2u * i] : 0u) | (2u * i + 1u < count ? v[2u * i + 1u] << 16 : 0u);
     }
     __device__ uint32_t field() const {
         v2us m = __builtin_bit_cast(v2us, d[0] & 0x7fff7fffu);
@@ -76,14 +77,15 @@ template <>
 struct Eight<float> {
     float v[8];
     __device__ void load(const float* p) {
-        const float4 a = reinterpret_cast<const float4*>(p)[0];
-        const float4 b = reinterpret_cast<const float4*>(p)[1];
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-        v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+        const v4u_any a = reinterpret_cast<const v4u_any*>(p)[0], b = reinterpret_cast<const v4u_any*>(p)[1];
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; ++i) v[i] = __uint_as_float(a[i]), v[i + 4u] = __uint_as_float(b[i]);
     }
     __device__ void gather(const float* p, uint32_t count) {
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; ++i) v[i] = i < count ? p[i] : 0.0f;
+        for (uint32_t i = 0; i < 8u; ++i) v[i] = p[min(i, count - 1u)];
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; ++i) v[i] = i < count ? v[i] : 0.0f;
     }
     __device__ uint32_t field() const {
         uint32_t m = 0;
@@ -120,9 +122,8 @@ constexpr uint32_t kQuantThreads = 256;
 
 template <typename T>
 __global__ __launch_bounds__(kQuantThreads) void mx_quantize_kernel(
-    const T* __restrict__ x, uint64_t stride, uint32_t rows, uint32_t columns, bool whole,
-    uint32_t lanes_log2, uint32_t* __restrict__ codes, uint32_t* __restrict__ scales,
-    T* __restrict__ rounded, bool rounded_whole) {
+    const T* __restrict__ x, uint64_t stride, uint32_t rows, uint32_t columns, uint32_t lanes_log2,
+    uint32_t* __restrict__ codes, uint32_t* __restrict__ scales, T* __restrict__ rounded) {
     const uint32_t lanes = 1u << lanes_log2;
     const uint32_t row = blockIdx.x * (kQuantThreads >> lanes_log2) + (threadIdx.x >> lanes_log2);
     if (row >= rows) return;
@@ -130,9 +131,9 @@ __global__ __launch_bounds__(kQuantThreads) void mx_quantize_kernel(
     const T* from = x + row * stride;
     const uint64_t first_eight = static_cast<uint64_t>(row) * (padded / 8u);
     for (uint32_t c = (threadIdx.x & (lanes - 1u)) * 8u; c < padded; c += lanes * 8u) {
-        Eight<T> e;
-        if (whole && c + 8u <= columns) e.load(from + c);
-        else e.gather(from + c, c < columns ? columns - c : 0u);
+        Eight<T> e{};
+        if (c + 8u <= columns) e.load(from + c);
+        else if (c < columns) e.gather(from + c, columns - c);
         uint32_t field = e.field();
         field = max(field, static_cast<uint32_t>(__shfl_xor(static_cast<int>(field), 1)));
         field = max(field, static_cast<uint32_t>(__shfl_xor(static_cast<int>(field), 2)));
@@ -144,29 +145,29 @@ __global__ __launch_bounds__(kQuantThreads) void mx_quantize_kernel(
         four |= static_cast<uint32_t>(__shfl_down(static_cast<int>(byte), 8)) << 16;
         four |= static_cast<uint32_t>(__shfl_down(static_cast<int>(byte), 12)) << 24;
         if ((c & 127u) == 0u) scales[(first_eight + c / 8u) / 16u] = four;
-        if (!rounded) continue;
+        if (!rounded || c >= columns) continue;
         float v[8];
         mx_values(q, byte, v);
         T* to = rounded + static_cast<uint64_t>(row) * columns + c;
-        if constexpr (sizeof(T) == 4u) {
-            if (rounded_whole && c + 8u <= columns) {
-                reinterpret_cast<float4*>(to)[0] = make_float4(v[0], v[1], v[2], v[3]);
-                reinterpret_cast<float4*>(to)[1] = make_float4(v[4], v[5], v[6], v[7]);
-            } else {
-                for (uint32_t i = 0; i < 8u && c + i < columns; ++i) to[i] = v[i];
-            }
-        } else {
-            if (rounded_whole && c + 8u <= columns) {
-                uint32_t d[4];
+        constexpr uint32_t kWords = sizeof(T) * 2u;
+        uint32_t d[kWords];
 #pragma unroll
-                for (uint32_t i = 0; i < 4u; ++i)  // two significant bits: exact in bf16
-                    d[i] = __float_as_uint(v[2 * i]) >> 16 |
-                           (__float_as_uint(v[2 * i + 1]) & 0xffff0000u);
-                *reinterpret_cast<uint4*>(to) = make_uint4(d[0], d[1], d[2], d[3]);
-            } else {
-                for (uint32_t i = 0; i < 8u && c + i < columns; ++i)
-                    to[i] = static_cast<uint16_t>(__float_as_uint(v[i]) >> 16);
-            }
+        for (uint32_t i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4u) d[i] = __float_as_uint(v[i]);
+            else d[i] = __float_as_uint(v[2 * i]) >> 16 |  // two significant bits: exact in bf16
+                        (__float_as_uint(v[2 * i + 1]) & 0xffff0000u);
+        }
+        if (c + 8u <= columns) {
+#pragma unroll
+            for (uint32_t i = 0; i < kWords; i += 4u)
+                reinterpret_cast<v4u_any*>(to)[i / 4u] = v4u_any{d[i], d[i + 1u], d[i + 2u], d[i + 3u]};
+            continue;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 7u; ++i) {
+            if (c + i >= columns) break;
+            if constexpr (sizeof(T) == 4u) to[i] = v[i];
+            else to[i] = static_cast<uint16_t>(d[i / 2u] >> i % 2u * 16u);
         }
     }
 }
@@ -177,6 +178,8 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+// at any element: rows of odd strides start anywhere
+typedef uint32_t v2u_any __attribute__((ext_vector_type(2), aligned(2)));
 
 // The block-scaled matrix instructions on 4-bit codes.  v_mfma_scale_f32_16x16x128:
 // lane l holds the 32 values k = 32 (l / 16) .. + 31 of row l % 16 of A and of B and
@@ -647,7 +650,6 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         using T = std::remove_pointer_t<decltype(c)>;
         constexpr uint32_t kSize = sizeof(T), kOut = kSwiglu ? kTN / 2u : kTN;  // tiles across
         constexpr uint32_t kFours = kOut * kAcc / 4u;                           // a lane's groups of four
-        const bool whole = reinterpret_cast<uintptr_t>(c) % 16u == 0u && p.c_stride * kSize % 16u == 0u;
         const uint32_t first_row = __builtin_amdgcn_readlane(known_first, t % 64u);
         const uint32_t count = __builtin_amdgcn_readlane(known_count, t % 64u);
         const uint32_t first_column = __builtin_amdgcn_readlane(known_column, t % 64u) * kColumns + wn * kOut * kMF;
@@ -660,8 +662,9 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
                 constexpr uint32_t kEach = sizeof(words) / kSize;
                 if (m >= count || column >= n_out) return;
                 T* to = row + column;
-                if (whole && column + kEach <= n_out) {
-                    *reinterpret_cast<std::remove_cv_t<std::remove_reference_t<decltype(words)>>*>(to) = words;
+                if (column + kEach <= n_out) {
+                    using At = std::conditional_t<sizeof(words) == 16u, v4u_any, v2u_any>;
+                    *reinterpret_cast<At*>(to) = words;
                     return;
                 }
 #pragma unroll
@@ -777,20 +780,14 @@ hipError_t launch_mx_quantize(const void* x, uint32_t dtype, uint64_t stride, ui
     uint32_t lanes = 4;
     while (lanes < 8u && (8u << lanes) < columns) ++lanes;
     const uint32_t per = kQuantThreads >> lanes, grid = (rows + per - 1u) / per;
-    const uint32_t size = dtype == Q38M_DTYPE_F32 ? 4u : 2u;
-    const bool whole = reinterpret_cast<uintptr_t>(x) % 16u == 0u && stride * size % 16u == 0u;
-    const bool rounded_whole = reinterpret_cast<uintptr_t>(rounded) % 16u == 0u &&
-                               static_cast<uint64_t>(columns) * size % 16u == 0u;
     if (dtype == Q38M_DTYPE_F32)
         mx_quantize_kernel<float><<<grid, kQuantThreads, 0, stream>>>(
-            static_cast<const float*>(x), stride, rows, columns, whole, lanes,
-            static_cast<uint32_t*>(codes), static_cast<uint32_t*>(scales),
-            static_cast<float*>(rounded), rounded_whole);
+            static_cast<const float*>(x), stride, rows, columns, lanes, static_cast<uint32_t*>(codes),
+            static_cast<uint32_t*>(scales), static_cast<float*>(rounded));
     else
         mx_quantize_kernel<uint16_t><<<grid, kQuantThreads, 0, stream>>>(
-            static_cast<const uint16_t*>(x), stride, rows, columns, whole, lanes,
-            static_cast<uint32_t*>(codes), static_cast<uint32_t*>(scales),
-            static_cast<uint16_t*>(rounded), rounded_whole);
+            static_cast<const uint16_t*>(x), stride, rows, columns, lanes, static_cast<uint32_t*>(codes),
+            static_cast<uint32_t*>(scales), static_cast<uint16_t*>(rounded));
     return hipGetLastError();
 }
 
@@ -843,22 +840,23 @@ hipError_t launch_tiles(const MxProduct& p, hipStream_t stream) {
 // Calls f with the shape that a product runs on, the one with the shortest stage.  The
 // figures of `each` are fitted to these, us on 16 x 64, 16 x 128, 32 x 128, 64 x 64, 128 x
 // 128 and 256 x 256 tiles:
-//   1 x 8,192 x 2,048        4.6   5.2     -   5.4     -     -
-//   32 x 4,096 x 4,096         -   7.4   7.9   7.8    11    22
-//   256 x 4,096 x 4,096        -  13.1   9.4   8.9    13    25
-//   509 x 2,048 x 8,192        -    23    16    14    22    44
-//   1,024 x 4,096 x 4,096      -    41    25    21    17    28
-//   4,096 x 4,096 x 4,096      -     -     -     -    49    42
-//   8,192 x 8,192 x 8,192      -     -     -     -   378   301
+//   1 x 8,192 x 2,048        4.5   5.1   5.2   5.2   6.8    13
+//   32 x 4,096 x 4,096       6.2   7.6   7.7   7.4    10    21
+//   256 x 4,096 x 4,096       14    13   9.3   8.7    12    24
+//   509 x 2,048 x 8,192       25    23    16    14    20    43
+//   1,024 x 4,096 x 4,096     44    42    26    21    17    28
+//   4,096 x 4,096 x 4,096    158   155    96    81    49    41
+//   8,192 x 8,192 x 8,192  1,409 1,108   638   531   346   280
 // and gate/up (1,024 x 2,048) of 512 experts, top-10, by tokens:
-//   1                        7.1   8.6     -   7.3     -     -
-//   64                        72    72     -    78     -     -
-//   512                      110   106     -   122     -     -
-//   1,024                      -   131   113   128   125   163
-//   2,048                      -   170   143   137   133   174
-//   4,096                      -   267   191   203   144   179
-//   8,192                      -   447   313   287   223   193
-//   32,768                     -     -     -     -   576   520
+//   1                        6.6   8.0   7.3   7.2   8.9    15
+//   64                        72    72    72    78    80   114
+//   512                      109   106   105   120   117   160
+//   1,024                    138   131   114   127   122   161
+//   2,048                    179   170   143   136   130   169
+//   4,096                    283   266   192   199   141   176
+//   8,192                    496   447   310   289   215   192
+//   16,384                   885   800   518   477   313   323
+//   32,768                 1,639 1,472   925   840   549   499
 // 256 x 256 tiles are for mx_wide products alone: without it they need registers that
 // their waves do not have.
 template <typename F>

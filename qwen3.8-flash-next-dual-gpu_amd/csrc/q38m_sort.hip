@@ -6,7 +6,8 @@
 // (expert, route number) the kept routes get the packed places 0, 1, ...; a
 // route whose id names no expert is dropped: its order entry lies behind the
 // last expert's and its inverse is Q38M_ROUTE_DROPPED.
-#include <initializer_list>
+#include <algorithm>
+#include <type_traits>
 
 #include "q38m_device.h"
 #include "q38m_internal.h"
@@ -100,8 +101,8 @@ struct WaveRoutes {
 
 // One workgroup sorts everything: each wave counts its own contiguous routes, the counts
 // become places by a sum over the waves of a key and over the keys.  What takes its time
-// is latency: ids read, LDS counters, the sums, writes (512 tokens, top-10: 9.9 us with
-// the ids read again for every step; see the table of cases).
+// is latency: ids read, LDS counters, the sums, writes (512 tokens, top-10, whose bytes
+// would take 0.01 us: 8.2 us; with the ids read again for every step 9.9).
 constexpr uint32_t kSmallWaves = 16;
 __global__ __launch_bounds__(kSmallWaves * 64) void sort_small_kernel(
     const int32_t* __restrict__ ids, uint32_t routes, uint32_t experts,
@@ -147,7 +148,8 @@ __global__ __launch_bounds__(kSmallWaves * 64) void sort_small_kernel(
 }
 
 // The same in three launches over chunks of routes: the chunks' counts; each key's
-// counts summed over the chunks in front; the scatter, which sums the keys' totals.
+// counts summed over the chunks in front; the scatter, which sums the keys' totals.  327,680
+// routes of 512 experts: 4.7, 6.3 and 6.0 us, all latency (their 5 MB would take 1 us).
 constexpr uint32_t kChunkWaves = 4, kChunkSteps = kSortChunk / (kChunkWaves * 64u);
 __global__ __launch_bounds__(kChunkWaves * 64) void sort_count_kernel(
     const int32_t* __restrict__ ids, uint32_t routes, uint32_t experts,
@@ -241,38 +243,28 @@ __global__ __launch_bounds__(kChunkWaves * 64) void sort_scatter_kernel(
 
 // ---- rows -------------------------------------------------------------------
 
-// 16 bytes, kStream: past the caches
-template <bool kStream>
-__device__ __forceinline__ uint4 get16(const void* p) {
-    if constexpr (kStream) return load_stream(static_cast<const uint4*>(p));
-    else return *static_cast<const uint4*>(p);
-}
-template <bool kStream>
-__device__ __forceinline__ void put16(void* p, uint4 w) {
-    if constexpr (kStream) {
-        const v4u_t v = {w.x, w.y, w.z, w.w};
-        __builtin_nontemporal_store(v, static_cast<v4u_t*>(p));
-    } else {
-        *static_cast<uint4*>(p) = w;
-    }
-}
+// 16 bytes at any element (a row of odd width starts anywhere)
+typedef uint32_t v4u_any __attribute__((ext_vector_type(4), aligned(2)));
 
-// kN consecutive values of a row, and as fp32 (back: one rounding).  kN = 8 is 16-byte
-// aligned; kN = 1 takes any row.
+// kN consecutive values of a row, and as fp32 (back: one rounding): 16 bytes, or one value
+// of a row that is narrower.  kStream: past the caches.  (Eight values of fp32, two
+// instructions that touch every second 16 bytes each: 2,929 x 10 rows of 2,048 sorted, there
+// and back 142 us instead of 138.  Rows of odd widths a value a lane: 9,983 x 10 rows of 601
+// bf16 126 us instead of 60.)
 template <typename T, uint32_t kN>
 struct Piece {
     static constexpr uint32_t kWords = (kN * sizeof(T) + 3u) / 4u;
+    static_assert(kN == 1u || kWords == 4u, "a value or 16 bytes");
     uint32_t d[kWords];
 
     template <bool kStream>
     __device__ static Piece get(const T* p) {
         Piece r;
-        if constexpr (kN == 8u) {
-#pragma unroll
-            for (uint32_t i = 0; i < kWords; i += 4u) {
-                const uint4 w = get16<kStream>(p + i * 4u / sizeof(T));
-                r.d[i] = w.x, r.d[i + 1u] = w.y, r.d[i + 2u] = w.z, r.d[i + 3u] = w.w;
-            }
+        if constexpr (kN != 1u) {
+            v4u_any w;
+            if constexpr (kStream) w = __builtin_nontemporal_load(reinterpret_cast<const v4u_any*>(p));
+            else w = *reinterpret_cast<const v4u_any*>(p);
+            r.d[0] = w.x, r.d[1] = w.y, r.d[2] = w.z, r.d[3] = w.w;
         } else if constexpr (sizeof(T) == 4u) {
             r.d[0] = __float_as_uint(*p);
         } else {
@@ -282,10 +274,10 @@ struct Piece {
     }
     template <bool kStream>
     __device__ void put(T* p) const {
-        if constexpr (kN == 8u) {
-#pragma unroll
-            for (uint32_t i = 0; i < kWords; i += 4u)
-                put16<kStream>(p + i * 4u / sizeof(T), make_uint4(d[i], d[i + 1u], d[i + 2u], d[i + 3u]));
+        if constexpr (kN != 1u) {
+            const v4u_any w = {d[0], d[1], d[2], d[3]};
+            if constexpr (kStream) __builtin_nontemporal_store(w, reinterpret_cast<v4u_any*>(p));
+            else *reinterpret_cast<v4u_any*>(p) = w;
         } else if constexpr (sizeof(T) == 4u) {
             *p = __uint_as_float(d[0]);
         } else {
@@ -314,7 +306,9 @@ struct Piece {
 constexpr uint32_t kRowThreads = 256;
 
 // A workgroup takes kRowThreads / lanes tokens, `lanes` (a power of two)
-// threads each, which walk the row kN values a thread.
+// threads each, which walk the row kN values a thread.  A row's last piece is
+// its last kN values, in part those of the piece in front: written twice, with
+// the same bits.
 struct RowPlace {
     uint32_t token, column, step;
 };
@@ -325,8 +319,10 @@ __device__ __forceinline__ RowPlace row_place(uint32_t lanes_log2) {
                     (threadIdx.x & (lanes - 1u)) * kN, lanes * kN};
 }
 
-// rows[inverse[t k + r]] = x[t] for every kept route
-template <typename T, uint32_t kN>
+// rows[inverse[t k + r]] = x[t] for every kept route: a token is read once and written
+// top_k times.  32,768 x 10 rows of 2,048 bf16: 257 us, 5.7 TB/s of 1.48 GB, nearly all of
+// it writes.
+template <typename T, uint32_t kN, bool kStream>
 __global__ __launch_bounds__(kRowThreads) void permute_kernel(
     const T* __restrict__ x, const uint32_t* __restrict__ inverse, uint32_t tokens,
     uint32_t top_k, uint32_t width, uint32_t lanes_log2, T* __restrict__ rows) {
@@ -334,28 +330,29 @@ __global__ __launch_bounds__(kRowThreads) void permute_kernel(
     if (p.token >= tokens) return;
     const uint32_t routes = tokens * top_k;
     const uint32_t* at = inverse + static_cast<size_t>(p.token) * top_k;
-    for (uint32_t c = p.column; c < width; c += p.step) {
+    for (uint32_t c0 = p.column; c0 < width; c0 += p.step) {
+        const uint32_t c = min(c0, width - kN);
         const auto v = Piece<T, kN>::template get<false>(x + static_cast<size_t>(p.token) * width + c);
         for (uint32_t r = 0; r < top_k; ++r)
-            if (at[r] < routes) v.template put<false>(rows + static_cast<size_t>(at[r]) * width + c);
+            if (at[r] < routes) v.template put<kStream>(rows + static_cast<size_t>(at[r]) * width + c);
     }
 }
 
 // y[t] = sum over t's kept routes, in rank order, of weight * row.  The rows of kRanks
-// routes are under way at once.  y goes past the caches, and the rows come past them where
-// they are more than the 256 MB behind the L2s hold: 1.3 GB of them cached / y past the
-// caches / both 325 / 265 / 239 us (6.2 TB/s), 21 MB of them 5.0 / 4.3 / 4.8.
+// routes are under way at once; y goes past the caches (21 MB of rows: 4.3 us, cached 5.0).
+// 32,768 x 10 rows of 2,048 bf16: 239 us, 6.2 TB/s of 1.48 GB.
 template <typename T, uint32_t kN, bool kStream>
 __global__ __launch_bounds__(kRowThreads) void unpermute_kernel(
     const T* __restrict__ rows, const uint32_t* __restrict__ inverse,
     const float* __restrict__ weights, uint32_t tokens, uint32_t top_k, uint32_t width,
     uint32_t lanes_log2, T* __restrict__ y) {
-    constexpr uint32_t kRanks = sizeof(T) == 2u ? 16u : 8u;
+    constexpr uint32_t kRanks = 16;
     const RowPlace p = row_place<kN>(lanes_log2);
     if (p.token >= tokens) return;
     const uint32_t routes = tokens * top_k;
     const size_t first = static_cast<size_t>(p.token) * top_k;
-    for (uint32_t c = p.column; c < width; c += p.step) {
+    for (uint32_t c0 = p.column; c0 < width; c0 += p.step) {
+        const uint32_t c = min(c0, width - kN);
         float sum[kN] = {};
         for (uint32_t r0 = 0; r0 < top_k; r0 += kRanks) {
             uint32_t at[kRanks];
@@ -389,14 +386,18 @@ __global__ __launch_bounds__(kRowThreads) void unpermute_kernel(
     }
 }
 
-// One wave per route: d_rows[at] = w dy[t], d_weights[route] = <dy[t], rows[at]>
-template <typename T, uint32_t kN>
+// d_rows[at] = w dy[t], d_weights[route] = <dy[t], rows[at]>: up to a wave's lanes (a power of
+// two) for each route.  dy[t] is read by each of its routes, from the caches but for the first.
+// 16,384 x 10 rows of 2,048
+// bf16: 275 us, 5.1 TB/s of 1.41 GB, read and written in nearly equal parts, as in a copy,
+// which reaches as much.
+template <typename T, uint32_t kN, bool kStream>
 __global__ __launch_bounds__(kRowThreads) void unpermute_backward_kernel(
     const T* __restrict__ dy, const T* __restrict__ rows, const uint32_t* __restrict__ inverse,
     const float* __restrict__ weights, uint32_t routes, uint32_t top_k, uint32_t width,
-    T* __restrict__ d_rows, float* __restrict__ d_weights) {
-    const uint32_t route = blockIdx.x * (kRowThreads / 64u) + (threadIdx.x >> 6);
-    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t lanes_log2, T* __restrict__ d_rows, float* __restrict__ d_weights) {
+    const RowPlace p = row_place<kN>(lanes_log2);
+    const uint32_t route = p.token;
     if (route >= routes) return;
     const uint32_t at = inverse[route];
     float dot = 0.0f;
@@ -404,33 +405,26 @@ __global__ __launch_bounds__(kRowThreads) void unpermute_backward_kernel(
         const float w = weights[route];
         const T* from = dy + static_cast<size_t>(route / top_k) * width;
         const size_t row = static_cast<size_t>(at) * width;
-        for (uint32_t c = lane * kN; c < width; c += 64u * kN) {
+        for (uint32_t c0 = p.column; c0 < width; c0 += p.step) {
+            const uint32_t c = min(c0, width - kN);
             float g[kN], v[kN];
             Piece<T, kN>::template get<false>(from + c).widen(g);
             if (d_weights) {
-                Piece<T, kN>::template get<false>(rows + row + c).widen(v);
+                Piece<T, kN>::template get<kStream>(rows + row + c).widen(v);
 #pragma unroll
-                for (uint32_t i = 0; i < kN; ++i) dot = __builtin_fmaf(g[i], v[i], dot);
+                for (uint32_t i = 0; i < kN; ++i)  // those of the piece in front are in its sum
+                    if (c + i >= c0) dot = __builtin_fmaf(g[i], v[i], dot);
             }
             if (d_rows) {
 #pragma unroll
                 for (uint32_t i = 0; i < kN; ++i) g[i] *= w;
-                Piece<T, kN>::round(g).template put<false>(d_rows + row + c);
+                Piece<T, kN>::round(g).template put<kStream>(d_rows + row + c);
             }
         }
     }
     if (!d_weights) return;
-#pragma unroll
-    for (uint32_t d = 32u; d != 0u; d >>= 1) dot += __shfl_xor(dot, d);
-    if (lane == 0u) d_weights[route] = dot;
-}
-
-// 16-byte pieces where every row starts on one
-bool whole_pieces(uint32_t width, std::initializer_list<const void*> ptrs) {
-    if (width % 8u != 0u) return false;
-    for (const void* p : ptrs)
-        if (reinterpret_cast<uintptr_t>(p) % 16u != 0u) return false;
-    return true;
+    for (uint32_t d = 1u << lanes_log2 >> 1; d != 0u; d >>= 1) dot += __shfl_xor(dot, d);
+    if (p.column == 0u) d_weights[route] = dot;
 }
 
 uint32_t row_lanes_log2(uint32_t width, uint32_t piece) {
@@ -444,56 +438,60 @@ uint32_t row_grid(uint32_t tokens, uint32_t lanes_log2) {
     return (tokens + per - 1u) / per;
 }
 
+// Calls f with the values a piece has and whether the rows (`sides` of them: read, written or
+// both) go past the caches: where they are more than the 256 MB behind the L2s hold.  10 rows
+// of 2,048 bf16 a token, cached / past the caches, us: written 20.8 / 23.7 for 120 MB, 139 /
+// 128 for 655, 283 / 257 for 1,342; back 20.5 / 21.4, 88.3 / 87.8 (492 MB), 265 / 239; both
+// ways in the gradient 288 / 275 for 1,342.
+template <typename T, typename F>
+void with_piece(uint32_t sides, uint32_t tokens, uint32_t top_k, uint32_t width, F f) {
+    constexpr uint64_t kCachedBytes = 256u << 20;
+    constexpr std::integral_constant<uint32_t, 16u / sizeof(T)> kWide{};
+    constexpr std::integral_constant<uint32_t, 1u> kNarrow{};
+    const bool streamed = static_cast<uint64_t>(tokens) * top_k * width * sizeof(T) * sides > kCachedBytes;
+    if (width >= kWide.value) {
+        if (streamed) f(kWide, std::true_type{});
+        else f(kWide, std::false_type{});
+    } else {
+        f(kNarrow, std::false_type{});
+    }
+}
+
 template <typename T>
 hipError_t permute(const T* x, const uint32_t* inverse, uint32_t tokens, uint32_t top_k,
                    uint32_t width, T* rows, hipStream_t stream) {
-    if (whole_pieces(width, {x, rows})) {
-        const uint32_t lanes = row_lanes_log2(width, 8u);
-        permute_kernel<T, 8><<<row_grid(tokens, lanes), kRowThreads, 0, stream>>>(
+    with_piece<T>(1u, tokens, top_k, width, [&](auto piece, auto streamed) {
+        constexpr uint32_t kN = decltype(piece)::value;
+        const uint32_t lanes = row_lanes_log2(width, kN);
+        permute_kernel<T, kN, decltype(streamed)::value><<<row_grid(tokens, lanes), kRowThreads, 0, stream>>>(
             x, inverse, tokens, top_k, width, lanes, rows);
-    } else {
-        const uint32_t lanes = row_lanes_log2(width, 1u);
-        permute_kernel<T, 1><<<row_grid(tokens, lanes), kRowThreads, 0, stream>>>(
-            x, inverse, tokens, top_k, width, lanes, rows);
-    }
-    return hipGetLastError();
-}
-
-constexpr uint64_t kCachedBytes = 256u << 20;
-
-template <typename T, uint32_t kN>
-hipError_t unpermute(const T* rows, const uint32_t* inverse, const float* weights,
-                     uint32_t tokens, uint32_t top_k, uint32_t width, T* y, hipStream_t stream) {
-    const uint32_t lanes = row_lanes_log2(width, kN), grid = row_grid(tokens, lanes);
-    if (static_cast<uint64_t>(tokens) * top_k * width * sizeof(T) > kCachedBytes)
-        unpermute_kernel<T, kN, true><<<grid, kRowThreads, 0, stream>>>(
-            rows, inverse, weights, tokens, top_k, width, lanes, y);
-    else
-        unpermute_kernel<T, kN, false><<<grid, kRowThreads, 0, stream>>>(
-            rows, inverse, weights, tokens, top_k, width, lanes, y);
+    });
     return hipGetLastError();
 }
 
 template <typename T>
 hipError_t unpermute(const T* rows, const uint32_t* inverse, const float* weights,
                      uint32_t tokens, uint32_t top_k, uint32_t width, T* y, hipStream_t stream) {
-    return whole_pieces(width, {rows, y})
-               ? unpermute<T, 8>(rows, inverse, weights, tokens, top_k, width, y, stream)
-               : unpermute<T, 1>(rows, inverse, weights, tokens, top_k, width, y, stream);
+    with_piece<T>(1u, tokens, top_k, width, [&](auto piece, auto streamed) {
+        constexpr uint32_t kN = decltype(piece)::value;
+        const uint32_t lanes = row_lanes_log2(width, kN);
+        unpermute_kernel<T, kN, decltype(streamed)::value><<<row_grid(tokens, lanes), kRowThreads, 0, stream>>>(
+            rows, inverse, weights, tokens, top_k, width, lanes, y);
+    });
+    return hipGetLastError();
 }
 
 template <typename T>
 hipError_t unpermute_backward(const T* dy, const T* rows, const uint32_t* inverse,
                               const float* weights, uint32_t tokens, uint32_t top_k,
                               uint32_t width, T* d_rows, float* d_weights, hipStream_t stream) {
-    const uint32_t routes = tokens * top_k;
-    const uint32_t grid = (routes + kRowThreads / 64u - 1u) / (kRowThreads / 64u);
-    if (whole_pieces(width, {dy, rows, d_rows}))
-        unpermute_backward_kernel<T, 8><<<grid, kRowThreads, 0, stream>>>(
-            dy, rows, inverse, weights, routes, top_k, width, d_rows, d_weights);
-    else
-        unpermute_backward_kernel<T, 1><<<grid, kRowThreads, 0, stream>>>(
-            dy, rows, inverse, weights, routes, top_k, width, d_rows, d_weights);
+    with_piece<T>(2u, tokens, top_k, width, [&](auto piece, auto streamed) {
+        constexpr uint32_t kN = decltype(piece)::value;
+        const uint32_t routes = tokens * top_k, lanes = std::min(row_lanes_log2(width, kN), 6u);
+        unpermute_backward_kernel<T, kN, decltype(streamed)::value>
+            <<<row_grid(routes, lanes), kRowThreads, 0, stream>>>(
+                dy, rows, inverse, weights, routes, top_k, width, lanes, d_rows, d_weights);
+    });
     return hipGetLastError();
 }
 
