@@ -2,8 +2,12 @@
 points that need no GPU: sizes, and every refusal before a device is
 touched."""
 import ctypes
+import os
+import subprocess
 
 import pytest
+
+from conftest import ROOT
 
 P = 0x100000  # a 16-byte aligned address that no refused call reads
 
@@ -168,3 +172,42 @@ def test_python_refusals(q38m):
     for bad in (ids.long(), ids.short(), ids[:5], ids.T.contiguous().T, ids.reshape(4, 6), ids):
         with pytest.raises(q38m.InvalidArgument):
             routes.sort(bad)
+
+
+def test_cpp_layer_of_the_guide(q38m, tmp_path):
+    """The guide's layer in C++ compiles against the wrapper, links, and throws what the entry
+    points refuse."""
+    guide = open(os.path.join(ROOT, "INTEGRATION.md")).read()
+    begin = guide.index("```cpp\n", guide.index("## 7. Microscaled experts")) + len("```cpp\n")
+    source = tmp_path / "layer.cpp"
+    source.write_text(guide[begin:guide.index("```\n", begin)] + r"""
+#include <cstdio>
+#include <stdexcept>
+template <typename F>
+void refused(F f) {
+    try {
+        f();
+    } catch (const std::invalid_argument&) {
+        return;
+    }
+    std::printf("accepted\n");
+}
+int main() {
+    MxLayer l{};
+    refused([&] { run_mx_layer(l, nullptr, nullptr, nullptr, nullptr, nullptr, 0); });
+    refused([&] { q38m::mx_quantize(&l, q38m::DtypeV1::kF32, 0, l.x_rows, nullptr, nullptr, 0); });
+    refused([&] { q38m::mx_gemm(l.x_rows, l.h_rows, nullptr, nullptr, 0, nullptr, 0); });
+    refused([&] { q38m::moe_permute_rows(&l, q38m::DtypeV1::kBf16, nullptr, 1, 1, 8, &l, nullptr, 0); });
+    refused([&] {
+        q38m::moe_unpermute_backward(&l, &l, q38m::DtypeV1::kBf16, nullptr, nullptr, 1, 1, 8, &l, nullptr,
+                                     nullptr, 0);
+    });
+    std::printf("ok\n");
+}
+""")
+    package = os.path.dirname(q38m.LIB_PATH)
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-I", os.path.join(ROOT, "include"), str(source),
+                    "-o", str(tmp_path / "layer"), "-L", package, "-lq38m", f"-Wl,-rpath,{package}",
+                    "-Wl,-rpath,/opt/rocm/lib"], check=True)
+    out = subprocess.run([str(tmp_path / "layer")], capture_output=True, text=True)
+    assert out.returncode == 0 and out.stdout == "ok\n", out.stdout + out.stderr
