@@ -3,12 +3,14 @@
 columns that end inside a tile and with several tiles a workgroup, against the
 plain 64-bit form.  The comments name the shape that the rule on sizes takes;
 test_gpu_mx.py derives the bounds."""
+import ctypes
+
 import numpy as np
 import pytest
 
 from conftest import load_oracle
-from helpers import device
-from test_gpu_mx import Encoded, check_product, close, encoded, run_experts, want_experts
+from helpers import device, host, stream, torch
+from test_gpu_mx import Encoded, check_product, close, encoded, product_bound, run_experts, want_experts, widen
 
 load_oracle()
 import mx_oracle as mx  # noqa: E402
@@ -58,3 +60,33 @@ def test_experts(q38m, swiglu, routes, experts, n, k):
         want, bound = want_experts(w.values, rows.values, offsets, packed, 1 if gather else 0, experts, k, swiglu)
         assert (words[kept:] == 0x4a4a).all(), "a dropped route's row was written"
         close(got[:kept], want[:kept], bound[:kept], dtype, (routes, experts, n, k, gather))
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 70, 1024), (300, 530, 512), (4000, 4000, 512)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_least_alignment(q38m, m, n, k, dtype):
+    """Scales 4 bytes and C one element behind a 16-byte boundary, rows of C an odd stride apart."""
+    t = torch()
+    print(f"alignment {m} x {n} x {k} {dtype}", flush=True)
+    rng = np.random.default_rng(m)
+    sides = []
+    for rows in (m, n):
+        codes, scales = encoded(rng, rows, k)
+        on_device, shifted = device(codes), t.zeros(scales.size + 4, dtype=t.uint8, device="cuda")
+        shifted[4:] = device(scales).reshape(-1)
+        sides.append((q38m.MxMatrix(on_device.data_ptr(), shifted.data_ptr() + 4, 1, rows, k), on_device, shifted,
+                      mx.decode(codes, scales, k)))
+    stride = n + 1 + n % 2
+    out = t.full((1 + m * stride + 8,), 0x4a4a, dtype=t.int16 if dtype == "bf16" else t.int32, device="cuda")
+    c = out.data_ptr() + out.element_size()
+    q38m.call("q38m_mx_gemm_v1", ctypes.byref(sides[0][0]), ctypes.byref(sides[1][0]),
+              *((None, c) if dtype == "bf16" else (c, None)), stride, stream(), 0)
+    t.cuda.synchronize()
+    words = host(out, np.uint16 if dtype == "bf16" else np.uint32)
+    assert words[0] == 0x4a4a and (words[1 + m * stride:] == 0x4a4a).all()
+    words = words[1:1 + m * stride].reshape(m, stride)
+    assert (words[:, n:] == 0x4a4a).all()
+    words = np.ascontiguousarray(words[:, :n])
+    got = widen(words) if dtype == "bf16" else words.view(np.float32).astype(np.float64)
+    want, size = mx.product(sides[0][3], sides[1][3])
+    close(got, want, product_bound(k, size), dtype, (m, n, k))
