@@ -438,14 +438,22 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     uint32_t found = 0, next_column = 0;
     RowTile next{0u, 0u, 0u};
     uint32_t data_source[kDataLoads], scale_source[kScaleLoads];
+    // what follows from the lane alone is computed anew in each use outside the stages, not kept
+    // in registers from one tile to the next
+    const auto fresh_lane = [&]() MX_INLINE {
+        uint32_t l = lane;
+        asm volatile("" : "+v"(l));
+        return l;
+    };
     const auto look_up = [&]() MX_INLINE {
         if (found == order.count) return;
+        const uint32_t own_lane = fresh_lane();
         if (found != 0u) order.at += order.step;
         const uint32_t row = order.row();
         next_column = order.column();
         if constexpr (kExperts) next = list.find(row);
         else next = RowTile{0u, row * kBM, static_cast<uint32_t>(min(p.routes - row * kBM, kBM))};
-        if (lane == found % 64u) {
+        if (own_lane == found % 64u) {
             known_first = next.first;
             known_count = next.count;
             known_column = next_column;
@@ -456,19 +464,18 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         for (uint32_t t = 0; t < kDataLoads; ++t) {
             const uint32_t i = wave + t * S::kWaves;
             if (t * S::kWaves < kDataA && data_live(t) && i < kDataA)
-                data_source[t] = p.packed[next.first + min(8u * i + (lane >> 3), next.count - 1u)];
+                data_source[t] = p.packed[next.first + min(8u * i + (own_lane >> 3), next.count - 1u)];
         }
 #pragma unroll
         for (uint32_t t = 0; t < kScaleLoads; ++t) {
             const uint32_t i = wave + t * S::kWaves;
             if (t * S::kWaves < kScaleA && scale_live(t) && i < kScaleA)
-                scale_source[t] = p.packed[next.first + min(kScaleRows * i + (kWide ? lane : lane >> 1), next.count - 1u)];
+                scale_source[t] = p.packed[next.first + min(kScaleRows * i + (kWide ? own_lane : own_lane >> 1), next.count - 1u)];
         }
     };
     // points the loads at the tile that was looked up, and looks up the one after it
     const auto point = [&]() MX_INLINE {
-        uint32_t own_lane = lane;  // the offsets are computed here, not kept from one tile to the next
-        asm volatile("" : "+v"(own_lane));
+        const uint32_t own_lane = fresh_lane();
         const bool gather = kExperts && p.packed;
         const uint64_t a_first = gather ? 0u : next.first;
         const uint64_t b_first = static_cast<uint64_t>(next.expert) * p.n + next_column * kColumns;
@@ -661,6 +668,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         using T = std::remove_pointer_t<decltype(c)>;
         constexpr uint32_t kSize = sizeof(T), kOut = kSwiglu ? kTN / 2u : kTN;  // tiles across
         constexpr uint32_t kFours = kOut * kAcc / 4u;                           // a lane's groups of four
+        const uint32_t own_lane = fresh_lane(), n = own_lane % kMF, q = own_lane / kMF;
         const uint32_t first_row = __builtin_amdgcn_readlane(known_first, t % 64u);
         const uint32_t count = __builtin_amdgcn_readlane(known_count, t % 64u);
         const uint32_t first_column = __builtin_amdgcn_readlane(known_column, t % 64u) * kColumns + wn * kOut * kMF;
