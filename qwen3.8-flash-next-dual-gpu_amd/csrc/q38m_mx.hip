@@ -334,8 +334,10 @@ struct MxOrder {
 // What bounds it: with few rows the latency of a stage (load, meet, read, multiply: 0.35 us
 // on 64 x 64 tiles); from tens of tokens on the weights' bytes (gate/up of 512 experts, 512
 // tokens: 106 us, 5.4 TB/s of 576 MB); large products the card's power (8,192^3 280 us, 3.9
-// PFLOP/s at 1.8 GHz) and, with few stages a tile, C's stores: gate/up of 32,768 tokens 492
-// us, 435 without them, 3.4 PFLOP/s on the rows of its 256-row tiles, 2.8 on those that count.
+// PFLOP/s at 1.8 GHz) and, with few stages a tile, C's stores and loads that memory answers
+// late: gate/up of 32,768 tokens 481 us, 3.4 PFLOP/s on the rows of its 256-row tiles, 2.9 on
+// those that count (an earlier form of 509 us took 435 without its stores; with four experts'
+// weights alone, which the L2s hold, 467 instead of 507).
 template <uint32_t kMF_, uint32_t kWM_, uint32_t kWN_, uint32_t kTM_, uint32_t kTN_, uint32_t kStages_>
 struct MxShape {
     static constexpr uint32_t kMF = kMF_, kWM = kWM_, kWN = kWN_, kTM = kTM_, kTN = kTN_;
@@ -438,11 +440,13 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     uint32_t found = 0, next_column = 0;
     RowTile next{0u, 0u, 0u};
     uint32_t data_source[kDataLoads], scale_source[kScaleLoads];
-    // what follows from the lane alone is computed anew in each use outside the stages, not kept
-    // in registers from one tile to the next
+    // On 256 x 256 tiles, which leave no registers over, what follows from the lane alone is
+    // computed anew in each use outside the stages (kept from tile to tile, 12 registers went to
+    // memory: 32,768-token gate/up 500 us instead of 481; where they are free keeping it is as
+    // fast or faster: 509 x 2,048 x 8,192 14.1 instead of 14.4).
     const auto fresh_lane = [&]() MX_INLINE {
         uint32_t l = lane;
-        asm volatile("" : "+v"(l));
+        if constexpr (S::kWaves == 8u) asm volatile("" : "+v"(l));
         return l;
     };
     const auto look_up = [&]() MX_INLINE {
@@ -873,9 +877,9 @@ hipError_t launch_tiles(const MxProduct& p, hipStream_t stream) {
 //   1,024                    138   131   114   127   122   161
 //   2,048                    179   170   143   136   130   169
 //   4,096                    283   266   192   199   141   176
-//   8,192                    496   447   310   289   215   192
-//   16,384                   885   800   518   477   313   323
-//   32,768                 1,639 1,472   925   840   549   499
+//   8,192                    496   447   310   289   215   184
+//   16,384                   885   800   518   477   313   310
+//   32,768                 1,639 1,472   925   840   549   481
 // 256 x 256 tiles are for mx_wide products alone: without it they need registers that
 // their waves do not have.
 template <typename F>
