@@ -229,6 +229,7 @@ __device__ __forceinline__ float swiglu(float g, float u) {
 
 struct RowTile {
     uint32_t expert, first, count;  // rows first .. first + count of the sorted order
+    bool alone;                     // all of the expert's rows
 };
 
 // The row tiles of the experts' rows, kRows at a time, found by a wave from the offsets
@@ -282,9 +283,9 @@ struct TileList {
         upto += __builtin_amdgcn_update_dpp(0, upto, 0x118, 0xf, 0xf, true);
         const uint32_t at = __builtin_ctzll(__ballot(upto > left));
         const uint32_t before = at != 0u ? __builtin_amdgcn_readlane(upto, at - 1u) : 0u;
-        const uint32_t first = __builtin_amdgcn_readlane(begin, at) + (left - before) * kRows;
-        const uint32_t count = min(__builtin_amdgcn_readlane(end, at) - first, kRows);
-        return RowTile{group * kPer + at, first, count};
+        const uint32_t from = __builtin_amdgcn_readlane(begin, at), to = __builtin_amdgcn_readlane(end, at);
+        const uint32_t first = from + (left - before) * kRows;
+        return RowTile{group * kPer + at, first, min(to - first, kRows), to - from <= kRows};
     }
 };
 
@@ -333,7 +334,7 @@ struct MxOrder {
 //
 // What bounds it: with few rows the latency of a stage (load, meet, read, multiply: 0.35 us
 // on 64 x 64 tiles); from tens of tokens on the weights' bytes (gate/up of 512 experts, 512
-// tokens: 106 us, 5.4 TB/s of 576 MB); large products the card's power (8,192^3 280 us, 3.9
+// tokens: 94 us, 6.1 TB/s of 576 MB); large products the card's power (8,192^3 280 us, 3.9
 // PFLOP/s at 1.8 GHz) and, with few stages a tile, C's stores and loads that memory answers
 // late: gate/up of 32,768 tokens 481 us, 3.4 PFLOP/s on the rows of its 256-row tiles, 2.9 on
 // those that count (an earlier form of 509 us took 435 without its stores; with four experts'
@@ -367,6 +368,12 @@ __device__ __forceinline__ void mx_load16(const uint8_t* base, uint32_t offset, 
                  "s"(mx_uniform(base)), "s"(lds)
                  : "memory");
 }
+// the same past the caches
+__device__ __forceinline__ void mx_load16_stream(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(offset),
+                 "s"(mx_uniform(base)), "s"(lds)
+                 : "memory");
+}
 __device__ __forceinline__ void mx_load4(const uint8_t* base, uint32_t offset, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset),
                  "s"(mx_uniform(base)), "s"(lds)
@@ -380,7 +387,7 @@ __device__ __forceinline__ void mx_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(kOutstanding) : "memory");
 }
 
-template <typename S, bool kExperts, bool kSwiglu, bool kWide>
+template <typename S, bool kExperts, bool kSwiglu, bool kWide, bool kStream>
 __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 4u) void mx_tile_kernel(MxProduct p) {
     constexpr uint32_t kMF = S::kMF, kTM = S::kTM, kTN = S::kTN, kBM = S::kBM, kBN = S::kBN;
     using Acc = std::conditional_t<kMF == 32u, v16f, v4f>;
@@ -438,7 +445,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     // the next tile to load, the `found`-th from one on, and the sources of its rows of A
     // where they are gathered: looked up a tile ahead, so that nobody waits for them
     uint32_t found = 0, next_column = 0;
-    RowTile next{0u, 0u, 0u};
+    RowTile next{0u, 0u, 0u, false};
     uint32_t data_source[kDataLoads], scale_source[kScaleLoads];
     // On 256 x 256 tiles, which leave no registers over, what follows from the lane alone is
     // computed anew in each use outside the stages (kept from tile to tile, 12 registers went to
@@ -456,7 +463,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         const uint32_t row = order.row();
         next_column = order.column();
         if constexpr (kExperts) next = list.find(row);
-        else next = RowTile{0u, row * kBM, static_cast<uint32_t>(min(p.routes - row * kBM, kBM))};
+        else next = RowTile{0u, row * kBM, static_cast<uint32_t>(min(p.routes - row * kBM, kBM)), false};
         if (own_lane == found % 64u) {
             known_first = next.first;
             known_count = next.count;
@@ -478,7 +485,9 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         }
     };
     // points the loads at the tile that was looked up, and looks up the one after it
+    bool stream = false;  // of the tile being loaded: no other row tile reads this B
     const auto point = [&]() MX_INLINE {
+        stream = kStream && next.alone;
         const uint32_t own_lane = fresh_lane();
         const bool gather = kExperts && p.packed;
         const uint64_t a_first = gather ? 0u : next.first;
@@ -549,8 +558,11 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
             const uint32_t piece = (lane & 7u) ^ ((4u * i + (lane >> 4)) & 7u);
             back = odd && from + 1u == stages && piece >= 4u ? 64u : 0u;
         }
-        mx_load16((t * S::kWaves >= kDataA || i >= kDataA ? b_base : a_base) + (from * 128ull), data[t] - back,
-                  __builtin_amdgcn_readfirstlane(ring_at + to * (S::kSlot * 16u) + i * 1024u));
+        const bool of_a = t * S::kWaves < kDataA && i < kDataA;
+        const uint8_t* base = (of_a ? a_base : b_base) + (from * 128ull);
+        const uint32_t at = __builtin_amdgcn_readfirstlane(ring_at + to * (S::kSlot * 16u) + i * 1024u);
+        if (kStream && stream && !of_a) mx_load16_stream(base, data[t] - back, at);
+        else mx_load16(base, data[t] - back, at);
     };
     // to the next stage to load, at a tile's first stage with a turn to take before its loads;
     // past the last tile the last stage again, into slots that nobody reads any more, so
@@ -846,17 +858,39 @@ bool mx_wide(const MxProduct& p) {
            reinterpret_cast<uintptr_t>(p.b_scales) % 16u == 0u;
 }
 
+// Whether an expert's weights that one row tile reads alone go past the caches: where those
+// of as many experts as may have a row are more than the 256 MB behind the L2s hold.
+// Gate/up of 512 experts and 512 tokens, the same weights call after call, cached / past the
+// caches, by bytes of codes: 201 MB 35.8 / 44.6 us, 268 MB 45.9 / 49.7, 302 MB 60 / 56, 537
+// MB 106 / 94 (6.1 TB/s); 537 MB of which a skewed routing reads 300 57 / 64.  Tiles of 16
+// and 32 rows alone: on 128 rows the choice between two loads costs what it gives (2,048
+// tokens 130 / 129, 4,096 141 / 137, 8,192 of them 212 / 227), so many weights do not come to
+// 64 rows, and in dense products the choice costs more (1 x 8,192 x 2,048 4.4 / 5.9).
+bool mx_streams(const MxProduct& p) {
+    return static_cast<uint64_t>(std::min(p.routes, p.experts)) * p.n * p.k128 * 64u > (256ull << 20);
+}
+
 template <typename S, bool kExperts, bool kSwiglu>
 hipError_t launch_tiles(const MxProduct& p, hipStream_t stream) {
     const uint64_t tiles = (mx_tiles<S>(p, kSwiglu) + kXcds - 1u) / kXcds * kXcds;
     const uint32_t grid = tiles < S::kResident * kCus ? static_cast<uint32_t>(tiles) : S::kResident * kCus;
-    if constexpr (!std::is_same_v<S, Mx256x256>) {
-        if (!mx_wide(p)) {
-            mx_tile_kernel<S, kExperts, kSwiglu, false><<<grid, 64u * S::kWaves, 0, stream>>>(p);
+    const auto launch = [&](auto wide, auto streamed) {
+        mx_tile_kernel<S, kExperts, kSwiglu, decltype(wide)::value, decltype(streamed)::value>
+            <<<grid, 64u * S::kWaves, 0, stream>>>(p);
+    };
+    if constexpr (kExperts && S::kBM <= 32u) {
+        if (mx_wide(p) && mx_streams(p)) {
+            launch(std::true_type{}, std::true_type{});
             return hipGetLastError();
         }
     }
-    mx_tile_kernel<S, kExperts, kSwiglu, true><<<grid, 64u * S::kWaves, 0, stream>>>(p);
+    if constexpr (!std::is_same_v<S, Mx256x256>) {
+        if (!mx_wide(p)) {
+            launch(std::false_type{}, std::false_type{});
+            return hipGetLastError();
+        }
+    }
+    launch(std::true_type{}, std::false_type{});
     return hipGetLastError();
 }
 
@@ -872,10 +906,10 @@ hipError_t launch_tiles(const MxProduct& p, hipStream_t stream) {
 //   8,192 x 8,192 x 8,192  1,409 1,108   638   531   346   280
 // and gate/up (1,024 x 2,048) of 512 experts, top-10, by tokens:
 //   1                        6.6   8.0   7.3   7.2   8.9    15
-//   64                        72    72    72    78    80   114
-//   512                      109   106   105   120   117   160
-//   1,024                    138   131   114   127   122   161
-//   2,048                    179   170   143   136   130   169
+//   64                        65    64    64    77    80   114
+//   512                       96    94    94   121   117   160
+//   1,024                    138   131   106   127   122   161
+//   2,048                    190   175   144   136   130   169
 //   4,096                    283   266   192   199   141   176
 //   8,192                    496   447   310   289   215   184
 //   16,384                   885   800   518   477   313   310

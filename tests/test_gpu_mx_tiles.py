@@ -10,6 +10,7 @@ import pytest
 
 from conftest import load_oracle
 from helpers import device, host, stream, torch
+from test_gpu_mx_layer import decode_rows, random_rows, spread
 from test_gpu_mx import Encoded, check_product, close, encoded, product_bound, run_experts, want_experts, widen
 
 load_oracle()
@@ -90,3 +91,37 @@ def test_least_alignment(q38m, m, n, k, dtype):
     got = widen(words) if dtype == "bf16" else words.view(np.float32).astype(np.float64)
     want, size = mx.product(sides[0][3], sides[1][3])
     close(got, want, product_bound(k, size), dtype, (m, n, k))
+
+
+@pytest.mark.parametrize("swiglu,routes,experts,n,k,kind", [
+    (False, 1396, 1024, 186, 4096, "even"), (True, 1100, 1024, 132, 4096, "even"),           # 16 x 64
+    (False, 600, 512, 1100, 2048, "even"), (True, 600, 512, 1100, 2048, "even"),             # 16 x 128
+    (False, 4000, 512, 1100, 2048, "skewed"), (True, 4000, 512, 1100, 2048, "skewed"),
+    (False, 9000, 512, 1100, 2048, "skewed"), (True, 9000, 512, 1100, 2048, "skewed"),       # 32 x 128
+    (True, 530, 40, 3594, 4096, "skewed")])
+def test_weights_past_the_caches(q38m, swiglu, routes, experts, n, k, kind):
+    """Weights of more than 256 MB: experts of one row tile and of several, compared at rows and
+    columns spread over the whole."""
+    t = torch()
+    print(f"past the caches {routes} of {experts}, {n} x {k} {kind} swiglu {swiglu}", flush=True)
+    rng = np.random.default_rng(routes + n)
+    ids = rng.integers(0, experts, size=(routes, 1)).astype(np.int32)
+    if kind == "skewed":
+        ids[rng.random(ids.shape) < 0.3] //= 64
+    offsets, packed, _ = mx.sort_routes(ids, experts)
+    w, rows = (random_rows(q38m, e, m, k, 122, 124) for e, m in ((experts, n), (1, routes)))
+    columns = n // 2 if swiglu else n
+    at, order = device(offsets), device(packed)
+    c = t.empty(routes, columns, dtype=t.float32, device="cuda")
+    q38m.call("q38m_mx_grouped_gemm_v1", ctypes.byref(w.desc), ctypes.byref(rows.desc), at.data_ptr(),
+              order.data_ptr(), 1, routes, q38m.MX_EPILOGUE_SWIGLU if swiglu else q38m.MX_EPILOGUE_NONE,
+              c.data_ptr(), None, stream(), 0)
+    places, some = spread(routes, 60), spread(columns, 50)
+    got = c[t.as_tensor(places, device="cuda")][:, t.as_tensor(some, device="cuda")].cpu().numpy().astype(np.float64)
+    a = decode_rows(rows, packed[places].astype(np.int64), k)
+    picked = np.concatenate((some, columns + some)) if swiglu else some
+    for i, p in enumerate(places):
+        expert = int(ids[packed[p], 0])
+        want, bound = want_experts(decode_rows(w, expert * n + picked, k), a[i:i + 1], np.array([0, 1]),
+                                   np.zeros(1, np.int64), 0, 1, k, swiglu)
+        close(got[i:i + 1], want, bound, "f32", (p, expert))
