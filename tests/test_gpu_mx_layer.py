@@ -345,10 +345,12 @@ def test_large_experts(q38m):
         close(got[i:i + 1], want, product_bound(k, size), "f32", (p, expert))
 
 
-def test_large_rows(q38m):
-    """560,000 routes of 8,192 bf16 values: 9.2 GB of rows, there, back and the gradients."""
+@pytest.mark.parametrize("width", [8192, 1201])
+def test_large_rows(q38m, width):
+    """560,000 routes of bf16 rows, 9.2 GB of them at 8,192 values and an odd start for every
+    second row at 1,201: there, back and the gradients."""
     t = torch()
-    tokens, top_k, experts, width = 70000, 8, 300, 8192
+    tokens, top_k, experts = 70000, 8, 300
     routes = tokens * top_k
     ids = t.randint(-20, experts, (tokens, top_k), dtype=t.int32, device="cuda")
     s = q38m.SortedRoutes(tokens, top_k, experts).sort(ids)
