@@ -362,22 +362,24 @@ __device__ __forceinline__ const uint8_t* mx_uniform(const uint8_t* p) {
     return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(high) << 32 | low);
 }
 
-// 16 bytes (4 bytes) a lane from base + offset to consecutive LDS from byte `lds` on
+// 16 bytes (4 bytes) a lane from base + offset to consecutive LDS from byte `lds` on.  The
+// compiler does not look into asm for the waits that its loads need: a scalar register that
+// a vector instruction wrote (mx_uniform's lane reads) is read five wait states later at the
+// earliest, m0 one after its write.  s_nop 3 is four, the move of m0 one.
+#define MX_LOAD_LDS(INSTRUCTION)                                       \
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\t" INSTRUCTION        \
+                 :                                                     \
+                 : "v"(offset), "s"(mx_uniform(base)), "s"(lds)        \
+                 : "memory")
 __device__ __forceinline__ void mx_load16(const uint8_t* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(offset),
-                 "s"(mx_uniform(base)), "s"(lds)
-                 : "memory");
+    MX_LOAD_LDS("global_load_lds_dwordx4 %0, %1");
 }
 // the same past the caches
 __device__ __forceinline__ void mx_load16_stream(const uint8_t* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(offset),
-                 "s"(mx_uniform(base)), "s"(lds)
-                 : "memory");
+    MX_LOAD_LDS("global_load_lds_dwordx4 %0, %1 nt");
 }
 __device__ __forceinline__ void mx_load4(const uint8_t* base, uint32_t offset, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(offset),
-                 "s"(mx_uniform(base)), "s"(lds)
-                 : "memory");
+    MX_LOAD_LDS("global_load_lds_dword %0, %1");
 }
 
 // until at most kOutstanding of the wave's loads are in flight and its LDS reads are

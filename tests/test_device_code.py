@@ -1,0 +1,60 @@
+"""The built library's device code keeps the waits that gfx950 leaves to the
+program.  The compiler inserts them for its own instructions; it does not look
+into inline assembly, where the products' loads to LDS are."""
+import pytest
+
+import device_code as dc
+
+LISTING = """
+0000000000000100 <kernel>:
+\tv_readfirstlane_b32 s4, v0        // 000000000100: 7E080500
+\tv_readfirstlane_b32 s5, v1        // 000000000104: 7E0A0501
+\ts_mov_b32 m0, s9                  // 000000000108: BEFC0009
+\ts_nop {0}                         // 00000000010C: BF800000
+\tglobal_load_lds_dwordx4 v3, s[4:5] // 000000000110: DDF48000 00040003
+\ts_cbranch_scc1 65531               // 000000000118: BF85FFFB <kernel+0x8>
+\ts_endpgm                          // 00000000011C: BF810000
+"""
+
+
+def scalar_m0(i):
+    return {"m0"} if i.name.startswith("s_") and i.operands[0] == "m0" else set()
+
+
+def lds_load(i):
+    return {"m0"} if "_lds_" in i.name and i.name.startswith(("global", "buffer")) else set()
+
+
+@pytest.mark.parametrize("nop,soon", [(0, ["s4", "s5"]), (2, ["s5"]), (3, [])])
+def test_the_check_counts(nop, soon):
+    """Wait states between the reads of lanes and the load: 1 + (nop + 1), one more for s4."""
+    found = dc.too_soon(dc.parse(LISTING.format(nop)), dc.memory_reads, dc.vector_writes, 5)
+    assert sorted(w.operands[0] for w, _ in found) == soon
+
+
+def test_the_check_follows_branches():
+    """The branch back to 0x108 leaves a write at 0x114 three wait states in front of the load."""
+    text = LISTING.format(0).replace("\ts_cbranch", "\tv_readlane_b32 s4, v9, 0 // 000000000114: D289\n\ts_cbranch")
+    found = dc.too_soon(dc.parse(text), dc.memory_reads, dc.vector_writes, 5)
+    assert 0x114 in {w.address for w, _ in found}
+
+
+@pytest.fixture(scope="module")
+def objects(q38m, tmp_path_factory):
+    found = dc.code_objects(q38m.LIB_PATH, tmp_path_factory.mktemp("code"))
+    assert len(found) >= 11  # one for each source
+    return [(o, dc.disassemble(o)) for o in found]
+
+
+def test_scalar_operands_of_memory_instructions_have_settled(objects):
+    """A scalar register that a vector instruction writes is read by a vector memory instruction
+    no earlier than five wait states later, m0 by a load to LDS one after a scalar write: the
+    hardware does not hold these back."""
+    loads = 0
+    for _, code in objects:
+        loads += sum(bool(lds_load(i)) for i in code)
+        for reads, writes, states in ((dc.memory_reads, dc.vector_writes, 5), (lds_load, scalar_m0, 1)):
+            found = dc.too_soon(code, reads, writes, states)
+            assert not found, [(w.kernel, hex(w.address), w.name, w.operands, hex(r.address), r.name, r.operands)
+                               for w, r in found[:3]] + [len(found)]
+    assert loads > 500  # the listing shows them
