@@ -370,7 +370,7 @@ __device__ __forceinline__ const uint8_t* mx_uniform(const uint8_t* p) {
     asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\t" INSTRUCTION        \
                  :                                                     \
                  : "v"(offset), "s"(mx_uniform(base)), "s"(lds)        \
-                 : "memory")
+                 : "memory", "m0")
 __device__ __forceinline__ void mx_load16(const uint8_t* base, uint32_t offset, uint32_t lds) {
     MX_LOAD_LDS("global_load_lds_dwordx4 %0, %1");
 }

@@ -1,9 +1,13 @@
 """The built library's device code keeps the waits that gfx950 leaves to the
 program.  The compiler inserts them for its own instructions; it does not look
 into inline assembly, where the products' loads to LDS are."""
+import os
+import re
+
 import pytest
 
 import device_code as dc
+from conftest import PACKAGE_DIR
 
 LISTING = """
 0000000000000100 <kernel>:
@@ -58,3 +62,36 @@ def test_scalar_operands_of_memory_instructions_have_settled(objects):
             assert not found, [(w.kernel, hex(w.address), w.name, w.operands, hex(r.address), r.name, r.operands)
                                for w, r in found[:3]] + [len(found)]
     assert loads > 500  # the listing shows them
+
+
+def test_m0_belongs_to_the_loads(objects):
+    """Every load to LDS has its own write of m0 right in front, and nothing else reads m0: no
+    value that the compiler keeps there is lost."""
+    for _, code in objects:
+        for k, i in enumerate(code):
+            if lds_load(i):
+                setting = next(p for p in reversed(code[:k]) if p.name != "s_nop")
+                assert scalar_m0(setting), (i.kernel, hex(i.address))
+            else:
+                reads = i.operands[1:] if scalar_m0(i) else i.operands
+                assert not any("m0" in dc.scalar_registers(o) for o in reads), (i.kernel, hex(i.address), i.name)
+
+
+def test_inline_assembly_names_what_it_writes():
+    """m0 is among the clobbers of every inline assembly that sets it."""
+    folder = os.path.join(PACKAGE_DIR, "csrc")
+    found = 0
+    for name in sorted(os.listdir(folder)):
+        text = open(os.path.join(folder, name)).read()
+        for start in (m.start() for m in re.finditer(r"\basm\b", text)):
+            depth, end = 0, text.index("(", start)
+            while True:
+                depth += {"(": 1, ")": -1}.get(text[end], 0)
+                end += 1
+                if depth == 0:
+                    break
+            statement = text[start:end]
+            if re.search(r"s_mov_b32 m0", statement):
+                found += 1
+                assert '"m0"' in statement, (name, statement)
+    assert found >= 2
