@@ -95,3 +95,12 @@ def test_inline_assembly_names_what_it_writes():
                 found += 1
                 assert '"m0"' in statement, (name, statement)
     assert found >= 2
+
+
+def test_product_kernels_keep_their_registers(objects):
+    """No microscaled kernel keeps a vector register in memory: 256 x 256 tiles have none to
+    spare, and a compiler that spills there would put memory into the innermost loop."""
+    kernels = {name: r for path, _ in objects for name, r in dc.resources(path).items() if "mx_" in name}
+    assert len([name for name in kernels if "mx_tile_kernel" in name]) >= 36
+    for name, r in kernels.items():
+        assert r["private_segment_fixed_size"] == 0 and r["vgpr_spill_count"] == 0, (name, r)
