@@ -651,7 +651,8 @@ int q38m_mx_gemm_v1(const q38m_mx_matrix_v1* a, const q38m_mx_matrix_v1* b,
  * an expert whose end is not behind its begin has no rows.
  * epilogue SWIGLU: weights' first half of rows is gate, the second half up;
  * C has half as many columns, h = g / (1 + exp(-g)) * u in fp32, rounded
- * once.  C is contiguous.  Rows of C that no expert has (dropped routes) are
+ * once: within 8 fp32 roundings, bf16 within 2^-17 h before its own; a zero
+ * where exp(-g) is past fp32 (g below -88.7).  C is contiguous.  Rows of C that no expert has (dropped routes) are
  * left as they were; a src(p) past A's rows reads A's last row.  One expert's
  * codes, and those of gathered rows, are below 4 GB. */
 #define Q38M_MX_EPILOGUE_NONE 0u

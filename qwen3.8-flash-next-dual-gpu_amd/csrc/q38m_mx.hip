@@ -205,23 +205,26 @@ __device__ __forceinline__ v16f mfma_mx(v4i a, uint32_t sa, v4i b, uint32_t sb, 
 }
 
 // h = g / (1 + exp(-g)) u on the base-2 exponential and reciprocal instructions (one
-// unit in the last place each).  The exponential's argument is held to 88, where it is
-// still finite: below g = -88 h is within 2^-126 |g u| of the formula's.  kExact puts the
-// rounding of -g log2 e back: within 8 roundings of h; without it, |g| roundings more,
-// 2^-17 of h at most, far below half a step of bf16.  (The contract's exp and an IEEE
-// division take three times the instructions: 32,768-token gate/up 750 -> 640 us.)
+// unit in the last place each).  The reciprocal gives zero in place of a result below the
+// smallest normal, so it is taken of a quarter of the sum, whose reciprocal never is, and a
+// multiplication takes the quarter back.  An exponential past 2^128 is infinite and h a zero,
+// as in the formula in fp32.  kExact puts the rounding of -g log2 e back (of an argument
+// held to where the exponential is long infinite or zero): within 8 roundings of h; without
+// it, |g| roundings more, 2^-17 of h at most, far below half a step of bf16.  (The contract's
+// exp and an IEEE division take three times the instructions: an earlier form of the
+// 32,768-token gate/up took 750 us with them and 640 without.)
 template <bool kExact>
 __device__ __forceinline__ float swiglu(float g, float u) {
     constexpr float kLog2e = 1.44269502162933349609375f;  // and what it lacks of log2 e
     constexpr float kLog2eLow = 1.92596299112661746887e-8f;
-    const float x = -__builtin_amdgcn_fmed3f(g, -88.0f, 88.0f);
+    const float x = kExact ? -__builtin_amdgcn_fmed3f(g, -128.0f, 128.0f) : -g;
     const float a = x * kLog2e;
     float e = __builtin_amdgcn_exp2f(a);
     if constexpr (kExact) {
         const float low = __builtin_fmaf(x, kLog2eLow, __builtin_fmaf(x, kLog2e, -a));
-        e = __builtin_fmaf(e * low, 0.693147180559945309f, e);
+        e = __builtin_fmaf(fminf(e, 0x1p127f) * low, 0.693147180559945309f, e);  // infinite stays
     }
-    return g * __builtin_amdgcn_rcpf(1.0f + e) * u;
+    return g * (0.25f * __builtin_amdgcn_rcpf(__builtin_fmaf(e, 0.25f, 0.25f))) * u;
 }
 
 // the kernel's steps, which share its registers
