@@ -286,11 +286,6 @@ struct MxProduct {
     uint64_t c_stride;
     uint32_t a_rows, routes, n, k128, experts, top_k;  // routes: C's rows
 };
-// row tiles that `routes` rows over `experts` experts need at most
-constexpr uint32_t mx_max_tasks(uint32_t routes, uint32_t experts, uint32_t tile) {
-    const uint32_t first = routes < experts ? routes : experts;
-    return first + (routes - first) / tile;
-}
 // whether the launch's grid holds the product
 bool mx_product_fits(const MxProduct& p, bool swiglu);
 hipError_t launch_mx_product(const MxProduct& p, bool swiglu, hipStream_t stream);

@@ -5,15 +5,15 @@
 // low nibble; codes past K are zero) and one scale byte for every 32 values.
 // Code c stands for (-1)^(c >> 3) * {0, .5, 1, 1.5, 2, 3, 4, 6}[c & 7], scale
 // byte s for 2^(s - 127), 255 for NaN.
-#include <algorithm>
-#include <cmath>
-#include <iterator>
 #include <type_traits>
 
 #include "q38m_device.h"
 #include "q38m_internal.h"
+#include "q38m_mx_tiles.h"
 
 namespace q38m {
+
+static_assert(kMxMaxExperts == kMaxSortExperts, "the offsets that the tiles keep");
 
 namespace {
 
@@ -299,17 +299,17 @@ struct TileList {
 // B.  (Each a run of consecutive tiles, with the same rows of A: gate/up of 512 experts
 // 112 instead of 108 us for 512 tokens, 316 instead of 182 for 2,048, 968 instead of 608
 // for 32,768: the workgroups stream B at different places.)
-constexpr uint32_t kXcds = 8, kCus = 256, kGroup = 4;
+constexpr uint32_t kGroup = 4;
 struct MxOrder {
     uint32_t rows, columns;   // of tiles
     uint32_t at, step, count;  // this workgroup's tiles
 
     __device__ MX_INLINE MxOrder(uint32_t rows_, uint32_t columns_) : rows(rows_), columns(columns_) {
         const uint64_t all = static_cast<uint64_t>(rows) * columns;
-        const uint32_t xcd = blockIdx.x % kXcds;
-        step = gridDim.x / kXcds;
-        at = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(xcd * all / kXcds)) + blockIdx.x / kXcds;
-        const uint32_t end = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>((xcd + 1u) * all / kXcds));
+        const uint32_t xcd = blockIdx.x % kMxXcds;
+        step = gridDim.x / kMxXcds;
+        at = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(xcd * all / kMxXcds)) + blockIdx.x / kMxXcds;
+        const uint32_t end = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>((xcd + 1u) * all / kMxXcds));
         count = at < end ? (end - at + step - 1u) / step : 0u;
     }
     __device__ MX_INLINE uint32_t height() const { return min(kGroup, rows - at / (kGroup * columns) * kGroup); }
@@ -318,6 +318,40 @@ struct MxOrder {
     }
     __device__ MX_INLINE uint32_t column() const { return at % (kGroup * columns) / height(); }
 };
+
+__device__ __forceinline__ const uint8_t* mx_uniform(const uint8_t* p) {
+    const uint64_t v = reinterpret_cast<uint64_t>(p);
+    const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
+    const uint32_t high = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
+    return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(high) << 32 | low);
+}
+
+// 16 bytes (4 bytes) a lane from base + offset to consecutive LDS from byte `lds` on.  The
+// compiler does not look into asm for the waits that its loads need: a scalar register that
+// a vector instruction wrote (mx_uniform's lane reads) is read five wait states later at the
+// earliest, m0 one after its write.  s_nop 3 is four, the move of m0 one.
+#define MX_LOAD_LDS(INSTRUCTION)                                       \
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\t" INSTRUCTION         \
+                 :                                                     \
+                 : "v"(offset), "s"(mx_uniform(base)), "s"(lds)        \
+                 : "memory", "m0")
+__device__ __forceinline__ void mx_load16(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    MX_LOAD_LDS("global_load_lds_dwordx4 %0, %1");
+}
+// the same past the caches
+__device__ __forceinline__ void mx_load16_stream(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    MX_LOAD_LDS("global_load_lds_dwordx4 %0, %1 nt");
+}
+__device__ __forceinline__ void mx_load4(const uint8_t* base, uint32_t offset, uint32_t lds) {
+    MX_LOAD_LDS("global_load_lds_dword %0, %1");
+}
+
+// until at most kOutstanding of the wave's loads are in flight and its LDS reads are
+// complete, then for the workgroup's waves to get there
+template <uint32_t kOutstanding>
+__device__ __forceinline__ void mx_barrier() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(kOutstanding) : "memory");
+}
 
 // Workgroups stay and compute tile after tile of kBM rows of C by kBN rows of B (with
 // the SwiGLU fold half of them gate, half up rows), kWM x kWN waves, each kTM x kTN
@@ -342,56 +376,6 @@ struct MxOrder {
 // late: gate/up of 32,768 tokens 481 us, 3.4 PFLOP/s on the rows of its 256-row tiles, 2.9 on
 // those that count (an earlier form of 509 us took 435 without its stores; with four experts'
 // weights alone, which the L2s hold, 467 instead of 507).
-template <uint32_t kMF_, uint32_t kWM_, uint32_t kWN_, uint32_t kTM_, uint32_t kTN_, uint32_t kStages_>
-struct MxShape {
-    static constexpr uint32_t kMF = kMF_, kWM = kWM_, kWN = kWN_, kTM = kTM_, kTN = kTN_;
-    static constexpr uint32_t kStages = kStages_, kWaves = kWM * kWN;
-    static constexpr uint32_t kBM = kWM * kTM * kMF, kBN = kWN * kTN * kMF, kRows = kBM + kBN;
-    static constexpr uint32_t kSteps = kMF / 8u;  // matrix instructions deep: 2 or 4
-    // 16-byte words of LDS: the ring, the scales' and the experts' offsets.  The scales
-    // of kStages stages may be under way: half as many pairs, begun and ended ones
-    static constexpr uint32_t kSlot = kRows * 8u, kScaleAt = kStages * kSlot;
-    static constexpr uint32_t kScaleWords = (kStages / 2u + 1u) * kRows;
-    static constexpr uint32_t kOffsetsAt = kScaleAt + kScaleWords;
-    static constexpr uint32_t kLds = kOffsetsAt + kMaxSortExperts / 4u;
-    static constexpr uint32_t kResident = 160u * 64u / kLds;  // workgroups a CU
-    static_assert(kResident != 0u, "160 KB of LDS");
-};
-
-__device__ __forceinline__ const uint8_t* mx_uniform(const uint8_t* p) {
-    const uint64_t v = reinterpret_cast<uint64_t>(p);
-    const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v));
-    const uint32_t high = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(v >> 32));
-    return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(high) << 32 | low);
-}
-
-// 16 bytes (4 bytes) a lane from base + offset to consecutive LDS from byte `lds` on.  The
-// compiler does not look into asm for the waits that its loads need: a scalar register that
-// a vector instruction wrote (mx_uniform's lane reads) is read five wait states later at the
-// earliest, m0 one after its write.  s_nop 3 is four, the move of m0 one.
-#define MX_LOAD_LDS(INSTRUCTION)                                       \
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\t" INSTRUCTION        \
-                 :                                                     \
-                 : "v"(offset), "s"(mx_uniform(base)), "s"(lds)        \
-                 : "memory", "m0")
-__device__ __forceinline__ void mx_load16(const uint8_t* base, uint32_t offset, uint32_t lds) {
-    MX_LOAD_LDS("global_load_lds_dwordx4 %0, %1");
-}
-// the same past the caches
-__device__ __forceinline__ void mx_load16_stream(const uint8_t* base, uint32_t offset, uint32_t lds) {
-    MX_LOAD_LDS("global_load_lds_dwordx4 %0, %1 nt");
-}
-__device__ __forceinline__ void mx_load4(const uint8_t* base, uint32_t offset, uint32_t lds) {
-    MX_LOAD_LDS("global_load_lds_dword %0, %1");
-}
-
-// until at most kOutstanding of the wave's loads are in flight and its LDS reads are
-// complete, then for the workgroup's waves to get there
-template <uint32_t kOutstanding>
-__device__ __forceinline__ void mx_barrier() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(kOutstanding) : "memory");
-}
-
 template <typename S, bool kExperts, bool kSwiglu, bool kWide, bool kStream>
 __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 4u) void mx_tile_kernel(MxProduct p) {
     constexpr uint32_t kMF = S::kMF, kTM = S::kTM, kTN = S::kTN, kBM = S::kBM, kBN = S::kBN;
@@ -805,13 +789,6 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     mx_barrier<0>();  // no load is under way to LDS that the next workgroup gets
 }
 
-using Mx256x256 = MxShape<32, 4, 2, 2, 4, 2>;
-using Mx128x128 = MxShape<32, 2, 2, 2, 2, 2>;
-using Mx64x64 = MxShape<16, 2, 2, 2, 2, 3>;
-using Mx32x128 = MxShape<16, 1, 4, 2, 2, 3>;
-using Mx16x128 = MxShape<16, 1, 4, 1, 2, 3>;
-using Mx16x64 = MxShape<16, 1, 2, 1, 2, 4>;
-
 }  // namespace
 
 hipError_t launch_mx_quantize(const void* x, uint32_t dtype, uint64_t stride, uint32_t rows,
@@ -833,108 +810,31 @@ hipError_t launch_mx_quantize(const void* x, uint32_t dtype, uint64_t stride, ui
 
 namespace {
 
-// tiles: a bound where the experts' rows are known to the device alone
-template <typename S>
-uint64_t mx_tiles(const MxProduct& p, bool swiglu) {
-    const uint64_t across = swiglu ? S::kBN / 2u : S::kBN, n_out = swiglu ? p.n / 2u : p.n;
-    const uint64_t rows = p.offsets ? mx_max_tasks(p.routes, p.experts, S::kBM)
-                                    : (static_cast<uint64_t>(p.routes) + S::kBM - 1u) / S::kBM;
-    return rows * ((n_out + across - 1u) / across);
-}
-
-// What a stage of all tiles takes, us: `each` for every 256 tiles.  An expert's last row
-// tile is taken to be half full.
-template <typename S>
-float stage_us(const MxProduct& p, bool swiglu, float each) {
-    const uint32_t across = swiglu ? S::kBN / 2u : S::kBN, n_out = swiglu ? p.n / 2u : p.n;
-    float rows = static_cast<float>((p.routes + S::kBM - 1u) / S::kBM);
-    if (p.offsets) {
-        const float active = static_cast<float>(p.routes < p.experts ? p.routes : p.experts);
-        const float of_each = static_cast<float>(p.routes) / active / S::kBM + 0.5f;
-        rows = active * (of_each > 1.0f ? of_each : 1.0f);
-    }
-    const float tiles = rows * static_cast<float>((n_out + across - 1u) / across);
-    return each * std::ceil(tiles / 256.0f);
-}
-
-// a row's scales of two stages are one 16-byte piece
-bool mx_wide(const MxProduct& p) {
-    return p.k128 % 4u == 0u && reinterpret_cast<uintptr_t>(p.a_scales) % 16u == 0u &&
-           reinterpret_cast<uintptr_t>(p.b_scales) % 16u == 0u;
-}
-
-// Whether an expert's weights that one row tile reads alone go past the caches: where those
-// of as many experts as may have a row are more than the 256 MB behind the L2s hold.
-// Gate/up of 512 experts and 512 tokens, the same weights call after call, cached / past the
-// caches, by bytes of codes: 201 MB 35.8 / 44.6 us, 268 MB 45.9 / 49.7, 302 MB 60 / 56, 537
-// MB 106 / 94 (6.1 TB/s); 537 MB of which a skewed routing reads 300 57 / 64.  Tiles of 16
-// and 32 rows alone: on 128 rows the choice between two loads costs what it gives (2,048
-// tokens 130 / 129, 4,096 141 / 137, 8,192 of them 212 / 227), so many weights do not come to
-// 64 rows, and in dense products the choice costs more (1 x 8,192 x 2,048 4.4 / 5.9).
-bool mx_streams(const MxProduct& p) {
-    return static_cast<uint64_t>(std::min(p.routes, p.experts)) * p.n * p.k128 * 64u > (256ull << 20);
+MxSizes sizes_of(const MxProduct& p, bool swiglu) {
+    return MxSizes{p.routes, p.n, p.k128, p.offsets ? p.experts : 0u, swiglu,
+                   mx_wide(p.k128, reinterpret_cast<uintptr_t>(p.a_scales), reinterpret_cast<uintptr_t>(p.b_scales))};
 }
 
 template <typename S, bool kExperts, bool kSwiglu>
-hipError_t launch_tiles(const MxProduct& p, hipStream_t stream) {
-    const uint64_t tiles = (mx_tiles<S>(p, kSwiglu) + kXcds - 1u) / kXcds * kXcds;
-    const uint32_t grid = tiles < S::kResident * kCus ? static_cast<uint32_t>(tiles) : S::kResident * kCus;
+hipError_t launch_tiles(const MxProduct& p, const MxSizes& sizes, hipStream_t stream) {
     const auto launch = [&](auto wide, auto streamed) {
         mx_tile_kernel<S, kExperts, kSwiglu, decltype(wide)::value, decltype(streamed)::value>
-            <<<grid, 64u * S::kWaves, 0, stream>>>(p);
+            <<<mx_grid<S>(sizes), 64u * S::kWaves, 0, stream>>>(p);
     };
     if constexpr (kExperts && S::kBM <= 32u) {
-        if (mx_wide(p) && mx_streams(p)) {
+        if (mx_streams<S>(sizes)) {
             launch(std::true_type{}, std::true_type{});
             return hipGetLastError();
         }
     }
     if constexpr (!std::is_same_v<S, Mx256x256>) {
-        if (!mx_wide(p)) {
+        if (!sizes.wide) {
             launch(std::false_type{}, std::false_type{});
             return hipGetLastError();
         }
     }
     launch(std::true_type{}, std::false_type{});
     return hipGetLastError();
-}
-
-// Calls f with the shape that a product runs on, the one with the shortest stage.  The
-// figures of `each` are fitted to these, us on 16 x 64, 16 x 128, 32 x 128, 64 x 64, 128 x
-// 128 and 256 x 256 tiles:
-//   1 x 8,192 x 2,048        4.5   5.1   5.2   5.2   6.8    13
-//   32 x 4,096 x 4,096       6.2   7.6   7.7   7.4    10    21
-//   256 x 4,096 x 4,096       14    13   9.3   8.7    12    24
-//   509 x 2,048 x 8,192       25    23    16    14    20    43
-//   1,024 x 4,096 x 4,096     44    42    26    21    17    28
-//   4,096 x 4,096 x 4,096    158   155    96    81    49    41
-//   8,192 x 8,192 x 8,192  1,409 1,108   638   531   346   280
-// and gate/up (1,024 x 2,048) of 512 experts, top-10, by tokens:
-//   1                        6.6   8.0   7.3   7.2   8.9    15
-//   64                        65    64    64    77    80   114
-//   512                       96    94    94   121   117   160
-//   1,024                    138   131   106   127   122   161
-//   2,048                    190   175   144   136   130   169
-//   4,096                    283   266   192   199   141   176
-//   8,192                    496   447   310   289   215   184
-//   16,384                   885   800   518   477   313   310
-//   32,768                 1,639 1,472   925   840   549   481
-// 256 x 256 tiles are for mx_wide products alone: without it they need registers that
-// their waves do not have.
-template <typename F>
-auto with_tiles(const MxProduct& p, bool swiglu, F f) {
-    const float us[] = {stage_us<Mx16x64>(p, swiglu, 0.2f),   stage_us<Mx16x128>(p, swiglu, 0.33f),
-                        stage_us<Mx32x128>(p, swiglu, 0.45f), stage_us<Mx64x64>(p, swiglu, 0.38f),
-                        stage_us<Mx128x128>(p, swiglu, 0.66f),
-                        stage_us<Mx256x256>(p, swiglu, mx_wide(p) ? 2.0f : 1e30f)};
-    switch (std::min_element(std::begin(us), std::end(us)) - us) {
-        case 0: return f(Mx16x64{});
-        case 1: return f(Mx16x128{});
-        case 2: return f(Mx32x128{});
-        case 3: return f(Mx64x64{});
-        case 4: return f(Mx128x128{});
-        default: return f(Mx256x256{});
-    }
 }
 
 }  // namespace
@@ -947,14 +847,18 @@ bool mx_product_fits(const MxProduct& p, bool swiglu) {
     const uint64_t b_rows = swiglu ? p.n : 256u, a_rows = p.packed ? p.a_rows : 256u;
     return p.n <= (1u << 28) && p.routes <= (1u << 28) && b_rows * row_bytes < (1ull << 32) &&
            a_rows * row_bytes < (1ull << 32) &&
-           with_tiles(p, swiglu, [&](auto s) { return mx_tiles<decltype(s)>(p, swiglu) < (1ull << 31); });
+           with_mx_tiles(sizes_of(p, swiglu), [&](auto s) {
+               return mx_tiles<decltype(s)>(sizes_of(p, swiglu)) < (1ull << 31);
+           });
 }
 
 hipError_t launch_mx_product(const MxProduct& p, bool swiglu, hipStream_t stream) {
-    return with_tiles(p, swiglu, [&](auto s) {
+    const MxSizes sizes = sizes_of(p, swiglu);
+    return with_mx_tiles(sizes, [&](auto s) {
         using S = decltype(s);
-        if (!p.offsets) return launch_tiles<S, false, false>(p, stream);
-        return swiglu ? launch_tiles<S, true, true>(p, stream) : launch_tiles<S, true, false>(p, stream);
+        if (!p.offsets) return launch_tiles<S, false, false>(p, sizes, stream);
+        return swiglu ? launch_tiles<S, true, true>(p, sizes, stream)
+                      : launch_tiles<S, true, false>(p, sizes, stream);
     });
 }
 
