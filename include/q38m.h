@@ -628,15 +628,18 @@ size_t q38m_mx_scale_bytes(uint32_t columns);
  * NULL, or the values that the codes stand for (exact in either type, NaN
  * where s = 255), contiguous rows of x's type -- what the products compute
  * with, for training with the rounding in the loop and for error
- * measurements. */
+ * measurements.  x_stride >= columns <= 2^24; experts * rows <= 2^23, more
+ * take several calls on parts of the buffers. */
 int q38m_mx_quantize_v1(const void* x, uint32_t dtype, uint64_t x_stride,
                         const q38m_mx_matrix_v1* dst, void* rounded, void* stream,
                         int device);
 
 /* C[m][n] = sum over k of A[m][k] * B[n][k], fp32 sums, one rounding (bf16:
  * to nearest even); exactly one of c_f32 / c_bf16, c_stride elements from
- * row to row.  a and b: experts = 1, equal columns.  Floating-point parity:
- * products and scales are exact, the order of the sum is the kernels'. */
+ * row to row.  a and b: experts = 1, equal columns <= 2^24, each at most 2^28
+ * rows, C fewer than 2^31 tiles (16 x 64 to 256 x 256 values, by the sizes).
+ * Floating-point parity: products and scales are exact, the order of the sum
+ * is the kernels'. */
 int q38m_mx_gemm_v1(const q38m_mx_matrix_v1* a, const q38m_mx_matrix_v1* b,
                     float* c_f32, uint16_t* c_bf16, uint64_t c_stride,
                     void* stream, int device);
@@ -653,8 +656,10 @@ int q38m_mx_gemm_v1(const q38m_mx_matrix_v1* a, const q38m_mx_matrix_v1* b,
  * C has half as many columns, h = g / (1 + exp(-g)) * u in fp32, rounded
  * once: within 8 fp32 roundings, bf16 within 2^-17 h before its own; a zero
  * where exp(-g) is past fp32 (g below -88.7).  C is contiguous.  Rows of C that no expert has (dropped routes) are
- * left as they were; a src(p) past A's rows reads A's last row.  One expert's
- * codes, and those of gathered rows, are below 4 GB. */
+ * left as they were; a src(p) past A's rows reads A's last row.  At most 1024
+ * experts, fewer than 2^24 routes, weights of at most 2^28 rows an expert,
+ * columns <= 2^24, fewer than 2^31 tiles of C; one expert's codes, and those
+ * of gathered rows, are below 4 GB. */
 #define Q38M_MX_EPILOGUE_NONE 0u
 #define Q38M_MX_EPILOGUE_SWIGLU 1u
 int q38m_mx_grouped_gemm_v1(const q38m_mx_matrix_v1* weights,
@@ -669,7 +674,8 @@ int q38m_mx_grouped_gemm_v1(const q38m_mx_matrix_v1* weights,
  * 101-104: expert-major, stable in the route index token * top_k + rank) for
  * any number of tokens, experts and ranks, in bf16 or fp32, with routes that
  * no expert takes, and the derivatives that training wants.
- * 1 <= experts <= 1024, top_k >= 1, tokens * top_k < 2^24.
+ * 1 <= experts <= 1024, top_k >= 1, 1 <= tokens * top_k < 2^24,
+ * 1 <= width <= 2^24.
  *
  * expert_ids int32 [tokens][top_k]; an id outside [0, experts) drops its
  * route.  Writes expert_offsets [experts + 1] (the last: the kept routes),

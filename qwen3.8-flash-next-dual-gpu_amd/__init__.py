@@ -472,7 +472,8 @@ class MxRows:
 
 def mx_quantize(x, experts=1, rounded=None, stream=None):
     """x [experts * rows][columns] on a GPU (bf16, raw bf16 words in 16-bit integers, or fp32;
-    any row stride, columns side by side) as MxRows.  rounded: None, or a contiguous tensor like
+    columns side by side, rows any stride apart but not one over the other; at most 2^23) as
+    MxRows.  rounded: None, or a contiguous tensor like
     x that gets the values the codes stand for."""
     torch = _torch()
     words = (torch.bfloat16, torch.int16, torch.uint16)

@@ -266,7 +266,7 @@ hipError_t launch_unpermute_backward(const void* dy, const void* rows, uint32_t 
                                      void* d_rows, float* d_weights, hipStream_t stream);
 
 // microscaled 4-bit rows (q38m_mx.hip)
-constexpr uint32_t kMaxMxRows = 1u << 23;  // a workgroup per row: grids below 2^32 threads
+constexpr uint32_t kMaxMxRows = 1u << 23;  // a workgroup per row: 2^31 threads, half of what a grid may have
 constexpr uint32_t mx_k128(uint32_t columns) { return (columns + 127u) / 128u; }
 // rounded may be null
 hipError_t launch_mx_quantize(const void* x, uint32_t dtype, uint64_t stride, uint32_t rows,
