@@ -248,6 +248,7 @@ CHECK_EXPERT = 1
 CHECK_TASK_ROWS = 2
 CHECK_ROUTE = 4
 CHECK_TOKEN = 8
+CHECK_OFFSETS = 16
 
 
 class PhaseRecord(ctypes.Structure):

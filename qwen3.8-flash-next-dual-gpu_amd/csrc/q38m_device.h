@@ -41,12 +41,15 @@ __device__ __forceinline__ uint2 load_stream(const uint2* p) {
 // of this translation unit (each unit has its own; q38m_checked_status_v1
 // ORs them) and is replaced by 0, an in-range value, so the kernel completes
 // without touching memory outside its buffers -- it never traps.  In the
-// product build checked() is the value itself.
+// product build checked() is the value itself.  Kernels whose contract says
+// what a value out of range does (skipped, held to the range) report it and
+// do that.
 enum CheckBit : uint32_t {
     kCheckExpert = 1u,    // task expert >= 512
     kCheckTaskRows = 2u,  // task rows > the largest task (128)
     kCheckRoute = 4u,     // inverse (assignment -> packed) index >= routes
-    kCheckToken = 8u,     // packed route index past the largest chunk
+    kCheckToken = 8u,     // packed route index past the largest chunk, or of no token row
+    kCheckOffsets = 16u,  // expert offsets that fall or lie past the routes
 };
 
 #ifdef Q38M_CHECKED
@@ -82,6 +85,16 @@ __device__ __forceinline__ uint32_t checked(uint32_t v, uint32_t limit, CheckBit
     (void)bit;
 #endif
     return v;
+}
+
+// sets the bit in the checked build alone
+__device__ __forceinline__ void report(bool out_of_range, CheckBit bit) {
+#ifdef Q38M_CHECKED
+    if (out_of_range) atomicOr(&g_checked_status, static_cast<uint32_t>(bit));
+#else
+    (void)out_of_range;
+    (void)bit;
+#endif
 }
 
 // ---- plan tasks ------------------------------------------------------------

@@ -397,6 +397,16 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         for (uint32_t e = threadIdx.x; e < kMaxSortExperts; e += 64u * S::kWaves)
             offsets[e] = e < p.experts ? p.offsets[e] : last_offset;
         __syncthreads();
+#ifdef Q38M_CHECKED
+        for (uint32_t e = threadIdx.x; e < p.experts; e += 64u * S::kWaves) {
+            const uint32_t end = p.offsets[e + 1u];
+            report(end < offsets[e] || end > p.routes, kCheckOffsets);
+        }
+        if (p.packed)  // each workgroup looks at a part of the sources
+            for (uint32_t i = offsets[0] + blockIdx.x * 64u * S::kWaves + threadIdx.x; i < min(last_offset, p.routes);
+                 i += gridDim.x * 64u * S::kWaves)
+                report(p.packed[i] / p.top_k >= p.a_rows, kCheckToken);
+#endif
     }
     const auto make_list = [&]() MX_INLINE {
         if constexpr (kExperts) return TileList<kBM>(offsets, last_offset, p.routes);

@@ -305,6 +305,12 @@ struct Piece {
 
 constexpr uint32_t kRowThreads = 256;
 
+// whether an inverse entry is a place
+__device__ __forceinline__ bool in_range(uint32_t at, uint32_t routes) {
+    report(at >= routes && at != Q38M_ROUTE_DROPPED, kCheckRoute);
+    return at < routes;
+}
+
 // A workgroup takes kRowThreads / lanes tokens, `lanes` (a power of two)
 // threads each, which walk the row kN values a thread.  A row's last piece is
 // its last kN values, in part those of the piece in front: written twice, with
@@ -334,7 +340,7 @@ __global__ __launch_bounds__(kRowThreads) void permute_kernel(
         const uint32_t c = min(c0, width - kN);
         const auto v = Piece<T, kN>::template get<false>(x + static_cast<size_t>(p.token) * width + c);
         for (uint32_t r = 0; r < top_k; ++r)
-            if (at[r] < routes) v.template put<kStream>(rows + static_cast<size_t>(at[r]) * width + c);
+            if (in_range(at[r], routes)) v.template put<kStream>(rows + static_cast<size_t>(at[r]) * width + c);
     }
 }
 
@@ -370,7 +376,7 @@ __global__ __launch_bounds__(kRowThreads) void unpermute_kernel(
 #pragma unroll
             for (uint32_t i = 0; i < kRanks; ++i) {
                 row[i] = Piece<T, kN>{};
-                if (at[i] < routes)
+                if (in_range(at[i], routes))
                     row[i] = Piece<T, kN>::template get<kStream>(rows + static_cast<size_t>(at[i]) * width + c);
             }
 #pragma unroll
@@ -401,7 +407,7 @@ __global__ __launch_bounds__(kRowThreads) void unpermute_backward_kernel(
     if (route >= routes) return;
     const uint32_t at = inverse[route];
     float dot = 0.0f;
-    if (at < routes) {
+    if (in_range(at, routes)) {
         const float w = weights[route];
         const T* from = dy + static_cast<size_t>(route / top_k) * width;
         const size_t row = static_cast<size_t>(at) * width;
