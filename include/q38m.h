@@ -651,7 +651,8 @@ int q38m_mx_gemm_v1(const q38m_mx_matrix_v1* a, const q38m_mx_matrix_v1* b,
  * packed_assignment NULL: src(p) = p and rows->rows = routes; else src(p) =
  * packed_assignment[p] / top_k (the token rows, as q38m_moe_grouped_gate_up_v1
  * gathers them).  routes: C's rows; offsets past it are taken as routes, and
- * an expert whose end is not behind its begin has no rows.
+ * an expert whose end is not behind its begin has no rows (a row that two
+ * experts' offsets hold after such a fall gets either's).
  * epilogue SWIGLU: weights' first half of rows is gate, the second half up;
  * C has half as many columns, h = g / (1 + exp(-g)) * u in fp32, rounded
  * once: within 8 fp32 roundings, bf16 within 2^-17 h before its own; a zero
