@@ -184,7 +184,7 @@ __device__ __forceinline__ uint32_t wave_top10(uint32_t k32, uint32_t expert, St
         const uint32_t cand = prefix | (1u << b);
         const uint64_t reach = __builtin_amdgcn_ballot_w64(k32 >= cand);
         uint32_t count;
-        asm("s_bcnt1_i32_b64 %0, %1" : "=s"(count) : "s"(reach));
+        asm("s_bcnt1_i32_b64 %0, %1" : "=s"(count) : "s"(reach) : "scc");
         prefix = count >= kTopK ? cand : prefix;
         // exactly ten keys reach the prefix: they are the wave's top 10
         // (below, "above" and the ties at the prefix make up exactly that
@@ -224,7 +224,7 @@ __device__ __forceinline__ void wave_top10_rows(const uint32_t (&k32)[kRows], ui
             const uint32_t cand = prefix[r] | (1u << b);
             const uint64_t reach = __builtin_amdgcn_ballot_w64(k32[r] >= cand);
             uint32_t count;
-            asm("s_bcnt1_i32_b64 %0, %1" : "=s"(count) : "s"(reach));
+            asm("s_bcnt1_i32_b64 %0, %1" : "=s"(count) : "s"(reach) : "scc");
             prefix[r] = count >= kTopK ? cand : prefix[r];
         }
     }
@@ -281,7 +281,7 @@ __device__ __forceinline__ void rank_candidates(const SelectLds& lds, int32_t* i
 // popcount of a wave-uniform 64-bit mask, on the scalar unit
 __device__ __forceinline__ uint32_t scalar_popcount(uint64_t mask) {
     uint32_t count;
-    asm("s_bcnt1_i32_b64 %0, %1" : "=s"(count) : "s"(mask));
+    asm("s_bcnt1_i32_b64 %0, %1" : "=s"(count) : "s"(mask) : "scc");
     return count;
 }
 

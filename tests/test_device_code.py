@@ -77,24 +77,28 @@ def test_m0_belongs_to_the_loads(objects):
                 assert not any("m0" in dc.scalar_registers(o) for o in reads), (i.kernel, hex(i.address), i.name)
 
 
-def test_inline_assembly_names_what_it_writes():
-    """m0 is among the clobbers of every inline assembly that sets it."""
+def assembly_statements():
+    """(file, statement) of every inline assembly."""
     folder = os.path.join(PACKAGE_DIR, "csrc")
-    found = 0
     for name in sorted(os.listdir(folder)):
         text = open(os.path.join(folder, name)).read()
-        for start in (m.start() for m in re.finditer(r"\basm\b", text)):
+        for start in (m.start() for m in re.finditer(r"\basm\b(?: volatile)?\(", text)):
             depth, end = 0, text.index("(", start)
             while True:
                 depth += {"(": 1, ")": -1}.get(text[end], 0)
                 end += 1
                 if depth == 0:
                     break
-            statement = text[start:end]
-            if re.search(r"s_mov_b32 m0", statement):
-                found += 1
-                assert '"m0"' in statement, (name, statement)
-    assert found >= 2
+            yield name, text[start:end]
+
+
+@pytest.mark.parametrize("writes,register,least", [("s_mov_b32 m0", "m0", 2), ("s_bcnt1_i32", "scc", 3)])
+def test_inline_assembly_names_what_it_writes(writes, register, least):
+    """m0 and the scalar condition bit are among the clobbers of every statement that sets them."""
+    found = [(name, text) for name, text in assembly_statements() if writes in text]
+    assert len(found) >= least
+    for name, text in found:
+        assert f'"{register}"' in text, (name, text)
 
 
 def test_product_kernels_keep_their_registers(objects):
