@@ -296,9 +296,9 @@ struct TileList {
 // column by column.  The dispatcher hands workgroups to the eight XCDs in turn, each
 // with an L2 of its own: an XCD has one contiguous eighth of the order, and its
 // workgroups take turns, so that those at work at the same time share rows of A and of
-// B.  (Each a run of consecutive tiles, with the same rows of A: gate/up of 512 experts
-// 112 instead of 108 us for 512 tokens, 316 instead of 182 for 2,048, 968 instead of 608
-// for 32,768: the workgroups stream B at different places.)
+// B.  (Each a run of consecutive tiles, with the same rows of A, streams B at different
+// places: gate/up of 512 experts, on an earlier form of the kernel, 112 us and in turns 108
+// for 512 tokens, 316 and 182 for 2,048, 968 and 608 for 32,768.)
 constexpr uint32_t kGroup = 4;
 struct MxOrder {
     uint32_t rows, columns;   // of tiles
@@ -369,13 +369,15 @@ __device__ __forceinline__ void mx_barrier() {
 // banks.  A load instruction fills 1 KB of consecutive LDS, eight rows; the swizzle is
 // in the addresses that its lanes read.
 //
-// What bounds it: with few rows the latency of a stage (load, meet, read, multiply: 0.35 us
-// on 64 x 64 tiles); from tens of tokens on the weights' bytes (gate/up of 512 experts, 512
-// tokens: 94 us, 6.1 TB/s of 576 MB); large products the card's power (8,192^3 280 us, 3.9
-// PFLOP/s at 1.8 GHz) and, with few stages a tile, C's stores and loads that memory answers
-// late: gate/up of 32,768 tokens 481 us, 3.4 PFLOP/s on the rows of its 256-row tiles, 2.9 on
-// those that count (an earlier form of 509 us took 435 without its stores; with four experts'
-// weights alone, which the L2s hold, 467 instead of 507).
+// What bounds it: with few rows a launch, its first loads and how fast the L2s answer (a
+// stage brings 43 to 56 KB a microsecond and CU to LDS on all five smaller shapes; 509 x 2,048
+// x 8,192 14.1 us, its vector L1s held up by answers under way half the time); from tens of
+// tokens on the weights' bytes (gate/up of 512 experts, 512 tokens: 94 us, 6.1 TB/s of 576
+// MB); large products the clock, 1.8 GHz under their load, and the same waits, which leave the
+// matrix pipes 57 % busy (8,192^3 278 us, 3.9 PFLOP/s); with few stages a tile, C's stores and
+// loads that memory answers late: gate/up of 32,768 tokens 480 us, 3.4 PFLOP/s on the rows of
+// its 256-row tiles, 2.9 on those that count (an earlier form of 509 us took 435 without its
+// stores; with four experts' weights alone, which the L2s hold, 467 instead of 507).
 template <typename S, bool kExperts, bool kSwiglu, bool kWide, bool kStream>
 __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 4u) void mx_tile_kernel(MxProduct p) {
     constexpr uint32_t kMF = S::kMF, kTM = S::kTM, kTN = S::kTN, kBM = S::kBM, kBN = S::kBN;
