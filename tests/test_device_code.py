@@ -1,4 +1,4 @@
-"""The built library's device code keeps the waits that gfx950 leaves to the
+"""The built libraries' device code keeps the waits that gfx950 leaves to the
 program.  The compiler inserts them for its own instructions; it does not look
 into inline assembly, where the products' loads to LDS are."""
 import os
@@ -43,9 +43,10 @@ def test_the_check_follows_branches():
     assert 0x114 in {w.address for w, _ in found}
 
 
-@pytest.fixture(scope="module")
-def objects(q38m, tmp_path_factory):
-    found = dc.code_objects(q38m.LIB_PATH, tmp_path_factory.mktemp("code"))
+@pytest.fixture(scope="module", params=["product", "checked"])
+def objects(q38m, request, tmp_path_factory):
+    library = q38m.LIB_PATH if request.param == "product" else q38m.CHECKED_LIB_PATH
+    found = dc.code_objects(library, tmp_path_factory.mktemp("code"))
     assert len(found) >= 11  # one for each source
     return [(o, dc.disassemble(o)) for o in found]
 
