@@ -460,6 +460,20 @@ def _stream_of(tensor, stream):
     return stream if stream is not None else _torch().cuda.current_stream(tensor.device)
 
 
+def _overlap(rows, flat):
+    """Whether one of the rows (columns side by side) shares memory with a contiguous tensor."""
+    if rows.numel() == 0:
+        return False
+    size = rows.element_size()
+    step = max(rows.stride(0), 1) * size  # from row to row
+    length = rows.shape[1] * size
+    begin = flat.data_ptr() - rows.data_ptr()
+    end = begin + flat.numel() * flat.element_size()
+    # the first row that ends behind `begin`
+    first = max((begin - length) // step + 1, 0)
+    return first < rows.shape[0] and first * step < end
+
+
 class MxRows:
     """Microscaled 4-bit rows resident in device memory plus their descriptor."""
 
@@ -475,7 +489,7 @@ def mx_quantize(x, experts=1, rounded=None, stream=None):
     """x [experts * rows][columns] on a GPU (bf16, raw bf16 words in 16-bit integers, or fp32;
     columns side by side, rows any stride apart but not one over the other; at most 2^23) as
     MxRows.  rounded: None, or a contiguous tensor like
-    x that gets the values the codes stand for."""
+    x, elsewhere in memory, that gets the values the codes stand for."""
     torch = _torch()
     words = (torch.bfloat16, torch.int16, torch.uint16)
     _require(x.dim() == 2 and (x.dtype == torch.float32 or x.dtype in words),
@@ -485,6 +499,7 @@ def mx_quantize(x, experts=1, rounded=None, stream=None):
     _require(rounded is None or (rounded.shape == x.shape and rounded.dtype == x.dtype and
                                  rounded.device == x.device and rounded.is_contiguous()),
              "rounded must be a contiguous tensor like x")
+    _require(rounded is None or not _overlap(x, rounded), "rounded must not overlap the rows")
     _require(x.is_cuda, "rows to quantise must be on a GPU")
     stream = _stream_of(x, stream)
     with torch.cuda.stream(stream):  # whose memory the rows are
