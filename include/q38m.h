@@ -656,11 +656,11 @@ int q38m_mx_gemm_v1(const q38m_mx_matrix_v1* a, const q38m_mx_matrix_v1* b,
  * epilogue SWIGLU: weights' first half of rows is gate, the second half up;
  * C has half as many columns, h = g / (1 + exp(-g)) * u in fp32, rounded
  * once: within 8 fp32 roundings, bf16 within 2^-17 h before its own; a zero
- * where exp(-g) is past fp32 (g below -88.7).  C is contiguous.  Rows of C that no expert has (dropped routes) are
- * left as they were; a src(p) past A's rows reads A's last row.  At most 1024
- * experts, fewer than 2^24 routes, weights of at most 2^28 rows an expert,
- * columns <= 2^24, fewer than 2^31 tiles of C; one expert's codes, and those
- * of gathered rows, are below 4 GB. */
+ * where exp(-g) is past fp32 (g below -88.7).  C is contiguous.  Rows of C
+ * that no expert has (dropped routes) are left as they were; a src(p) past A's
+ * rows reads A's last row.  At most 1024 experts, fewer than 2^24 routes,
+ * weights of at most 2^28 rows an expert, columns <= 2^24, fewer than 2^31
+ * tiles of C; one expert's codes, and those of gathered rows, are below 4 GB. */
 #define Q38M_MX_EPILOGUE_NONE 0u
 #define Q38M_MX_EPILOGUE_SWIGLU 1u
 int q38m_mx_grouped_gemm_v1(const q38m_mx_matrix_v1* weights,
