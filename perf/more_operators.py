@@ -414,7 +414,7 @@ def _calls(s):
     experts, top_k, offsets = c["experts"], c["top_k"], s["offsets"].data_ptr()
     packed = s["packed"].data_ptr() if c["up"] else None
     if c["kind"] == "experts":
-        epilogue = q.MX_EPILOGUE_SWIGLU if c["up"] else q.MX_EPILOGUE_NONE
+        epilogue = q.EPILOGUE_SWIGLU if c["up"] else q.EPILOGUE_NONE
         return [("q38m_moe_expert_gemm_v1", t(s["w"], experts), t(s["rows"]), offsets, packed, top_k, epilogue,
                  t(s["c"]), t(s["pre"]))]
     return [("q38m_moe_expert_backward_rows_v1", t(s["w"], experts), t(s["dc"]), offsets, t(s["pre"]),
