@@ -721,6 +721,130 @@ int q38m_moe_unpermute_backward_v1(const void* dy, const void* rows, uint32_t dt
                                    uint32_t top_k, uint32_t width, void* d_rows,
                                    float* d_weights, void* stream, int device);
 
+/* ---- bf16 products with epilogues and gradients ------------------------
+ * No counterpart in the reference, which only serves: the dense products of
+ * q38m_dense_gemm_bf16's kind with bias, activation and residual in one launch,
+ * the experts' products over sorted rows in bf16, and the derivatives of both.
+ *
+ * A matrix is `rows` rows of `columns` values (experts times, one below the
+ * other), row_stride elements from row to row (at least `columns`; any, where
+ * there is one row).  bf16 is raw words; where a call takes either type the
+ * descriptor says which.  Every operand that a product multiplies is bf16.
+ * Sums are fp32, and each output is rounded once (to nearest even).  Data is
+ * aligned to its elements; operands whose rows all start at 16 bytes (data
+ * and row_stride multiples of 16 bytes) run on the fast kernels, which read
+ * a row in aligned pieces of 16 bytes, the last one whole: up to seven values
+ * behind a row's last one are read, and do not count whatever they hold.
+ * Descriptors that are not needed are NULL.  Outputs overlap no input and no
+ * other output, but a residual may be the output that it is added to (the
+ * same data, type and stride).  rows <= 2^28, columns <= 2^24,
+ * experts <= 1024; a product has fewer than 2^31 tiles of 16 x 64 values.
+ * Floating-point parity: the order of a sum is the kernels', and it is the
+ * same in every call with the same sizes and strides. */
+typedef struct q38m_tensor_v1 {
+    void* data;
+    uint64_t row_stride;
+    uint32_t dtype;   /* Q38M_DTYPE_* */
+    uint32_t experts; /* 1: a plain matrix */
+    uint32_t rows;    /* of one expert */
+    uint32_t columns;
+} q38m_tensor_v1;
+
+/* Activations act(z); s(z) = 1 / (1 + exp(-z)), Phi the normal distribution's
+ * integral:
+ *   RELU max(z, 0); SILU z s(z); SIGMOID s(z); GELU z Phi(z);
+ *   GELU_TANH z s(2 t), t = sqrt(2 / pi) (z + 0.044715 z^3)
+ * computed in fp32, within 8 * 2^-24 max(1, |z|), and so are the derivatives
+ * (RELU's is 0 at 0).  An exponential below the smallest normal is a zero. */
+#define Q38M_ACT_NONE 0u
+#define Q38M_ACT_RELU 1u
+#define Q38M_ACT_SILU 2u
+#define Q38M_ACT_SIGMOID 3u
+#define Q38M_ACT_GELU 4u
+#define Q38M_ACT_GELU_TANH 5u
+
+/* Scratch that each of the three q38m_linear products of a layer with this
+ * many rows, outputs (weight rows) and inputs (weight columns) takes; 0: none
+ * is needed and it may be NULL.  16-byte aligned.  Two calls that may run at
+ * the same time need two (captured graphs that replay together too). */
+size_t q38m_linear_scratch_bytes(uint32_t rows, uint32_t outputs, uint32_t inputs);
+
+/* y = act(x weight^T + bias) + residual: x [rows][inputs], weight
+ * [outputs][inputs], bias [1][outputs], residual and y [rows][outputs].  bias,
+ * residual, y and pre are bf16 or fp32.  pre: NULL, or gets x weight^T + bias
+ * [rows][outputs], what the derivative of the activation wants. */
+int q38m_linear_v1(const q38m_tensor_v1* x, const q38m_tensor_v1* weight,
+                   const q38m_tensor_v1* bias, uint32_t activation,
+                   const q38m_tensor_v1* residual, const q38m_tensor_v1* y,
+                   const q38m_tensor_v1* pre, void* scratch, size_t scratch_bytes,
+                   void* stream, int device);
+
+/* dx = (dz weight) * act'(pre) + residual: dz [rows][outputs] the gradient of
+ * x weight^T + bias, pre [rows][inputs] what the activation in front of x was
+ * taken of (NULL with Q38M_ACT_NONE), residual [rows][inputs] the gradient
+ * that x gets otherwise (through a skip connection). */
+int q38m_linear_backward_input_v1(const q38m_tensor_v1* dz, const q38m_tensor_v1* weight,
+                                  const q38m_tensor_v1* pre, uint32_t activation,
+                                  const q38m_tensor_v1* residual, const q38m_tensor_v1* dx,
+                                  void* scratch, size_t scratch_bytes, void* stream,
+                                  int device);
+
+/* d_weight = dz^T x + residual [outputs][inputs] (residual: what the weight's
+ * gradient was before, d_weight itself to add up in place) and d_bias = the
+ * sum of dz's rows [1][outputs].  Either output may be NULL; x too where
+ * d_weight is. */
+int q38m_linear_backward_weight_v1(const q38m_tensor_v1* dz, const q38m_tensor_v1* x,
+                                   const q38m_tensor_v1* residual,
+                                   const q38m_tensor_v1* d_weight,
+                                   const q38m_tensor_v1* d_bias, void* scratch,
+                                   size_t scratch_bytes, void* stream, int device);
+
+/* dz = dy * act'(pre), [rows][columns] each, bf16 or fp32 (a layer's first step
+ * where its gradient does not come out of q38m_linear_backward_input_v1). */
+int q38m_linear_backward_activation_v1(const q38m_tensor_v1* dy, const q38m_tensor_v1* pre,
+                                       uint32_t activation, const q38m_tensor_v1* dz,
+                                       void* stream, int device);
+
+/* The experts' products over rows sorted by expert, with q38m_mx_grouped_gemm_v1's
+ * order, offsets and gather: for p in [expert_offsets[e], expert_offsets[e + 1]),
+ * c[p] = rows[src(p)] weights[e]^T, src(p) = p (packed_assignment NULL,
+ * rows->rows = c->rows) or packed_assignment[p] / top_k.  c->rows are the
+ * routes, below 2^24; offsets past them are taken as them, and an expert whose
+ * end is not behind its begin has no rows (a row that two experts' offsets hold
+ * after such a fall gets either's).  Rows of c that no expert has are left as
+ * they were; a src(p) past the rows reads the last one.
+ * epilogue SWIGLU: weights' first half of rows is gate, the second up; c has
+ * half as many columns, h = g / (1 + exp(-g)) u (a zero for g below -88.7), and
+ * pre (NULL, or bf16 or fp32 [routes][weights->rows]) gets gate and up.
+ * NONE: pre is NULL.  c: bf16 or fp32.  Gathered rows and one expert's matrix
+ * are below 4 GB. */
+#define Q38M_EPILOGUE_NONE 0u
+#define Q38M_EPILOGUE_SWIGLU 1u
+int q38m_moe_expert_gemm_v1(const q38m_tensor_v1* weights, const q38m_tensor_v1* rows,
+                            const uint32_t* expert_offsets, const uint32_t* packed_assignment,
+                            uint32_t top_k, uint32_t epilogue, const q38m_tensor_v1* c,
+                            const q38m_tensor_v1* pre, void* stream, int device);
+
+/* d_rows[p] = d_c[p] weights[e], in the sorted order (for gathered rows
+ * q38m_moe_unpermute_rows_v1 with NULL weights brings it to the tokens).  pre
+ * NULL: d_rows [routes][weights->columns].  Else the rows came out of the
+ * SWIGLU epilogue, pre [routes][2 weights->columns] is what it kept, and d_rows
+ * [routes][2 weights->columns] gets the gradients of gate, dh u s(g) (1 + g (1
+ * - s(g))), and of up, dh g s(g).  pre and d_rows are bf16 or fp32. */
+int q38m_moe_expert_backward_rows_v1(const q38m_tensor_v1* weights, const q38m_tensor_v1* d_c,
+                                     const uint32_t* expert_offsets, const q38m_tensor_v1* pre,
+                                     const q38m_tensor_v1* d_rows, void* stream, int device);
+
+/* d_weights[e] = sum over e's p of d_c[p]^T rows[src(p)] + residual[e]
+ * ([experts][d_c->columns][rows->columns], bf16 or fp32): zeros, or the
+ * residual, for an expert without rows.  src(p) as above. */
+int q38m_moe_expert_backward_weights_v1(const q38m_tensor_v1* d_c, const q38m_tensor_v1* rows,
+                                        const uint32_t* expert_offsets,
+                                        const uint32_t* packed_assignment, uint32_t top_k,
+                                        const q38m_tensor_v1* residual,
+                                        const q38m_tensor_v1* d_weights, void* stream,
+                                        int device);
+
 /* ---- deterministic synthetic data (counter-based SplitMix64) --------- */
 #define Q38M_SYNTH_NORMAL_F32 1u     /* sigma*N(0,1) (+ bias[i % bias_len]) */
 #define Q38M_SYNTH_NORMAL_BF16 2u    /* bf16(sigma*N(0,1)) */

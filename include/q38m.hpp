@@ -338,6 +338,79 @@ inline void moe_unpermute_backward(const void* dy, const void* rows, DtypeV1 dty
                                          width, d_rows, d_weights, stream, device));
 }
 
+// ---- bf16 products with epilogues and gradients: no reference counterpart; the
+// entry points of the same names in q38m.h.  A null pointer is nothing.
+using TensorV1 = q38m_tensor_v1;
+
+enum class ActivationV1 : std::uint32_t {
+    kNone = Q38M_ACT_NONE,
+    kRelu = Q38M_ACT_RELU,
+    kSilu = Q38M_ACT_SILU,
+    kSigmoid = Q38M_ACT_SIGMOID,
+    kGelu = Q38M_ACT_GELU,
+    kGeluTanh = Q38M_ACT_GELU_TANH,
+};
+enum class EpilogueV1 : std::uint32_t {
+    kNone = Q38M_EPILOGUE_NONE,
+    kSwiglu = Q38M_EPILOGUE_SWIGLU,
+};
+
+inline void linear(const TensorV1& x, const TensorV1& weight, const TensorV1* bias,
+                   ActivationV1 activation, const TensorV1* residual, const TensorV1& y,
+                   const TensorV1* pre, void* scratch, std::size_t scratch_bytes, void* stream,
+                   int device) {
+    check(q38m_linear_v1(&x, &weight, bias, static_cast<std::uint32_t>(activation), residual, &y,
+                         pre, scratch, scratch_bytes, stream, device));
+}
+
+inline void linear_backward_input(const TensorV1& dz, const TensorV1& weight,
+                                  const TensorV1* pre, ActivationV1 activation,
+                                  const TensorV1* residual, const TensorV1& dx, void* scratch,
+                                  std::size_t scratch_bytes, void* stream, int device) {
+    check(q38m_linear_backward_input_v1(&dz, &weight, pre, static_cast<std::uint32_t>(activation),
+                                        residual, &dx, scratch, scratch_bytes, stream, device));
+}
+
+inline void linear_backward_weight(const TensorV1& dz, const TensorV1* x,
+                                   const TensorV1* residual, const TensorV1* d_weight,
+                                   const TensorV1* d_bias, void* scratch,
+                                   std::size_t scratch_bytes, void* stream, int device) {
+    check(q38m_linear_backward_weight_v1(&dz, x, residual, d_weight, d_bias, scratch,
+                                         scratch_bytes, stream, device));
+}
+
+inline void linear_backward_activation(const TensorV1& dy, const TensorV1& pre,
+                                       ActivationV1 activation, const TensorV1& dz, void* stream,
+                                       int device) {
+    check(q38m_linear_backward_activation_v1(&dy, &pre, static_cast<std::uint32_t>(activation),
+                                             &dz, stream, device));
+}
+
+inline void moe_expert_gemm(const TensorV1& weights, const TensorV1& rows,
+                            const std::uint32_t* expert_offsets,
+                            const std::uint32_t* packed_assignment, std::uint32_t top_k,
+                            EpilogueV1 epilogue, const TensorV1& c, const TensorV1* pre,
+                            void* stream, int device) {
+    check(q38m_moe_expert_gemm_v1(&weights, &rows, expert_offsets, packed_assignment, top_k,
+                                  static_cast<std::uint32_t>(epilogue), &c, pre, stream, device));
+}
+
+inline void moe_expert_backward_rows(const TensorV1& weights, const TensorV1& d_c,
+                                     const std::uint32_t* expert_offsets, const TensorV1* pre,
+                                     const TensorV1& d_rows, void* stream, int device) {
+    check(q38m_moe_expert_backward_rows_v1(&weights, &d_c, expert_offsets, pre, &d_rows, stream,
+                                           device));
+}
+
+inline void moe_expert_backward_weights(const TensorV1& d_c, const TensorV1& rows,
+                                        const std::uint32_t* expert_offsets,
+                                        const std::uint32_t* packed_assignment,
+                                        std::uint32_t top_k, const TensorV1* residual,
+                                        const TensorV1& d_weights, void* stream, int device) {
+    check(q38m_moe_expert_backward_weights_v1(&d_c, &rows, expert_offsets, packed_assignment,
+                                              top_k, residual, &d_weights, stream, device));
+}
+
 inline bool cuda_q38_moe_prefill_compiled() { return q38m_moe_compiled() == 1; }
 inline bool cuda_q38_moe_compiled() { return q38m_moe_compiled() == 1; }
 

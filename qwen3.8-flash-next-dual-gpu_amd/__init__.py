@@ -52,6 +52,9 @@ MX_BLOCK = 32
 MX_EPILOGUE_NONE = 0
 MX_EPILOGUE_SWIGLU = 1
 ROUTE_DROPPED = 0xffffffff
+EPILOGUE_NONE = 0
+EPILOGUE_SWIGLU = 1
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "sigmoid": 3, "gelu": 4, "gelu_tanh": 5}
 
 SYNTH_NORMAL_F32 = 1
 SYNTH_NORMAL_BF16 = 2
@@ -120,11 +123,18 @@ class MxMatrix(ctypes.Structure):
                 ("columns", ctypes.c_uint32), ("reserved", ctypes.c_uint32)]
 
 
+class Tensor(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_uint64),
+                ("dtype", ctypes.c_uint32), ("experts", ctypes.c_uint32),
+                ("rows", ctypes.c_uint32), ("columns", ctypes.c_uint32)]
+
+
 class WideWorkspace(ctypes.Structure):
     _fields_ = [("step", PrefillWorkspace), ("plan_scratch", ctypes.c_void_p)]
 
 
 _P = ctypes.c_void_p
+_T = ctypes.POINTER(Tensor)
 _U32 = ctypes.c_uint32
 _U64 = ctypes.c_uint64
 _I32 = ctypes.c_int32
@@ -216,6 +226,14 @@ SIGNATURES = {
     "q38m_moe_unpermute_rows_v1": (_INT, [_P, _U32, _P, _P, _U32, _U32, _U32, _P, _P, _INT]),
     "q38m_moe_unpermute_backward_v1": (_INT, [_P, _P, _U32, _P, _P, _U32, _U32, _U32, _P, _P, _P,
                                               _INT]),
+    "q38m_linear_scratch_bytes": (_SZ, [_U32, _U32, _U32]),
+    "q38m_linear_v1": (_INT, [_T, _T, _T, _U32, _T, _T, _T, _P, _SZ, _P, _INT]),
+    "q38m_linear_backward_input_v1": (_INT, [_T, _T, _T, _U32, _T, _T, _P, _SZ, _P, _INT]),
+    "q38m_linear_backward_weight_v1": (_INT, [_T, _T, _T, _T, _T, _P, _SZ, _P, _INT]),
+    "q38m_linear_backward_activation_v1": (_INT, [_T, _T, _U32, _T, _P, _INT]),
+    "q38m_moe_expert_gemm_v1": (_INT, [_T, _T, _P, _P, _U32, _U32, _T, _T, _P, _INT]),
+    "q38m_moe_expert_backward_rows_v1": (_INT, [_T, _T, _P, _T, _T, _P, _INT]),
+    "q38m_moe_expert_backward_weights_v1": (_INT, [_T, _T, _P, _P, _U32, _T, _T, _P, _INT]),
     "q38m_synth_fill": (_INT, [_U32, _U64, _U64, _U64, _F, _I32, _I32, _P, _U32, _P, _P, _INT]),
     "q38m_moe_compiled": (_INT, []),
     "q38m_last_error": (ctypes.c_char_p, []),
@@ -508,6 +526,31 @@ def mx_quantize(x, experts=1, rounded=None, stream=None):
          x.stride(0) if x.shape[0] > 1 else x.shape[1], ctypes.byref(out.desc), ptr(rounded),
          stream.cuda_stream, device_index(x))
     return out
+
+
+def describe(x, experts=1):
+    """The descriptor of a matrix on a GPU: [rows][columns], experts' matrices one below the other
+    ([experts][rows][columns]), or a vector as one row.  bf16, raw bf16 words in 16-bit integers, or
+    fp32; columns side by side, rows and experts one stride apart.  The tensor is the caller's to keep."""
+    torch = _torch()
+    words = (torch.bfloat16, torch.int16, torch.uint16)
+    _require(x.dtype == torch.float32 or x.dtype in words, "a bf16 or fp32 tensor is wanted")
+    _require(x.is_cuda, "the tensor must be on a GPU")
+    _require(1 <= x.dim() <= 3 and x.numel() > 0, "a vector, a matrix or experts' matrices are wanted")
+    if x.dim() == 1:
+        x = x.unsqueeze(0)
+    if x.dim() == 3:
+        _require(experts in (1, x.shape[0]), "the experts are not the tensor's")
+        experts = x.shape[0]
+        _require(experts == 1 or x.shape[1] == 1 or x.stride(0) == x.shape[1] * x.stride(1),
+                 "experts' matrices must lie one below the other")
+        stride = x.stride(0) if x.shape[1] == 1 else x.stride(1)
+        x = x.as_strided((experts * x.shape[1], x.shape[2]), (stride, x.stride(2)))
+    _require(x.shape[1] == 1 or x.stride(1) == 1, "columns must lie side by side")
+    _require(experts > 0 and x.shape[0] % experts == 0, "the experts' rows must be equally many")
+    return Tensor(ptr(x), x.stride(0) if x.shape[0] > 1 else x.shape[1],
+                  DTYPE_F32 if x.dtype == torch.float32 else DTYPE_BF16, experts,
+                  x.shape[0] // experts, x.shape[1])
 
 
 class SortedRoutes:

@@ -1096,6 +1096,235 @@ int q38m_moe_unpermute_backward_v1(const void* dy, const void* rows, uint32_t dt
                   "unpermute_backward_kernel");
 }
 
+// ---- bf16 products with epilogues and gradients ------------------------
+
+namespace {
+
+using q38m::LinearEpilogue;
+using q38m::LinearFold;
+using q38m::LinearMatrix;
+using q38m::LinearOrder;
+using q38m::LinearProduct;
+
+bool valid_tensor(const q38m_tensor_v1* t) {
+    if (!t || !t->data || !valid_dtype(t->dtype) || !element_aligned(t->data, t->dtype) ||
+        t->experts == 0u || t->experts > q38m::kMaxSortExperts || t->rows == 0u ||
+        t->rows > q38m::kMaxLinearRows || t->columns == 0u || t->columns > kMaxWidth)
+        return false;
+    const uint64_t rows = static_cast<uint64_t>(t->experts) * t->rows;
+    return rows == 1u || (t->row_stride >= t->columns && t->row_stride <= (1ull << 40) &&
+                          rows <= (1ull << 62) / t->row_stride);
+}
+
+bool has_shape(const q38m_tensor_v1* t, uint32_t experts, uint32_t rows, uint32_t columns) {
+    return valid_tensor(t) && t->experts == experts && t->rows == rows && t->columns == columns;
+}
+
+// absent, or of this shape
+bool valid_optional(const q38m_tensor_v1* t, uint32_t experts, uint32_t rows, uint32_t columns) {
+    return !t || has_shape(t, experts, rows, columns);
+}
+
+bool valid_operand(const q38m_tensor_v1* t) {
+    return valid_tensor(t) && t->dtype == Q38M_DTYPE_BF16;
+}
+
+uint64_t stride_of(const q38m_tensor_v1* t) {  // one row: any
+    return static_cast<uint64_t>(t->experts) * t->rows == 1u ? t->columns : t->row_stride;
+}
+
+// a residual that is the output is read and written element by element
+bool valid_residual(const q38m_tensor_v1* residual, const q38m_tensor_v1* out) {
+    return !residual || residual->data != out->data ||
+           (residual->dtype == out->dtype && stride_of(residual) == stride_of(out));
+}
+
+LinearMatrix view(const q38m_tensor_v1* t) {
+    return t ? LinearMatrix{t->data, stride_of(t), t->dtype == Q38M_DTYPE_F32} : LinearMatrix{};
+}
+
+const uint16_t* words(const q38m_tensor_v1* t) { return static_cast<const uint16_t*>(t->data); }
+
+bool valid_activation(uint32_t activation) { return activation <= Q38M_ACT_GELU_TANH; }
+
+bool valid_scratch(const void* scratch, size_t bytes, size_t needed) {
+    return needed == 0u || (scratch && bytes >= needed && aligned(scratch, 16));
+}
+
+// Offsets, packed assignment and the rows that they sort.
+bool valid_sorted(const uint32_t* offsets, const uint32_t* packed, uint32_t top_k,
+                  const q38m_tensor_v1* rows, uint32_t routes) {
+    return offsets && aligned(offsets, 4) && aligned(packed, 4) && top_k != 0u &&
+           routes <= q38m::kMaxSortRoutes && rows->experts == 1u && (packed || rows->rows == routes);
+}
+
+int run_linear(const LinearProduct& p, LinearOrder order, LinearFold fold, void* scratch,
+               void* stream, int device) {
+    if (!q38m::linear_fits(p, order, fold))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "bf16 product too large for one call");
+    if (int rc = select_device(device)) return rc;
+    return finish(q38m::launch_linear(p, order, fold, scratch, as_stream(stream)),
+                  "bf16 product kernel");
+}
+
+}  // namespace
+
+size_t q38m_linear_scratch_bytes(uint32_t rows, uint32_t outputs, uint32_t inputs) {
+    if (rows == 0u || rows > q38m::kMaxLinearRows || outputs == 0u || outputs > kMaxWidth ||
+        inputs == 0u || inputs > kMaxWidth)
+        return 0u;
+    return q38m::linear_scratch_bytes(rows, outputs, inputs);
+}
+
+int q38m_linear_v1(const q38m_tensor_v1* x, const q38m_tensor_v1* weight,
+                   const q38m_tensor_v1* bias, uint32_t activation,
+                   const q38m_tensor_v1* residual, const q38m_tensor_v1* y,
+                   const q38m_tensor_v1* pre, void* scratch, size_t scratch_bytes,
+                   void* stream, int device) {
+    if (!valid_operand(x) || !valid_operand(weight) || x->experts != 1u || weight->experts != 1u ||
+        x->columns != weight->columns || weight->rows > kMaxWidth ||
+        !has_shape(y, 1, x->rows, weight->rows) ||
+        !valid_optional(bias, 1, 1, weight->rows) ||
+        !valid_optional(residual, 1, x->rows, weight->rows) ||
+        !valid_optional(pre, 1, x->rows, weight->rows) || !valid_residual(residual, y) ||
+        !valid_activation(activation))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid linear layer");
+    if (!valid_scratch(scratch, scratch_bytes,
+                       q38m_linear_scratch_bytes(x->rows, weight->rows, x->columns)))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "linear scratch is missing, small or unaligned");
+    const LinearProduct p{words(x), words(weight), stride_of(x), stride_of(weight), nullptr,
+                          nullptr, x->rows, weight->rows, x->columns, 0u, 1u, 1u,
+                          LinearEpilogue{view(y), view(bias), view(residual), view(pre),
+                                         activation, false}};
+    return run_linear(p, LinearOrder::kNT, LinearFold::kPlain, scratch, stream, device);
+}
+
+int q38m_linear_backward_input_v1(const q38m_tensor_v1* dz, const q38m_tensor_v1* weight,
+                                  const q38m_tensor_v1* pre, uint32_t activation,
+                                  const q38m_tensor_v1* residual, const q38m_tensor_v1* dx,
+                                  void* scratch, size_t scratch_bytes, void* stream,
+                                  int device) {
+    if (!valid_operand(dz) || !valid_operand(weight) || dz->experts != 1u ||
+        weight->experts != 1u || dz->columns != weight->rows ||
+        !has_shape(dx, 1, dz->rows, weight->columns) ||
+        !valid_optional(pre, 1, dz->rows, weight->columns) ||
+        !valid_optional(residual, 1, dz->rows, weight->columns) || !valid_residual(residual, dx) ||
+        !valid_activation(activation) || (!pre && activation != Q38M_ACT_NONE))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid linear input gradient");
+    if (!valid_scratch(scratch, scratch_bytes,
+                       q38m_linear_scratch_bytes(dz->rows, weight->rows, weight->columns)))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "linear scratch is missing, small or unaligned");
+    const LinearProduct p{words(dz), words(weight), stride_of(dz), stride_of(weight), nullptr,
+                          nullptr, dz->rows, weight->columns, dz->columns, 0u, 1u, 1u,
+                          LinearEpilogue{view(dx), LinearMatrix{}, view(residual), view(pre),
+                                         activation, true}};
+    return run_linear(p, LinearOrder::kNN, LinearFold::kPlain, scratch, stream, device);
+}
+
+int q38m_linear_backward_weight_v1(const q38m_tensor_v1* dz, const q38m_tensor_v1* x,
+                                   const q38m_tensor_v1* residual,
+                                   const q38m_tensor_v1* d_weight,
+                                   const q38m_tensor_v1* d_bias, void* scratch,
+                                   size_t scratch_bytes, void* stream, int device) {
+    if (!valid_operand(dz) || dz->experts != 1u || (!d_weight && !d_bias) ||
+        (d_weight && (!valid_operand(x) || x->experts != 1u || x->rows != dz->rows ||
+                      !has_shape(d_weight, 1, dz->columns, x->columns) ||
+                      !valid_optional(residual, 1, dz->columns, x->columns) ||
+                      !valid_residual(residual, d_weight))) ||
+        (!d_weight && residual) || !valid_optional(d_bias, 1, 1, dz->columns))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid linear weight gradient");
+    const uint32_t inputs = d_weight ? x->columns : 1u;
+    if (!valid_scratch(scratch, scratch_bytes,
+                       q38m_linear_scratch_bytes(dz->rows, dz->columns, inputs)))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "linear scratch is missing, small or unaligned");
+    if (d_weight) {
+        const LinearProduct p{words(dz), words(x), stride_of(dz), stride_of(x), nullptr, nullptr,
+                              dz->columns, x->columns, dz->rows, 0u, 1u, 1u,
+                              LinearEpilogue{view(d_weight), LinearMatrix{}, view(residual),
+                                             LinearMatrix{}, Q38M_ACT_NONE, true}};
+        if (int rc = run_linear(p, LinearOrder::kTN, LinearFold::kPlain, scratch, stream, device))
+            return rc;
+    } else if (int rc = select_device(device)) {
+        return rc;
+    }
+    if (!d_bias) return finish(hipSuccess, "");
+    return finish(q38m::launch_bias_backward(words(dz), stride_of(dz), dz->rows, dz->columns,
+                                             view(d_bias), scratch, as_stream(stream)),
+                  "bias gradient kernels");
+}
+
+int q38m_linear_backward_activation_v1(const q38m_tensor_v1* dy, const q38m_tensor_v1* pre,
+                                       uint32_t activation, const q38m_tensor_v1* dz,
+                                       void* stream, int device) {
+    if (!valid_tensor(dy) || dy->experts != 1u || !has_shape(pre, 1, dy->rows, dy->columns) ||
+        !has_shape(dz, 1, dy->rows, dy->columns) || !valid_activation(activation))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid activation gradient");
+    if (int rc = select_device(device)) return rc;
+    return finish(q38m::launch_activation_backward(view(dy), view(pre), activation, view(dz),
+                                                   dy->rows, dy->columns, as_stream(stream)),
+                  "activation_backward_kernel");
+}
+
+int q38m_moe_expert_gemm_v1(const q38m_tensor_v1* weights, const q38m_tensor_v1* rows,
+                            const uint32_t* expert_offsets, const uint32_t* packed_assignment,
+                            uint32_t top_k, uint32_t epilogue, const q38m_tensor_v1* c,
+                            const q38m_tensor_v1* pre, void* stream, int device) {
+    const bool swiglu = epilogue == Q38M_EPILOGUE_SWIGLU;
+    if (!valid_operand(weights) || !valid_operand(rows) || !valid_tensor(c) ||
+        weights->columns != rows->columns || weights->rows > kMaxWidth ||
+        !valid_sorted(expert_offsets, packed_assignment, top_k, rows, c->rows) ||
+        (!swiglu && epilogue != Q38M_EPILOGUE_NONE) || (swiglu && weights->rows % 2u != 0u) ||
+        !has_shape(c, 1, c->rows, swiglu ? weights->rows / 2u : weights->rows) ||
+        (pre && !swiglu) || !valid_optional(pre, 1, c->rows, weights->rows))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid expert product");
+    const LinearProduct p{words(rows), words(weights), stride_of(rows), stride_of(weights),
+                          expert_offsets, packed_assignment, c->rows, weights->rows,
+                          weights->columns, rows->rows, weights->experts, top_k,
+                          LinearEpilogue{view(c), LinearMatrix{}, LinearMatrix{}, view(pre),
+                                         Q38M_ACT_NONE, false}};
+    return run_linear(p, LinearOrder::kNT, swiglu ? LinearFold::kSwiglu : LinearFold::kPlain,
+                      nullptr, stream, device);
+}
+
+int q38m_moe_expert_backward_rows_v1(const q38m_tensor_v1* weights, const q38m_tensor_v1* d_c,
+                                     const uint32_t* expert_offsets, const q38m_tensor_v1* pre,
+                                     const q38m_tensor_v1* d_rows, void* stream, int device) {
+    if (!valid_operand(weights) || !valid_operand(d_c) || weights->rows != d_c->columns ||
+        !valid_sorted(expert_offsets, nullptr, 1u, d_c, d_c->rows) ||
+        (pre && weights->columns > kMaxWidth / 2u) ||
+        !has_shape(d_rows, 1, d_c->rows, pre ? 2u * weights->columns : weights->columns) ||
+        !valid_optional(pre, 1, d_c->rows, 2u * weights->columns))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid expert row gradient");
+    const LinearProduct p{words(d_c), words(weights), stride_of(d_c), stride_of(weights),
+                          expert_offsets, nullptr, d_c->rows, weights->columns, weights->rows,
+                          d_c->rows, weights->experts, 1u,
+                          LinearEpilogue{view(d_rows), LinearMatrix{}, LinearMatrix{}, view(pre),
+                                         Q38M_ACT_NONE, true}};
+    return run_linear(p, LinearOrder::kNN, pre ? LinearFold::kSwigluGrad : LinearFold::kPlain,
+                      nullptr, stream, device);
+}
+
+int q38m_moe_expert_backward_weights_v1(const q38m_tensor_v1* d_c, const q38m_tensor_v1* rows,
+                                        const uint32_t* expert_offsets,
+                                        const uint32_t* packed_assignment, uint32_t top_k,
+                                        const q38m_tensor_v1* residual,
+                                        const q38m_tensor_v1* d_weights, void* stream,
+                                        int device) {
+    if (!valid_operand(d_c) || !valid_operand(rows) || d_c->experts != 1u ||
+        !valid_sorted(expert_offsets, packed_assignment, top_k, rows, d_c->rows) ||
+        !valid_tensor(d_weights) ||
+        !has_shape(d_weights, d_weights->experts, d_c->columns, rows->columns) ||
+        !valid_optional(residual, d_weights->experts, d_c->columns, rows->columns) ||
+        !valid_residual(residual, d_weights))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid expert weight gradient");
+    const LinearProduct p{words(d_c), words(rows), stride_of(d_c), stride_of(rows),
+                          expert_offsets, packed_assignment, d_c->columns, rows->columns,
+                          d_c->rows, rows->rows, d_weights->experts, top_k,
+                          LinearEpilogue{view(d_weights), LinearMatrix{}, view(residual),
+                                         LinearMatrix{}, Q38M_ACT_NONE, true}};
+    return run_linear(p, LinearOrder::kTN, LinearFold::kPlain, nullptr, stream, device);
+}
+
 int q38m_synth_fill(uint32_t kind, uint64_t seed, uint64_t tag, uint64_t count, float sigma,
                     int32_t lo, int32_t hi, const float* bias, uint32_t bias_len, void* out,
                     void* stream, int device) {

@@ -290,4 +290,50 @@ struct MxProduct {
 bool mx_product_fits(const MxProduct& p, bool swiglu);
 hipError_t launch_mx_product(const MxProduct& p, bool swiglu, hipStream_t stream);
 
+// bf16 products with epilogues and gradients (q38m_linear.hip)
+constexpr uint32_t kMaxLinearRows = 1u << 28;
+// an element of a matrix of either type; null: not there
+struct LinearMatrix {
+    void* data;
+    uint64_t stride;  // elements
+    bool f32;
+};
+// What becomes of a product's fp32 sums v.  Forward: pre = v + bias, c = act(pre) +
+// residual.  Gradient (slope): c = v * act'(pre) + residual.
+struct LinearEpilogue {
+    LinearMatrix c, bias, residual, pre;
+    uint32_t activation;
+    bool slope;
+};
+// kNT: C = A B^T, rows of A and B as stored; kNN: C = A B, K along B's stored rows;
+// kTN: C = A^T B, K along both's.  The stored rows along K are `depth`, of kTN with
+// offsets an expert's part of them.
+enum class LinearOrder { kNT, kNN, kTN };
+enum class LinearFold { kPlain, kSwiglu, kSwigluGrad };
+struct LinearProduct {
+    const uint16_t* a;
+    const uint16_t* b;
+    uint64_t a_stride, b_stride;  // elements from stored row to stored row
+    const uint32_t* offsets;      // null: the dense product
+    const uint32_t* packed;       // null, or gathers kNT's rows of A, kTN's of B
+    uint32_t rows;                // of C; kTN with offsets: of an expert
+    uint32_t columns;             // of C in front of a fold
+    uint32_t depth;               // K; kTN with offsets: all experts' rows (routes)
+    uint32_t source_rows;         // gathered: the rows to choose from
+    uint32_t experts, top_k;
+    LinearEpilogue e;
+};
+size_t linear_scratch_bytes(uint32_t rows, uint32_t outputs, uint32_t inputs);
+// whether its tiles can be counted and an expert's (gathered) rows reached
+bool linear_fits(const LinearProduct& p, LinearOrder order, LinearFold fold);
+hipError_t launch_linear(const LinearProduct& p, LinearOrder order, LinearFold fold, void* scratch,
+                         hipStream_t stream);
+hipError_t launch_activation_backward(const LinearMatrix& dy, const LinearMatrix& pre,
+                                      uint32_t activation, const LinearMatrix& dz, uint32_t rows,
+                                      uint32_t columns, hipStream_t stream);
+// sums of the columns of bf16 rows
+hipError_t launch_bias_backward(const uint16_t* dz, uint64_t stride, uint32_t rows,
+                                uint32_t columns, const LinearMatrix& d_bias, void* scratch,
+                                hipStream_t stream);
+
 }  // namespace q38m
