@@ -1129,8 +1129,9 @@ bool valid_operand(const q38m_tensor_v1* t) {
     return valid_tensor(t) && t->dtype == Q38M_DTYPE_BF16;
 }
 
-uint64_t stride_of(const q38m_tensor_v1* t) {  // one row: any
-    return static_cast<uint64_t>(t->experts) * t->rows == 1u ? t->columns : t->row_stride;
+uint64_t stride_of(const q38m_tensor_v1* t) {  // one row: any, so that the next would start at 16 bytes
+    return static_cast<uint64_t>(t->experts) * t->rows == 1u ? (t->columns + 7u) / 8u * 8u
+                                                             : t->row_stride;
 }
 
 // a residual that is the output is read and written element by element

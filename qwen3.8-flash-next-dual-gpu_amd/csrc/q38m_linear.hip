@@ -9,6 +9,7 @@
 
 #include "q38m_device.h"
 #include "q38m_internal.h"
+#include "q38m_linear_tiles.h"
 #include "q38m_product.h"
 
 namespace q38m {
@@ -412,6 +413,555 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearProduct p) {
     }
 }
 
+// ---- products of rows at 16 bytes -------------------------------------------------
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+// v_mfma_f32_32x32x16_bf16: lane l holds k = 8 (l / 32) .. + 7 of row l % 32 of A and of B;
+// D lane l: rows 8 (i / 4) + 4 (l / 32) + i % 4 of A, row l % 32 of B.
+// v_mfma_f32_16x16x32_bf16: k = 8 (l / 16) .. + 7 of row l % 16; D lane l: rows 4 (l / 16)
+// + i of A, row l % 16 of B.
+__device__ __forceinline__ v4f mfma_bf16(v4i a, v4i b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v16f mfma_bf16(v4i a, v4i b, v16f c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// The block of LDS that holds an operand's 64 values of K for kWidth rows of C (columns of
+// C): 128 bytes for each of them.
+//
+// Along K (as stored): a row's 64 values are eight 16-byte pieces, at positions p ^ (r / 2
+// % 8), so that the lanes of a read, one piece of 16 or 32 consecutive rows, spread over
+// all 64 banks.
+//
+// Across K: a stored row has kWidth values of one k, in units of 32 bytes.  A transposing
+// read (ds_read_b64_tr_b16) takes for 16 lanes four k by 16 columns, one unit of each k:
+// lane i gives the address of a quarter (i % 4) of k i / 4's unit and gets column i's four
+// values.  The units of k lie at positions u ^ x(k), where x differs between the eight k
+// whose units 32 lanes read together.
+template <bool kAcross, uint32_t kWidth>
+struct Block {
+    static constexpr uint32_t kUnits = kWidth / 16u;
+    static constexpr uint32_t kRowLanes = kWidth / 8u;  // 16-byte pieces of a stored row across K
+    static_assert(!kAcross || kWidth >= 64u, "a load instruction brings whole stored rows");
+
+    // the stored row (across K: the k) and 16-byte piece of it of load instruction i's lane
+    __device__ MX_INLINE static uint32_t row(uint32_t i, uint32_t lane) {
+        if constexpr (kAcross) return i * (64u / kRowLanes) + lane / kRowLanes;
+        else return 8u * i + (lane >> 3);
+    }
+    __device__ MX_INLINE static uint32_t piece(uint32_t i, uint32_t lane) {
+        if constexpr (kAcross) return (lane % kRowLanes) ^ (flip(row(i, lane)) << 1);
+        else return (lane & 7u) ^ (row(i, lane) >> 1 & 7u);
+    }
+    __device__ MX_INLINE static uint32_t flip(uint32_t k) {
+        if constexpr (kUnits >= 8u) return (k & 3u) << 1 | (k >> 3 & 1u);
+        else return k & 2u | (k >> 3 & 1u);
+    }
+};
+
+// Workgroups stay and compute tile after tile of kBM x kBN values of C (with the SwiGLU fold
+// half of the columns gate, half up), kWM x kWN waves, each kTM x kTN matrix-instruction
+// tiles of kMF rows.  K goes through LDS in stages of 64 values, in a ring of kStages slots,
+// loaded straight from memory; the stages of a tile follow those of the tile before without
+// a gap.
+template <typename S, LinearOrder kOrder, bool kExperts, LinearFold kFold>
+__global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 4u) void linear_tile_kernel(
+    LinearProduct p, uint32_t each) {
+    constexpr uint32_t kMF = S::kMF, kTM = S::kTM, kTN = S::kTN, kBM = S::kBM, kBN = S::kBN;
+    constexpr bool kAcrossA = kOrder == LinearOrder::kTN, kAcrossB = kOrder != LinearOrder::kNT;
+    constexpr bool kSwiglu = kFold == LinearFold::kSwiglu;
+    constexpr bool kRagged = kExperts && kAcrossA;  // K is the expert's rows
+    using A = Block<kAcrossA, kBM>;
+    using B = Block<kAcrossB, kBN>;
+    using Acc = std::conditional_t<kMF == 32u, v16f, v4f>;
+    constexpr uint32_t kAcc = kMF == 32u ? 16u : 4u;
+    __shared__ v4i ring[kExperts ? S::kLds : S::kOffsetsAt];
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __builtin_assume(wave < S::kWaves);  // settles at compile time which loads are of A and which of B
+    const uint32_t n_out = kSwiglu ? p.columns / 2u : p.columns;
+    constexpr uint32_t kColumns = kSwiglu ? kBN / 2u : kBN;
+    const uint32_t columns = (n_out + kColumns - 1u) / kColumns;
+
+    // ---- this workgroup's tiles ----
+    uint32_t* offsets = reinterpret_cast<uint32_t*>(ring + S::kOffsetsAt);
+    const uint32_t last_offset = kExperts ? p.offsets[p.experts] : 0u;
+    const uint32_t routes = kRagged ? p.depth : p.rows;
+    if constexpr (kExperts) {
+        for (uint32_t e = threadIdx.x; e < kMaxSortExperts; e += 64u * S::kWaves)
+            offsets[e] = e < p.experts ? p.offsets[e] : last_offset;
+        __syncthreads();
+#ifdef Q38M_CHECKED
+        for (uint32_t e = threadIdx.x; e < p.experts; e += 64u * S::kWaves) {
+            const uint32_t end = p.offsets[e + 1u];
+            report(end < offsets[e] || end > routes, kCheckOffsets);
+        }
+        if (p.packed)  // each workgroup looks at a part of the sources
+            for (uint32_t i = offsets[0] + blockIdx.x * 64u * S::kWaves + threadIdx.x; i < min(last_offset, routes);
+                 i += gridDim.x * 64u * S::kWaves)
+                report(p.packed[i] / p.top_k >= p.source_rows, kCheckToken);
+#endif
+    }
+    // K that is ragged: an expert's rows are one "row tile" of the list
+    const auto make_list = [&]() MX_INLINE {
+        if constexpr (kExperts) return TileList<kRagged ? 1u << 24 : kBM>(offsets, last_offset, routes);
+        else return 0;
+    };
+    const auto list = make_list();
+    const uint32_t of_rows = (p.rows + kBM - 1u) / kBM;  // row tiles of a matrix C
+    const auto row_tiles = [&]() MX_INLINE {
+        if constexpr (kRagged) return list.total * of_rows;
+        else if constexpr (kExperts) return list.total;
+        else return of_rows * ((p.depth + each - 1u) / each);
+    };
+    if constexpr (kRagged) {
+        // experts without rows: zeros, and what they are added to, unless that is there already
+        if (p.e.residual.data != p.e.c.data)
+            for (uint32_t e = 0; e < p.experts; ++e) {
+                const uint32_t begin = offsets[e], end = e + 1u < kMaxSortExperts ? offsets[e + 1u] : last_offset;
+                if (min(end, routes) > min(begin, routes)) continue;
+                for (uint32_t r = blockIdx.x; r < p.rows; r += gridDim.x)
+                    for (uint32_t c = threadIdx.x * 8u; c < n_out; c += S::kWaves * 512u) {
+                        float v[8] = {};
+                        finish_plain(p.e, static_cast<uint64_t>(e) * p.rows + r, c, n_out, v);
+                    }
+            }
+    }
+    MxOrder order(row_tiles(), columns);
+    if (order.count == 0u) return;
+    // what is known of the tiles being loaded: lane t % 64 holds the t-th
+    uint32_t known_first = 0, known_count = 0, known_column = 0, known_depth = 0, known_matrix = 0;
+
+    // ---- loads: instructions dealt to the waves, the left over ones to the first: 1 KB of
+    // data each.  Those of A first, then of B, each instruction of one of them: a base of its
+    // tile and stage for all lanes and an offset below 4 GB for each ----
+    constexpr uint32_t kDataA = kBM / 8u, kData = S::kRows / 8u;
+    constexpr uint32_t kDataEach = kData / S::kWaves, kDataRest = kData % S::kWaves;
+    constexpr uint32_t kDataLoads = kDataEach + (kDataRest != 0u ? 1u : 0u);
+    const bool data_rest = kDataRest != 0u && wave < kDataRest;
+    const auto data_live = [&](uint32_t t) MX_INLINE { return kDataRest == 0u || t < kDataEach || data_rest; };
+    const auto of_a = [&](uint32_t t) MX_INLINE { return t * S::kWaves < kDataA && wave + t * S::kWaves < kDataA; };
+    const uint32_t a_bytes = static_cast<uint32_t>(p.a_stride) * 2u, b_bytes = static_cast<uint32_t>(p.b_stride) * 2u;
+    const uint64_t a_step = kAcrossA ? 64ull * a_bytes : 128u, b_step = kAcrossB ? 64ull * b_bytes : 128u;
+    const uint8_t* a_all = reinterpret_cast<const uint8_t*>(p.a);
+    const uint8_t* b_all = reinterpret_cast<const uint8_t*>(p.b);
+    const bool gather = kExperts && kOrder != LinearOrder::kNN && p.packed;
+    const uint8_t *a_base, *b_base;  // of the stage being loaded
+    uint32_t data[kDataLoads];
+    // the next tile to load, the `found`-th from one on, looked up a tile ahead, so that nobody
+    // waits; with the sources of its rows of A where they are gathered
+    uint32_t found = 0, next_column = 0, next_from = 0, next_depth = 0;
+    RowTile next{0u, 0u, 0u, false};
+    uint32_t source[kDataLoads];
+    const auto fresh_lane = [&]() MX_INLINE {
+        uint32_t l = lane;
+        if constexpr (S::kWaves == 8u) asm volatile("" : "+v"(l));
+        return l;
+    };
+    const auto look_up = [&]() MX_INLINE {
+        if (found == order.count) return;
+        const uint32_t own_lane = fresh_lane();
+        if (found != 0u) order.at += order.step;
+        const uint32_t row = order.row();
+        next_column = order.column();
+        next_from = 0u;
+        next_depth = p.depth;
+        uint32_t matrix = 0;
+        if constexpr (kRagged) {
+            const RowTile all = list.find(row / of_rows);
+            next = RowTile{all.expert, row % of_rows * kBM, 0u, false};
+            next.count = min(p.rows - next.first, kBM);
+            next_from = all.first;
+            next_depth = all.count;
+            matrix = all.expert;
+        } else if constexpr (kExperts) {
+            next = list.find(row);
+        } else {
+            matrix = row / of_rows;  // the part of K, whose sums are a matrix of their own
+            next = RowTile{0u, row % of_rows * kBM, 0u, false};
+            next.count = min(p.rows - next.first, kBM);
+            next_from = matrix * each;
+            next_depth = min(p.depth - next_from, each);
+        }
+        if (own_lane == found % 64u) {
+            known_first = next.first;
+            known_count = next.count;
+            known_column = next_column;
+            known_depth = next_depth;
+            known_matrix = matrix;
+        }
+        ++found;
+        if constexpr (kExperts && !kAcrossB) {
+            if (!p.packed) return;
+#pragma unroll
+            for (uint32_t t = 0; t < kDataLoads; ++t)
+                if (data_live(t) && of_a(t))
+                    source[t] = p.packed[next.first + min(A::row(wave + t * S::kWaves, own_lane), next.count - 1u)];
+        }
+    };
+    uint32_t from = 0, stages = 0, depth = 0, k_from = 0;  // of the tile being loaded: the stage, and its K
+    // points the loads at the tile that was looked up, and looks up the one after it
+    uint32_t a_last = 0, b_last = 0;  // across K: the last piece that is there of a stored row
+    const auto point = [&]() MX_INLINE {
+        const uint32_t own_lane = fresh_lane();
+        depth = next_depth;
+        stages = (depth + 63u) / 64u;
+        k_from = next_from;
+        if constexpr (kAcrossA) {
+            a_base = a_all + static_cast<uint64_t>(next_from) * a_bytes + 2ull * next.first;
+        } else {
+            a_base = a_all + (gather ? 0ull : static_cast<uint64_t>(next.first) * a_bytes) + 2ull * next_from;
+        }
+        const uint64_t b_first = kRagged ? (gather ? 0u : next_from)
+                                 : kExperts ? static_cast<uint64_t>(next.expert) * (kAcrossB ? p.depth : p.columns)
+                                            : (kAcrossB ? next_from : 0u);
+        b_base = b_all + (b_first + (kAcrossB ? 0u : next_column * kColumns)) * b_bytes +
+                 2ull * (kAcrossB ? next_column * kColumns : next_from);
+        a_base = mx_uniform(a_base);
+        b_base = mx_uniform(b_base);
+        a_last = (next.count - 1u) / 8u;
+        b_last = (min(p.columns - next_column * kColumns, kBN) - 1u) / 8u;
+#pragma unroll
+        for (uint32_t t = 0; t < kDataLoads; ++t) {
+            if (!data_live(t)) continue;
+            const uint32_t i = wave + t * S::kWaves;
+            if (of_a(t)) {
+                const uint32_t r = A::row(i, own_lane), piece = A::piece(i, own_lane);
+                if constexpr (kAcrossA) data[t] = r * a_bytes + 16u * min(piece, a_last);
+                else data[t] = (gather ? min(source[t] / p.top_k, p.source_rows - 1u) : min(r, next.count - 1u)) * a_bytes + 16u * piece;
+            } else {
+                const uint32_t r = B::row(i - kDataA, own_lane), piece = B::piece(i - kDataA, own_lane);
+                if constexpr (kAcrossB) {
+                    data[t] = r * b_bytes + 16u * min(piece, b_last);
+                } else {
+                    uint32_t column = r, up = 0;
+                    if constexpr (kSwiglu) {  // a wave's tiles: half of them gate, half up
+                        const uint32_t tile = r / kMF % kTN;
+                        column = r / (kTN * kMF) * (kTN / 2u * kMF) + tile % (kTN / 2u) * kMF + r % kMF;
+                        up = tile >= kTN / 2u ? n_out : 0u;
+                    }
+                    data[t] = (min(column, n_out - 1u - next_column * kColumns) + up) * b_bytes + 16u * piece;
+                }
+            }
+        }
+        look_up();
+    };
+    // gathered stored rows along K: the stage's sources, looked up a stage ahead
+    const auto look_ahead = [&](uint32_t first, uint32_t stage, uint32_t count) MX_INLINE {
+#pragma unroll
+        for (uint32_t t = 0; t < kDataLoads; ++t) {
+            const uint32_t i = wave + t * S::kWaves;
+            if (data_live(t) && !of_a(t))
+                source[t] = p.packed[first + min(stage * 64u + B::row(i - kDataA, lane), count - 1u)];
+        }
+    };
+    const auto take_sources = [&]() MX_INLINE {
+#pragma unroll
+        for (uint32_t t = 0; t < kDataLoads; ++t) {
+            const uint32_t i = wave + t * S::kWaves;
+            if (data_live(t) && !of_a(t))
+                data[t] = min(source[t] / p.top_k, p.source_rows - 1u) * b_bytes + 16u * min(B::piece(i - kDataA, lane), b_last);
+        }
+        if (from + 1u < stages) look_ahead(k_from, from + 1u, depth);
+        else look_ahead(next_from, 0u, next_depth);
+    };
+    // a tile's last stage where K ends inside it: what lies behind is another piece, or row, of it
+    const auto hold_back = [&]() MX_INLINE {
+        const uint32_t valid = depth - from * 64u;
+        if (valid >= 64u) return;
+#pragma unroll
+        for (uint32_t t = 0; t < kDataLoads; ++t) {
+            if (!data_live(t)) continue;
+            const uint32_t i = wave + t * S::kWaves;
+            const auto behind = [&](uint32_t at, uint32_t last) MX_INLINE { return at > last ? at - last : 0u; };
+            if (of_a(t)) {
+                if constexpr (kAcrossA) data[t] -= behind(A::row(i, lane), valid - 1u) * a_bytes;
+                else data[t] -= behind(A::piece(i, lane), (valid - 1u) / 8u) * 16u;
+            } else if constexpr (kAcrossB) {
+                if (!(kRagged && gather)) data[t] -= behind(B::row(i - kDataA, lane), valid - 1u) * b_bytes;
+            } else {
+                data[t] -= behind(B::piece(i - kDataA, lane), (valid - 1u) / 8u) * 16u;
+            }
+        }
+    };
+    look_up();
+    uint32_t tiles_left = order.count;  // with the one being loaded
+    bool turn = false, moved = false;
+    point();
+    if constexpr (kRagged) {
+        if (gather) {
+            look_ahead(k_from, 0u, depth);
+            take_sources();
+        }
+    }
+    if (stages == 1u) hold_back();
+    uint32_t to = 0;  // the slot that is loaded
+    const uint32_t ring_at = static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) v4i*)ring));
+    const auto load_data = [&](uint32_t t) MX_INLINE {
+        if (!data_live(t)) return;
+        const uint32_t i = wave + t * S::kWaves;
+        const uint32_t at = __builtin_amdgcn_readfirstlane(ring_at + to * (S::kSlot * 16u) + i * 1024u);
+        mx_load16(of_a(t) ? a_base : b_base, data[t], at);
+    };
+    // to the next stage to load; past the last tile the last stage again, into slots that nobody
+    // reads any more, so that the count of loads under way is always the same
+    const auto load_next = [&]() MX_INLINE {
+        to = to + 1u == S::kStages ? 0u : to + 1u;
+        if (from + 1u < stages) {
+            ++from;
+            a_base += a_step;
+            if (!(kRagged && gather)) b_base += b_step;
+            moved = true;
+        } else if (tiles_left != 1u) {
+            turn = true;
+        }
+    };
+    // what the next stage's loads need, behind the barrier in front of them
+    const auto take_turn = [&]() MX_INLINE {
+        if (turn) {
+            turn = false;
+            moved = true;
+            --tiles_left;
+            from = 0;
+            point();
+        }
+        if constexpr (kRagged) {
+            if (gather) take_sources();
+        }
+        if (moved && from + 1u == stages) hold_back();
+        moved = false;
+    };
+
+    // ---- products ----
+    const uint32_t wm = wave / S::kWN, wn = wave % S::kWN;
+    const uint32_t n = lane % kMF, q = lane / kMF;
+    Acc acc[kTN][kTM];
+#pragma unroll
+    for (uint32_t j = 0; j < kTN; ++j)
+#pragma unroll
+        for (uint32_t i = 0; i < kTM; ++i) acc[j][i] = Acc{};
+    constexpr uint32_t kReads = kTM + kTN;
+    // where a lane's fragments start in a slot, bytes
+    uint32_t part_at[kReads];
+#pragma unroll
+    for (uint32_t i = 0; i < kReads; ++i) {
+        const uint32_t tile = i < kTM ? wm * kTM + i : wn * kTN + i - kTM;
+        const uint32_t block = i < kTM ? 0u : kBM * 128u;
+        const bool across = i < kTM ? kAcrossA : kAcrossB;
+        const uint32_t width = i < kTM ? kBM : kBN;
+        if (across) {
+            const uint32_t k = 8u * q + lane % 16u / 4u, unit = tile * (kMF / 16u) + lane % kMF / 16u;
+            const uint32_t flip = i < kTM ? A::flip(k) : B::flip(k);
+            part_at[i] = block + k * 2u * width + (unit ^ flip) * 32u + lane % 4u * 8u;
+        } else {
+            part_at[i] = block + (tile * kMF + n) * 128u;
+        }
+    }
+    const uint32_t swizzle = n >> 1 & 7u;  // along K, as of every kMF-th row after it
+    v4i part[2][kReads];  // a step's fragments of A, then of B, and the next step's
+    uint32_t slot = 0;    // of the stage whose fragments are read
+    auto* lds = (__attribute__((address_space(3))) char*)ring;
+    const auto read = [&](uint32_t c, uint32_t i) MX_INLINE {
+        const uint32_t at = slot * (S::kSlot * 16u) + part_at[i];
+        if (i < kTM ? kAcrossA : kAcrossB) {
+            const uint32_t row = (i < kTM ? kBM : kBN) * 2u;
+            const v4s low = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) v4s*)(lds + at + 512u / kMF * c * row));
+            const v4s high = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) v4s*)(lds + at + (512u / kMF * c + 4u) * row));
+            const v2u a = __builtin_bit_cast(v2u, low), b = __builtin_bit_cast(v2u, high);
+            part[c % 2u][i] = v4i{static_cast<int>(a.x), static_cast<int>(a.y), static_cast<int>(b.x), static_cast<int>(b.y)};
+        } else {
+            part[c % 2u][i] = *(__attribute__((address_space(3))) v4i*)(lds + at + ((64u / kMF * c + q) ^ swizzle) * 16u);
+        }
+    };
+    // zeros behind the `valid` values of K of the stage in this slot, of both operands: what
+    // was loaded there may be anything, NaN too
+    const auto clear = [&](uint32_t valid) MX_INLINE {
+        const uint32_t first = slot * S::kSlot;
+        const auto part_of = [&](uint32_t w, bool across, uint32_t width, uint32_t block) MX_INLINE {
+            const uint32_t at = first + block + w;
+            if (across) {
+                if (w / (width / 8u) >= valid) ring[at] = v4i{0, 0, 0, 0};
+                return;
+            }
+            const uint32_t row = w / 8u, k = 8u * ((w & 7u) ^ (row >> 1 & 7u));
+            if (k >= valid) {
+                ring[at] = v4i{0, 0, 0, 0};
+            } else if (k + 8u > valid) {
+                v4i v = ring[at];
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) {
+                    if (k + 2u * e >= valid) v[e] = 0;
+                    else if (k + 2u * e + 1u >= valid) v[e] &= 0xffff;
+                }
+                ring[at] = v;
+            }
+        };
+#pragma unroll 1
+        for (uint32_t w = threadIdx.x; w < kBM * 8u; w += 64u * S::kWaves) part_of(w, kAcrossA, kBM, 0u);
+#pragma unroll 1
+        for (uint32_t w = threadIdx.x; w < kBN * 8u; w += 64u * S::kWaves) part_of(w, kAcrossB, kBN, kBM * 8u);
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    // the matrix instructions of step c, `ops` other operations among them from the first on
+    const auto multiply = [&](auto step, auto ops, auto op) MX_INLINE {
+        constexpr uint32_t kC = decltype(step)::value, kOps = decltype(ops)::value, kAll = kTM * kTN;
+        constexpr uint32_t kPer = (kOps + kAll - 1u) / kAll;
+#pragma unroll
+        for (uint32_t m = 0; m < kAll; ++m) {
+            const uint32_t j = m / kTM, i = m % kTM;
+            acc[j][i] = mfma_bf16(part[kC % 2u][kTM + j], part[kC % 2u][i], acc[j][i]);
+#pragma unroll
+            for (uint32_t o = m * kPer; o < (m + 1u) * kPer && o < kOps; ++o) op(o);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    constexpr uint32_t kEarly = (kDataLoads + 1u) / 2u;  // data loads in the step behind the barrier, the rest a step later
+
+    // A stage in kSteps steps, software pipelined: a step's fragments are read while the step in
+    // front of it is multiplied.  In front of the last step the workgroup meets: the next stage
+    // (`valid` values of K) has come and this one is read, so its slot takes the kStages-th after it.
+    const auto stage = [&](uint32_t valid) MX_INLINE {
+        constexpr uint32_t kLater = S::kStages - 2u;  // loads of the stages behind the next may be under way
+        const auto step = [&](auto c) MX_INLINE {
+            constexpr uint32_t kC = decltype(c)::value;
+            constexpr uint32_t kLoads = kC == 0u ? kDataLoads - kEarly : 0u;
+            multiply(c, std::integral_constant<uint32_t, kReads + kLoads>{}, [&](uint32_t o) MX_INLINE {
+                if (o < kReads) read(kC + 1u, o);
+                else load_data(kEarly + o - kReads);
+            });
+            if constexpr (kC == 0u) load_next();
+        };
+        step(std::integral_constant<uint32_t, 0>{});
+        if constexpr (S::kSteps > 2u) {
+            step(std::integral_constant<uint32_t, 1>{});
+            step(std::integral_constant<uint32_t, 2>{});
+        }
+        if (data_rest) mx_barrier<(kDataEach + (kDataRest != 0u ? 1u : 0u)) * kLater>();
+        else mx_barrier<kDataEach * kLater>();
+        take_turn();
+        slot = slot + 1u == S::kStages ? 0u : slot + 1u;
+        if (valid < 64u) clear(valid);
+        multiply(std::integral_constant<uint32_t, S::kSteps - 1u>{}, std::integral_constant<uint32_t, kReads + kEarly>{},
+                 [&](uint32_t o) MX_INLINE {
+                     if (o < kReads) read(0u, o);
+                     else load_data(o - kReads);
+                 });
+    };
+
+    // ---- C: a lane has four consecutive columns of a row and trades one of two such groups with
+    // the lane that has the columns beside the other's, which gives both of them eight ----
+    const auto store = [&](uint32_t t) MX_INLINE {
+        constexpr uint32_t kOut = kSwiglu ? kTN / 2u : kTN;  // tiles across
+        constexpr uint32_t kFours = kOut * kAcc / 4u;        // a lane's groups of four
+        constexpr uint32_t kN = kFours == 1u ? 4u : 8u;
+        const uint32_t own_lane = fresh_lane(), n = own_lane % kMF, q = own_lane / kMF;
+        const uint32_t count = __builtin_amdgcn_readlane(known_count, t % 64u);
+        const uint64_t first_row = static_cast<uint64_t>(__builtin_amdgcn_readlane(known_matrix, t % 64u)) * p.rows +
+                                   __builtin_amdgcn_readlane(known_first, t % 64u);
+        const uint32_t first_column = __builtin_amdgcn_readlane(known_column, t % 64u) * kColumns + wn * kOut * kMF;
+        // the columns of group f start at kGap f + 4 q of the wave's
+        constexpr uint32_t kGap = kMF == 32u ? 8u : 16u;
+#pragma unroll
+        for (uint32_t i = 0; i < kTM; ++i) {
+            const uint32_t m = (wm * kTM + i) * kMF + n;
+            if ((wm * kTM + i) * kMF >= count) break;
+            const auto values = [&](uint32_t f, uint32_t shift, float (&v)[kN]) MX_INLINE {
+                const auto sum = [&](uint32_t g, uint32_t e) MX_INLINE {
+                    return acc[g / (kAcc / 4u) + shift][i][4u * (g % (kAcc / 4u)) + e];
+                };
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) {
+                    if constexpr (kN == 4u) {
+                        v[e] = sum(f, e);
+                    } else {
+                        const uint32_t a = __float_as_uint(sum(f, e)), b = __float_as_uint(sum(f + 1u, e));
+                        const auto both = [&]() MX_INLINE {
+                            if constexpr (kMF == 32u) return __builtin_amdgcn_permlane32_swap(a, b, false, false);
+                            else return __builtin_amdgcn_permlane16_swap(a, b, false, false);
+                        }();
+                        v[e] = __uint_as_float(both[0]);
+                        v[4u + e] = __uint_as_float(both[1]);
+                    }
+                }
+            };
+#pragma unroll
+            for (uint32_t f = 0; f < kFours; f += kN / 4u) {
+                const uint32_t column = first_column + (kN == 4u      ? 4u * q
+                                                        : kMF == 32u ? kGap * (f + q)
+                                                                      : kGap * (f + q % 2u) + 4u * (q & 2u));
+                float v[kN];
+                values(f, 0u, v);
+                [[maybe_unused]] float u[kN];
+                if constexpr (kSwiglu) values(f, kOut, u);
+                if (m >= count || column >= n_out) continue;
+                if constexpr (kSwiglu) finish_swiglu(p.e, first_row + m, column, n_out, v, u);
+                else if constexpr (kFold == LinearFold::kSwigluGrad) finish_swiglu_grad(p.e, first_row + m, column, n_out, v);
+                else finish_plain(p.e, first_row + m, column, n_out, v);
+            }
+        }
+    };
+
+    // all stages that the ring holds under way, but for the last one's later loads
+#pragma unroll
+    for (uint32_t s = 0; s < S::kStages; ++s) {
+#pragma unroll
+        for (uint32_t t = 0; t < (s + 1u < S::kStages ? kDataLoads : kEarly); ++t) load_data(t);
+        if (s + 1u < S::kStages) {
+            load_next();
+            take_turn();
+        }
+    }
+    // the first stage has come when no more than the others' loads are under way
+    constexpr uint32_t kFirst = kDataEach * (S::kStages - 2u) + (kEarly < kDataEach ? kEarly : kDataEach);
+    mx_barrier<kFirst>();
+    const auto depth_of = [&](uint32_t t) MX_INLINE -> uint32_t {
+        return __builtin_amdgcn_readlane(known_depth, t % 64u);
+    };
+    uint32_t left = depth_of(0u);  // values of K of the tile that are not multiplied yet
+    if (left < 64u) clear(left);
+#pragma unroll
+    for (uint32_t i = 0; i < kReads; ++i) read(0u, i);
+    for (uint32_t t = 0;; ++t) {
+        const uint32_t after = t + 1u == order.count ? 64u : depth_of(t + 1u);
+        for (; left > 64u; left -= 64u) stage(left - 64u);
+        stage(after);
+        store(t);
+        if (t + 1u == order.count) break;
+        left = after;
+#pragma unroll
+        for (uint32_t j = 0; j < kTN; ++j)
+#pragma unroll
+            for (uint32_t i = 0; i < kTM; ++i) acc[j][i] = Acc{};
+    }
+    mx_barrier<0>();  // no load is under way to LDS that the next workgroup gets
+}
+
+// Sums of the parts of K, in their order, and the epilogue: eight columns of a row a thread.
+__global__ __launch_bounds__(256) void linear_join_kernel(const float* __restrict__ parts, uint32_t count, uint32_t rows,
+                                                          uint32_t columns, LinearEpilogue e) {
+    const uint32_t pieces = (columns + 7u) / 8u;
+    const uint64_t all = static_cast<uint64_t>(rows) * pieces;
+    const LinearMatrix m{const_cast<float*>(parts), columns, true};
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < all; i += gridDim.x * 256ull) {
+        const uint64_t row = i / pieces;
+        const uint32_t column = static_cast<uint32_t>(i % pieces) * 8u;
+        float v[8];
+        load_row(m, row * columns + column, columns - column, v);
+        for (uint32_t s = 1; s < count; ++s) {
+            float w[8];
+            load_row(m, (static_cast<uint64_t>(s) * rows + row) * columns + column, columns - column, w);
+#pragma unroll
+            for (uint32_t k = 0; k < 8u; ++k) v[k] += w[k];
+        }
+        finish_plain(e, row, column, columns, v);
+    }
+}
+
 // ---- activation and bias gradients ------------------------------------------------
 
 // Eight columns of a row for each thread; memory bounds it.
@@ -489,22 +1039,89 @@ uint64_t any_tiles(const LinearProduct& p, LinearOrder order, LinearFold fold) {
     return rows * ((columns + across - 1u) / across);
 }
 
+LinearSizes linear_sizes(const LinearProduct& p, LinearOrder order, LinearFold fold) {
+    return LinearSizes{p.rows, p.columns, p.depth, p.offsets ? p.experts : 0u, fold == LinearFold::kSwiglu,
+                       order == LinearOrder::kTN};
+}
+
+// Whether every operand row starts at 16 bytes, and a lane's offsets from its tile's base are
+// 32-bit numbers: 256 rows along K, 64 across it, all those that are gathered, and the distance
+// from gate to up.
+bool linear_on_tiles(const LinearProduct& p, LinearOrder order, LinearFold fold) {
+    if ((reinterpret_cast<uintptr_t>(p.a) | reinterpret_cast<uintptr_t>(p.b)) % 16u != 0u ||
+        (p.a_stride | p.b_stride) % 8u != 0u)
+        return false;
+    const uint64_t limit = 1ull << 31;  // of elements
+    const uint64_t a_rows = order == LinearOrder::kNT && p.packed ? p.source_rows : 256u;
+    const uint64_t b_rows = order == LinearOrder::kTN && p.packed ? p.source_rows
+                            : fold == LinearFold::kSwiglu        ? p.columns + 256ull
+                                                                 : 256u;
+    return p.a_stride < limit && p.b_stride < limit && std::max<uint64_t>(a_rows, 256u) * p.a_stride < limit &&
+           std::max<uint64_t>(b_rows, 256u) * p.b_stride < limit;
+}
+
+template <typename S, LinearOrder kOrder, bool kExperts, LinearFold kFold>
+hipError_t launch_tiles(const LinearProduct& p, const LinearSizes& sizes, uint32_t splits, void* scratch,
+                        hipStream_t stream) {
+    const uint32_t each = kExperts ? 0u : linear_each(p.depth, splits);
+    const uint32_t parts = kExperts ? 1u : (p.depth + each - 1u) / each;
+    LinearProduct q = p;
+    if (parts > 1u) {
+        q.e = LinearEpilogue{};
+        q.e.c = LinearMatrix{scratch, p.columns, true};
+    }
+    linear_tile_kernel<S, kOrder, kExperts, kFold>
+        <<<linear_grid<S>(sizes, parts), 64u * S::kWaves, 0, stream>>>(q, each);
+    if (parts == 1u) return hipGetLastError();
+    if (hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
+    const uint64_t pieces = static_cast<uint64_t>(p.rows) * ((p.columns + 7u) / 8u);
+    const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>((pieces + 255u) / 256u, 16u * kMxCus));
+    linear_join_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(scratch), parts, p.rows, p.columns, p.e);
+    return hipGetLastError();
+}
+
+size_t split_bytes(const LinearSizes& p) {
+    return with_linear_tiles(p, [&](auto, uint32_t splits) -> size_t {
+        const uint32_t each = linear_each(p.depth, splits), parts = (p.depth + each - 1u) / each;
+        return parts > 1u ? static_cast<size_t>(parts) * p.rows * p.columns * sizeof(float) : 0u;
+    });
+}
+
 }  // namespace
 
-size_t linear_scratch_bytes(uint32_t rows, uint32_t outputs, uint32_t) {
+size_t linear_scratch_bytes(uint32_t rows, uint32_t outputs, uint32_t inputs) {
     const uint32_t parts = bias_parts(rows, outputs);
-    return parts > 1u ? static_cast<size_t>(parts) * outputs * sizeof(float) : 0u;
+    size_t most = parts > 1u ? static_cast<size_t>(parts) * outputs * sizeof(float) : 0u;
+    most = std::max(most, split_bytes(LinearSizes{rows, outputs, inputs, 0u, false, false}));
+    most = std::max(most, split_bytes(LinearSizes{rows, inputs, outputs, 0u, false, false}));
+    return std::max(most, split_bytes(LinearSizes{outputs, inputs, rows, 0u, false, true}));
 }
 
 bool linear_fits(const LinearProduct& p, LinearOrder order, LinearFold fold) {
-    return any_tiles(p, order, fold) < (1ull << 31);
+    if (any_tiles(p, order, fold) >= (1ull << 31)) return false;
+    const LinearSizes sizes = linear_sizes(p, order, fold);
+    return with_linear_tiles(sizes, [&](auto s, uint32_t splits) {
+        return linear_tiles<decltype(s)>(sizes) * splits < (1ull << 31);
+    });
 }
 
-hipError_t launch_linear(const LinearProduct& p, LinearOrder order, LinearFold fold, void*, hipStream_t stream) {
-    const uint32_t grid = static_cast<uint32_t>(any_tiles(p, order, fold));
-    const auto launch = [&](auto o, auto experts, auto f) {
-        linear_any_kernel<decltype(o)::value, decltype(experts)::value, decltype(f)::value>
-            <<<grid, 256, 0, stream>>>(p);
+hipError_t launch_linear(const LinearProduct& p, LinearOrder order, LinearFold fold, void* scratch, hipStream_t stream) {
+    const LinearSizes sizes = linear_sizes(p, order, fold);
+    const bool on_tiles = linear_on_tiles(p, order, fold);
+    const auto launch = [&](auto o, auto experts, auto f) -> hipError_t {
+        constexpr LinearOrder kOrder = decltype(o)::value;
+        constexpr bool kExperts = decltype(experts)::value;
+        constexpr LinearFold kFold = decltype(f)::value;
+        if (!on_tiles) {
+            linear_any_kernel<kOrder, kExperts, kFold>
+                <<<static_cast<uint32_t>(any_tiles(p, order, fold)), 256, 0, stream>>>(p);
+            return hipGetLastError();
+        }
+        return with_linear_tiles(sizes, [&](auto s, uint32_t splits) -> hipError_t {
+            using S = decltype(s);
+            if constexpr (kOrder == LinearOrder::kTN && S::kBM < 64u) return hipErrorInvalidValue;  // the rule takes none
+            else return launch_tiles<S, kOrder, kExperts, kFold>(p, sizes, splits, scratch, stream);
+        });
     };
     using NT = std::integral_constant<LinearOrder, LinearOrder::kNT>;
     using NN = std::integral_constant<LinearOrder, LinearOrder::kNN>;
@@ -513,19 +1130,15 @@ hipError_t launch_linear(const LinearProduct& p, LinearOrder order, LinearFold f
     using Swiglu = std::integral_constant<LinearFold, LinearFold::kSwiglu>;
     using SwigluGrad = std::integral_constant<LinearFold, LinearFold::kSwigluGrad>;
     if (!p.offsets) {
-        if (order == LinearOrder::kNT) launch(NT{}, std::false_type{}, Plain{});
-        else if (order == LinearOrder::kNN) launch(NN{}, std::false_type{}, Plain{});
-        else launch(TN{}, std::false_type{}, Plain{});
-    } else if (fold == LinearFold::kSwiglu) {
-        launch(NT{}, std::true_type{}, Swiglu{});
-    } else if (fold == LinearFold::kSwigluGrad) {
-        launch(NN{}, std::true_type{}, SwigluGrad{});
-    } else {
-        if (order == LinearOrder::kNT) launch(NT{}, std::true_type{}, Plain{});
-        else if (order == LinearOrder::kNN) launch(NN{}, std::true_type{}, Plain{});
-        else launch(TN{}, std::true_type{}, Plain{});
+        if (order == LinearOrder::kNT) return launch(NT{}, std::false_type{}, Plain{});
+        if (order == LinearOrder::kNN) return launch(NN{}, std::false_type{}, Plain{});
+        return launch(TN{}, std::false_type{}, Plain{});
     }
-    return hipGetLastError();
+    if (fold == LinearFold::kSwiglu) return launch(NT{}, std::true_type{}, Swiglu{});
+    if (fold == LinearFold::kSwigluGrad) return launch(NN{}, std::true_type{}, SwigluGrad{});
+    if (order == LinearOrder::kNT) return launch(NT{}, std::true_type{}, Plain{});
+    if (order == LinearOrder::kNN) return launch(NN{}, std::true_type{}, Plain{});
+    return launch(TN{}, std::true_type{}, Plain{});
 }
 
 hipError_t launch_activation_backward(const LinearMatrix& dy, const LinearMatrix& pre,
