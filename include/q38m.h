@@ -763,10 +763,11 @@ typedef struct q38m_tensor_v1 {
 #define Q38M_ACT_GELU 4u
 #define Q38M_ACT_GELU_TANH 5u
 
-/* Scratch that each of the three q38m_linear products of a layer with this
- * many rows, outputs (weight rows) and inputs (weight columns) takes; 0: none
- * is needed and it may be NULL.  16-byte aligned.  Two calls that may run at
- * the same time need two (captured graphs that replay together too). */
+/* Scratch that any of the three q38m_linear products of a layer with this many
+ * rows, outputs (weight rows) and inputs (weight columns) takes at most (a
+ * call that is given less than it needs is refused); 0: none is needed and it
+ * may be NULL.  16-byte aligned.  Two calls that may run at the same time need
+ * two (captured graphs that replay together too). */
 size_t q38m_linear_scratch_bytes(uint32_t rows, uint32_t outputs, uint32_t inputs);
 
 /* y = act(x weight^T + bias) + residual: x [rows][inputs], weight

@@ -1160,11 +1160,13 @@ bool valid_sorted(const uint32_t* offsets, const uint32_t* packed, uint32_t top_
 }
 
 int run_linear(const LinearProduct& p, LinearOrder order, LinearFold fold, void* scratch,
-               void* stream, int device) {
-    if (!q38m::linear_fits(p, order, fold))
-        return fail(Q38M_ERR_INVALID_ARGUMENT, "bf16 product too large for one call");
+               size_t scratch_bytes, void* stream, int device) {
+    const q38m::LinearRun run = q38m::linear_run(p, order, fold);
+    if (!run.fits) return fail(Q38M_ERR_INVALID_ARGUMENT, "bf16 product too large for one call");
+    if (!valid_scratch(scratch, scratch_bytes, run.scratch_bytes))
+        return fail(Q38M_ERR_INVALID_ARGUMENT, "linear scratch is missing, small or unaligned");
     if (int rc = select_device(device)) return rc;
-    return finish(q38m::launch_linear(p, order, fold, scratch, as_stream(stream)),
+    return finish(q38m::launch_linear(p, order, fold, run, scratch, as_stream(stream)),
                   "bf16 product kernel");
 }
 
@@ -1190,14 +1192,12 @@ int q38m_linear_v1(const q38m_tensor_v1* x, const q38m_tensor_v1* weight,
         !valid_optional(pre, 1, x->rows, weight->rows) || !valid_residual(residual, y) ||
         !valid_activation(activation))
         return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid linear layer");
-    if (!valid_scratch(scratch, scratch_bytes,
-                       q38m_linear_scratch_bytes(x->rows, weight->rows, x->columns)))
-        return fail(Q38M_ERR_INVALID_ARGUMENT, "linear scratch is missing, small or unaligned");
     const LinearProduct p{words(x), words(weight), stride_of(x), stride_of(weight), nullptr,
                           nullptr, x->rows, weight->rows, x->columns, 0u, 1u, 1u,
                           LinearEpilogue{view(y), view(bias), view(residual), view(pre),
-                                         activation, false}};
-    return run_linear(p, LinearOrder::kNT, LinearFold::kPlain, scratch, stream, device);
+                                         activation}};
+    return run_linear(p, LinearOrder::kNT, LinearFold::kForward, scratch, scratch_bytes, stream,
+                      device);
 }
 
 int q38m_linear_backward_input_v1(const q38m_tensor_v1* dz, const q38m_tensor_v1* weight,
@@ -1212,14 +1212,12 @@ int q38m_linear_backward_input_v1(const q38m_tensor_v1* dz, const q38m_tensor_v1
         !valid_optional(residual, 1, dz->rows, weight->columns) || !valid_residual(residual, dx) ||
         !valid_activation(activation) || (!pre && activation != Q38M_ACT_NONE))
         return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid linear input gradient");
-    if (!valid_scratch(scratch, scratch_bytes,
-                       q38m_linear_scratch_bytes(dz->rows, weight->rows, weight->columns)))
-        return fail(Q38M_ERR_INVALID_ARGUMENT, "linear scratch is missing, small or unaligned");
     const LinearProduct p{words(dz), words(weight), stride_of(dz), stride_of(weight), nullptr,
                           nullptr, dz->rows, weight->columns, dz->columns, 0u, 1u, 1u,
                           LinearEpilogue{view(dx), LinearMatrix{}, view(residual), view(pre),
-                                         activation, true}};
-    return run_linear(p, LinearOrder::kNN, LinearFold::kPlain, scratch, stream, device);
+                                         activation}};
+    return run_linear(p, LinearOrder::kNN, LinearFold::kSlope, scratch, scratch_bytes, stream,
+                      device);
 }
 
 int q38m_linear_backward_weight_v1(const q38m_tensor_v1* dz, const q38m_tensor_v1* x,
@@ -1234,16 +1232,16 @@ int q38m_linear_backward_weight_v1(const q38m_tensor_v1* dz, const q38m_tensor_v
                       !valid_residual(residual, d_weight))) ||
         (!d_weight && residual) || !valid_optional(d_bias, 1, 1, dz->columns))
         return fail(Q38M_ERR_INVALID_ARGUMENT, "invalid linear weight gradient");
-    const uint32_t inputs = d_weight ? x->columns : 1u;
-    if (!valid_scratch(scratch, scratch_bytes,
-                       q38m_linear_scratch_bytes(dz->rows, dz->columns, inputs)))
+    if (d_bias && !valid_scratch(scratch, scratch_bytes,
+                                 q38m::bias_scratch_bytes(dz->rows, dz->columns)))
         return fail(Q38M_ERR_INVALID_ARGUMENT, "linear scratch is missing, small or unaligned");
     if (d_weight) {
         const LinearProduct p{words(dz), words(x), stride_of(dz), stride_of(x), nullptr, nullptr,
                               dz->columns, x->columns, dz->rows, 0u, 1u, 1u,
                               LinearEpilogue{view(d_weight), LinearMatrix{}, view(residual),
-                                             LinearMatrix{}, Q38M_ACT_NONE, true}};
-        if (int rc = run_linear(p, LinearOrder::kTN, LinearFold::kPlain, scratch, stream, device))
+                                             LinearMatrix{}, Q38M_ACT_NONE}};
+        if (int rc = run_linear(p, LinearOrder::kTN, LinearFold::kAdd, scratch, scratch_bytes,
+                                stream, device))
             return rc;
     } else if (int rc = select_device(device)) {
         return rc;
@@ -1282,9 +1280,9 @@ int q38m_moe_expert_gemm_v1(const q38m_tensor_v1* weights, const q38m_tensor_v1*
                           expert_offsets, packed_assignment, c->rows, weights->rows,
                           weights->columns, rows->rows, weights->experts, top_k,
                           LinearEpilogue{view(c), LinearMatrix{}, LinearMatrix{}, view(pre),
-                                         Q38M_ACT_NONE, false}};
-    return run_linear(p, LinearOrder::kNT, swiglu ? LinearFold::kSwiglu : LinearFold::kPlain,
-                      nullptr, stream, device);
+                                         Q38M_ACT_NONE}};
+    return run_linear(p, LinearOrder::kNT, swiglu ? LinearFold::kSwiglu : LinearFold::kStore,
+                      nullptr, 0u, stream, device);
 }
 
 int q38m_moe_expert_backward_rows_v1(const q38m_tensor_v1* weights, const q38m_tensor_v1* d_c,
@@ -1300,9 +1298,9 @@ int q38m_moe_expert_backward_rows_v1(const q38m_tensor_v1* weights, const q38m_t
                           expert_offsets, nullptr, d_c->rows, weights->columns, weights->rows,
                           d_c->rows, weights->experts, 1u,
                           LinearEpilogue{view(d_rows), LinearMatrix{}, LinearMatrix{}, view(pre),
-                                         Q38M_ACT_NONE, true}};
-    return run_linear(p, LinearOrder::kNN, pre ? LinearFold::kSwigluGrad : LinearFold::kPlain,
-                      nullptr, stream, device);
+                                         Q38M_ACT_NONE}};
+    return run_linear(p, LinearOrder::kNN, pre ? LinearFold::kSwigluGrad : LinearFold::kStore,
+                      nullptr, 0u, stream, device);
 }
 
 int q38m_moe_expert_backward_weights_v1(const q38m_tensor_v1* d_c, const q38m_tensor_v1* rows,
@@ -1322,8 +1320,8 @@ int q38m_moe_expert_backward_weights_v1(const q38m_tensor_v1* d_c, const q38m_te
                           expert_offsets, packed_assignment, d_c->columns, rows->columns,
                           d_c->rows, rows->rows, d_weights->experts, top_k,
                           LinearEpilogue{view(d_weights), LinearMatrix{}, view(residual),
-                                         LinearMatrix{}, Q38M_ACT_NONE, true}};
-    return run_linear(p, LinearOrder::kTN, LinearFold::kPlain, nullptr, stream, device);
+                                         LinearMatrix{}, Q38M_ACT_NONE}};
+    return run_linear(p, LinearOrder::kTN, LinearFold::kAdd, nullptr, 0u, stream, device);
 }
 
 int q38m_synth_fill(uint32_t kind, uint64_t seed, uint64_t tag, uint64_t count, float sigma,

@@ -8,6 +8,7 @@
 #include <stdint.h>
 
 #include "q38m.h"
+#include "q38m_linear_tiles.h"
 
 namespace q38m {
 
@@ -299,17 +300,18 @@ struct LinearMatrix {
     bool f32;
 };
 // What becomes of a product's fp32 sums v.  Forward: pre = v + bias, c = act(pre) +
-// residual.  Gradient (slope): c = v * act'(pre) + residual.
+// residual.  Gradient: c = v * act'(pre) + residual.
 struct LinearEpilogue {
     LinearMatrix c, bias, residual, pre;
     uint32_t activation;
-    bool slope;
 };
 // kNT: C = A B^T, rows of A and B as stored; kNN: C = A B, K along B's stored rows;
 // kTN: C = A^T B, K along both's.  The stored rows along K are `depth`, of kTN with
 // offsets an expert's part of them.
 enum class LinearOrder { kNT, kNN, kTN };
-enum class LinearFold { kPlain, kSwiglu, kSwigluGrad };
+// What an epilogue does: store alone, add the residual, the forward or the gradient one,
+// the SwiGLU fold of gate and up columns, or its derivative.
+enum class LinearFold { kStore, kAdd, kForward, kSlope, kSwiglu, kSwigluGrad };
 struct LinearProduct {
     const uint16_t* a;
     const uint16_t* b;
@@ -324,10 +326,17 @@ struct LinearProduct {
     LinearEpilogue e;
 };
 size_t linear_scratch_bytes(uint32_t rows, uint32_t outputs, uint32_t inputs);
-// whether its tiles can be counted and an expert's (gathered) rows reached
-bool linear_fits(const LinearProduct& p, LinearOrder order, LinearFold fold);
-hipError_t launch_linear(const LinearProduct& p, LinearOrder order, LinearFold fold, void* scratch,
-                         hipStream_t stream);
+size_t bias_scratch_bytes(uint32_t rows, uint32_t columns);
+// How a product is run: on tiles, or where its operands' rows do not start at 16 bytes on the
+// kernel for any strides; whether its tiles can be counted, and the scratch it takes.
+struct LinearRun {
+    LinearPlan plan;
+    bool on_tiles, fits;
+    size_t scratch_bytes;
+};
+LinearRun linear_run(const LinearProduct& p, LinearOrder order, LinearFold fold);
+hipError_t launch_linear(const LinearProduct& p, LinearOrder order, LinearFold fold, const LinearRun& run,
+                         void* scratch, hipStream_t stream);
 hipError_t launch_activation_backward(const LinearMatrix& dy, const LinearMatrix& pre,
                                       uint32_t activation, const LinearMatrix& dz, uint32_t rows,
                                       uint32_t columns, hipStream_t stream);

@@ -17,6 +17,15 @@ namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
+// f(0) .. f(kCount - 1) with the numbers as constants of the program
+template <uint32_t kCount, uint32_t kFirst = 0u, typename F>
+__device__ MX_INLINE void each_of(F f) {
+    if constexpr (kFirst < kCount) {
+        f(std::integral_constant<uint32_t, kFirst>{});
+        each_of<kCount, kFirst + 1u>(f);
+    }
+}
+
 // ---- activations --------------------------------------------------------------
 
 // Phi(-|z|), with a = |z|, t = 1 / (1 + 0.3 a): exp(-a^2 / 2) times a polynomial in t,
@@ -125,142 +134,177 @@ __device__ __forceinline__ void times_slope(uint32_t activation, const float (&z
 
 // ---- epilogue -------------------------------------------------------------------
 
-// kN (4 or 8) consecutive elements of a matrix, `live` of them there
+// kN (8, 4 or 1) consecutive elements of a matrix, as they lie there (fp32 in all words,
+// bf16 in the first half of them), and as numbers
 template <uint32_t kN>
-__device__ __forceinline__ void load_row(const LinearMatrix& m, uint64_t at, uint32_t live, float (&v)[kN]) {
-    if (m.f32) {
-        const float* p = static_cast<const float*>(m.data) + at;
-        if (live >= kN) {
+struct Raw {
+    uint32_t d[kN];
+
+    __device__ __forceinline__ void load(LinearMatrix m, uint64_t at) {
+        if (m.f32) {
+            const float* p = static_cast<const float*>(m.data) + at;
+            if constexpr (kN == 1u) {
+                d[0] = __float_as_uint(*p);
+            } else {
 #pragma unroll
-            for (uint32_t i = 0; i < kN; i += 4u) {
-                const v4u_any w = *reinterpret_cast<const v4u_any*>(p + i);
-                v[i] = __uint_as_float(w.x), v[i + 1u] = __uint_as_float(w.y);
-                v[i + 2u] = __uint_as_float(w.z), v[i + 3u] = __uint_as_float(w.w);
+                for (uint32_t i = 0; i < kN; i += 4u) {
+                    const v4u_any w = *reinterpret_cast<const v4u_any*>(p + i);
+                    d[i] = w.x, d[i + 1u] = w.y, d[i + 2u] = w.z, d[i + 3u] = w.w;
+                }
             }
             return;
         }
-#pragma unroll
-        for (uint32_t i = 0; i < kN; ++i) v[i] = i < live ? p[i] : 0.0f;
-        return;
-    }
-    const uint16_t* p = static_cast<const uint16_t*>(m.data) + at;
-    if (live >= kN) {
-        uint32_t d[kN / 2u];
-        if constexpr (kN == 8u) {
-            const v4u_any w = *reinterpret_cast<const v4u_any*>(p);
-            d[0] = w.x, d[1] = w.y, d[2] = w.z, d[3] = w.w;
-        } else {
+        const uint16_t* p = static_cast<const uint16_t*>(m.data) + at;
+        if constexpr (kN == 1u) {
+            d[0] = *p;
+        } else if constexpr (kN == 4u) {
             const v2u_any w = *reinterpret_cast<const v2u_any*>(p);
             d[0] = w.x, d[1] = w.y;
+        } else {
+            const v4u_any w = *reinterpret_cast<const v4u_any*>(p);
+            d[0] = w.x, d[1] = w.y, d[2] = w.z, d[3] = w.w;
         }
-#pragma unroll
-        for (uint32_t i = 0; i < kN; i += 2u) {
-            v[i] = __uint_as_float(d[i / 2u] << 16);
-            v[i + 1u] = __uint_as_float(d[i / 2u] & 0xffff0000u);
-        }
-        return;
     }
+    __device__ __forceinline__ void values(LinearMatrix m, float (&v)[kN]) const {
+        if (m.f32) {
 #pragma unroll
-    for (uint32_t i = 0; i < kN; ++i) v[i] = i < live ? bf16_to_f32(p[i]) : 0.0f;
+            for (uint32_t i = 0; i < kN; ++i) v[i] = __uint_as_float(d[i]);
+            return;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i)
+            v[i] = __uint_as_float(i % 2u != 0u ? d[i / 2u] & 0xffff0000u : d[i / 2u] << 16);
+    }
+};
+
+template <uint32_t kN>
+__device__ __forceinline__ void load_row(LinearMatrix m, uint64_t at, float (&v)[kN]) {
+    Raw<kN> raw;
+    raw.load(m, at);
+    raw.values(m, v);
 }
 
 template <uint32_t kN>
-__device__ __forceinline__ void store_row(const LinearMatrix& m, uint64_t at, uint32_t live, const float (&v)[kN]) {
+__device__ __forceinline__ void store_row(LinearMatrix m, uint64_t at, const float (&v)[kN]) {
     if (m.f32) {
         float* p = static_cast<float*>(m.data) + at;
-        if (live >= kN) {
+        if constexpr (kN == 1u) {
+            *p = v[0];
+        } else {
 #pragma unroll
             for (uint32_t i = 0; i < kN; i += 4u)
                 *reinterpret_cast<v4u_any*>(p + i) = v4u_any{__float_as_uint(v[i]), __float_as_uint(v[i + 1u]),
                                                              __float_as_uint(v[i + 2u]), __float_as_uint(v[i + 3u])};
-            return;
         }
-#pragma unroll
-        for (uint32_t i = 0; i < kN - 1u; ++i)
-            if (i < live) p[i] = v[i];
         return;
     }
     uint16_t* p = static_cast<uint16_t*>(m.data) + at;
-    uint32_t d[kN / 2u];
+    if constexpr (kN == 1u) {
+        *p = static_cast<uint16_t>(f32_to_bf16(v[0]));
+    } else {
+        uint32_t d[kN / 2u];
 #pragma unroll
-    for (uint32_t i = 0; i < kN; i += 2u) d[i / 2u] = f32_to_bf16(v[i]) | f32_to_bf16(v[i + 1u]) << 16;
-    if (live >= kN) {
+        for (uint32_t i = 0; i < kN; i += 2u) d[i / 2u] = f32_to_bf16(v[i]) | f32_to_bf16(v[i + 1u]) << 16;
         if constexpr (kN == 8u) *reinterpret_cast<v4u_any*>(p) = v4u_any{d[0], d[1], d[2], d[3]};
         else *reinterpret_cast<v2u_any*>(p) = v2u_any{d[0], d[1]};
-        return;
     }
-#pragma unroll
-    for (uint32_t i = 0; i < kN - 1u; ++i)
-        if (i < live) p[i] = static_cast<uint16_t>(d[i / 2u] >> i % 2u * 16u);
 }
 
-// The epilogue of kN sums of row `row`, columns from `column` on (below n of them).
-template <uint32_t kN>
-__device__ __forceinline__ void finish_plain(const LinearEpilogue& e, uint64_t row, uint32_t column, uint32_t n,
-                                             float (&v)[kN]) {
-    const uint32_t live = n - column;
-    if (e.slope) {
+// A lane's kN consecutive values of a row of C and of what lies beside it, `shift` columns
+// on where a fold has two halves.
+struct InRow {
+    uint64_t row;
+    uint32_t column;
+
+    template <uint32_t kN>
+    __device__ __forceinline__ void load(LinearMatrix m, uint32_t shift, float (&v)[kN]) const {
+        load_row(m, row * m.stride + shift + column, v);
+    }
+    template <uint32_t kN>
+    __device__ __forceinline__ void store(LinearMatrix m, uint32_t shift, const float (&v)[kN]) const {
+        store_row(m, row * m.stride + shift + column, v);
+    }
+    template <uint32_t kN>
+    __device__ __forceinline__ void load_bias(LinearMatrix m, float (&v)[kN]) const {
+        load_row(m, column, v);
+    }
+};
+
+// The epilogue of a lane's kN sums; n: the columns of C in front of what a fold puts beside
+// them; u: the sums of up beside gate's.
+template <LinearFold kFold, typename Access, uint32_t kN>
+__device__ __forceinline__ void finish_all(LinearEpilogue e, Access at, uint32_t n, float (&v)[kN],
+                                           const float (&u)[kN]) {
+    if constexpr (kFold == LinearFold::kSwiglu) {  // pre: n columns of gate, then n of up
+        if (e.pre.data) {
+            at.store(e.pre, 0u, v);
+            at.store(e.pre, n, u);
+        }
+        if (e.c.f32) {
+#pragma unroll
+            for (uint32_t i = 0; i < kN; ++i) v[i] = swiglu<true>(v[i], u[i]);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < kN; ++i) v[i] = swiglu<false>(v[i], u[i]);
+        }
+    } else if constexpr (kFold == LinearFold::kSwigluGrad) {  // of gate dh u (s + g s(g) s(-g)), of up dh g s
+        // up's first, so that few values are held at a time
+        float gate[kN], other[kN];
+        at.load(e.pre, 0u, gate);
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i) {
+            const Sigmoid y(gate[i]);
+            other[i] = v[i] * (gate[i] * y.s);
+            v[i] *= __builtin_fmaf(held(gate[i]), y.both, y.s);
+        }
+        at.store(e.c, n, other);
+        __builtin_amdgcn_sched_barrier(0);
+        at.load(e.pre, n, other);
+#pragma unroll
+        for (uint32_t i = 0; i < kN; ++i) v[i] *= other[i];
+    } else if constexpr (kFold == LinearFold::kSlope) {
         if (e.activation != Q38M_ACT_NONE) {
             float z[kN];
-            load_row(e.pre, row * e.pre.stride + column, live, z);
+            at.load(e.pre, 0u, z);
             times_slope(e.activation, z, v);
         }
-    } else {
+    } else if constexpr (kFold == LinearFold::kForward) {
         if (e.bias.data) {
             float b[kN];
-            load_row(e.bias, column, live, b);
+            at.load_bias(e.bias, b);
 #pragma unroll
             for (uint32_t i = 0; i < kN; ++i) v[i] += b[i];
         }
-        if (e.pre.data) store_row(e.pre, row * e.pre.stride + column, live, v);
+        if (e.pre.data) at.store(e.pre, 0u, v);
         activate(e.activation, v);
     }
-    if (e.residual.data) {
-        float r[kN];
-        load_row(e.residual, row * e.residual.stride + column, live, r);
+    if constexpr (kFold == LinearFold::kForward || kFold == LinearFold::kSlope || kFold == LinearFold::kAdd) {
+        if (e.residual.data) {
+            float r[kN];
+            at.load(e.residual, 0u, r);
 #pragma unroll
-        for (uint32_t i = 0; i < kN; ++i) v[i] += r[i];
+            for (uint32_t i = 0; i < kN; ++i) v[i] += r[i];
+        }
     }
-    store_row(e.c, row * e.c.stride + column, live, v);
+    at.store(e.c, 0u, v);
 }
 
-// Gate and up sums of the same columns; pre has n columns of gate, then n of up.
-template <uint32_t kN>
-__device__ __forceinline__ void finish_swiglu(const LinearEpilogue& e, uint64_t row, uint32_t column, uint32_t n,
-                                              const float (&gate)[kN], const float (&up)[kN]) {
-    const uint32_t live = n - column;
-    if (e.pre.data) {
-        store_row(e.pre, row * e.pre.stride + column, live, gate);
-        store_row(e.pre, row * e.pre.stride + n + column, live, up);
+// kN sums of a row, columns from `column` on; those that are below n one by one where not all
+// are: the sums move through the first place, so that one copy of the code does for all.
+template <LinearFold kFold, uint32_t kN>
+__device__ __forceinline__ void finish(LinearEpilogue e, uint64_t row, uint32_t column, uint32_t n,
+                                       float (&v)[kN], float (&u)[kN]) {
+    if (column + kN <= n) {
+        finish_all<kFold>(e, InRow{row, column}, n, v, u);
+        return;
     }
-    float h[kN];
-    if (e.c.f32) {
+#pragma unroll 1
+    for (; column < n; ++column) {
+        float one[1] = {v[0]}, up[1] = {u[0]};
+        finish_all<kFold>(e, InRow{row, column}, n, one, up);
 #pragma unroll
-        for (uint32_t i = 0; i < kN; ++i) h[i] = swiglu<true>(gate[i], up[i]);
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < kN; ++i) h[i] = swiglu<false>(gate[i], up[i]);
+        for (uint32_t i = 0; i + 1u < kN; ++i) v[i] = v[i + 1u], u[i] = u[i + 1u];
     }
-    store_row(e.c, row * e.c.stride + column, live, h);
-}
-
-// The gradients of gate and up of h's: dh u (s + g s(g) s(-g)) and dh g s.
-template <uint32_t kN>
-__device__ __forceinline__ void finish_swiglu_grad(const LinearEpilogue& e, uint64_t row, uint32_t column, uint32_t n,
-                                                   const float (&dh)[kN]) {
-    const uint32_t live = n - column;
-    float g[kN], u[kN];
-    load_row(e.pre, row * e.pre.stride + column, live, g);
-    load_row(e.pre, row * e.pre.stride + n + column, live, u);
-    float dg[kN], du[kN];
-#pragma unroll
-    for (uint32_t i = 0; i < kN; ++i) {
-        const Sigmoid y(g[i]);
-        dg[i] = dh[i] * u[i] * __builtin_fmaf(held(g[i]), y.both, y.s);
-        du[i] = dh[i] * (g[i] * y.s);
-    }
-    store_row(e.c, row * e.c.stride + column, live, dg);
-    store_row(e.c, row * e.c.stride + n + column, live, du);
 }
 
 // ---- products of any strides ----------------------------------------------------
@@ -401,14 +445,8 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearProduct p) {
             const uint32_t column = column0 + (kFold == LinearFold::kSwiglu ? wn * 16u : wn * 32u + j * 16u) + 4u * q;
             if (column >= n_out) continue;
             float v[4] = {acc[j][i][0], acc[j][i][1], acc[j][i][2], acc[j][i][3]};
-            if constexpr (kFold == LinearFold::kSwiglu) {
-                const float u[4] = {acc[1][i][0], acc[1][i][1], acc[1][i][2], acc[1][i][3]};
-                finish_swiglu(p.e, row, column, n_out, v, u);
-            } else if constexpr (kFold == LinearFold::kSwigluGrad) {
-                finish_swiglu_grad(p.e, row, column, n_out, v);
-            } else {
-                finish_plain(p.e, row, column, n_out, v);
-            }
+            float u[4] = {acc[1][i][0], acc[1][i][1], acc[1][i][2], acc[1][i][3]};
+            finish<kFold>(p.e, row, column, n_out, v, u);
         }
     }
 }
@@ -416,6 +454,7 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearProduct p) {
 // ---- products of rows at 16 bytes -------------------------------------------------
 
 typedef short v4s __attribute__((ext_vector_type(4)));
+constexpr int kVmcnt0 = 0x0f70;  // a wait for all of a wave's loads and stores
 
 // v_mfma_f32_32x32x16_bf16: lane l holds k = 8 (l / 32) .. + 7 of row l % 32 of A and of B;
 // D lane l: rows 8 (i / 4) + 4 (l / 32) + i % 4 of A, row l % 32 of B.
@@ -461,6 +500,109 @@ struct Block {
     }
 };
 
+// Transposes four registers over four lanes: lane i's register k becomes lane k's register i.
+__device__ MX_INLINE v4u transpose_quad(v4u r, uint32_t lane) {
+    const bool odd = (lane & 1u) != 0u, high = (lane & 2u) != 0u;
+    const uint32_t a = __builtin_amdgcn_mov_dpp(odd ? r.x : r.y, 0xb1, 0xf, 0xf, true);  // of lane ^ 1
+    const uint32_t b = __builtin_amdgcn_mov_dpp(odd ? r.z : r.w, 0xb1, 0xf, 0xf, true);
+    r = odd ? v4u{a, r.y, b, r.w} : v4u{r.x, a, r.z, b};
+    const uint32_t c = __builtin_amdgcn_mov_dpp(high ? r.x : r.z, 0x4e, 0xf, 0xf, true);  // of lane ^ 2
+    const uint32_t d = __builtin_amdgcn_mov_dpp(high ? r.y : r.w, 0x4e, 0xf, 0xf, true);
+    return high ? v4u{c, d, r.z, r.w} : v4u{r.x, r.y, c, d};
+}
+
+// 64 columns of the 32 rows that two of a wave's 32 x 32 tiles side by side have: lane l has of row
+// n = l % 32 the columns 16 k + 8 q .. + 7, q = l / 32, k = 0 .. 3.  Memory is read and written in
+// whole lines, past the caches: four lanes' pieces of 16 bytes change places, so that a lane has
+// its neighbours' rows in turn and a piece of each, and eight lanes a line.  Each lane its own
+// row's pieces, 32 bytes of a line at a time, past the caches or not: 16,384 tokens' gate/up weight
+// gradient in fp32 2,650 us, in whole lines 2,270, past the caches too 2,090; part lines past
+// the caches cost the rows' products more than a fifth.
+struct Span {
+    uint64_t row;           // of C: the tile's first
+    uint32_t first, count;  // the lane's row of the tile, the tile's rows
+    uint32_t column;        // the span's first
+    uint32_t lane;
+
+    __device__ MX_INLINE uint64_t place(LinearMatrix m, uint32_t r) const {
+        return (row + min(r, count - 1u)) * m.stride + column;
+    }
+    // the pieces of row first / 4 * 4 + k: bf16 columns 16 (n % 4) + 8 q, fp32 columns 32 half + 8 (n % 4) + 4 q
+    __device__ MX_INLINE uint32_t row_of(uint32_t k) const { return (first & ~3u) + k; }
+    __device__ MX_INLINE uint32_t column_of() const { return 16u * (lane & 3u) + lane / 32u * 8u; }
+    __device__ MX_INLINE uint32_t wide_column_of() const { return 8u * (lane & 3u) + lane / 32u * 4u; }
+
+    __device__ MX_INLINE void load(LinearMatrix m, uint32_t shift, float (&v)[32]) const {
+        if (m.f32) {
+            each_of<2>([&](auto hc) MX_INLINE {
+                constexpr uint32_t half = decltype(hc)::value;
+                v4u d[4];  // dword e of the pieces k
+                each_of<4>([&](auto kc) MX_INLINE {
+                    constexpr uint32_t k = decltype(kc)::value;
+                    const v4u_any w = __builtin_nontemporal_load(reinterpret_cast<const v4u_any*>(
+                        static_cast<const float*>(m.data) + place(m, row_of(k)) + shift + 32u * half + wide_column_of()));
+                    d[0][k] = w.x, d[1][k] = w.y, d[2][k] = w.z, d[3][k] = w.w;
+                });
+                each_of<4>([&](auto e) MX_INLINE { d[decltype(e)::value] = transpose_quad(d[decltype(e)::value], lane); });
+                each_of<8>([&](auto c) MX_INLINE {  // four columns of both lanes of a row to eight of each
+                    constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
+                    const auto both = __builtin_amdgcn_permlane32_swap(d[e][2u * k], d[e][2u * k + 1u], false, false);
+                    v[16u * half + 8u * k + e] = __uint_as_float(both[0]);
+                    v[16u * half + 8u * k + 4u + e] = __uint_as_float(both[1]);
+                });
+            });
+            return;
+        }
+        v4u d[4];
+        each_of<4>([&](auto kc) MX_INLINE {
+            constexpr uint32_t k = decltype(kc)::value;
+            const v4u_any w = __builtin_nontemporal_load(reinterpret_cast<const v4u_any*>(static_cast<const uint16_t*>(m.data) + place(m, row_of(k)) +
+                                                                shift + column_of()));
+            d[0][k] = w.x, d[1][k] = w.y, d[2][k] = w.z, d[3][k] = w.w;
+        });
+        each_of<4>([&](auto e) MX_INLINE { d[decltype(e)::value] = transpose_quad(d[decltype(e)::value], lane); });
+        each_of<16>([&](auto c) MX_INLINE {
+            constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
+            v[8u * k + 2u * e] = __uint_as_float(d[e][k] << 16);
+            v[8u * k + 2u * e + 1u] = __uint_as_float(d[e][k] & 0xffff0000u);
+        });
+    }
+    __device__ MX_INLINE void store(LinearMatrix m, uint32_t shift, const float (&v)[32]) const {
+        if (m.f32) {
+            each_of<2>([&](auto hc) MX_INLINE {
+                constexpr uint32_t half = decltype(hc)::value;
+                v4u d[4];
+                each_of<8>([&](auto c) MX_INLINE {
+                    constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
+                    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[16u * half + 8u * k + e]),
+                                                                       __float_as_uint(v[16u * half + 8u * k + 4u + e]), false, false);
+                    d[e][2u * k] = both[0];
+                    d[e][2u * k + 1u] = both[1];
+                });
+                each_of<4>([&](auto e) MX_INLINE { d[decltype(e)::value] = transpose_quad(d[decltype(e)::value], lane); });
+                each_of<4>([&](auto kc) MX_INLINE {
+                    constexpr uint32_t k = decltype(kc)::value;
+                    if (row_of(k) >= count) return;
+                    __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]}, reinterpret_cast<v4u_any*>(static_cast<float*>(m.data) + place(m, row_of(k)) + shift + 32u * half +
+                                                wide_column_of()));
+                });
+            });
+            return;
+        }
+        v4u d[4];
+        each_of<16>([&](auto c) MX_INLINE {
+            constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
+            d[e][k] = f32_to_bf16(v[8u * k + 2u * e]) | f32_to_bf16(v[8u * k + 2u * e + 1u]) << 16;
+        });
+        each_of<4>([&](auto e) MX_INLINE { d[decltype(e)::value] = transpose_quad(d[decltype(e)::value], lane); });
+        each_of<4>([&](auto kc) MX_INLINE {
+            constexpr uint32_t k = decltype(kc)::value;
+            if (row_of(k) >= count) return;
+            __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]}, reinterpret_cast<v4u_any*>(static_cast<uint16_t*>(m.data) + place(m, row_of(k)) + shift + column_of()));
+        });
+    }
+};
+
 // Workgroups stay and compute tile after tile of kBM x kBN values of C (with the SwiGLU fold
 // half of the columns gate, half up), kWM x kWN waves, each kTM x kTN matrix-instruction
 // tiles of kMF rows.  K goes through LDS in stages of 64 values, in a ring of kStages slots,
@@ -472,7 +614,9 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     constexpr uint32_t kMF = S::kMF, kTM = S::kTM, kTN = S::kTN, kBM = S::kBM, kBN = S::kBN;
     constexpr bool kAcrossA = kOrder == LinearOrder::kTN, kAcrossB = kOrder != LinearOrder::kNT;
     constexpr bool kSwiglu = kFold == LinearFold::kSwiglu;
-    constexpr bool kRagged = kExperts && kAcrossA;  // K is the expert's rows
+    constexpr bool kRagged = kExperts && kAcrossA;   // K is the expert's rows
+    constexpr bool kListed = kExperts && !kAcrossA;  // rows of C are
+    static_assert(!kSwiglu || kTN % 2u == 0u, "a wave's tiles: half of them gate, half up");
     using A = Block<kAcrossA, kBM>;
     using B = Block<kAcrossB, kBN>;
     using Acc = std::conditional_t<kMF == 32u, v16f, v4f>;
@@ -518,21 +662,28 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     };
     if constexpr (kRagged) {
         // experts without rows: zeros, and what they are added to, unless that is there already
-        if (p.e.residual.data != p.e.c.data)
+        if (p.e.residual.data != p.e.c.data) {
+            const uint32_t pieces = (n_out + 7u) / 8u, threads = gridDim.x * 64u * S::kWaves;
+            const uint64_t all = static_cast<uint64_t>(p.rows) * pieces;
+            uint32_t start = blockIdx.x * 64u * S::kWaves + threadIdx.x;  // the threads go round the experts' pieces
             for (uint32_t e = 0; e < p.experts; ++e) {
                 const uint32_t begin = offsets[e], end = e + 1u < kMaxSortExperts ? offsets[e + 1u] : last_offset;
                 if (min(end, routes) > min(begin, routes)) continue;
-                for (uint32_t r = blockIdx.x; r < p.rows; r += gridDim.x)
-                    for (uint32_t c = threadIdx.x * 8u; c < n_out; c += S::kWaves * 512u) {
-                        float v[8] = {};
-                        finish_plain(p.e, static_cast<uint64_t>(e) * p.rows + r, c, n_out, v);
-                    }
+                uint64_t i = start;
+                for (; i < all; i += threads) {
+                    const uint64_t row = static_cast<uint64_t>(e) * p.rows + i / pieces;
+                    float v[8] = {}, u[8] = {};
+                    finish<kFold>(p.e, row, static_cast<uint32_t>(i % pieces) * 8u, n_out, v, u);
+                }
+                start = static_cast<uint32_t>(i - all);
             }
+        }
     }
     MxOrder order(row_tiles(), columns);
     if (order.count == 0u) return;
     // what is known of the tiles being loaded: lane t % 64 holds the t-th
-    uint32_t known_first = 0, known_count = 0, known_column = 0, known_depth = 0, known_matrix = 0;
+    uint32_t known_first = 0, known_column = 0, known_depth = 0;
+    [[maybe_unused]] uint32_t known_count = 0, known_matrix = 0;
 
     // ---- loads: instructions dealt to the waves, the left over ones to the first: 1 KB of
     // data each.  Those of A first, then of B, each instruction of one of them: a base of its
@@ -587,10 +738,10 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         }
         if (own_lane == found % 64u) {
             known_first = next.first;
-            known_count = next.count;
+            if constexpr (kListed) known_count = next.count;
+            else known_matrix = matrix;
             known_column = next_column;
             known_depth = next_depth;
-            known_matrix = matrix;
         }
         ++found;
         if constexpr (kExperts && !kAcrossB) {
@@ -688,7 +839,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     };
     look_up();
     uint32_t tiles_left = order.count;  // with the one being loaded
-    bool turn = false, moved = false;
+    uint32_t moved = 0u;  // what the next loads are for: 1, the next stage; 2, the next tile; 0, the same stage
     point();
     if constexpr (kRagged) {
         if (gather) {
@@ -710,20 +861,16 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     // reads any more, so that the count of loads under way is always the same
     const auto load_next = [&]() MX_INLINE {
         to = to + 1u == S::kStages ? 0u : to + 1u;
-        if (from + 1u < stages) {
-            ++from;
-            a_base += a_step;
-            if (!(kRagged && gather)) b_base += b_step;
-            moved = true;
-        } else if (tiles_left != 1u) {
-            turn = true;
-        }
+        const bool within = from + 1u < stages;
+        moved = within ? 1u : tiles_left != 1u ? 2u : 0u;
+        if (!within) return;
+        ++from;
+        a_base += a_step;
+        if (!(kRagged && gather)) b_base += b_step;
     };
     // what the next stage's loads need, behind the barrier in front of them
     const auto take_turn = [&]() MX_INLINE {
-        if (turn) {
-            turn = false;
-            moved = true;
+        if (moved == 2u) {
             --tiles_left;
             from = 0;
             point();
@@ -731,18 +878,87 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         if constexpr (kRagged) {
             if (gather) take_sources();
         }
-        if (moved && from + 1u == stages) hold_back();
-        moved = false;
+        if (moved != 0u && from + 1u == stages) hold_back();
     };
 
     // ---- products ----
     const uint32_t wm = wave / S::kWN, wn = wave % S::kWN;
     const uint32_t n = lane % kMF, q = lane / kMF;
     Acc acc[kTN][kTM];
+    constexpr uint32_t kOut = kSwiglu ? kTN / 2u : kTN;  // column tiles of C
+    constexpr uint32_t kGap = kMF == 32u ? 8u : 16u;     // the columns of a lane's group f of four: from kGap f + 4 q on
+    const auto first_row = [&](uint32_t t) MX_INLINE {
+        const uint32_t first = __builtin_amdgcn_readlane(known_first, t % 64u);
+        if constexpr (kListed) return static_cast<uint64_t>(first);
+        else return static_cast<uint64_t>(__builtin_amdgcn_readlane(known_matrix, t % 64u)) * p.rows + first;
+    };
+    const auto count_of = [&](uint32_t t) MX_INLINE -> uint32_t {
+        if constexpr (kListed) return __builtin_amdgcn_readlane(known_count, t % 64u);
+        else return min(p.rows - __builtin_amdgcn_readlane(known_first, t % 64u), kBM);
+    };
+    const auto first_column = [&](uint32_t t) MX_INLINE {
+        return __builtin_amdgcn_readlane(known_column, t % 64u) * kColumns + wn * kOut * kMF;
+    };
+    // Sums that are stored as they are go to memory in whole lines.  With the other folds the
+    // exchange between lanes costs what it gives (in half lines, for want of registers: gate/up of
+    // 32,768 tokens 1,594 us and so 1,647, down's row gradient of 16,384 763 and 884).
+    constexpr bool kSpans = kMF == 32u && kOut % 2u == 0u && (kFold == LinearFold::kStore || kFold == LinearFold::kAdd);
+    [[maybe_unused]] const auto span = [&](uint32_t t, uint32_t i, uint32_t place) MX_INLINE {
+        const uint32_t own_lane = fresh_lane();
+        return Span{first_row(t), (wm * kTM + i) * kMF + (own_lane & 31u), count_of(t), first_column(t) + 64u * place, own_lane};
+    };
+    // The sums of tile t begin with what it is added to, or with zeros.
+    const auto begin = [&](uint32_t t) MX_INLINE {
+        if (kFold == LinearFold::kAdd && p.e.residual.data) {
+            const LinearMatrix r = p.e.residual;
+            const uint32_t own_lane = fresh_lane(), n = own_lane % kMF, q = own_lane / kMF;
+            const uint32_t last = count_of(t) - 1u;
+            each_of<kTM>([&](auto ic) MX_INLINE {
+                constexpr uint32_t i = decltype(ic)::value;
+                if constexpr (kSpans) {
+                    if (first_column(t) + 32u * kOut <= n_out) {
+                        each_of<kOut / 2u>([&](auto pc) MX_INLINE {
+                            constexpr uint32_t place = decltype(pc)::value;
+                            float v[32];
+                            span(t, i, place).load(r, 0u, v);
+                            each_of<16>([&](auto c) MX_INLINE {
+                                constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
+                                constexpr uint32_t f = 2u * (4u * place + k);
+                                const auto both = __builtin_amdgcn_permlane32_swap(
+                                    __float_as_uint(v[8u * k + e]), __float_as_uint(v[8u * k + 4u + e]), false, false);
+                                acc[f / 4u][i][4u * (f % 4u) + e] = __uint_as_float(both[0]);
+                                acc[f / 4u][i][4u * (f % 4u + 1u) + e] = __uint_as_float(both[1]);
+                            });
+                        });
+                        return;
+                    }
+                }
+                const uint64_t at = (first_row(t) + min((wm * kTM + i) * kMF + n, last)) * r.stride;
+                each_of<kTN * kAcc / 4u>([&](auto c) MX_INLINE {
+                    constexpr uint32_t f = decltype(c)::value, j = f / (kAcc / 4u), e = f % (kAcc / 4u) * 4u;
+                    const uint32_t column = first_column(t) + kGap * f + 4u * q;
+                    if (column + 4u <= n_out) {
+                        float v[4];
+                        load_row(r, at + column, v);
+                        each_of<4>([&](auto k) MX_INLINE { acc[j][i][e + decltype(k)::value] = v[decltype(k)::value]; });
+                        return;
+                    }
+                    each_of<4>([&](auto k) MX_INLINE {  // those behind the last column are not stored
+                        float v[1];
+                        load_row(r, at + min(column + decltype(k)::value, n_out - 1u), v);
+                        acc[j][i][e + decltype(k)::value] = v[0];
+                    });
+                });
+            });
+            // the compiler would wait for them in the stages, where other loads are under way
+            __builtin_amdgcn_s_waitcnt(kVmcnt0);
+            return;
+        }
 #pragma unroll
-    for (uint32_t j = 0; j < kTN; ++j)
+        for (uint32_t j = 0; j < kTN; ++j)
 #pragma unroll
-        for (uint32_t i = 0; i < kTM; ++i) acc[j][i] = Acc{};
+            for (uint32_t i = 0; i < kTM; ++i) acc[j][i] = Acc{};
+    };
     constexpr uint32_t kReads = kTM + kTN;
     // where a lane's fragments start in a slot, bytes
     uint32_t part_at[kReads];
@@ -856,54 +1072,71 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     // ---- C: a lane has four consecutive columns of a row and trades one of two such groups with
     // the lane that has the columns beside the other's, which gives both of them eight ----
     const auto store = [&](uint32_t t) MX_INLINE {
-        constexpr uint32_t kOut = kSwiglu ? kTN / 2u : kTN;  // tiles across
-        constexpr uint32_t kFours = kOut * kAcc / 4u;        // a lane's groups of four
+        constexpr LinearFold kEnd = kFold == LinearFold::kAdd ? LinearFold::kStore : kFold;  // begun with
+        constexpr uint32_t kFours = kOut * kAcc / 4u;                                        // a lane's groups of four
         constexpr uint32_t kN = kFours == 1u ? 4u : 8u;
         const uint32_t own_lane = fresh_lane(), n = own_lane % kMF, q = own_lane / kMF;
-        const uint32_t count = __builtin_amdgcn_readlane(known_count, t % 64u);
-        const uint64_t first_row = static_cast<uint64_t>(__builtin_amdgcn_readlane(known_matrix, t % 64u)) * p.rows +
-                                   __builtin_amdgcn_readlane(known_first, t % 64u);
-        const uint32_t first_column = __builtin_amdgcn_readlane(known_column, t % 64u) * kColumns + wn * kOut * kMF;
-        // the columns of group f start at kGap f + 4 q of the wave's
-        constexpr uint32_t kGap = kMF == 32u ? 8u : 16u;
-#pragma unroll
-        for (uint32_t i = 0; i < kTM; ++i) {
+        const uint32_t count = count_of(t);
+        const uint64_t row0 = first_row(t);
+        const uint32_t column0 = first_column(t);
+        each_of<kTM>([&](auto ic) MX_INLINE {
+            constexpr uint32_t i = decltype(ic)::value;
             const uint32_t m = (wm * kTM + i) * kMF + n;
-            if ((wm * kTM + i) * kMF >= count) break;
-            const auto values = [&](uint32_t f, uint32_t shift, float (&v)[kN]) MX_INLINE {
-                const auto sum = [&](uint32_t g, uint32_t e) MX_INLINE {
-                    return acc[g / (kAcc / 4u) + shift][i][4u * (g % (kAcc / 4u)) + e];
-                };
-#pragma unroll
-                for (uint32_t e = 0; e < 4u; ++e) {
+            if ((wm * kTM + i) * kMF >= count) return;
+            asm volatile("" ::: "memory");  // a row's bias is not kept for the next one
+            const auto values = [&](auto fc, auto shift, auto& v, auto at) MX_INLINE {
+                constexpr uint32_t f = decltype(fc)::value, kShift = decltype(shift)::value, kAt = decltype(at)::value;
+                constexpr uint32_t kEach = kAcc / 4u;
+                each_of<4>([&](auto ec) MX_INLINE {
+                    constexpr uint32_t e = decltype(ec)::value;
                     if constexpr (kN == 4u) {
-                        v[e] = sum(f, e);
+                        v[kAt + e] = acc[f / kEach + kShift][i][4u * (f % kEach) + e];
                     } else {
-                        const uint32_t a = __float_as_uint(sum(f, e)), b = __float_as_uint(sum(f + 1u, e));
+                        const uint32_t a = __float_as_uint(acc[f / kEach + kShift][i][4u * (f % kEach) + e]);
+                        const uint32_t b = __float_as_uint(acc[(f + 1u) / kEach + kShift][i][4u * ((f + 1u) % kEach) + e]);
                         const auto both = [&]() MX_INLINE {
                             if constexpr (kMF == 32u) return __builtin_amdgcn_permlane32_swap(a, b, false, false);
                             else return __builtin_amdgcn_permlane16_swap(a, b, false, false);
                         }();
-                        v[e] = __uint_as_float(both[0]);
-                        v[4u + e] = __uint_as_float(both[1]);
+                        v[kAt + e] = __uint_as_float(both[0]);
+                        v[kAt + 4u + e] = __uint_as_float(both[1]);
                     }
-                }
+                });
             };
-#pragma unroll
-            for (uint32_t f = 0; f < kFours; f += kN / 4u) {
-                const uint32_t column = first_column + (kN == 4u      ? 4u * q
-                                                        : kMF == 32u ? kGap * (f + q)
-                                                                      : kGap * (f + q % 2u) + 4u * (q & 2u));
-                float v[kN];
-                values(f, 0u, v);
-                [[maybe_unused]] float u[kN];
-                if constexpr (kSwiglu) values(f, kOut, u);
-                if (m >= count || column >= n_out) continue;
-                if constexpr (kSwiglu) finish_swiglu(p.e, first_row + m, column, n_out, v, u);
-                else if constexpr (kFold == LinearFold::kSwigluGrad) finish_swiglu_grad(p.e, first_row + m, column, n_out, v);
-                else finish_plain(p.e, first_row + m, column, n_out, v);
+            using None = std::integral_constant<uint32_t, 0u>;
+            using Up = std::integral_constant<uint32_t, kSwiglu ? kOut : 0u>;
+            if constexpr (kSpans) {
+                if (column0 + 32u * kOut <= n_out) {
+                    each_of<kOut / 2u>([&](auto pc) MX_INLINE {
+                        constexpr uint32_t place = decltype(pc)::value;
+                        float v[32], u[32] = {};
+                        each_of<4>([&](auto kc) MX_INLINE {
+                            constexpr uint32_t k = decltype(kc)::value;
+                            using Group = std::integral_constant<uint32_t, 2u * (4u * place + k)>;
+                            using At = std::integral_constant<uint32_t, 8u * k>;
+                            values(Group{}, None{}, v, At{});
+                        });
+                        finish_all<kEnd>(p.e, span(t, i, place), n_out, v, u);
+                        if constexpr (S::kWaves == 8u) __builtin_amdgcn_sched_barrier(0);
+                    });
+                    return;
+                }
             }
-        }
+            each_of<kFours * 4u / kN>([&](auto gc) MX_INLINE {
+                constexpr uint32_t f = decltype(gc)::value * (kN / 4u);
+                const uint32_t column = column0 + (kN == 4u      ? 4u * q
+                                                   : kMF == 32u ? kGap * (f + q)
+                                                                 : kGap * (f + q % 2u) + 4u * (q & 2u));
+                float v[kN], u[kN] = {};
+                values(std::integral_constant<uint32_t, f>{}, None{}, v, None{});
+                if constexpr (kSwiglu) values(std::integral_constant<uint32_t, f>{}, Up{}, u, None{});
+                if (m < count && column < n_out) finish<kEnd>(p.e, row0 + m, column, n_out, v, u);
+                if constexpr (S::kWaves == 8u) __builtin_amdgcn_sched_barrier(0);
+            });
+        });
+        // The compiler cannot tell that a load under a condition is used under the same one, and
+        // would wait for it in the next tile's stages: it is told here that none is under way.
+        if constexpr (kEnd != LinearFold::kStore && kEnd != LinearFold::kSwiglu) __builtin_amdgcn_s_waitcnt(kVmcnt0);
     };
 
     // all stages that the ring holds under way, but for the last one's later loads
@@ -926,6 +1159,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     if (left < 64u) clear(left);
 #pragma unroll
     for (uint32_t i = 0; i < kReads; ++i) read(0u, i);
+    begin(0u);
     for (uint32_t t = 0;; ++t) {
         const uint32_t after = t + 1u == order.count ? 64u : depth_of(t + 1u);
         for (; left > 64u; left -= 64u) stage(left - 64u);
@@ -933,32 +1167,42 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         store(t);
         if (t + 1u == order.count) break;
         left = after;
-#pragma unroll
-        for (uint32_t j = 0; j < kTN; ++j)
-#pragma unroll
-            for (uint32_t i = 0; i < kTM; ++i) acc[j][i] = Acc{};
+        begin(t + 1u);
     }
     mx_barrier<0>();  // no load is under way to LDS that the next workgroup gets
 }
 
-// Sums of the parts of K, in their order, and the epilogue: eight columns of a row a thread.
+// Sums of the parts of K, in their order, and the epilogue: eight columns of a row a thread,
+// one where a row's end comes before.
+template <LinearFold kFold, uint32_t kN>
+__device__ __forceinline__ void join_columns(const float* parts, uint32_t count, uint32_t rows, uint64_t row,
+                                             uint32_t column, uint32_t columns, LinearEpilogue e) {
+    const LinearMatrix m{const_cast<float*>(parts), columns, true};
+    float v[kN], u[kN] = {};
+    load_row(m, row * columns + column, v);
+#pragma unroll 4
+    for (uint32_t s = 1; s < count; ++s) {
+        float w[kN];
+        load_row(m, (static_cast<uint64_t>(s) * rows + row) * columns + column, w);
+#pragma unroll
+        for (uint32_t k = 0; k < kN; ++k) v[k] += w[k];
+    }
+    finish_all<kFold>(e, InRow{row, column}, columns, v, u);
+}
+
+template <LinearFold kFold>
 __global__ __launch_bounds__(256) void linear_join_kernel(const float* __restrict__ parts, uint32_t count, uint32_t rows,
                                                           uint32_t columns, LinearEpilogue e) {
     const uint32_t pieces = (columns + 7u) / 8u;
     const uint64_t all = static_cast<uint64_t>(rows) * pieces;
-    const LinearMatrix m{const_cast<float*>(parts), columns, true};
     for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < all; i += gridDim.x * 256ull) {
         const uint64_t row = i / pieces;
-        const uint32_t column = static_cast<uint32_t>(i % pieces) * 8u;
-        float v[8];
-        load_row(m, row * columns + column, columns - column, v);
-        for (uint32_t s = 1; s < count; ++s) {
-            float w[8];
-            load_row(m, (static_cast<uint64_t>(s) * rows + row) * columns + column, columns - column, w);
-#pragma unroll
-            for (uint32_t k = 0; k < 8u; ++k) v[k] += w[k];
+        uint32_t column = static_cast<uint32_t>(i % pieces) * 8u;
+        if (column + 8u <= columns) {
+            join_columns<kFold, 8>(parts, count, rows, row, column, columns, e);
+            continue;
         }
-        finish_plain(e, row, column, columns, v);
+        for (; column < columns; ++column) join_columns<kFold, 1>(parts, count, rows, row, column, columns, e);
     }
 }
 
@@ -970,12 +1214,19 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(LinearMatrix d
                                                                   uint32_t row_pieces, uint32_t columns) {
     for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < pieces; i += gridDim.x * 256ull) {
         const uint64_t row = i / row_pieces;
-        const uint32_t column = static_cast<uint32_t>(i % row_pieces) * 8u, live = columns - column;
-        float v[8], z[8];
-        load_row(dy, row * dy.stride + column, live, v);
-        load_row(pre, row * pre.stride + column, live, z);
-        times_slope(activation, z, v);
-        store_row(dz, row * dz.stride + column, live, v);
+        uint32_t column = static_cast<uint32_t>(i % row_pieces) * 8u;
+        const auto part = [&](auto count) {
+            float v[decltype(count)::value], z[decltype(count)::value];
+            load_row(dy, row * dy.stride + column, v);
+            load_row(pre, row * pre.stride + column, z);
+            times_slope(activation, z, v);
+            store_row(dz, row * dz.stride + column, v);
+        };
+        if (column + 8u <= columns) {
+            part(std::integral_constant<uint32_t, 8>{});
+            continue;
+        }
+        for (; column < columns; ++column) part(std::integral_constant<uint32_t, 1>{});
     }
 }
 
@@ -990,15 +1241,20 @@ __global__ __launch_bounds__(256) void bias_sum_kernel(const uint16_t* __restric
     const uint32_t column = blockIdx.x * kBiasColumns + threadIdx.x % 8u * 8u;
     const uint32_t from = blockIdx.y * each, to = min(rows - from, each) + from;
     float sum[8] = {};
-    if (column < columns) {
-        const LinearMatrix m{const_cast<uint16_t*>(dz), stride, false};
+    const LinearMatrix m{const_cast<uint16_t*>(dz), stride, false};
+    if (column + 8u <= columns) {
 #pragma unroll 4
         for (uint32_t r = from + threadIdx.x / 8u; r < to; r += 32u) {
             float v[8];
-            load_row(m, r * stride + column, columns - column, v);
+            load_row(m, r * stride + column, v);
 #pragma unroll
             for (uint32_t i = 0; i < 8u; ++i) sum[i] += v[i];
         }
+    } else if (column < columns) {
+        for (uint32_t r = from + threadIdx.x / 8u; r < to; r += 32u)
+#pragma unroll
+            for (uint32_t i = 0; i < 7u; ++i)
+                if (column + i < columns) sum[i] += bf16_to_f32(dz[r * stride + column + i]);
     }
 #pragma unroll
     for (uint32_t i = 0; i < 8u; ++i) sums[threadIdx.x / 8u][threadIdx.x % 8u * 8u + i] = sum[i];
@@ -1060,85 +1316,104 @@ bool linear_on_tiles(const LinearProduct& p, LinearOrder order, LinearFold fold)
            std::max<uint64_t>(b_rows, 256u) * p.b_stride < limit;
 }
 
+// 256 x 256 tiles leave the SwiGLU's gradient too few registers.
+bool linear_wide(LinearFold fold) { return fold != LinearFold::kSwigluGrad; }
+
+size_t part_bytes(const LinearSizes& p, const LinearPlan& plan) {
+    const uint32_t parts = p.experts != 0u ? 1u : linear_parts(p.depth, plan.splits);
+    return parts > 1u ? static_cast<size_t>(parts) * p.rows * p.columns * sizeof(float) : 0u;
+}
+
 template <typename S, LinearOrder kOrder, bool kExperts, LinearFold kFold>
 hipError_t launch_tiles(const LinearProduct& p, const LinearSizes& sizes, uint32_t splits, void* scratch,
                         hipStream_t stream) {
-    const uint32_t each = kExperts ? 0u : linear_each(p.depth, splits);
-    const uint32_t parts = kExperts ? 1u : (p.depth + each - 1u) / each;
-    LinearProduct q = p;
-    if (parts > 1u) {
-        q.e = LinearEpilogue{};
-        q.e.c = LinearMatrix{scratch, p.columns, true};
+    if constexpr ((kOrder == LinearOrder::kTN && S::kBM < 64u) ||
+                  (kFold == LinearFold::kSwigluGrad && S::kBM == 256u)) {
+        return hipErrorInvalidValue;  // the rule takes none
+    } else {
+        const uint32_t each = kExperts ? 0u : linear_each(p.depth, splits);
+        const uint32_t parts = kExperts ? 1u : linear_parts(p.depth, splits);
+        LinearProduct q = p;
+        if (parts > 1u) {
+            q.e = LinearEpilogue{};
+            q.e.c = LinearMatrix{scratch, p.columns, true};
+        }
+        linear_tile_kernel<S, kOrder, kExperts, kFold>
+            <<<linear_grid<S>(sizes, parts), 64u * S::kWaves, 0, stream>>>(q, each);
+        if constexpr (!kExperts) {
+            if (parts > 1u) {
+                if (hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
+                const uint64_t pieces = static_cast<uint64_t>(p.rows) * ((p.columns + 7u) / 8u);
+                const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>((pieces + 255u) / 256u, 16u * kMxCus));
+                linear_join_kernel<kFold><<<grid, 256, 0, stream>>>(static_cast<const float*>(scratch), parts, p.rows,
+                                                                   p.columns, p.e);
+            }
+        }
+        return hipGetLastError();
     }
-    linear_tile_kernel<S, kOrder, kExperts, kFold>
-        <<<linear_grid<S>(sizes, parts), 64u * S::kWaves, 0, stream>>>(q, each);
-    if (parts == 1u) return hipGetLastError();
-    if (hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
-    const uint64_t pieces = static_cast<uint64_t>(p.rows) * ((p.columns + 7u) / 8u);
-    const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>((pieces + 255u) / 256u, 16u * kMxCus));
-    linear_join_kernel<<<grid, 256, 0, stream>>>(static_cast<const float*>(scratch), parts, p.rows, p.columns, p.e);
-    return hipGetLastError();
-}
-
-size_t split_bytes(const LinearSizes& p) {
-    return with_linear_tiles(p, [&](auto, uint32_t splits) -> size_t {
-        const uint32_t each = linear_each(p.depth, splits), parts = (p.depth + each - 1u) / each;
-        return parts > 1u ? static_cast<size_t>(parts) * p.rows * p.columns * sizeof(float) : 0u;
-    });
 }
 
 }  // namespace
 
 size_t linear_scratch_bytes(uint32_t rows, uint32_t outputs, uint32_t inputs) {
-    const uint32_t parts = bias_parts(rows, outputs);
-    size_t most = parts > 1u ? static_cast<size_t>(parts) * outputs * sizeof(float) : 0u;
-    most = std::max(most, split_bytes(LinearSizes{rows, outputs, inputs, 0u, false, false}));
-    most = std::max(most, split_bytes(LinearSizes{rows, inputs, outputs, 0u, false, false}));
-    return std::max(most, split_bytes(LinearSizes{outputs, inputs, rows, 0u, false, true}));
+    size_t most = bias_scratch_bytes(rows, outputs);
+    for (const LinearSizes& s : {LinearSizes{rows, outputs, inputs, 0u, false, false},
+                                 LinearSizes{rows, inputs, outputs, 0u, false, false},
+                                 LinearSizes{outputs, inputs, rows, 0u, false, true}})
+        most = std::max(most, part_bytes(s, linear_plan(s, true)));
+    return most;
 }
 
-bool linear_fits(const LinearProduct& p, LinearOrder order, LinearFold fold) {
-    if (any_tiles(p, order, fold) >= (1ull << 31)) return false;
+size_t bias_scratch_bytes(uint32_t rows, uint32_t columns) {
+    const uint32_t parts = bias_parts(rows, columns);
+    return parts > 1u ? static_cast<size_t>(parts) * columns * sizeof(float) : 0u;
+}
+
+LinearRun linear_run(const LinearProduct& p, LinearOrder order, LinearFold fold) {
     const LinearSizes sizes = linear_sizes(p, order, fold);
-    return with_linear_tiles(sizes, [&](auto s, uint32_t splits) {
-        return linear_tiles<decltype(s)>(sizes) * splits < (1ull << 31);
+    if (!linear_on_tiles(p, order, fold)) return LinearRun{{}, false, any_tiles(p, order, fold) < (1ull << 31), 0u};
+    const LinearPlan plan = linear_plan(sizes, linear_wide(fold));
+    const bool fits = with_linear_shape(plan, [&](auto s) {
+        return linear_tiles<decltype(s)>(sizes) * plan.splits < (1ull << 31);
     });
+    return LinearRun{plan, true, fits, part_bytes(sizes, plan)};
 }
 
-hipError_t launch_linear(const LinearProduct& p, LinearOrder order, LinearFold fold, void* scratch, hipStream_t stream) {
+hipError_t launch_linear(const LinearProduct& p, LinearOrder order, LinearFold fold, const LinearRun& run, void* scratch,
+                         hipStream_t stream) {
     const LinearSizes sizes = linear_sizes(p, order, fold);
-    const bool on_tiles = linear_on_tiles(p, order, fold);
     const auto launch = [&](auto o, auto experts, auto f) -> hipError_t {
         constexpr LinearOrder kOrder = decltype(o)::value;
         constexpr bool kExperts = decltype(experts)::value;
         constexpr LinearFold kFold = decltype(f)::value;
-        if (!on_tiles) {
+        if (!run.on_tiles) {
             linear_any_kernel<kOrder, kExperts, kFold>
                 <<<static_cast<uint32_t>(any_tiles(p, order, fold)), 256, 0, stream>>>(p);
             return hipGetLastError();
         }
-        return with_linear_tiles(sizes, [&](auto s, uint32_t splits) -> hipError_t {
-            using S = decltype(s);
-            if constexpr (kOrder == LinearOrder::kTN && S::kBM < 64u) return hipErrorInvalidValue;  // the rule takes none
-            else return launch_tiles<S, kOrder, kExperts, kFold>(p, sizes, splits, scratch, stream);
+        return with_linear_shape(run.plan, [&](auto s) -> hipError_t {
+            return launch_tiles<decltype(s), kOrder, kExperts, kFold>(p, sizes, run.plan.splits, scratch, stream);
         });
     };
     using NT = std::integral_constant<LinearOrder, LinearOrder::kNT>;
     using NN = std::integral_constant<LinearOrder, LinearOrder::kNN>;
     using TN = std::integral_constant<LinearOrder, LinearOrder::kTN>;
-    using Plain = std::integral_constant<LinearFold, LinearFold::kPlain>;
+    using Store = std::integral_constant<LinearFold, LinearFold::kStore>;
+    using Add = std::integral_constant<LinearFold, LinearFold::kAdd>;
+    using Forward = std::integral_constant<LinearFold, LinearFold::kForward>;
+    using Slope = std::integral_constant<LinearFold, LinearFold::kSlope>;
     using Swiglu = std::integral_constant<LinearFold, LinearFold::kSwiglu>;
     using SwigluGrad = std::integral_constant<LinearFold, LinearFold::kSwigluGrad>;
     if (!p.offsets) {
-        if (order == LinearOrder::kNT) return launch(NT{}, std::false_type{}, Plain{});
-        if (order == LinearOrder::kNN) return launch(NN{}, std::false_type{}, Plain{});
-        return launch(TN{}, std::false_type{}, Plain{});
+        if (order == LinearOrder::kNT) return launch(NT{}, std::false_type{}, Forward{});
+        if (order == LinearOrder::kNN) return launch(NN{}, std::false_type{}, Slope{});
+        return launch(TN{}, std::false_type{}, Add{});
     }
     if (fold == LinearFold::kSwiglu) return launch(NT{}, std::true_type{}, Swiglu{});
     if (fold == LinearFold::kSwigluGrad) return launch(NN{}, std::true_type{}, SwigluGrad{});
-    if (order == LinearOrder::kNT) return launch(NT{}, std::true_type{}, Plain{});
-    if (order == LinearOrder::kNN) return launch(NN{}, std::true_type{}, Plain{});
-    return launch(TN{}, std::true_type{}, Plain{});
+    if (order == LinearOrder::kNT) return launch(NT{}, std::true_type{}, Store{});
+    if (order == LinearOrder::kNN) return launch(NN{}, std::true_type{}, Store{});
+    return launch(TN{}, std::true_type{}, Add{});
 }
 
 hipError_t launch_activation_backward(const LinearMatrix& dy, const LinearMatrix& pre,

@@ -5,8 +5,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstddef>
 #include <cstdint>
-#include <iterator>
 
 #include "q38m_mx_tiles.h"
 
@@ -65,22 +65,105 @@ uint32_t linear_grid(const LinearSizes& p, uint32_t splits) {
     return tiles < S::kResident * kMxCus ? static_cast<uint32_t>(tiles) : S::kResident * kMxCus;
 }
 
-// Values of K in each part of a dense product that is cut along K.
+// Values of K in each part of a dense product that is cut along K, and the parts that come of it.
 constexpr uint32_t linear_each(uint32_t depth, uint32_t splits) {
     return ((depth + splits - 1u) / splits + 63u) / 64u * 64u;
 }
+constexpr uint32_t linear_parts(uint32_t depth, uint32_t splits) {
+    const uint32_t each = linear_each(depth, splits);
+    return (depth + each - 1u) / each;
+}
 
+// What a product is run on: the shape's number in LinearCost's order, and into how many parts its
+// K is cut, whose sums go through the scratch.
+struct LinearPlan {
+    uint32_t shape, splits;
+};
+
+constexpr uint32_t kLinearShapes = 5, kLinearMaxSplits = 32;
+constexpr size_t kLinearMaxPartBytes = 256u << 20;
+
+// What a product takes, us: a launch, and for every tile that a CU computes after another its
+// stages and its end.  A stage takes `alone` at least, the answer's way from memory, and `each` for
+// each of the workgroups that a CU holds.  The figures are fitted to graphs of 4,389 dense
+// products of 1 to 8,192 rows (outputs and inputs 512 to 8,192, all three orders, K in 1 to 32
+// parts) and of 860 experts' products (1 to 16,384 tokens, 8, 64 and 512 experts) on every shape.
+// Taking the least, the rule's products are within 1.02 of the fastest shape's time in the
+// geometric mean, and 1.2 at most but for weights' gradients of one or four tokens (1.65), which
+// are mostly zeros written.
+struct LinearCost {
+    float alone, each, end;
+};
+constexpr LinearCost kDenseCost[kLinearShapes] = {
+    {1.17f, 1.18f, 5.8f}, {0.65f, 0.45f, 1.33f}, {0.297f, 0.143f, 0.49f}, {0.295f, 0.225f, 0.61f}, {0.289f, 0.202f, 0.51f}};
+constexpr LinearCost kExpertCost[kLinearShapes] = {
+    {1.09f, 0.965f, 4.1f}, {0.65f, 0.395f, 0.94f}, {0.297f, 0.152f, 0.345f}, {0.19f, 0.248f, 0.43f}, {0.31f, 0.236f, 0.36f}};
+constexpr LinearCost kRaggedCost[kLinearShapes] = {
+    {1.34f, 1.365f, 5.8f}, {0.5f, 0.468f, 1.33f}, {0.297f, 0.106f, 0.49f}, {}, {}};
+constexpr float kLaunchUs = 2.9f, kJoinUs = 2.5f, kJoinPartUs = 0.123f, kJoinMbUs = 1.26f;  // MB of a part's sums
+
+// tiles * parts of `stages` stages each
+template <typename S>
+float linear_us(float tiles, float stages, const LinearCost& c) {
+    const float held = std::min(static_cast<float>(S::kResident), std::ceil(tiles / 256.0f));
+    return kLaunchUs + std::ceil(tiles / (256.0f * held)) * (stages * std::max(c.alone, held * c.each) + held * c.end);
+}
+
+template <typename S>
+float linear_expert_us(const LinearSizes& p, uint32_t shape) {
+    const uint32_t across = p.swiglu ? S::kBN / 2u : S::kBN;
+    const float columns = static_cast<float>((p.across() + across - 1u) / across);
+    const uint32_t routes = p.ragged ? p.depth : p.rows;
+    const float active = static_cast<float>(std::min(routes, p.experts)), rows = static_cast<float>(routes) / active;
+    if (p.ragged)
+        return linear_us<S>(active * static_cast<float>((p.rows + S::kBM - 1u) / S::kBM) * columns, rows / 64.0f + 1.0f,
+                            kRaggedCost[shape]);
+    // an expert's last row tile is partly full
+    const float tiles = routes <= p.experts ? 1.0f : std::max(1.0f, rows / S::kBM + 0.43f);
+    return linear_us<S>(active * tiles * columns, static_cast<float>((p.depth + 63u) / 64u), kExpertCost[shape]);
+}
+
+// The plan with the least time.  wide: 256 x 256 tiles are there for it.  K that lies across A's
+// rows takes tiles of 64 rows and more: fewer would not fill a load instruction.
+inline LinearPlan linear_plan(const LinearSizes& p, bool wide) {
+    LinearPlan best{2u, 1u};
+    float least = 1e30f;
+    const auto look = [&](auto s, uint32_t shape) {
+        using S = decltype(s);
+        if ((shape == 0u && !wide) || (p.ragged && S::kBM < 64u)) return;
+        if (p.experts != 0u) {
+            const float us = linear_expert_us<S>(p, shape);
+            if (us < least) least = us, best = LinearPlan{shape, 1u};
+            return;
+        }
+        const float tiles = static_cast<float>(linear_tiles<S>(p)), part_mb = static_cast<float>(p.rows) * p.columns * 4e-6f;
+        for (uint32_t splits = 1; splits <= kLinearMaxSplits; splits *= 2u) {
+            if (splits != 1u && (tiles * splits > 1024.0f || p.depth / splits < 128u ||
+                                 part_mb * splits > kLinearMaxPartBytes * 1e-6f))
+                break;
+            float us = linear_us<S>(tiles * splits, static_cast<float>(linear_each(p.depth, splits) / 64u), kDenseCost[shape]);
+            if (splits != 1u) us += kJoinUs + splits * (kJoinPartUs + kJoinMbUs * part_mb * 0.25f);
+            if (us < least) least = us, best = LinearPlan{shape, splits};
+        }
+    };
+    look(Linear256x256{}, 0u);
+    look(Linear128x128{}, 1u);
+    look(Linear64x64{}, 2u);
+    look(Linear32x128{}, 3u);
+    look(Linear16x128{}, 4u);
+    return best;
+}
+
+// Calls f with the plan's shape.
 template <typename F>
-auto with_linear_tiles(const LinearSizes& p, F f) {
-    const uint64_t rows = p.experts != 0u && !p.ragged
-                              ? p.rows / std::max(1u, std::min(p.rows, p.experts))
-                              : p.rows;
-    const bool few = !p.ragged;
-    if (few && rows <= 16u) return f(Linear16x128{}, 1u);
-    if (few && rows <= 32u) return f(Linear32x128{}, 1u);
-    if (linear_tiles<Linear256x256>(p) >= 200u && rows > 128u) return f(Linear256x256{}, 1u);
-    if (linear_tiles<Linear128x128>(p) >= 200u && rows > 64u) return f(Linear128x128{}, 1u);
-    return f(Linear64x64{}, 1u);
+auto with_linear_shape(const LinearPlan& plan, F f) {
+    switch (plan.shape) {
+        case 0: return f(Linear256x256{});
+        case 1: return f(Linear128x128{});
+        case 2: return f(Linear64x64{});
+        case 3: return f(Linear32x128{});
+        default: return f(Linear16x128{});
+    }
 }
 
 }  // namespace q38m
