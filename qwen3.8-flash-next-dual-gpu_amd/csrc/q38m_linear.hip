@@ -364,9 +364,17 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearProduct p) {
 
     // each thread's piece of eight values: along K, row t / 4 and piece t % 4; across K,
     // stored row t / 8 and columns from 8 (t % 8) on
-    const auto source = [&](uint32_t place) {
-        return p.packed ? min(p.packed[place] / p.top_k, p.source_rows - 1u) : place;
+    const auto source = [&](uint32_t place) -> uint32_t {
+        if (!p.packed) return place;
+        const uint32_t row = p.packed[place] / p.top_k;
+        report(row >= p.source_rows, kCheckToken);
+        return min(row, p.source_rows - 1u);
     };
+#ifdef Q38M_CHECKED
+    if constexpr (kExperts)
+        for (uint32_t e = blockIdx.x * 256u + t; e < p.experts; e += gridDim.x * 256u)
+            report(p.offsets[e + 1u] < p.offsets[e] || p.offsets[e + 1u] > (kAcrossA ? p.depth : p.rows), kCheckOffsets);
+#endif
     const uint32_t r = t / 4u;
     const uint16_t *a_from, *b_from;
     int32_t a_live = 0, b_live = 0;  // across K: columns there
@@ -1172,6 +1180,158 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     mx_barrier<0>();  // no load is under way to LDS that the next workgroup gets
 }
 
+// Few rows (generated tokens, experts of a few rows): a workgroup has 16 rows of C by 16 or 32
+// columns (with the SwiGLU fold 16 of gate and 16 of up), and its waves a part of K each, whose
+// sums meet in LDS in the waves' order.  A wave streams its part through a ring of its own, 64
+// values of K of all rows at a time, and waits for no other, so a CU has the bytes of many stages
+// under way from its first clocks on; what bounds it is a launch, the first answers from memory
+// and, of larger matrices, memory's rate (1 x 8,192 x 2,048 5.1 us, 6.6 TB/s of weights that the
+// caches behind the L2s hold; on 16 x 128 tiles with K in four parts and their join 9.9).
+template <typename S, bool kExperts, LinearFold kFold>
+__global__ __launch_bounds__(64u * S::kWaves) void linear_few_kernel(LinearProduct p) {
+    constexpr bool kSwiglu = kFold == LinearFold::kSwiglu;
+    constexpr uint32_t kFewRows = S::kRows, kFewWaves = S::kWaves, kFewStages = S::kStages, kTiles = S::kTiles;
+    static_assert(!kSwiglu || kTiles == 2u, "a tile of gate, one of up");
+    constexpr uint32_t kRowsB = 16u * kTiles, kRows = kFewRows + kRowsB, kSlot = kRows * 8u;  // 16-byte words
+    constexpr uint32_t kAcross = kSwiglu ? kRowsB / 2u : kRowsB;
+    __shared__ v4i ring[kFewWaves * kFewStages * kSlot];
+    __shared__ uint32_t offsets[kExperts ? kMaxSortExperts : 1u];
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t n_out = kSwiglu ? p.columns / 2u : p.columns;
+    const uint32_t columns = (n_out + kAcross - 1u) / kAcross;
+    const uint32_t row_tile = blockIdx.x / columns, column0 = blockIdx.x % columns * kAcross;
+    RowTile tile{0u, row_tile * kFewRows, 0u, false};
+    if constexpr (kExperts) {
+        const uint32_t last = p.offsets[p.experts];
+        for (uint32_t e = threadIdx.x; e < kMaxSortExperts; e += 64u * kFewWaves) offsets[e] = e < p.experts ? p.offsets[e] : last;
+        __syncthreads();
+#ifdef Q38M_CHECKED
+        for (uint32_t e = threadIdx.x; e < p.experts; e += 64u * kFewWaves)
+            report(p.offsets[e + 1u] < offsets[e] || p.offsets[e + 1u] > p.rows, kCheckOffsets);
+#endif
+        const TileList<kFewRows> list(offsets, last, p.rows);
+        if (row_tile >= list.total) return;
+        tile = list.find(row_tile);
+    } else {
+        tile.count = min(p.rows - tile.first, kFewRows);
+    }
+    const bool all_rows = tile.count > 8u;  // else the second eight rows of A are not loaded, and their sums not stored
+
+    // this wave's stages, and its loads: two of A (one), four of B, eight rows each
+    const uint32_t stages = (p.depth + 63u) / 64u;
+    const uint32_t first = wave * stages / kFewWaves, end = (wave + 1u) * stages / kFewWaves;
+    const uint32_t a_bytes = static_cast<uint32_t>(p.a_stride) * 2u, b_bytes = static_cast<uint32_t>(p.b_stride) * 2u;
+    const bool gather = kExperts && p.packed;
+    const uint8_t* a_base = reinterpret_cast<const uint8_t*>(p.a) + (gather ? 0ull : static_cast<uint64_t>(tile.first) * a_bytes);
+    const uint8_t* b_base = reinterpret_cast<const uint8_t*>(p.b) +
+                            (static_cast<uint64_t>(tile.expert) * p.columns + column0) * b_bytes;
+    a_base = mx_uniform(a_base);
+    b_base = mx_uniform(b_base);
+    constexpr uint32_t kLoads = kRows / 8u;
+    uint32_t data[kLoads];
+    each_of<kLoads>([&](auto tc) MX_INLINE {
+        constexpr uint32_t t = decltype(tc)::value;
+        const uint32_t r = 8u * t + (lane >> 3), piece = (lane & 7u) ^ (r >> 1 & 7u);
+        if constexpr (t < kFewRows / 8u) {
+            uint32_t row = min(r, tile.count - 1u);
+            if (gather) {
+                row = p.packed[tile.first + row] / p.top_k;
+                report(row >= p.source_rows, kCheckToken);
+                row = min(row, p.source_rows - 1u);
+            }
+            data[t] = row * a_bytes + 16u * piece;
+        } else {
+            uint32_t column = r - kFewRows, up = 0;
+            if constexpr (kSwiglu) {  // 16 of gate, 16 of up
+                up = column / 16u * n_out;
+                column %= 16u;
+            }
+            data[t] = (min(column, n_out - 1u - column0) + up) * b_bytes + 16u * piece;
+        }
+    });
+    const uint32_t ring_at = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(
+        reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) v4i*)ring)) + wave * (kFewStages * kSlot * 16u));
+    const auto load = [&](uint32_t s, uint32_t slot) MX_INLINE {
+        const uint32_t valid = p.depth - s * 64u;
+        const uint64_t shift = s * 128ull;
+        each_of<kLoads>([&](auto tc) MX_INLINE {
+            constexpr uint32_t t = decltype(tc)::value;
+            if (t == 1u && !all_rows) return;
+            uint32_t at = data[t];
+            if (valid < 64u) {  // a piece behind K is another of the row
+                const uint32_t piece = (lane & 7u) ^ ((8u * t + (lane >> 3)) >> 1 & 7u), last = (valid - 1u) / 8u;
+                at -= piece > last ? (piece - last) * 16u : 0u;
+            }
+            mx_load16((t < kFewRows / 8u ? a_base : b_base) + shift, at, ring_at + slot * (kSlot * 16u) + t * 1024u);
+        });
+    };
+    v4f acc[kTiles] = {};
+    const uint32_t n = lane % 16u, q = lane / 16u, swizzle = n >> 1 & 7u;
+    const uint32_t count = end - first;
+    each_of<kFewStages - 1u>([&](auto s) MX_INLINE {
+        if (decltype(s)::value < count) load(first + decltype(s)::value, decltype(s)::value);
+    });
+    uint32_t slot = 0;
+    for (uint32_t s = 0; s < count; ++s) {
+        // the stages behind this one may be under way; this one's fragments were read two stages ago
+        if (s + kFewStages - 1u < count) {
+            load(first + s + kFewStages - 1u, slot == 0u ? kFewStages - 1u : slot - 1u);
+            if (all_rows) asm volatile("s_waitcnt vmcnt(%0)" ::"i"((kFewStages - 1u) * kLoads) : "memory");
+            else asm volatile("s_waitcnt vmcnt(%0)" ::"i"((kFewStages - 1u) * (kLoads - 1u)) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        v4i* at = ring + (wave * kFewStages + slot) * kSlot;
+        const uint32_t valid = p.depth - (first + s) * 64u;
+        if (valid < 64u) {  // zeros behind K, of both operands
+            for (uint32_t w = lane; w < kSlot; w += 64u) {
+                const uint32_t k = 8u * ((w & 7u) ^ (w >> 4 & 7u));
+                if (k + 8u <= valid) continue;
+                v4i v = k >= valid ? v4i{0, 0, 0, 0} : at[w];
+#pragma unroll
+                for (uint32_t e = 0; e < 4u; ++e) {
+                    if (k + 2u * e >= valid) v[e] = 0;
+                    else if (k + 2u * e + 1u >= valid) v[e] &= 0xffff;
+                }
+                at[w] = v;
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+#pragma unroll
+        for (uint32_t c = 0; c < 2u; ++c) {
+            const uint32_t piece = (4u * c + q) ^ swizzle;
+            const v4i a = at[n * 8u + piece];
+            each_of<kTiles>([&](auto jc) MX_INLINE {
+                constexpr uint32_t j = decltype(jc)::value;
+                acc[j] = mfma_bf16(at[(kFewRows + 16u * j + n) * 8u + piece], a, acc[j]);
+            });
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its slot is loaded anew a stage on
+        slot = slot + 1u == kFewStages ? 0u : slot + 1u;
+    }
+    __syncthreads();
+    v4f* sums = reinterpret_cast<v4f*>(ring);
+    each_of<kTiles>([&](auto j) MX_INLINE { sums[(wave * kTiles + decltype(j)::value) * 64u + lane] = acc[decltype(j)::value]; });
+    __syncthreads();
+    if (wave >= (kSwiglu ? 1u : kTiles)) return;
+    const auto joined = [&](uint32_t half) MX_INLINE {
+        v4f sum = sums[half * 64u + lane];
+#pragma unroll
+        for (uint32_t w = 1; w < kFewWaves; ++w) sum += sums[(w * kTiles + half) * 64u + lane];
+        return sum;
+    };
+    const uint32_t column = column0 + (kSwiglu ? 0u : wave * 16u) + 4u * q;
+    const v4f sum = joined(kSwiglu ? 0u : wave);
+    float v[4] = {sum[0], sum[1], sum[2], sum[3]}, u[4] = {};
+    if constexpr (kSwiglu) {
+        const v4f up = joined(1u);
+        u[0] = up[0], u[1] = up[1], u[2] = up[2], u[3] = up[3];
+    }
+    if (n < tile.count && column < n_out)
+        finish<kFold>(p.e, static_cast<uint64_t>(tile.first) + n, column, n_out, v, u);
+}
+
 // Sums of the parts of K, in their order, and the epilogue: eight columns of a row a thread,
 // one where a row's end comes before.
 template <LinearFold kFold, uint32_t kN>
@@ -1297,7 +1457,7 @@ uint64_t any_tiles(const LinearProduct& p, LinearOrder order, LinearFold fold) {
 
 LinearSizes linear_sizes(const LinearProduct& p, LinearOrder order, LinearFold fold) {
     return LinearSizes{p.rows, p.columns, p.depth, p.offsets ? p.experts : 0u, fold == LinearFold::kSwiglu,
-                       order == LinearOrder::kTN};
+                       order == LinearOrder::kTN, order == LinearOrder::kNT};
 }
 
 // Whether every operand row starts at 16 bytes, and a lane's offsets from its tile's base are
@@ -1357,9 +1517,9 @@ hipError_t launch_tiles(const LinearProduct& p, const LinearSizes& sizes, uint32
 
 size_t linear_scratch_bytes(uint32_t rows, uint32_t outputs, uint32_t inputs) {
     size_t most = bias_scratch_bytes(rows, outputs);
-    for (const LinearSizes& s : {LinearSizes{rows, outputs, inputs, 0u, false, false},
-                                 LinearSizes{rows, inputs, outputs, 0u, false, false},
-                                 LinearSizes{outputs, inputs, rows, 0u, false, true}})
+    for (const LinearSizes& s : {LinearSizes{rows, outputs, inputs, 0u, false, false, true},
+                                 LinearSizes{rows, inputs, outputs, 0u, false, false, false},
+                                 LinearSizes{outputs, inputs, rows, 0u, false, true, false}})
         most = std::max(most, part_bytes(s, linear_plan(s, true)));
     return most;
 }
@@ -1373,6 +1533,7 @@ LinearRun linear_run(const LinearProduct& p, LinearOrder order, LinearFold fold)
     const LinearSizes sizes = linear_sizes(p, order, fold);
     if (!linear_on_tiles(p, order, fold)) return LinearRun{{}, false, any_tiles(p, order, fold) < (1ull << 31), 0u};
     const LinearPlan plan = linear_plan(sizes, linear_wide(fold));
+    if (plan.few()) return LinearRun{plan, true, true, 0u};
     const bool fits = with_linear_shape(plan, [&](auto s) {
         return linear_tiles<decltype(s)>(sizes) * plan.splits < (1ull << 31);
     });
@@ -1390,6 +1551,19 @@ hipError_t launch_linear(const LinearProduct& p, LinearOrder order, LinearFold f
             linear_any_kernel<kOrder, kExperts, kFold>
                 <<<static_cast<uint32_t>(any_tiles(p, order, fold)), 256, 0, stream>>>(p);
             return hipGetLastError();
+        }
+        if constexpr (kOrder == LinearOrder::kNT) {
+            if (run.plan.few())
+                return with_few_shape(run.plan, [&](auto s) -> hipError_t {
+                    using S = decltype(s);
+                    if constexpr (kFold == LinearFold::kSwiglu && S::kTiles != 2u) {
+                        return hipErrorInvalidValue;  // the rule takes none
+                    } else {
+                        linear_few_kernel<S, kExperts, kFold>
+                            <<<static_cast<uint32_t>(few_blocks<S>(sizes)), 64u * S::kWaves, 0, stream>>>(p);
+                        return hipGetLastError();
+                    }
+                });
         }
         return with_linear_shape(run.plan, [&](auto s) -> hipError_t {
             return launch_tiles<decltype(s), kOrder, kExperts, kFold>(p, sizes, run.plan.splits, scratch, stream);

@@ -34,12 +34,26 @@ using Linear64x64 = LinearShape<16, 2, 2, 2, 2, 3>;
 using Linear32x128 = LinearShape<16, 1, 4, 2, 2, 3>;
 using Linear16x128 = LinearShape<16, 1, 4, 1, 2, 3>;
 
+// The form for few rows: kRows rows of C by 16 kTiles columns a workgroup, its kWaves waves a part
+// of K each, in rings of kStages slots.
+template <uint32_t kWaves_, uint32_t kStages_, uint32_t kTiles_>
+struct FewShape {
+    static constexpr uint32_t kRows = 16, kWaves = kWaves_, kStages = kStages_, kTiles = kTiles_;
+    static constexpr uint32_t kLds = kWaves * kStages * (kRows + 16u * kTiles) * 8u + kMxMaxExperts / 4u;
+    static constexpr uint32_t kResident = 160u * 64u / kLds;  // workgroups a CU
+};
+
+using Few8x16 = FewShape<8, 3, 1>;
+using Few8x32 = FewShape<8, 2, 2>;
+using Few4x32 = FewShape<4, 3, 2>;
+
 // What the rule goes by.
 struct LinearSizes {
     uint32_t rows, columns, depth;  // of C in front of a fold, and K (all experts' rows where K is ragged)
     uint32_t experts;               // 0: the dense product
     bool swiglu;
-    bool ragged;  // K is an expert's rows, C has `rows` rows for each
+    bool ragged;  // K lies across A's stored rows; by expert: it is the expert's, and C has `rows` rows for each
+    bool along;   // K lies along the stored rows of both operands
 
     constexpr uint32_t across() const { return swiglu ? columns / 2u : columns; }
 };
@@ -74,13 +88,23 @@ constexpr uint32_t linear_parts(uint32_t depth, uint32_t splits) {
     return (depth + each - 1u) / each;
 }
 
-// What a product is run on: the shape's number in LinearCost's order, and into how many parts its
-// K is cut, whose sums go through the scratch.
+// Workgroups of the form for few rows, a bound where the experts' rows are known to the device alone.
+template <typename S>
+uint64_t few_blocks(const LinearSizes& p) {
+    const uint64_t across = p.swiglu ? 8u * S::kTiles : 16u * S::kTiles;
+    const uint64_t rows = p.experts != 0u ? mx_max_tasks(p.rows, p.experts, S::kRows)
+                                          : (static_cast<uint64_t>(p.rows) + S::kRows - 1u) / S::kRows;
+    return rows * ((p.across() + across - 1u) / across);
+}
+
+// What a product is run on: the shape's number in LinearCost's order, or kFew and on of the form
+// for few rows, and into how many parts its K is cut, whose sums go through the scratch.
 struct LinearPlan {
     uint32_t shape, splits;
+    constexpr bool few() const { return shape >= 5u; }
 };
 
-constexpr uint32_t kLinearShapes = 5, kLinearMaxSplits = 32;
+constexpr uint32_t kLinearShapes = 5, kFew = 5, kLinearMaxSplits = 32;
 constexpr size_t kLinearMaxPartBytes = 256u << 20;
 
 // What a product takes, us: a launch, and for every tile that a CU computes after another its
@@ -125,7 +149,24 @@ float linear_expert_us(const LinearSizes& p, uint32_t shape) {
 
 // The plan with the least time.  wide: 256 x 256 tiles are there for it.  K that lies across A's
 // rows takes tiles of 64 rows and more: fewer would not fill a load instruction.
+//
+// The form for few rows takes products of so few workgroups that the card holds all of them at
+// once: as few waves a tile's stages in turn would leave most of it idle.  us on 8 waves by 16
+// columns, 8 by 32 and 4 by 32, and on the best tiles with K cut:
+//   1 x 2,048 x 2,048 (64 workgroups of 32 columns)    3.7   4.2   5.1    8.2
+//   1 x 2,048 x 8,192 (64)                             7.9   9.6    13     11
+//   1 x 8,192 x 2,048 (256)                            6.9   5.1   5.8    9.9
+//   128 x 2,048 x 2,048 (512)                           12   7.8   6.2     11
+//   61 x 8,192 x 512 (1,024)                            14   8.7   5.9    6.1
+//   512 x 512 x 8,192 (512)                             29    21    20     18
+//   gate/up of one token, 10 of 512 experts (320)              10.4    9.6   14.8
+//   down of one token (640)                             13   9.0   6.9    6.2
 inline LinearPlan linear_plan(const LinearSizes& p, bool wide) {
+    if (p.along) {
+        if (!p.swiglu && few_blocks<Few8x32>(p) <= 128u) return LinearPlan{kFew, 1u};
+        if (few_blocks<Few8x32>(p) <= 256u) return LinearPlan{kFew + 1u, 1u};
+        if (few_blocks<Few4x32>(p) <= 512u && p.depth <= 4096u) return LinearPlan{kFew + 2u, 1u};
+    }
     LinearPlan best{2u, 1u};
     float least = 1e30f;
     const auto look = [&](auto s, uint32_t shape) {
@@ -154,7 +195,17 @@ inline LinearPlan linear_plan(const LinearSizes& p, bool wide) {
     return best;
 }
 
-// Calls f with the plan's shape.
+// Calls f with the plan's form for few rows.
+template <typename F>
+auto with_few_shape(const LinearPlan& plan, F f) {
+    switch (plan.shape) {
+        case kFew: return f(Few8x16{});
+        case kFew + 1u: return f(Few8x32{});
+        default: return f(Few4x32{});
+    }
+}
+
+// Calls f with the plan's tile shape.
 template <typename F>
 auto with_linear_shape(const LinearPlan& plan, F f) {
     switch (plan.shape) {
