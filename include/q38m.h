@@ -735,12 +735,14 @@ int q38m_moe_unpermute_backward_v1(const void* dy, const void* rows, uint32_t dt
  * and row_stride multiples of 16 bytes) run on the fast kernels, which read
  * a row in aligned pieces of 16 bytes, the last one whole: up to seven values
  * behind a row's last one are read, and do not count whatever they hold.
+ * Others are copied so (q38m_linear_*, where the scratch has room) or run on
+ * a slower kernel.
  * Descriptors that are not needed are NULL.  Outputs overlap no input and no
  * other output, but a residual may be the output that it is added to (the
  * same data, type and stride).  rows <= 2^28, columns <= 2^24,
  * experts <= 1024; a product has fewer than 2^31 tiles of 16 x 64 values.
  * Floating-point parity: the order of a sum is the kernels', and it is the
- * same in every call with the same sizes and strides. */
+ * same in every call with the same sizes, strides and scratch. */
 typedef struct q38m_tensor_v1 {
     void* data;
     uint64_t row_stride;
@@ -764,9 +766,11 @@ typedef struct q38m_tensor_v1 {
 #define Q38M_ACT_GELU_TANH 5u
 
 /* Scratch that any of the three q38m_linear products of a layer with this many
- * rows, outputs (weight rows) and inputs (weight columns) takes at most (a
- * call that is given less than it needs is refused); 0: none is needed and it
- * may be NULL.  16-byte aligned.  Two calls that may run at the same time need
+ * rows, outputs (weight rows) and inputs (weight columns) takes at most, of
+ * contiguous matrices; a call that is given less than it needs is refused.  For
+ * the copies of a matrix whose row_stride alone is no multiple of 8, rows *
+ * ((columns + 7) / 8) * 16 bytes more.  0: none is needed and it may be NULL.
+ * 16-byte aligned.  Two calls that may run at the same time need
  * two (captured graphs that replay together too). */
 size_t q38m_linear_scratch_bytes(uint32_t rows, uint32_t outputs, uint32_t inputs);
 

@@ -1161,7 +1161,7 @@ bool valid_sorted(const uint32_t* offsets, const uint32_t* packed, uint32_t top_
 
 int run_linear(const LinearProduct& p, LinearOrder order, LinearFold fold, void* scratch,
                size_t scratch_bytes, void* stream, int device) {
-    const q38m::LinearRun run = q38m::linear_run(p, order, fold);
+    const q38m::LinearRun run = q38m::linear_run(p, order, fold, scratch ? scratch_bytes : 0u);
     if (!run.fits) return fail(Q38M_ERR_INVALID_ARGUMENT, "bf16 product too large for one call");
     if (!valid_scratch(scratch, scratch_bytes, run.scratch_bytes))
         return fail(Q38M_ERR_INVALID_ARGUMENT, "linear scratch is missing, small or unaligned");

@@ -327,14 +327,15 @@ struct LinearProduct {
 };
 size_t linear_scratch_bytes(uint32_t rows, uint32_t outputs, uint32_t inputs);
 size_t bias_scratch_bytes(uint32_t rows, uint32_t columns);
-// How a product is run: on tiles, or where its operands' rows do not start at 16 bytes on the
-// kernel for any strides; whether its tiles can be counted, and the scratch it takes.
+// How a product is run: on tiles, for which operands whose rows do not start at 16 bytes are copied
+// to the scratch where it has room for them (the dense products), or on the kernel for any
+// strides; whether its tiles can be counted, and the scratch it takes.
 struct LinearRun {
     LinearPlan plan;
-    bool on_tiles, fits;
+    bool on_tiles, fits, copy_a, copy_b;
     size_t scratch_bytes;
 };
-LinearRun linear_run(const LinearProduct& p, LinearOrder order, LinearFold fold);
+LinearRun linear_run(const LinearProduct& p, LinearOrder order, LinearFold fold, size_t scratch_bytes);
 hipError_t launch_linear(const LinearProduct& p, LinearOrder order, LinearFold fold, const LinearRun& run,
                          void* scratch, hipStream_t stream);
 hipError_t launch_activation_backward(const LinearMatrix& dy, const LinearMatrix& pre,

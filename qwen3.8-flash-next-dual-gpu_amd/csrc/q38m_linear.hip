@@ -1366,6 +1366,18 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const float* __restric
     }
 }
 
+// Rows of any stride and alignment to rows at 16 bytes: a piece of eight values a thread, zeros behind
+// a row's end.  Memory bounds it.
+__global__ __launch_bounds__(256) void linear_rows_kernel(const uint16_t* __restrict__ from, uint64_t stride,
+                                                          uint64_t pieces, uint32_t row_pieces, uint32_t columns,
+                                                          v4u* __restrict__ to) {
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < pieces; i += gridDim.x * 256ull) {
+        const uint64_t row = i / row_pieces;
+        const uint32_t column = static_cast<uint32_t>(i % row_pieces) * 8u;
+        to[i] = load_eight(from + row * stride + column, static_cast<int32_t>(columns - column));
+    }
+}
+
 // ---- activation and bias gradients ------------------------------------------------
 
 // Eight columns of a row for each thread; memory bounds it.
@@ -1515,12 +1527,77 @@ hipError_t launch_tiles(const LinearProduct& p, const LinearSizes& sizes, uint32
 
 }  // namespace
 
+namespace {
+
+struct Operand {  // as it is stored
+    const uint16_t* data;
+    uint64_t stride;
+    uint32_t rows, columns;
+    bool at_16() const { return reinterpret_cast<uintptr_t>(data) % 16u == 0u && stride % 8u == 0u; }
+    uint64_t row_pieces() const { return (columns + 7ull) / 8u; }
+    size_t copy_bytes() const { return rows * row_pieces() * 16u; }
+};
+
+Operand operand_a(const LinearProduct& p, LinearOrder order) {
+    return order == LinearOrder::kTN ? Operand{p.a, p.a_stride, p.depth, p.rows} : Operand{p.a, p.a_stride, p.rows, p.depth};
+}
+Operand operand_b(const LinearProduct& p, LinearOrder order) {
+    return order == LinearOrder::kNT ? Operand{p.b, p.b_stride, p.columns, p.depth} : Operand{p.b, p.b_stride, p.depth, p.columns};
+}
+
+size_t up_to_16(size_t bytes) { return (bytes + 15u) / 16u * 16u; }
+
+// The parts of K, and in front of them copies of operands whose rows do not start at 16 bytes.
+LinearRun run_with_copies(const LinearProduct& p, LinearOrder order, LinearFold fold) {
+    LinearProduct q = p;
+    const Operand a = operand_a(p, order), b = operand_b(p, order);
+    LinearRun run{};
+    run.copy_a = !a.at_16();
+    run.copy_b = !b.at_16();
+    if (run.copy_a) q.a = nullptr, q.a_stride = a.row_pieces() * 8u;
+    if (run.copy_b) q.b = nullptr, q.b_stride = b.row_pieces() * 8u;
+    const LinearSizes sizes = linear_sizes(p, order, fold);
+    run.plan = linear_plan(sizes, linear_wide(fold));
+    run.on_tiles = linear_on_tiles(q, order, fold);
+    run.fits = run.plan.few() || with_linear_shape(run.plan, [&](auto s) {
+        return linear_tiles<decltype(s)>(sizes) * run.plan.splits < (1ull << 31);
+    });
+    run.scratch_bytes = run.plan.few() ? 0u : part_bytes(sizes, run.plan);
+    if (run.copy_a) run.scratch_bytes = up_to_16(run.scratch_bytes) + a.copy_bytes();
+    if (run.copy_b) run.scratch_bytes = up_to_16(run.scratch_bytes) + b.copy_bytes();
+    return run;
+}
+
+// Whether copies pay: the kernel for any strides goes through K 32 values at a time, 8.9 us for 1,000
+// of them where its tiles are at work at the same time, the copies are a launch each and their bytes.
+// us without and with copies, rows x outputs x inputs, all odd: 61 x 2,001 x 501 10 and 13, 1 x 8,191 x
+// 2,001 34 and 22, 512 x 8,191 x 501 21 and 33, 4,001 x 8,191 x 501 142 and 93, x 8,001 1,899 and 563;
+// the input's gradient of 61 x 333 x 501 15 and 11, of 4,001 x 8,191 x 2,001 703 and 191; the weight's of
+// 61 x 2,001 x 2,001 10 and 12, of 512 x 2,001 x 2,001 42 and 20.
+bool copies_pay(const LinearProduct& p) {
+    const double products = static_cast<double>(p.rows) * p.columns * p.depth;
+    return p.depth >= 320u || (p.depth >= 96u && products >= 3e9);
+}
+
+// Contiguous matrices of a layer: null data has the alignment that a copy would have.
+LinearProduct layer_product(uint32_t rows, uint32_t columns, uint32_t depth, uint64_t a_stride, uint64_t b_stride) {
+    return LinearProduct{nullptr, nullptr, a_stride, b_stride, nullptr, nullptr, rows, columns, depth, 0u, 1u, 1u, {}};
+}
+
+}  // namespace
+
 size_t linear_scratch_bytes(uint32_t rows, uint32_t outputs, uint32_t inputs) {
+    const auto stride = [&](uint32_t of, uint64_t columns) { return of == 1u ? (columns + 7u) / 8u * 8u : columns; };
+    const uint64_t x = stride(rows, inputs), w = stride(outputs, inputs), dz = stride(rows, outputs);
     size_t most = bias_scratch_bytes(rows, outputs);
-    for (const LinearSizes& s : {LinearSizes{rows, outputs, inputs, 0u, false, false, true},
-                                 LinearSizes{rows, inputs, outputs, 0u, false, false, false},
-                                 LinearSizes{outputs, inputs, rows, 0u, false, true, false}})
-        most = std::max(most, part_bytes(s, linear_plan(s, true)));
+    const auto with = [&](const LinearProduct& p, LinearOrder order, LinearFold fold) {
+        const LinearRun run = run_with_copies(p, order, fold);
+        if (run.on_tiles && run.fits && ((!run.copy_a && !run.copy_b) || copies_pay(p)))
+            most = std::max(most, run.scratch_bytes);
+    };
+    with(layer_product(rows, outputs, inputs, x, w), LinearOrder::kNT, LinearFold::kForward);
+    with(layer_product(rows, inputs, outputs, dz, w), LinearOrder::kNN, LinearFold::kSlope);
+    with(layer_product(outputs, inputs, rows, dz, x), LinearOrder::kTN, LinearFold::kAdd);
     return most;
 }
 
@@ -1529,20 +1606,41 @@ size_t bias_scratch_bytes(uint32_t rows, uint32_t columns) {
     return parts > 1u ? static_cast<size_t>(parts) * columns * sizeof(float) : 0u;
 }
 
-LinearRun linear_run(const LinearProduct& p, LinearOrder order, LinearFold fold) {
-    const LinearSizes sizes = linear_sizes(p, order, fold);
-    if (!linear_on_tiles(p, order, fold)) return LinearRun{{}, false, any_tiles(p, order, fold) < (1ull << 31), 0u};
-    const LinearPlan plan = linear_plan(sizes, linear_wide(fold));
-    if (plan.few()) return LinearRun{plan, true, true, 0u};
-    const bool fits = with_linear_shape(plan, [&](auto s) {
-        return linear_tiles<decltype(s)>(sizes) * plan.splits < (1ull << 31);
-    });
-    return LinearRun{plan, true, fits, part_bytes(sizes, plan)};
+LinearRun linear_run(const LinearProduct& p, LinearOrder order, LinearFold fold, size_t scratch_bytes) {
+    LinearRun run = run_with_copies(p, order, fold);
+    const bool copies = run.copy_a || run.copy_b;
+    // experts' rows are not copied: their calls have no scratch
+    if (run.on_tiles && (!copies || (!p.offsets && copies_pay(p) && scratch_bytes >= run.scratch_bytes)))
+        return run;
+    return LinearRun{{2u, 1u}, false, any_tiles(p, order, fold) < (1ull << 31), false, false, 0u};
 }
 
-hipError_t launch_linear(const LinearProduct& p, LinearOrder order, LinearFold fold, const LinearRun& run, void* scratch,
+hipError_t launch_linear(const LinearProduct& given, LinearOrder order, LinearFold fold, const LinearRun& run, void* scratch,
                          hipStream_t stream) {
+    LinearProduct p = given;
     const LinearSizes sizes = linear_sizes(p, order, fold);
+    size_t used = !run.on_tiles || run.plan.few() ? 0u : part_bytes(sizes, run.plan);
+    const auto copy = [&](const Operand& o) -> const uint16_t* {
+        used = up_to_16(used);
+        v4u* to = reinterpret_cast<v4u*>(static_cast<uint8_t*>(scratch) + used);
+        used += o.copy_bytes();
+        const uint64_t pieces = o.rows * o.row_pieces();
+        const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>((pieces + 255u) / 256u, 16u * kMxCus));
+        linear_rows_kernel<<<grid, 256, 0, stream>>>(o.data, o.stride, pieces, static_cast<uint32_t>(o.row_pieces()), o.columns, to);
+        return reinterpret_cast<const uint16_t*>(to);
+    };
+    if (run.copy_a) {
+        const Operand a = operand_a(p, order);
+        p.a = copy(a);
+        p.a_stride = a.row_pieces() * 8u;
+    }
+    if (run.copy_b) {
+        const Operand b = operand_b(p, order);
+        p.b = copy(b);
+        p.b_stride = b.row_pieces() * 8u;
+    }
+    if (run.copy_a || run.copy_b)
+        if (hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
     const auto launch = [&](auto o, auto experts, auto f) -> hipError_t {
         constexpr LinearOrder kOrder = decltype(o)::value;
         constexpr bool kExperts = decltype(experts)::value;

@@ -7,7 +7,7 @@ import pytest
 
 from helpers import stream, torch
 from linear_cases import (ACT_ERROR, F32_ROUND, Matrix, check_backward_input, check_backward_weight, check_linear,
-                          close, lin, output, run_linear, scratch_for, sync)
+                          close, lin, output, product_bound, run_linear, scratch_for, sync)
 
 pytestmark = pytest.mark.gpu
 
@@ -272,3 +272,24 @@ def test_long_rows_past_32_bits(q38m):
     b = x[-100:].double()
     # zeros add nothing and no error
     close(dw.double(), a.T @ b, (a.abs().T @ b.abs()) * 300 * 2.0 ** -23, "f32", "dw")
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 333, 2001), (17, 401, 333), (700, 513, 65), (131, 1001, 1003)])
+def test_odd_rows_copied_and_not(q38m, m, n, k):
+    """Contiguous odd rows: with the scratch that a layer is told to bring, and with none where that
+    is taken too; strides that the scratch was not sized for, with room and without."""
+    t = torch()
+    big = t.empty(1 << 26, dtype=t.uint8, device="cuda")
+    for spare in (0, 3):
+        x, w = Matrix(q38m, 1, m, k, spare=spare, shift=spare), Matrix(q38m, 2, n, k, sigma=k ** -0.5, spare=spare)
+        dz = Matrix(q38m, 3, m, n, spare=spare)
+        _, at, nbytes = scratch_for(q38m, m, n, k)
+        for place, room in ((at, nbytes), (None, 0), (big.data_ptr(), big.numel())):
+            y, dx = output(q38m, m, n, "f32", 1), output(q38m, m, k, "f32", 1)
+            dw = output(q38m, n, k, "f32", 1)
+            q38m.call("q38m_linear_v1", x.arg, w.arg, None, 0, None, y.arg, None, place, room, stream(), 0)
+            q38m.call("q38m_linear_backward_input_v1", dz.arg, w.arg, None, 0, None, dx.arg, place, room, stream(), 0)
+            q38m.call("q38m_linear_backward_weight_v1", dz.arg, x.arg, None, dw.arg, None, place, room, stream(), 0)
+            sync()
+            for got, a, b in ((y, x.values, w.values.T), (dx, dz.values, w.values), (dw, dz.values.T, x.values)):
+                close(got.got(), a @ b, product_bound(a.shape[1], a.abs() @ b.abs()), "f32", (spare, room))
