@@ -735,14 +735,16 @@ int q38m_moe_unpermute_backward_v1(const void* dy, const void* rows, uint32_t dt
  * and row_stride multiples of 16 bytes) run on the fast kernels, which read
  * a row in aligned pieces of 16 bytes, the last one whole: up to seven values
  * behind a row's last one are read, and do not count whatever they hold.
- * Others are copied so (q38m_linear_*, where the scratch has room) or run on
- * a slower kernel.
+ * Others are copied so (q38m_linear_*, where that pays and the scratch has
+ * room) or run on a slower kernel, and so do rows too far apart for 32-bit
+ * offsets (256 of them, all that are gathered, or from gate to up: 4 GB).
  * Descriptors that are not needed are NULL.  Outputs overlap no input and no
  * other output, but a residual may be the output that it is added to (the
  * same data, type and stride).  rows <= 2^28, columns <= 2^24,
- * experts <= 1024; a product has fewer than 2^31 tiles of 16 x 64 values.
+ * experts <= 1024; a product has fewer than 2^31 tiles (16 x 128 to 256 x 256
+ * values, by the sizes; on the slower kernel 2^24, of 64 x 64).
  * Floating-point parity: the order of a sum is the kernels', and it is the
- * same in every call with the same sizes, strides and scratch. */
+ * same in every call with the same sizes, strides, alignments and scratch size. */
 typedef struct q38m_tensor_v1 {
     void* data;
     uint64_t row_stride;
@@ -816,13 +818,13 @@ int q38m_linear_backward_activation_v1(const q38m_tensor_v1* dy, const q38m_tens
  * rows->rows = c->rows) or packed_assignment[p] / top_k.  c->rows are the
  * routes, below 2^24; offsets past them are taken as them, and an expert whose
  * end is not behind its begin has no rows (a row that two experts' offsets hold
- * after such a fall gets either's).  Rows of c that no expert has are left as
- * they were; a src(p) past the rows reads the last one.
+ * after such a fall gets either's, and where falls make the experts' rows more
+ * than the routes some may be left as they were).  Rows of c that no expert has
+ * are left as they were; a src(p) past the rows reads the last one.
  * epilogue SWIGLU: weights' first half of rows is gate, the second up; c has
  * half as many columns, h = g / (1 + exp(-g)) u (a zero for g below -88.7), and
  * pre (NULL, or bf16 or fp32 [routes][weights->rows]) gets gate and up.
- * NONE: pre is NULL.  c: bf16 or fp32.  Gathered rows and one expert's matrix
- * are below 4 GB. */
+ * NONE: pre is NULL.  c: bf16 or fp32. */
 #define Q38M_EPILOGUE_NONE 0u
 #define Q38M_EPILOGUE_SWIGLU 1u
 int q38m_moe_expert_gemm_v1(const q38m_tensor_v1* weights, const q38m_tensor_v1* rows,

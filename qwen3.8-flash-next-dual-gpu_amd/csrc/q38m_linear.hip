@@ -564,8 +564,8 @@ struct Span {
         v4u d[4];
         each_of<4>([&](auto kc) MX_INLINE {
             constexpr uint32_t k = decltype(kc)::value;
-            const v4u_any w = __builtin_nontemporal_load(reinterpret_cast<const v4u_any*>(static_cast<const uint16_t*>(m.data) + place(m, row_of(k)) +
-                                                                shift + column_of()));
+            const uint16_t* from = static_cast<const uint16_t*>(m.data) + place(m, row_of(k)) + shift + column_of();
+            const v4u_any w = __builtin_nontemporal_load(reinterpret_cast<const v4u_any*>(from));
             d[0][k] = w.x, d[1][k] = w.y, d[2][k] = w.z, d[3][k] = w.w;
         });
         each_of<4>([&](auto e) MX_INLINE { d[decltype(e)::value] = transpose_quad(d[decltype(e)::value], lane); });
@@ -591,8 +591,8 @@ struct Span {
                 each_of<4>([&](auto kc) MX_INLINE {
                     constexpr uint32_t k = decltype(kc)::value;
                     if (row_of(k) >= count) return;
-                    __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]}, reinterpret_cast<v4u_any*>(static_cast<float*>(m.data) + place(m, row_of(k)) + shift + 32u * half +
-                                                wide_column_of()));
+                    float* to = static_cast<float*>(m.data) + place(m, row_of(k)) + shift + 32u * half + wide_column_of();
+                    __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]}, reinterpret_cast<v4u_any*>(to));
                 });
             });
             return;
@@ -606,7 +606,8 @@ struct Span {
         each_of<4>([&](auto kc) MX_INLINE {
             constexpr uint32_t k = decltype(kc)::value;
             if (row_of(k) >= count) return;
-            __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]}, reinterpret_cast<v4u_any*>(static_cast<uint16_t*>(m.data) + place(m, row_of(k)) + shift + column_of()));
+            uint16_t* to = static_cast<uint16_t*>(m.data) + place(m, row_of(k)) + shift + column_of();
+            __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]}, reinterpret_cast<v4u_any*>(to));
         });
     }
 };
@@ -616,6 +617,20 @@ struct Span {
 // tiles of kMF rows.  K goes through LDS in stages of 64 values, in a ring of kStages slots,
 // loaded straight from memory; the stages of a tile follow those of the tile before without
 // a gap.
+//
+// What bounds it, by counters:
+// - large products (8,192^3 840 us without an epilogue, 1,309 TFLOP/s; across K of one or both
+//   operands 814 and 800): the card's clock, 1.7 GHz of 2.4 under this load, and matrix pipes busy
+//   for 72 % of the rest, the L1s' answers under way for most of what is left; no LDS conflicts.
+//   128 x 128 tiles move twice as much through LDS for the same products and take 1,016 us.
+// - many experts' products with much to store (gate/up of 32,768 tokens 1,600 us, 859 TFLOP/s of
+//   rows that are there): row tiles that an expert's last rows fill partly, a sixth of the products,
+//   and the stores, during which this workgroup multiplies nothing: a second set of sums does not fit
+//   the registers.
+// - experts of few rows (512 tokens 355 us, 6.1 TB/s) and weights' gradients in fp32 (16,384 tokens
+//   2,090 us, 5.4 TB/s read and written): memory.
+// - few tiles (509 x 2,048 x 8,192 31 us and a join of 4): one stage's latency after another, so K
+//   is cut until the card is full, and the parts' sums are joined by a second launch in their order.
 template <typename S, LinearOrder kOrder, bool kExperts, LinearFold kFold>
 __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 4u) void linear_tile_kernel(
     LinearProduct p, uint32_t each) {
@@ -1367,7 +1382,7 @@ __global__ __launch_bounds__(256) void linear_join_kernel(const float* __restric
 }
 
 // Rows of any stride and alignment to rows at 16 bytes: a piece of eight values a thread, zeros behind
-// a row's end.  Memory bounds it.
+// a row's end.  Memory bounds it: read once, written once, and read again by the product.
 __global__ __launch_bounds__(256) void linear_rows_kernel(const uint16_t* __restrict__ from, uint64_t stride,
                                                           uint64_t pieces, uint32_t row_pieces, uint32_t columns,
                                                           v4u* __restrict__ to) {
@@ -1380,7 +1395,8 @@ __global__ __launch_bounds__(256) void linear_rows_kernel(const uint16_t* __rest
 
 // ---- activation and bias gradients ------------------------------------------------
 
-// Eight columns of a row for each thread; memory bounds it.
+// Eight columns of a row for each thread; memory bounds it (16,384 x 8,192 bf16 with GELU 160 us,
+// 5.1 TB/s; fp32 305, 5.3).
 __global__ __launch_bounds__(256) void activation_backward_kernel(LinearMatrix dy, LinearMatrix pre,
                                                                   uint32_t activation, LinearMatrix dz, uint64_t pieces,
                                                                   uint32_t row_pieces, uint32_t columns) {
@@ -1404,7 +1420,9 @@ __global__ __launch_bounds__(256) void activation_backward_kernel(LinearMatrix d
 
 // Sums of 64 columns over `each` rows for each workgroup: 8 columns and every 32nd row for
 // a thread, its sum then joined with the other rows' in their order.  One part of the rows
-// writes d_bias, several their partial sums [part][columns], which a second launch joins.
+// writes d_bias, several their partial sums [part][columns], which a second launch joins: no
+// atomics, so that the order is always the same.  Memory bounds it where there is much of it
+// (131,072 x 8,192 388 us, 5.5 TB/s; 4,096 x 8,192 16 us, 5 of them the second launch).
 constexpr uint32_t kBiasColumns = 64, kBiasRows = 256, kBiasParts = 64;
 
 __global__ __launch_bounds__(256) void bias_sum_kernel(const uint16_t* __restrict__ dz, uint64_t stride, uint32_t rows,
@@ -1525,10 +1543,6 @@ hipError_t launch_tiles(const LinearProduct& p, const LinearSizes& sizes, uint32
     }
 }
 
-}  // namespace
-
-namespace {
-
 struct Operand {  // as it is stored
     const uint16_t* data;
     uint64_t stride;
@@ -1612,7 +1626,7 @@ LinearRun linear_run(const LinearProduct& p, LinearOrder order, LinearFold fold,
     // experts' rows are not copied: their calls have no scratch
     if (run.on_tiles && (!copies || (!p.offsets && copies_pay(p) && scratch_bytes >= run.scratch_bytes)))
         return run;
-    return LinearRun{{2u, 1u}, false, any_tiles(p, order, fold) < (1ull << 31), false, false, 0u};
+    return LinearRun{{2u, 1u}, false, any_tiles(p, order, fold) < (1ull << 24), false, false, 0u};  // threads of a launch
 }
 
 hipError_t launch_linear(const LinearProduct& given, LinearOrder order, LinearFold fold, const LinearRun& run, void* scratch,

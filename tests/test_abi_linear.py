@@ -76,6 +76,7 @@ def test_linear_refusals(q38m):
     call(**long, scratch=P + 8)
     call(**long, nbytes=0)
     call(x=t(1 << 28, 1 << 10), w=t(1 << 24, 1 << 10), y=t(1 << 28, 1 << 24))  # 2^31 tiles and more
+    call(x=t(1 << 28, 1), w=t(256, 1), y=t(1 << 28, 256))  # odd rows: 2^24 tiles of 64 x 64
 
 
 def test_input_gradient_refusals(q38m):
