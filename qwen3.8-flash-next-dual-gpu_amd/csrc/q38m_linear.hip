@@ -622,7 +622,7 @@ struct Span {
 // - large products (8,192^3 840 us without an epilogue, 1,309 TFLOP/s; across K of one or both
 //   operands 814 and 800): the card's clock, 1.7 GHz of 2.4 under this load, and matrix pipes busy
 //   for 72 % of the rest, the L1s' answers under way for most of what is left; no LDS conflicts.
-//   128 x 128 tiles move twice as much through LDS for the same products and take 1,016 us.
+//   128 x 128 tiles move twice as much through LDS for the same products (with GELU 1,159 us, 942).
 // - many experts' products with much to store (gate/up of 32,768 tokens 1,600 us, 859 TFLOP/s of
 //   rows that are there): row tiles that an expert's last rows fill partly, a sixth of the products,
 //   and the stores, during which this workgroup multiplies nothing: a second set of sums does not fit
@@ -686,19 +686,29 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     if constexpr (kRagged) {
         // experts without rows: zeros, and what they are added to, unless that is there already
         if (p.e.residual.data != p.e.c.data) {
+            // The threads of all workgroups go round these experts' pieces of eight values; 64 experts are
+            // looked at in one, and no piece's place is divided out (bf16 gradients of 512 experts, 61
+            // tokens: 221 us, 168 of them for the experts that have rows; one expert after another, with
+            // a division a piece, 300).
             const uint32_t pieces = (n_out + 7u) / 8u, threads = gridDim.x * 64u * S::kWaves;
-            const uint64_t all = static_cast<uint64_t>(p.rows) * pieces;
-            uint32_t start = blockIdx.x * 64u * S::kWaves + threadIdx.x;  // the threads go round the experts' pieces
-            for (uint32_t e = 0; e < p.experts; ++e) {
-                const uint32_t begin = offsets[e], end = e + 1u < kMaxSortExperts ? offsets[e + 1u] : last_offset;
-                if (min(end, routes) > min(begin, routes)) continue;
-                uint64_t i = start;
-                for (; i < all; i += threads) {
-                    const uint64_t row = static_cast<uint64_t>(e) * p.rows + i / pieces;
-                    float v[8] = {}, u[8] = {};
-                    finish<kFold>(p.e, row, static_cast<uint32_t>(i % pieces) * 8u, n_out, v, u);
+            const uint32_t start = blockIdx.x * 64u * S::kWaves + threadIdx.x;
+            const uint32_t step_rows = threads / pieces, step_pieces = threads % pieces;
+            uint32_t row = start / pieces, piece = start % pieces;
+            for (uint32_t e0 = 0; e0 < p.experts; e0 += 64u) {
+                const uint32_t own = e0 + lane;  // offsets has kMaxSortExperts, a multiple of 64
+                const uint32_t begin = offsets[own], end = own + 1u < kMaxSortExperts ? offsets[own + 1u] : last_offset;
+                uint64_t empty = __ballot(own < p.experts && min(end, routes) <= min(begin, routes));
+                for (; empty != 0u; empty &= empty - 1u) {
+                    const uint64_t first = static_cast<uint64_t>(e0 + __builtin_ctzll(empty)) * p.rows;
+                    while (row < p.rows) {
+                        float v[8] = {}, u[8] = {};
+                        finish<kFold>(p.e, first + row, piece * 8u, n_out, v, u);
+                        row += step_rows;
+                        piece += step_pieces;
+                        if (piece >= pieces) piece -= pieces, ++row;
+                    }
+                    row -= p.rows;
                 }
-                start = static_cast<uint32_t>(i - all);
             }
         }
     }
