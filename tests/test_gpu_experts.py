@@ -262,3 +262,60 @@ def test_streams(q38m):
         for i in range(5):
             for a, b in zip(alone, o[i]):
                 assert t.equal(a.view, b.view)
+
+
+@pytest.mark.parametrize("tokens,top_k,experts", [(3, 4, 24), (90, 6, 96)])
+def test_graphs_with_other_routes(q38m, tokens, top_k, experts):
+    """A layer's products captured once and replayed with routes that change between the replays, experts
+    with and without rows among them: every replay equals the eager calls bit for bit."""
+    t = torch()
+    hidden, middle, routes = 136, 72, tokens * top_k
+    x, dy = Matrix(q38m, 1, tokens, hidden), Matrix(q38m, 2, routes, hidden)
+    up = Matrix(q38m, 3, 2 * middle, hidden, sigma=0.1, experts=experts)
+    down = Matrix(q38m, 4, hidden, middle, sigma=0.1, experts=experts)
+    routing = q38m.SortedRoutes(tokens, top_k, experts)
+    at, packed = q38m.ptr(routing.offsets), q38m.ptr(routing.packed)
+
+    def buffers():
+        return (output(q38m, routes, middle), output(q38m, routes, 2 * middle, "f32"), output(q38m, routes, hidden),
+                output(q38m, routes, 2 * middle), output(q38m, routes, hidden),
+                output(q38m, 2 * middle, hidden, "f32", experts=experts), output(q38m, hidden, middle, experts=experts))
+
+    def run(o):
+        h, pre, y, dgu, dx, dup, ddown = o
+        q38m.call("q38m_moe_expert_gemm_v1", up.arg, x.arg, at, packed, top_k, 1, h.arg, pre.arg, stream(), 0)
+        q38m.call("q38m_moe_expert_gemm_v1", down.arg, h.arg, at, None, 1, 0, y.arg, None, stream(), 0)
+        q38m.call("q38m_moe_expert_backward_rows_v1", down.arg, dy.arg, at, pre.arg, dgu.arg, stream(), 0)
+        q38m.call("q38m_moe_expert_backward_rows_v1", up.arg, dgu.arg, at, None, dx.arg, stream(), 0)
+        q38m.call("q38m_moe_expert_backward_weights_v1", dgu.arg, x.arg, at, packed, top_k, dup.arg, dup.arg, stream(), 0)
+        q38m.call("q38m_moe_expert_backward_weights_v1", dy.arg, h.arg, at, None, 1, None, ddown.arg, stream(), 0)
+
+    def ids(seed):
+        some = t.randperm(experts, generator=t.Generator().manual_seed(seed))[:max(top_k, experts // (seed + 1))]
+        picks = t.rand(tokens, len(some), generator=t.Generator().manual_seed(seed)).argsort(1)[:, :top_k]
+        return some[picks].int().cuda()
+
+    eager, replayed = buffers(), buffers()
+    routing.sort(ids(0))
+    run(eager)
+    graph = t.cuda.CUDAGraph()
+    with t.cuda.graph(graph):
+        run(replayed)
+    for seed in range(4):
+        routing.sort(ids(seed))
+        for o in (eager, replayed):
+            o[5].view.fill_(1.0)
+        run(eager)
+        graph.replay()
+        sync()
+        for a, b in zip(eager, replayed):
+            assert t.equal(a.view, b.view), seed
+
+
+@pytest.mark.parametrize("n,k,counts", [(2, 1100001, [0, 5, 0]), (700, 3, [0] * 130 + [1] + [0] * 77), (1, 1, [0] * 70)])
+def test_weight_gradient_of_experts_without_rows(q38m, n, k, counts):
+    """Rows of more pieces than there are threads, many experts' zeros, and no rows at all."""
+    s = Sorted(counts, 0 if sum(counts) else 3)
+    for spare in ((0, 0, 0), (-n % 8, -k % 8, 0)):  # on either kernel
+        check_experts_weights(q38m, 11, s, n, k, None, "bf16", spare)
+        check_experts_weights(q38m, 12, s, n, k, "f32", "f32", spare)
