@@ -230,6 +230,19 @@ struct InRow {
     }
 };
 
+// The gradients of gate, dh u (s + g s(g) s(-g)), in place of dh, and of up, dh g s, of up.
+template <uint32_t kN>
+__device__ __forceinline__ void swiglu_slopes(const float (&gate)[kN], float (&up)[kN], float (&dh)[kN]) {
+#pragma unroll
+    for (uint32_t i = 0; i < kN; ++i) {
+        const Sigmoid y(gate[i]);
+        const float of_up = dh[i] * (gate[i] * y.s);
+        dh[i] *= __builtin_fmaf(held(gate[i]), y.both, y.s);
+        dh[i] *= up[i];
+        up[i] = of_up;
+    }
+}
+
 // The epilogue of a lane's kN sums; n: the columns of C in front of what a fold puts beside
 // them; u: the sums of up beside gate's.
 template <LinearFold kFold, typename Access, uint32_t kN>
@@ -247,21 +260,12 @@ __device__ __forceinline__ void finish_all(LinearEpilogue e, Access at, uint32_t
 #pragma unroll
             for (uint32_t i = 0; i < kN; ++i) v[i] = swiglu<false>(v[i], u[i]);
         }
-    } else if constexpr (kFold == LinearFold::kSwigluGrad) {  // of gate dh u (s + g s(g) s(-g)), of up dh g s
-        // up's first, so that few values are held at a time
-        float gate[kN], other[kN];
+    } else if constexpr (kFold == LinearFold::kSwigluGrad) {
+        float gate[kN], up[kN];
         at.load(e.pre, 0u, gate);
-#pragma unroll
-        for (uint32_t i = 0; i < kN; ++i) {
-            const Sigmoid y(gate[i]);
-            other[i] = v[i] * (gate[i] * y.s);
-            v[i] *= __builtin_fmaf(held(gate[i]), y.both, y.s);
-        }
-        at.store(e.c, n, other);
-        __builtin_amdgcn_sched_barrier(0);
-        at.load(e.pre, n, other);
-#pragma unroll
-        for (uint32_t i = 0; i < kN; ++i) v[i] *= other[i];
+        at.load(e.pre, n, up);
+        swiglu_slopes(gate, up, v);
+        at.store(e.c, n, up);
     } else if constexpr (kFold == LinearFold::kSlope) {
         if (e.activation != Q38M_ACT_NONE) {
             float z[kN];
@@ -1155,14 +1159,44 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
                     return;
                 }
             }
-            each_of<kFours * 4u / kN>([&](auto gc) MX_INLINE {
+            const auto column_of = [&](uint32_t f) MX_INLINE {
+                return column0 + (kN == 4u ? 4u * q : kMF == 32u ? kGap * (f + q) : kGap * (f + q % 2u) + 4u * (q & 2u));
+            };
+            // what the SwiGLU's derivative reads of a row, under way together: gate's, then up's
+            constexpr uint32_t kGroups = kFours * 4u / kN;
+            constexpr bool kBeside = kFold == LinearFold::kSwigluGrad && kN == 8u;
+            [[maybe_unused]] Raw<kN> beside[kBeside ? 2u * kGroups : 1u];
+            if constexpr (kBeside) {
+                if (n_out >= kN) {
+                    const uint64_t at = (row0 + min(m, count - 1u)) * p.e.pre.stride;
+                    each_of<kGroups>([&](auto gc) MX_INLINE {
+                        constexpr uint32_t g = decltype(gc)::value;
+                        const uint32_t column = min(column_of(g * (kN / 4u)), n_out - kN);
+                        beside[g].load(p.e.pre, at + column);
+                        beside[kGroups + g].load(p.e.pre, at + n_out + column);
+                    });
+                }
+            }
+            each_of<kGroups>([&](auto gc) MX_INLINE {
                 constexpr uint32_t f = decltype(gc)::value * (kN / 4u);
-                const uint32_t column = column0 + (kN == 4u      ? 4u * q
-                                                   : kMF == 32u ? kGap * (f + q)
-                                                                 : kGap * (f + q % 2u) + 4u * (q & 2u));
+                const uint32_t column = column_of(f);
                 float v[kN], u[kN] = {};
                 values(std::integral_constant<uint32_t, f>{}, None{}, v, None{});
                 if constexpr (kSwiglu) values(std::integral_constant<uint32_t, f>{}, Up{}, u, None{});
+                if constexpr (kBeside) {
+                    if (column + kN <= n_out) {
+                        float gate[kN];
+                        beside[decltype(gc)::value].values(p.e.pre, gate);
+                        beside[kGroups + decltype(gc)::value].values(p.e.pre, u);
+                        swiglu_slopes(gate, u, v);
+                        if (m < count) {
+                            const InRow at{row0 + m, column};
+                            at.store(p.e.c, n_out, u);
+                            at.store(p.e.c, 0u, v);
+                        }
+                        return;
+                    }
+                }
                 if (m < count && column < n_out) finish<kEnd>(p.e, row0 + m, column, n_out, v, u);
                 if constexpr (S::kWaves == 8u) __builtin_amdgcn_sched_barrier(0);
             });
