@@ -623,8 +623,8 @@ struct Span {
 // a gap.
 //
 // What bounds it, by counters:
-// - large products (8,192^3 840 us without an epilogue, 1,309 TFLOP/s; across K of one or both
-//   operands 814 and 800): the card's clock, 1.7 GHz of 2.4 under this load, and matrix pipes busy
+// - large products (8,192^3 819 us without an epilogue, 1,343 TFLOP/s; across K of one or both
+//   operands 808 and 800): the card's clock, 1.7 GHz of 2.4 under this load, and matrix pipes busy
 //   for 72 % of the rest, the L1s' answers under way for most of what is left; no LDS conflicts.
 //   128 x 128 tiles move twice as much through LDS for the same products (with GELU 1,159 us, 942).
 // - many experts' products with much to store (gate/up of 32,768 tokens 1,600 us, 859 TFLOP/s of
@@ -1735,7 +1735,13 @@ hipError_t launch_linear(const LinearProduct& given, LinearOrder order, LinearFo
     using Swiglu = std::integral_constant<LinearFold, LinearFold::kSwiglu>;
     using SwigluGrad = std::integral_constant<LinearFold, LinearFold::kSwigluGrad>;
     if (!p.offsets) {
+        // Where nothing is done to the sums but a residual's addition they begin with it, and go to memory in
+        // whole lines: the input's gradient 8,192 x 512 x 8,192 (rows x outputs x inputs) with a residual 128
+        // us and so 102, without one 81 and 74; forward 8,192 x 8,192 x 2,048 276 and 249, 240 and 226.
+        const bool as_they_are = p.e.activation == Q38M_ACT_NONE && !p.e.bias.data;
+        if (order == LinearOrder::kNT && as_they_are && !p.e.pre.data) return launch(NT{}, std::false_type{}, Add{});
         if (order == LinearOrder::kNT) return launch(NT{}, std::false_type{}, Forward{});
+        if (order == LinearOrder::kNN && as_they_are) return launch(NN{}, std::false_type{}, Add{});
         if (order == LinearOrder::kNN) return launch(NN{}, std::false_type{}, Slope{});
         return launch(TN{}, std::false_type{}, Add{});
     }
