@@ -293,3 +293,32 @@ def test_odd_rows_copied_and_not(q38m, m, n, k):
             sync()
             for got, a, b in ((y, x.values, w.values.T), (dx, dz.values, w.values), (dw, dz.values.T, x.values)):
                 close(got.got(), a @ b, product_bound(a.shape[1], a.abs() @ b.abs()), "f32", (spare, room))
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 256, 8192), (5, 264, 2048), (1030, 520, 640)])
+def test_residual_larger_than_the_sums(q38m, m, n, k):
+    """A residual of a thousand times the sums' size is a term of them at most: the bound of a sum of
+    one term more, whichever it begins with."""
+    t = torch()
+    for rows, outputs, inputs, name in ((m, n, k, "forward"), (m, k, n, "input"), (k, m, n, "weight")):
+        if name == "forward":
+            a, b = Matrix(q38m, 1, rows, inputs), Matrix(q38m, 2, outputs, inputs, sigma=inputs ** -0.5)
+            shape, product = (rows, outputs), lambda a, b: a @ b.T
+        elif name == "input":
+            a, b = Matrix(q38m, 1, rows, outputs), Matrix(q38m, 2, outputs, inputs, sigma=outputs ** -0.5)
+            shape, product = (rows, inputs), lambda a, b: a @ b
+        else:
+            a, b = Matrix(q38m, 1, rows, outputs), Matrix(q38m, 2, rows, inputs, sigma=rows ** -0.5)
+            shape, product = (outputs, inputs), lambda a, b: a.T @ b
+        depth = {"forward": inputs, "input": outputs, "weight": rows}[name]
+        r, y = Matrix(q38m, 3, *shape, "f32", sigma=1000.0), output(q38m, *shape, "f32")
+        _, at, nbytes = scratch_for(q38m, rows, outputs, inputs)
+        if name == "forward":
+            q38m.call("q38m_linear_v1", a.arg, b.arg, None, 0, r.arg, y.arg, None, at, nbytes, stream(), 0)
+        elif name == "input":
+            q38m.call("q38m_linear_backward_input_v1", a.arg, b.arg, None, 0, r.arg, y.arg, at, nbytes, stream(), 0)
+        else:
+            q38m.call("q38m_linear_backward_weight_v1", a.arg, b.arg, r.arg, y.arg, None, at, nbytes, stream(), 0)
+        sync()
+        size = product(a.values.abs(), b.values.abs()) + r.values.abs()
+        close(y.got(), product(a.values, b.values) + r.values, product_bound(depth + 1, size), "f32", (name, m, n, k))
