@@ -730,9 +730,9 @@ int q38m_moe_unpermute_backward_v1(const void* dy, const void* rows, uint32_t dt
  * other), row_stride elements from row to row (at least `columns`; any, where
  * there is one row).  bf16 is raw words; where a call takes either type the
  * descriptor says which.  Every operand that a product multiplies is bf16.
- * Sums are fp32 (where only a residual is added to them they begin with it, so
- * it counts in their error as a term does), and each output is rounded once (to
- * nearest even).  Data is aligned to its elements; operands whose rows all start at 16 bytes (data
+ * Sums are fp32, a residual is added to the whole sum in fp32 (one rounding,
+ * whatever its size), and each output is rounded once (to nearest even).  Data
+ * is aligned to its elements; operands whose rows all start at 16 bytes (data
  * and row_stride multiples of 16 bytes) run on the fast kernels, which read
  * a row in aligned pieces of 16 bytes, the last one whole: up to seven values
  * behind a row's last one are read, and do not count whatever they hold.

@@ -544,64 +544,43 @@ struct Span {
     __device__ MX_INLINE uint32_t column_of() const { return 16u * (lane & 3u) + lane / 32u * 8u; }
     __device__ MX_INLINE uint32_t wide_column_of() const { return 8u * (lane & 3u) + lane / 32u * 4u; }
 
-    __device__ MX_INLINE void load(LinearMatrix m, uint32_t shift, float (&v)[32]) const {
-        if (m.f32) {
-            each_of<2>([&](auto hc) MX_INLINE {
-                constexpr uint32_t half = decltype(hc)::value;
-                v4u d[4];  // dword e of the pieces k
-                each_of<4>([&](auto kc) MX_INLINE {
-                    constexpr uint32_t k = decltype(kc)::value;
-                    const v4u_any w = __builtin_nontemporal_load(reinterpret_cast<const v4u_any*>(
-                        static_cast<const float*>(m.data) + place(m, row_of(k)) + shift + 32u * half + wide_column_of()));
-                    d[0][k] = w.x, d[1][k] = w.y, d[2][k] = w.z, d[3][k] = w.w;
-                });
-                each_of<4>([&](auto e) MX_INLINE { d[decltype(e)::value] = transpose_quad(d[decltype(e)::value], lane); });
-                each_of<8>([&](auto c) MX_INLINE {  // four columns of both lanes of a row to eight of each
-                    constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
-                    const auto both = __builtin_amdgcn_permlane32_swap(d[e][2u * k], d[e][2u * k + 1u], false, false);
-                    v[16u * half + 8u * k + e] = __uint_as_float(both[0]);
-                    v[16u * half + 8u * k + 4u + e] = __uint_as_float(both[1]);
-                });
-            });
-            return;
-        }
-        v4u d[4];
-        each_of<4>([&](auto kc) MX_INLINE {
-            constexpr uint32_t k = decltype(kc)::value;
-            const uint16_t* from = static_cast<const uint16_t*>(m.data) + place(m, row_of(k)) + shift + column_of();
-            const v4u_any w = __builtin_nontemporal_load(reinterpret_cast<const v4u_any*>(from));
-            d[0][k] = w.x, d[1][k] = w.y, d[2][k] = w.z, d[3][k] = w.w;
+    // a half's values as its pieces have them in fp32: d[e][k] is value e of piece k
+    __device__ MX_INLINE void turn_half(const float (&v)[32], uint32_t half, v4u (&d)[4]) const {
+        each_of<8>([&](auto c) MX_INLINE {
+            constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
+            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[16u * half + 8u * k + e]),
+                                                               __float_as_uint(v[16u * half + 8u * k + 4u + e]), false, false);
+            d[e][2u * k] = both[0];
+            d[e][2u * k + 1u] = both[1];
         });
         each_of<4>([&](auto e) MX_INLINE { d[decltype(e)::value] = transpose_quad(d[decltype(e)::value], lane); });
-        each_of<16>([&](auto c) MX_INLINE {
-            constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
-            v[8u * k + 2u * e] = __uint_as_float(d[e][k] << 16);
-            v[8u * k + 2u * e + 1u] = __uint_as_float(d[e][k] & 0xffff0000u);
-        });
     }
-    __device__ MX_INLINE void store(LinearMatrix m, uint32_t shift, const float (&v)[32]) const {
+    __device__ MX_INLINE float* wide_piece(LinearMatrix m, uint32_t half, uint32_t k) const {
+        return static_cast<float*>(m.data) + place(m, row_of(k)) + 32u * half + wide_column_of();
+    }
+    __device__ MX_INLINE uint16_t* piece(LinearMatrix m, uint32_t k) const {
+        return static_cast<uint16_t*>(m.data) + place(m, row_of(k)) + column_of();
+    }
+    template <typename T>
+    __device__ MX_INLINE static T stream(const void* from) {
+        return __builtin_nontemporal_load(static_cast<const T*>(from));
+    }
+
+    __device__ MX_INLINE void store(LinearMatrix m, const float (&v)[32]) const {
+        v4u d[4];
         if (m.f32) {
             each_of<2>([&](auto hc) MX_INLINE {
                 constexpr uint32_t half = decltype(hc)::value;
-                v4u d[4];
-                each_of<8>([&](auto c) MX_INLINE {
-                    constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
-                    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[16u * half + 8u * k + e]),
-                                                                       __float_as_uint(v[16u * half + 8u * k + 4u + e]), false, false);
-                    d[e][2u * k] = both[0];
-                    d[e][2u * k + 1u] = both[1];
-                });
-                each_of<4>([&](auto e) MX_INLINE { d[decltype(e)::value] = transpose_quad(d[decltype(e)::value], lane); });
+                turn_half(v, half, d);
                 each_of<4>([&](auto kc) MX_INLINE {
                     constexpr uint32_t k = decltype(kc)::value;
                     if (row_of(k) >= count) return;
-                    float* to = static_cast<float*>(m.data) + place(m, row_of(k)) + shift + 32u * half + wide_column_of();
-                    __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]}, reinterpret_cast<v4u_any*>(to));
+                    __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]},
+                                                reinterpret_cast<v4u_any*>(wide_piece(m, half, k)));
                 });
             });
             return;
         }
-        v4u d[4];
         each_of<16>([&](auto c) MX_INLINE {
             constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
             d[e][k] = f32_to_bf16(v[8u * k + 2u * e]) | f32_to_bf16(v[8u * k + 2u * e + 1u]) << 16;
@@ -610,11 +589,58 @@ struct Span {
         each_of<4>([&](auto kc) MX_INLINE {
             constexpr uint32_t k = decltype(kc)::value;
             if (row_of(k) >= count) return;
-            uint16_t* to = static_cast<uint16_t*>(m.data) + place(m, row_of(k)) + shift + column_of();
-            __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]}, reinterpret_cast<v4u_any*>(to));
+            __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]}, reinterpret_cast<v4u_any*>(piece(m, k)));
+        });
+    }
+
+    // A residual is added to whole sums where a half's pieces have them, so it changes no places.  What is
+    // read of it at a time: of fp32 a half's pieces; of bf16 both halves', eight columns of half q from
+    // 8 (n % 4) on, which two lanes of a row trade for four of both halves, and trade sums back to be
+    // stored so.  (Four bf16 columns a lane, half a line at a time: forward 8,192 x 8,192 x 512 into fp32
+    // 140 us, so 115.)
+    __device__ MX_INLINE uint16_t* half_piece(LinearMatrix m, uint32_t k) const {
+        return static_cast<uint16_t*>(m.data) + place(m, row_of(k)) + lane / 32u * 32u + 8u * (lane & 3u);
+    }
+    __device__ MX_INLINE static void trade(v4u& w) {
+        const auto low = __builtin_amdgcn_permlane32_swap(w.x, w.z, false, false);
+        const auto high = __builtin_amdgcn_permlane32_swap(w.y, w.w, false, false);
+        w = v4u{low[0], high[0], low[1], high[1]};
+    }
+    __device__ MX_INLINE void read(LinearMatrix r, uint32_t half, v4u (&w)[4]) const {
+        each_of<4>([&](auto kc) MX_INLINE {
+            constexpr uint32_t k = decltype(kc)::value;
+            if (r.f32) w[k] = stream<v4u_any>(wide_piece(r, half, k));
+            else w[k] = stream<v4u_any>(half_piece(r, k));
+        });
+    }
+    __device__ MX_INLINE void store_sums(LinearMatrix m, LinearMatrix r, uint32_t half, const float (&v)[32], v4u (&w)[4],
+                                         v4u (&packed)[4]) const {
+        v4u d[4];
+        turn_half(v, half, d);
+        each_of<4>([&](auto kc) MX_INLINE {
+            constexpr uint32_t k = decltype(kc)::value;
+            if (!r.f32 && half == 0u) trade(w[k]);
+            each_of<4>([&](auto ec) MX_INLINE {
+                constexpr uint32_t e = decltype(ec)::value;
+                uint32_t other = w[k][e];
+                if (!r.f32) other = e % 2u != 0u ? w[k][2u * half + e / 2u] & 0xffff0000u : w[k][2u * half + e / 2u] << 16;
+                d[e][k] = __float_as_uint(__uint_as_float(d[e][k]) + __uint_as_float(other));
+            });
+            if (!m.f32) {
+                packed[k][2u * half] = f32_to_bf16(__uint_as_float(d[0][k])) | f32_to_bf16(__uint_as_float(d[1][k])) << 16;
+                packed[k][2u * half + 1u] = f32_to_bf16(__uint_as_float(d[2][k])) | f32_to_bf16(__uint_as_float(d[3][k])) << 16;
+                if (half == 0u) return;
+                trade(packed[k]);
+                if (row_of(k) < count) __builtin_nontemporal_store(v4u_any(packed[k]), reinterpret_cast<v4u_any*>(half_piece(m, k)));
+            } else if (row_of(k) < count) {
+                __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]},
+                                            reinterpret_cast<v4u_any*>(wide_piece(m, half, k)));
+            }
         });
     }
 };
+
+constexpr uint32_t kTyped = 4u;  // of a tile kernel's kTypes
 
 // Workgroups stay and compute tile after tile of kBM x kBN values of C (with the SwiGLU fold
 // half of the columns gate, half up), kWM x kWN waves, each kTM x kTN matrix-instruction
@@ -635,9 +661,18 @@ struct Span {
 //   2,090 us, 5.4 TB/s read and written): memory.
 // - few tiles (509 x 2,048 x 8,192 31 us and a join of 4): one stage's latency after another, so K
 //   is cut until the card is full, and the parts' sums are joined by a second launch in their order.
-template <typename S, LinearOrder kOrder, bool kExperts, LinearFold kFold>
+//
+// kTypes: 0, or kTyped and whether C (1) and the residual (2) are fp32, where a residual is added and
+// the sums stored in whole lines: with a way through for each type at run time the compiler kept 40 to
+// 640 registers of 256 x 256 tiles in memory, with one for each kernel none, or 5 to 20 of experts' tiles
+// and of fp32 residuals of bf16 sums, read and written where a tile begins and where its K or it ends.
+template <typename S, LinearOrder kOrder, bool kExperts, LinearFold kFold, uint32_t kTypes = 0u>
 __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 4u) void linear_tile_kernel(
     LinearProduct p, uint32_t each) {
+    if constexpr ((kTypes & kTyped) != 0u) {
+        p.e.c.f32 = (kTypes & 1u) != 0u;
+        p.e.residual.f32 = (kTypes & 2u) != 0u;
+    }
     constexpr uint32_t kMF = S::kMF, kTM = S::kTM, kTN = S::kTN, kBM = S::kBM, kBN = S::kBN;
     constexpr bool kAcrossA = kOrder == LinearOrder::kTN, kAcrossB = kOrder != LinearOrder::kNT;
     constexpr bool kSwiglu = kFold == LinearFold::kSwiglu;
@@ -940,57 +975,12 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     // exchange between lanes costs what it gives (in half lines, for want of registers: gate/up of
     // 32,768 tokens 1,594 us and so 1,647, down's row gradient of 16,384 763 and 884).
     constexpr bool kSpans = kMF == 32u && kOut % 2u == 0u && (kFold == LinearFold::kStore || kFold == LinearFold::kAdd);
+    static_assert(kTypes != 0u || !kSpans || kFold == LinearFold::kStore, "the types of what is added");
     [[maybe_unused]] const auto span = [&](uint32_t t, uint32_t i, uint32_t place) MX_INLINE {
         const uint32_t own_lane = fresh_lane();
         return Span{first_row(t), (wm * kTM + i) * kMF + (own_lane & 31u), count_of(t), first_column(t) + 64u * place, own_lane};
     };
-    // The sums of tile t begin with what it is added to, or with zeros.
-    const auto begin = [&](uint32_t t) MX_INLINE {
-        if (kFold == LinearFold::kAdd && p.e.residual.data) {
-            const LinearMatrix r = p.e.residual;
-            const uint32_t own_lane = fresh_lane(), n = own_lane % kMF, q = own_lane / kMF;
-            const uint32_t last = count_of(t) - 1u;
-            each_of<kTM>([&](auto ic) MX_INLINE {
-                constexpr uint32_t i = decltype(ic)::value;
-                if constexpr (kSpans) {
-                    if (first_column(t) + 32u * kOut <= n_out) {
-                        each_of<kOut / 2u>([&](auto pc) MX_INLINE {
-                            constexpr uint32_t place = decltype(pc)::value;
-                            float v[32];
-                            span(t, i, place).load(r, 0u, v);
-                            each_of<16>([&](auto c) MX_INLINE {
-                                constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
-                                constexpr uint32_t f = 2u * (4u * place + k);
-                                const auto both = __builtin_amdgcn_permlane32_swap(
-                                    __float_as_uint(v[8u * k + e]), __float_as_uint(v[8u * k + 4u + e]), false, false);
-                                acc[f / 4u][i][4u * (f % 4u) + e] = __uint_as_float(both[0]);
-                                acc[f / 4u][i][4u * (f % 4u + 1u) + e] = __uint_as_float(both[1]);
-                            });
-                        });
-                        return;
-                    }
-                }
-                const uint64_t at = (first_row(t) + min((wm * kTM + i) * kMF + n, last)) * r.stride;
-                each_of<kTN * kAcc / 4u>([&](auto c) MX_INLINE {
-                    constexpr uint32_t f = decltype(c)::value, j = f / (kAcc / 4u), e = f % (kAcc / 4u) * 4u;
-                    const uint32_t column = first_column(t) + kGap * f + 4u * q;
-                    if (column + 4u <= n_out) {
-                        float v[4];
-                        load_row(r, at + column, v);
-                        each_of<4>([&](auto k) MX_INLINE { acc[j][i][e + decltype(k)::value] = v[decltype(k)::value]; });
-                        return;
-                    }
-                    each_of<4>([&](auto k) MX_INLINE {  // those behind the last column are not stored
-                        float v[1];
-                        load_row(r, at + min(column + decltype(k)::value, n_out - 1u), v);
-                        acc[j][i][e + decltype(k)::value] = v[0];
-                    });
-                });
-            });
-            // the compiler would wait for them in the stages, where other loads are under way
-            __builtin_amdgcn_s_waitcnt(kVmcnt0);
-            return;
-        }
+    const auto begin = [&]() MX_INLINE {
 #pragma unroll
         for (uint32_t j = 0; j < kTN; ++j)
 #pragma unroll
@@ -1075,10 +1065,13 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     };
     constexpr uint32_t kEarly = (kDataLoads + 1u) / 2u;  // data loads in the step behind the barrier, the rest a step later
 
+    // The first fragments of the next tile are read behind the tile's end where a residual's values take
+    // their registers.
+    constexpr bool kReadBehind = kSpans && kFold == LinearFold::kAdd && kOrder == LinearOrder::kNT;
     // A stage in kSteps steps, software pipelined: a step's fragments are read while the step in
     // front of it is multiplied.  In front of the last step the workgroup meets: the next stage
     // (`valid` values of K) has come and this one is read, so its slot takes the kStages-th after it.
-    const auto stage = [&](uint32_t valid) MX_INLINE {
+    const auto stage = [&](uint32_t valid, auto read_next) MX_INLINE {
         constexpr uint32_t kLater = S::kStages - 2u;  // loads of the stages behind the next may be under way
         const auto step = [&](auto c) MX_INLINE {
             constexpr uint32_t kC = decltype(c)::value;
@@ -1101,21 +1094,35 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         if (valid < 64u) clear(valid);
         multiply(std::integral_constant<uint32_t, S::kSteps - 1u>{}, std::integral_constant<uint32_t, kReads + kEarly>{},
                  [&](uint32_t o) MX_INLINE {
-                     if (o < kReads) read(0u, o);
-                     else load_data(o - kReads);
+                     if (o >= kReads) load_data(o - kReads);
+                     else if (decltype(read_next)::value) read(0u, o);
                  });
     };
 
     // ---- C: a lane has four consecutive columns of a row and trades one of two such groups with
     // the lane that has the columns beside the other's, which gives both of them eight ----
     const auto store = [&](uint32_t t) MX_INLINE {
-        constexpr LinearFold kEnd = kFold == LinearFold::kAdd ? LinearFold::kStore : kFold;  // begun with
-        constexpr uint32_t kFours = kOut * kAcc / 4u;                                        // a lane's groups of four
+        using None = std::integral_constant<uint32_t, 0u>;
+        constexpr uint32_t kFours = kOut * kAcc / 4u;  // a lane's groups of four
         constexpr uint32_t kN = kFours == 1u ? 4u : 8u;
         const uint32_t own_lane = fresh_lane(), n = own_lane % kMF, q = own_lane / kMF;
         const uint32_t count = count_of(t);
         const uint64_t row0 = first_row(t);
         const uint32_t column0 = first_column(t);
+        // The residual's reads, numbered: one for a span of bf16, two of fp32.  In a forward product the next
+        // one is under way while one's values are added (8,192 x 8,192 x 512 in bf16 104 us, so 98); with K
+        // across the rows that kept 30 to 80 registers in memory and took up to half as long again.
+        constexpr uint32_t kPlaces = kOut / 2u, kReadsEach = (kTypes & 2u) != 0u ? 2u : 1u;
+        constexpr uint32_t kAhead = kOrder == LinearOrder::kNT ? 1u : 0u;
+        [[maybe_unused]] v4u residual[kAhead + 1u][4];
+        [[maybe_unused]] const auto read_residual = [&](auto bc) MX_INLINE {
+            constexpr uint32_t b = decltype(bc)::value, at = b / kReadsEach;
+            if constexpr (at < kTM * kPlaces)
+                span(t, at / kPlaces, at % kPlaces).read(p.e.residual, b % kReadsEach, residual[b % (kAhead + 1u)]);
+        };
+        if constexpr (kSpans && kFold == LinearFold::kAdd && kAhead != 0u) {
+            if (column0 + 32u * kOut <= n_out) read_residual(None{});
+        }
         each_of<kTM>([&](auto ic) MX_INLINE {
             constexpr uint32_t i = decltype(ic)::value;
             const uint32_t m = (wm * kTM + i) * kMF + n;
@@ -1140,20 +1147,30 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
                     }
                 });
             };
-            using None = std::integral_constant<uint32_t, 0u>;
             using Up = std::integral_constant<uint32_t, kSwiglu ? kOut : 0u>;
             if constexpr (kSpans) {
                 if (column0 + 32u * kOut <= n_out) {
-                    each_of<kOut / 2u>([&](auto pc) MX_INLINE {
+                    each_of<kPlaces>([&](auto pc) MX_INLINE {
                         constexpr uint32_t place = decltype(pc)::value;
-                        float v[32], u[32] = {};
+                        float v[32];
                         each_of<4>([&](auto kc) MX_INLINE {
                             constexpr uint32_t k = decltype(kc)::value;
                             using Group = std::integral_constant<uint32_t, 2u * (4u * place + k)>;
                             using At = std::integral_constant<uint32_t, 8u * k>;
                             values(Group{}, None{}, v, At{});
                         });
-                        finish_all<kEnd>(p.e, span(t, i, place), n_out, v, u);
+                        const Span own = span(t, i, place);
+                        if constexpr (kFold == LinearFold::kAdd) {
+                            v4u packed[4];
+                            each_of<2>([&](auto hc) MX_INLINE {
+                                constexpr uint32_t half = decltype(hc)::value;
+                                constexpr uint32_t b = (i * kPlaces + place) * kReadsEach + (kReadsEach == 2u ? half : 0u);
+                                if constexpr (kReadsEach == 2u || half == 0u) read_residual(std::integral_constant<uint32_t, b + kAhead>{});
+                                own.store_sums(p.e.c, p.e.residual, half, v, residual[b % (kAhead + 1u)], packed);
+                            });
+                        } else {
+                            own.store(p.e.c, v);
+                        }
                         if constexpr (S::kWaves == 8u) __builtin_amdgcn_sched_barrier(0);
                     });
                     return;
@@ -1197,13 +1214,13 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
                         return;
                     }
                 }
-                if (m < count && column < n_out) finish<kEnd>(p.e, row0 + m, column, n_out, v, u);
+                if (m < count && column < n_out) finish<kFold>(p.e, row0 + m, column, n_out, v, u);
                 if constexpr (S::kWaves == 8u) __builtin_amdgcn_sched_barrier(0);
             });
         });
         // The compiler cannot tell that a load under a condition is used under the same one, and
         // would wait for it in the next tile's stages: it is told here that none is under way.
-        if constexpr (kEnd != LinearFold::kStore && kEnd != LinearFold::kSwiglu) __builtin_amdgcn_s_waitcnt(kVmcnt0);
+        if constexpr (kFold != LinearFold::kStore && kFold != LinearFold::kSwiglu) __builtin_amdgcn_s_waitcnt(kVmcnt0);
     };
 
     // all stages that the ring holds under way, but for the last one's later loads
@@ -1226,15 +1243,19 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     if (left < 64u) clear(left);
 #pragma unroll
     for (uint32_t i = 0; i < kReads; ++i) read(0u, i);
-    begin(0u);
+    begin();
     for (uint32_t t = 0;; ++t) {
         const uint32_t after = t + 1u == order.count ? 64u : depth_of(t + 1u);
-        for (; left > 64u; left -= 64u) stage(left - 64u);
-        stage(after);
+        for (; left > 64u; left -= 64u) stage(left - 64u, std::true_type{});
+        stage(after, std::bool_constant<!kReadBehind>{});
         store(t);
         if (t + 1u == order.count) break;
         left = after;
-        begin(t + 1u);
+        begin();
+        if constexpr (kReadBehind) {
+#pragma unroll
+            for (uint32_t i = 0; i < kReads; ++i) read(0u, i);
+        }
     }
     mx_barrier<0>();  // no load is under way to LDS that the next workgroup gets
 }
@@ -1572,8 +1593,28 @@ hipError_t launch_tiles(const LinearProduct& p, const LinearSizes& sizes, uint32
             q.e = LinearEpilogue{};
             q.e.c = LinearMatrix{scratch, p.columns, true};
         }
-        linear_tile_kernel<S, kOrder, kExperts, kFold>
-            <<<linear_grid<S>(sizes, parts), 64u * S::kWaves, 0, stream>>>(q, each);
+        const auto start = [&](auto fold, auto types) {
+            linear_tile_kernel<S, kOrder, kExperts, decltype(fold)::value, decltype(types)::value>
+                <<<linear_grid<S>(sizes, parts), 64u * S::kWaves, 0, stream>>>(q, each);
+        };
+        const auto no_types = std::integral_constant<uint32_t, 0u>{};
+        if constexpr (kFold == LinearFold::kAdd) {
+            const std::integral_constant<LinearFold, kFold> add{};
+            if (parts > 1u) {  // the join adds the residual
+                start(std::integral_constant<LinearFold, LinearFold::kStore>{}, no_types);
+            } else if constexpr (S::kMF == 32u) {
+                switch ((p.e.c.f32 ? 1u : 0u) + (p.e.residual.f32 ? 2u : 0u)) {
+                    case 0: start(add, std::integral_constant<uint32_t, kTyped>{}); break;
+                    case 1: start(add, std::integral_constant<uint32_t, kTyped + 1u>{}); break;
+                    case 2: start(add, std::integral_constant<uint32_t, kTyped + 2u>{}); break;
+                    default: start(add, std::integral_constant<uint32_t, kTyped + 3u>{});
+                }
+            } else {
+                start(add, no_types);
+            }
+        } else {
+            start(std::integral_constant<LinearFold, kFold>{}, no_types);
+        }
         if constexpr (!kExperts) {
             if (parts > 1u) {
                 if (hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
@@ -1734,22 +1775,25 @@ hipError_t launch_linear(const LinearProduct& given, LinearOrder order, LinearFo
     using Slope = std::integral_constant<LinearFold, LinearFold::kSlope>;
     using Swiglu = std::integral_constant<LinearFold, LinearFold::kSwiglu>;
     using SwigluGrad = std::integral_constant<LinearFold, LinearFold::kSwigluGrad>;
+    const auto added = [&](auto o, auto experts) {
+        return p.e.residual.data ? launch(o, experts, Add{}) : launch(o, experts, Store{});
+    };
     if (!p.offsets) {
-        // Where nothing is done to the sums but a residual's addition they begin with it, and go to memory in
-        // whole lines: the input's gradient 8,192 x 512 x 8,192 (rows x outputs x inputs) with a residual 128
-        // us and so 102, without one 81 and 74; forward 8,192 x 8,192 x 2,048 276 and 249, 240 and 226.
+        // Where nothing is done to the sums but a residual's addition they go to memory in whole lines: the
+        // input's gradient 8,192 x 512 x 8,192 (rows x outputs x inputs) with a residual 128 us and so 99,
+        // without one 81 and 74; forward 8,192 x 8,192 x 2,048 276 and 240, 240 and 226.
         const bool as_they_are = p.e.activation == Q38M_ACT_NONE && !p.e.bias.data;
-        if (order == LinearOrder::kNT && as_they_are && !p.e.pre.data) return launch(NT{}, std::false_type{}, Add{});
+        if (order == LinearOrder::kNT && as_they_are && !p.e.pre.data) return added(NT{}, std::false_type{});
         if (order == LinearOrder::kNT) return launch(NT{}, std::false_type{}, Forward{});
-        if (order == LinearOrder::kNN && as_they_are) return launch(NN{}, std::false_type{}, Add{});
+        if (order == LinearOrder::kNN && as_they_are) return added(NN{}, std::false_type{});
         if (order == LinearOrder::kNN) return launch(NN{}, std::false_type{}, Slope{});
-        return launch(TN{}, std::false_type{}, Add{});
+        return added(TN{}, std::false_type{});
     }
     if (fold == LinearFold::kSwiglu) return launch(NT{}, std::true_type{}, Swiglu{});
     if (fold == LinearFold::kSwigluGrad) return launch(NN{}, std::true_type{}, SwigluGrad{});
     if (order == LinearOrder::kNT) return launch(NT{}, std::true_type{}, Store{});
     if (order == LinearOrder::kNN) return launch(NN{}, std::true_type{}, Store{});
-    return launch(TN{}, std::true_type{}, Add{});
+    return added(TN{}, std::true_type{});
 }
 
 hipError_t launch_activation_backward(const LinearMatrix& dy, const LinearMatrix& pre,
