@@ -337,7 +337,7 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearProduct p) {
     constexpr bool kAcrossA = kOrder == LinearOrder::kTN, kAcrossB = kOrder != LinearOrder::kNT;
     constexpr uint32_t kAcross = kFold == LinearFold::kSwiglu ? kAnyTile / 2u : kAnyTile;
     __shared__ __align__(16) uint16_t lds[2][kAnyTile * kAnyPitch];
-    __shared__ uint32_t offsets[kExperts && !kAcrossA ? kMaxSortExperts : 1u];
+    __shared__ v4i offset_words[kExperts && !kAcrossA ? kMaxSortExperts / 4u : 1u];
     const uint32_t t = threadIdx.x, lane = t & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const uint32_t n_out = kFold == LinearFold::kSwiglu ? p.columns / 2u : p.columns;
@@ -355,10 +355,11 @@ __global__ __launch_bounds__(256) void linear_any_kernel(LinearProduct p) {
         k_first = min(p.offsets[tile.expert], p.depth);
         depth = max(min(p.offsets[tile.expert + 1u], p.depth), k_first) - k_first;
     } else if constexpr (kExperts) {
+        uint32_t* offsets = reinterpret_cast<uint32_t*>(offset_words);
         const uint32_t last = p.offsets[p.experts];
         for (uint32_t e = t; e < kMaxSortExperts; e += 256u) offsets[e] = e < p.experts ? p.offsets[e] : last;
         __syncthreads();
-        const TileList<kAnyTile> list(offsets, last, p.rows);
+        const TileList<kAnyTile> list(offset_words, last, p.rows);
         if (row_tile >= list.total) return;
         tile = list.find(row_tile);
     } else {
@@ -712,7 +713,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     }
     // K that is ragged: an expert's rows are one "row tile" of the list
     const auto make_list = [&]() MX_INLINE {
-        if constexpr (kExperts) return TileList<kRagged ? 1u << 24 : kBM>(offsets, last_offset, routes);
+        if constexpr (kExperts) return TileList<kRagged ? 1u << 24 : kBM>(ring + S::kOffsetsAt, last_offset, routes);
         else return 0;
     };
     const auto list = make_list();
@@ -1275,7 +1276,7 @@ __global__ __launch_bounds__(64u * S::kWaves) void linear_few_kernel(LinearProdu
     constexpr uint32_t kRowsB = 16u * kTiles, kRows = kFewRows + kRowsB, kSlot = kRows * 8u;  // 16-byte words
     constexpr uint32_t kAcross = kSwiglu ? kRowsB / 2u : kRowsB;
     __shared__ v4i ring[kFewWaves * kFewStages * kSlot];
-    __shared__ uint32_t offsets[kExperts ? kMaxSortExperts : 1u];
+    __shared__ v4i offset_words[kExperts ? kMaxSortExperts / 4u : 1u];
     const uint32_t lane = threadIdx.x & 63u;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t n_out = kSwiglu ? p.columns / 2u : p.columns;
@@ -1283,6 +1284,7 @@ __global__ __launch_bounds__(64u * S::kWaves) void linear_few_kernel(LinearProdu
     const uint32_t row_tile = blockIdx.x / columns, column0 = blockIdx.x % columns * kAcross;
     RowTile tile{0u, row_tile * kFewRows, 0u, false};
     if constexpr (kExperts) {
+        uint32_t* offsets = reinterpret_cast<uint32_t*>(offset_words);
         const uint32_t last = p.offsets[p.experts];
         for (uint32_t e = threadIdx.x; e < kMaxSortExperts; e += 64u * kFewWaves) offsets[e] = e < p.experts ? p.offsets[e] : last;
         __syncthreads();
@@ -1290,7 +1292,7 @@ __global__ __launch_bounds__(64u * S::kWaves) void linear_few_kernel(LinearProdu
         for (uint32_t e = threadIdx.x; e < p.experts; e += 64u * kFewWaves)
             report(p.offsets[e + 1u] < offsets[e] || p.offsets[e + 1u] > p.rows, kCheckOffsets);
 #endif
-        const TileList<kFewRows> list(offsets, last, p.rows);
+        const TileList<kFewRows> list(offset_words, last, p.rows);
         if (row_tile >= list.total) return;
         tile = list.find(row_tile);
     } else {

@@ -256,7 +256,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
 #endif
     }
     const auto make_list = [&]() MX_INLINE {
-        if constexpr (kExperts) return TileList<kBM>(offsets, last_offset, p.routes);
+        if constexpr (kExperts) return TileList<kBM>(ring + S::kOffsetsAt, last_offset, p.routes);
         else return 0;
     };
     const auto list = make_list();

@@ -53,7 +53,8 @@ struct RowTile {
 };
 
 // The row tiles of the experts' rows, kRows at a time, found by a wave from the offsets
-// (LDS, all of kMaxSortExperts; those past the experts are the last one, `last`).  Lane l
+// (LDS, all of kMaxSortExperts, in words of 16 bytes because they are read so; those past
+// the experts are the last one, `last`).  Lane l
 // keeps the row tiles of the first 16 (l + 1) experts.  Offsets past `routes` count as
 // routes, an end that is not behind its begin as no rows.
 template <uint32_t kRows>
@@ -63,13 +64,13 @@ struct TileList {
     const uint32_t* offsets;
     uint32_t last, routes, sum, total;
 
-    __device__ MX_INLINE TileList(const uint32_t* offsets_, uint32_t last_, uint32_t routes_)
-        : offsets(offsets_), last(last_), routes(routes_), sum(0) {
+    __device__ MX_INLINE TileList(const v4i* words, uint32_t last_, uint32_t routes_)
+        : offsets(reinterpret_cast<const uint32_t*>(words)), last(last_), routes(routes_), sum(0) {
         const uint32_t lane = threadIdx.x & 63u;
         uint32_t at[kPer + 1];
 #pragma unroll
         for (uint32_t i = 0; i < kPer; i += 4u) {
-            const v4i w = reinterpret_cast<const v4i*>(offsets)[(lane * kPer + i) / 4u];
+            const v4i w = words[(lane * kPer + i) / 4u];
             at[i] = w[0], at[i + 1u] = w[1], at[i + 2u] = w[2], at[i + 3u] = w[3];
         }
         at[kPer] = __shfl_down(at[0], 1);
