@@ -788,9 +788,14 @@ int q38m_linear_v1(const q38m_tensor_v1* x, const q38m_tensor_v1* weight,
                    void* stream, int device);
 
 /* dx = (dz weight) * act'(pre) + residual: dz [rows][outputs] the gradient of
- * x weight^T + bias, pre [rows][inputs] what the activation in front of x was
- * taken of (NULL with Q38M_ACT_NONE), residual [rows][inputs] the gradient
- * that x gets otherwise (through a skip connection). */
+ * x weight^T + bias, the others [rows][inputs].  With Q38M_ACT_NONE (pre NULL)
+ * dx is the gradient of x, and residual the one that x gets otherwise (through
+ * a skip connection).  With an activation x is act(pre), dx the gradient of
+ * pre (the layer in front's dz), and residual the one that pre gets otherwise:
+ * through a skip that leaves in front of the activation.  The gradient of one
+ * that leaves behind it, from x, is multiplied by act'(pre) too: it is added
+ * by a call with Q38M_ACT_NONE, whose dx (fp32 loses nothing) goes through
+ * q38m_linear_backward_activation_v1. */
 int q38m_linear_backward_input_v1(const q38m_tensor_v1* dz, const q38m_tensor_v1* weight,
                                   const q38m_tensor_v1* pre, uint32_t activation,
                                   const q38m_tensor_v1* residual, const q38m_tensor_v1* dx,
