@@ -545,34 +545,25 @@ struct Span {
     __device__ MX_INLINE uint32_t column_of() const { return 16u * (lane & 3u) + lane / 32u * 8u; }
     __device__ MX_INLINE uint32_t wide_column_of() const { return 8u * (lane & 3u) + lane / 32u * 4u; }
 
-    // a half's values as its pieces have them in fp32: d[e][k] is value e of piece k
-    __device__ MX_INLINE void turn_half(const float (&v)[32], uint32_t half, v4u (&d)[4]) const {
-        each_of<8>([&](auto c) MX_INLINE {
-            constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
-            const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[16u * half + 8u * k + e]),
-                                                               __float_as_uint(v[16u * half + 8u * k + 4u + e]), false, false);
-            d[e][2u * k] = both[0];
-            d[e][2u * k + 1u] = both[1];
-        });
-        each_of<4>([&](auto e) MX_INLINE { d[decltype(e)::value] = transpose_quad(d[decltype(e)::value], lane); });
-    }
     __device__ MX_INLINE float* wide_piece(LinearMatrix m, uint32_t half, uint32_t k) const {
         return static_cast<float*>(m.data) + place(m, row_of(k)) + 32u * half + wide_column_of();
     }
     __device__ MX_INLINE uint16_t* piece(LinearMatrix m, uint32_t k) const {
         return static_cast<uint16_t*>(m.data) + place(m, row_of(k)) + column_of();
     }
-    template <typename T>
-    __device__ MX_INLINE static T stream(const void* from) {
-        return __builtin_nontemporal_load(static_cast<const T*>(from));
-    }
-
     __device__ MX_INLINE void store(LinearMatrix m, const float (&v)[32]) const {
         v4u d[4];
         if (m.f32) {
             each_of<2>([&](auto hc) MX_INLINE {
                 constexpr uint32_t half = decltype(hc)::value;
-                turn_half(v, half, d);
+                each_of<8>([&](auto c) MX_INLINE {
+                    constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
+                    const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[16u * half + 8u * k + e]),
+                                                                       __float_as_uint(v[16u * half + 8u * k + 4u + e]), false, false);
+                    d[e][2u * k] = both[0];
+                    d[e][2u * k + 1u] = both[1];
+                });
+                each_of<4>([&](auto e) MX_INLINE { d[decltype(e)::value] = transpose_quad(d[decltype(e)::value], lane); });
                 each_of<4>([&](auto kc) MX_INLINE {
                     constexpr uint32_t k = decltype(kc)::value;
                     if (row_of(k) >= count) return;
@@ -594,54 +585,43 @@ struct Span {
         });
     }
 
-    // A residual is added to whole sums where a half's pieces have them, so it changes no places.  What is
-    // read of it at a time: of fp32 a half's pieces; of bf16 both halves', eight columns of half q from
-    // 8 (n % 4) on, which two lanes of a row trade for four of both halves, and trade sums back to be
-    // stored so.  (Four bf16 columns a lane, half a line at a time: forward 8,192 x 8,192 x 512 into fp32
-    // 140 us, so 115.)
-    __device__ MX_INLINE uint16_t* half_piece(LinearMatrix m, uint32_t k) const {
-        return static_cast<uint16_t*>(m.data) + place(m, row_of(k)) + lane / 32u * 32u + 8u * (lane & 3u);
-    }
-    __device__ MX_INLINE static void trade(v4u& w) {
-        const auto low = __builtin_amdgcn_permlane32_swap(w.x, w.z, false, false);
-        const auto high = __builtin_amdgcn_permlane32_swap(w.y, w.w, false, false);
-        w = v4u{low[0], high[0], low[1], high[1]};
-    }
-    __device__ MX_INLINE void read(LinearMatrix r, uint32_t half, v4u (&w)[4]) const {
-        each_of<4>([&](auto kc) MX_INLINE {
-            constexpr uint32_t k = decltype(kc)::value;
-            if (r.f32) w[k] = stream<v4u_any>(wide_piece(r, half, k));
-            else w[k] = stream<v4u_any>(half_piece(r, k));
-        });
-    }
-    __device__ MX_INLINE void store_sums(LinearMatrix m, LinearMatrix r, uint32_t half, const float (&v)[32], v4u (&w)[4],
-                                         v4u (&packed)[4]) const {
-        v4u d[4];
-        turn_half(v, half, d);
-        each_of<4>([&](auto kc) MX_INLINE {
-            constexpr uint32_t k = decltype(kc)::value;
-            if (!r.f32 && half == 0u) trade(w[k]);
-            each_of<4>([&](auto ec) MX_INLINE {
-                constexpr uint32_t e = decltype(ec)::value;
-                uint32_t other = w[k][e];
-                if (!r.f32) other = e % 2u != 0u ? w[k][2u * half + e / 2u] & 0xffff0000u : w[k][2u * half + e / 2u] << 16;
-                d[e][k] = __float_as_uint(__uint_as_float(d[e][k]) + __uint_as_float(other));
+    // m's values, added to the lane's groups of four that the sums are stored from: group 2 k + c has
+    // columns 16 k + 8 c + 4 q of its row.
+    template <typename F>
+    __device__ MX_INLINE void read(LinearMatrix m, F add) const {
+        v4u d[4];  // [e][k]: dword e of piece k
+        const auto load = [&](auto piece_of) MX_INLINE {
+            each_of<4>([&](auto kc) MX_INLINE {
+                constexpr uint32_t k = decltype(kc)::value;
+                const v4u_any w = __builtin_nontemporal_load(reinterpret_cast<const v4u_any*>(piece_of(k)));
+                d[0][k] = w.x, d[1][k] = w.y, d[2][k] = w.z, d[3][k] = w.w;
             });
-            if (!m.f32) {
-                packed[k][2u * half] = f32_to_bf16(__uint_as_float(d[0][k])) | f32_to_bf16(__uint_as_float(d[1][k])) << 16;
-                packed[k][2u * half + 1u] = f32_to_bf16(__uint_as_float(d[2][k])) | f32_to_bf16(__uint_as_float(d[3][k])) << 16;
-                if (half == 0u) return;
-                trade(packed[k]);
-                if (row_of(k) < count) __builtin_nontemporal_store(v4u_any(packed[k]), reinterpret_cast<v4u_any*>(half_piece(m, k)));
-            } else if (row_of(k) < count) {
-                __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]},
-                                            reinterpret_cast<v4u_any*>(wide_piece(m, half, k)));
-            }
+            each_of<4>([&](auto e) MX_INLINE { d[decltype(e)::value] = transpose_quad(d[decltype(e)::value], lane); });
+        };
+        if (m.f32) {
+            each_of<2>([&](auto hc) MX_INLINE {
+                constexpr uint32_t half = decltype(hc)::value;
+                load([&](uint32_t k) MX_INLINE { return wide_piece(m, half, k); });
+                each_of<16>([&](auto c) MX_INLINE {
+                    constexpr uint32_t k = decltype(c)::value / 4u, e = decltype(c)::value % 4u;
+                    add(std::integral_constant<uint32_t, 4u * half + k>{}, std::integral_constant<uint32_t, e>{},
+                        __uint_as_float(d[e][k]));
+                });
+            });
+            return;
+        }
+        load([&](uint32_t k) MX_INLINE { return piece(m, k); });
+        each_of<8>([&](auto c) MX_INLINE {  // eight columns of a row a lane to four of both of its groups
+            constexpr uint32_t k = decltype(c)::value / 2u, e = decltype(c)::value % 2u;
+            const auto both = __builtin_amdgcn_permlane32_swap(d[e][k], d[2u + e][k], false, false);
+            each_of<2>([&](auto gc) MX_INLINE {
+                const std::integral_constant<uint32_t, 2u * k + decltype(gc)::value> group;
+                add(group, std::integral_constant<uint32_t, 2u * e>{}, __uint_as_float(both[decltype(gc)::value] << 16));
+                add(group, std::integral_constant<uint32_t, 2u * e + 1u>{}, __uint_as_float(both[decltype(gc)::value] & 0xffff0000u));
+            });
         });
     }
 };
-
-constexpr uint32_t kTyped = 4u;  // of a tile kernel's kTypes
 
 // Workgroups stay and compute tile after tile of kBM x kBN values of C (with the SwiGLU fold
 // half of the columns gate, half up), kWM x kWN waves, each kTM x kTN matrix-instruction
@@ -662,18 +642,9 @@ constexpr uint32_t kTyped = 4u;  // of a tile kernel's kTypes
 //   2,090 us, 5.4 TB/s read and written): memory.
 // - few tiles (509 x 2,048 x 8,192 31 us and a join of 4): one stage's latency after another, so K
 //   is cut until the card is full, and the parts' sums are joined by a second launch in their order.
-//
-// kTypes: 0, or kTyped and whether C (1) and the residual (2) are fp32, where a residual is added and
-// the sums stored in whole lines: with a way through for each type at run time the compiler kept 40 to
-// 640 registers of 256 x 256 tiles in memory, with one for each kernel none, or 5 to 20 of experts' tiles
-// and of fp32 residuals of bf16 sums, read and written where a tile begins and where its K or it ends.
-template <typename S, LinearOrder kOrder, bool kExperts, LinearFold kFold, uint32_t kTypes = 0u>
+template <typename S, LinearOrder kOrder, bool kExperts, LinearFold kFold>
 __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 4u) void linear_tile_kernel(
     LinearProduct p, uint32_t each) {
-    if constexpr ((kTypes & kTyped) != 0u) {
-        p.e.c.f32 = (kTypes & 1u) != 0u;
-        p.e.residual.f32 = (kTypes & 2u) != 0u;
-    }
     constexpr uint32_t kMF = S::kMF, kTM = S::kTM, kTN = S::kTN, kBM = S::kBM, kBN = S::kBN;
     constexpr bool kAcrossA = kOrder == LinearOrder::kTN, kAcrossB = kOrder != LinearOrder::kNT;
     constexpr bool kSwiglu = kFold == LinearFold::kSwiglu;
@@ -976,7 +947,6 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     // exchange between lanes costs what it gives (in half lines, for want of registers: gate/up of
     // 32,768 tokens 1,594 us and so 1,647, down's row gradient of 16,384 763 and 884).
     constexpr bool kSpans = kMF == 32u && kOut % 2u == 0u && (kFold == LinearFold::kStore || kFold == LinearFold::kAdd);
-    static_assert(kTypes != 0u || !kSpans || kFold == LinearFold::kStore, "the types of what is added");
     [[maybe_unused]] const auto span = [&](uint32_t t, uint32_t i, uint32_t place) MX_INLINE {
         const uint32_t own_lane = fresh_lane();
         return Span{first_row(t), (wm * kTM + i) * kMF + (own_lane & 31u), count_of(t), first_column(t) + 64u * place, own_lane};
@@ -1066,13 +1036,10 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     };
     constexpr uint32_t kEarly = (kDataLoads + 1u) / 2u;  // data loads in the step behind the barrier, the rest a step later
 
-    // The first fragments of the next tile are read behind the tile's end where a residual's values take
-    // their registers.
-    constexpr bool kReadBehind = kSpans && kFold == LinearFold::kAdd && kOrder == LinearOrder::kNT;
     // A stage in kSteps steps, software pipelined: a step's fragments are read while the step in
     // front of it is multiplied.  In front of the last step the workgroup meets: the next stage
     // (`valid` values of K) has come and this one is read, so its slot takes the kStages-th after it.
-    const auto stage = [&](uint32_t valid, auto read_next) MX_INLINE {
+    const auto stage = [&](uint32_t valid) MX_INLINE {
         constexpr uint32_t kLater = S::kStages - 2u;  // loads of the stages behind the next may be under way
         const auto step = [&](auto c) MX_INLINE {
             constexpr uint32_t kC = decltype(c)::value;
@@ -1095,8 +1062,8 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         if (valid < 64u) clear(valid);
         multiply(std::integral_constant<uint32_t, S::kSteps - 1u>{}, std::integral_constant<uint32_t, kReads + kEarly>{},
                  [&](uint32_t o) MX_INLINE {
-                     if (o >= kReads) load_data(o - kReads);
-                     else if (decltype(read_next)::value) read(0u, o);
+                     if (o < kReads) read(0u, o);
+                     else load_data(o - kReads);
                  });
     };
 
@@ -1110,19 +1077,22 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         const uint32_t count = count_of(t);
         const uint64_t row0 = first_row(t);
         const uint32_t column0 = first_column(t);
-        // The residual's reads, numbered: one for a span of bf16, two of fp32.  In a forward product the next
-        // one is under way while one's values are added (8,192 x 8,192 x 512 in bf16 104 us, so 98); with K
-        // across the rows that kept 30 to 80 registers in memory and took up to half as long again.
-        constexpr uint32_t kPlaces = kOut / 2u, kReadsEach = (kTypes & 2u) != 0u ? 2u : 1u;
-        constexpr uint32_t kAhead = kOrder == LinearOrder::kNT ? 1u : 0u;
-        [[maybe_unused]] v4u residual[kAhead + 1u][4];
-        [[maybe_unused]] const auto read_residual = [&](auto bc) MX_INLINE {
-            constexpr uint32_t b = decltype(bc)::value, at = b / kReadsEach;
-            if constexpr (at < kTM * kPlaces)
-                span(t, at / kPlaces, at % kPlaces).read(p.e.residual, b % kReadsEach, residual[b % (kAhead + 1u)]);
-        };
-        if constexpr (kSpans && kFold == LinearFold::kAdd && kAhead != 0u) {
-            if (column0 + 32u * kOut <= n_out) read_residual(None{});
+        // A residual is added to all of a wave's sums in front of their stores.  (A span's values where its
+        // stores have them, a kernel for each pair of types, which kept none or 5 to 20 registers in memory:
+        // gate/up weights of 16,384 tokens added up in fp32 1,930 us, so 2,006, but memory that is read and
+        // written by turns costs a short batch's: 61 x 8,192 x 2,048 29.4, so 26.2.)
+        constexpr uint32_t kPlaces = kOut / 2u;
+        if constexpr (kSpans && kFold == LinearFold::kAdd) {
+            if (column0 + 32u * kOut <= n_out && p.e.residual.data)
+                each_of<kTM * kPlaces>([&](auto sc) MX_INLINE {
+                    constexpr uint32_t i = decltype(sc)::value / kPlaces, place = decltype(sc)::value % kPlaces;
+                    if ((wm * kTM + i) * kMF >= count) return;
+                    span(t, i, place).read(p.e.residual, [&](auto fc, auto ec, float v) MX_INLINE {
+                        constexpr uint32_t f = 8u * place + decltype(fc)::value;
+                        acc[f / 4u][i][4u * (f % 4u) + decltype(ec)::value] += v;
+                    });
+                    if constexpr (S::kWaves == 8u) __builtin_amdgcn_sched_barrier(0);
+                });
         }
         each_of<kTM>([&](auto ic) MX_INLINE {
             constexpr uint32_t i = decltype(ic)::value;
@@ -1160,18 +1130,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
                             using At = std::integral_constant<uint32_t, 8u * k>;
                             values(Group{}, None{}, v, At{});
                         });
-                        const Span own = span(t, i, place);
-                        if constexpr (kFold == LinearFold::kAdd) {
-                            v4u packed[4];
-                            each_of<2>([&](auto hc) MX_INLINE {
-                                constexpr uint32_t half = decltype(hc)::value;
-                                constexpr uint32_t b = (i * kPlaces + place) * kReadsEach + (kReadsEach == 2u ? half : 0u);
-                                if constexpr (kReadsEach == 2u || half == 0u) read_residual(std::integral_constant<uint32_t, b + kAhead>{});
-                                own.store_sums(p.e.c, p.e.residual, half, v, residual[b % (kAhead + 1u)], packed);
-                            });
-                        } else {
-                            own.store(p.e.c, v);
-                        }
+                        span(t, i, place).store(p.e.c, v);
                         if constexpr (S::kWaves == 8u) __builtin_amdgcn_sched_barrier(0);
                     });
                     return;
@@ -1247,16 +1206,12 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     begin();
     for (uint32_t t = 0;; ++t) {
         const uint32_t after = t + 1u == order.count ? 64u : depth_of(t + 1u);
-        for (; left > 64u; left -= 64u) stage(left - 64u, std::true_type{});
-        stage(after, std::bool_constant<!kReadBehind>{});
+        for (; left > 64u; left -= 64u) stage(left - 64u);
+        stage(after);
         store(t);
         if (t + 1u == order.count) break;
         left = after;
         begin();
-        if constexpr (kReadBehind) {
-#pragma unroll
-            for (uint32_t i = 0; i < kReads; ++i) read(0u, i);
-        }
     }
     mx_barrier<0>();  // no load is under way to LDS that the next workgroup gets
 }
@@ -1595,28 +1550,8 @@ hipError_t launch_tiles(const LinearProduct& p, const LinearSizes& sizes, uint32
             q.e = LinearEpilogue{};
             q.e.c = LinearMatrix{scratch, p.columns, true};
         }
-        const auto start = [&](auto fold, auto types) {
-            linear_tile_kernel<S, kOrder, kExperts, decltype(fold)::value, decltype(types)::value>
-                <<<linear_grid<S>(sizes, parts), 64u * S::kWaves, 0, stream>>>(q, each);
-        };
-        const auto no_types = std::integral_constant<uint32_t, 0u>{};
-        if constexpr (kFold == LinearFold::kAdd) {
-            const std::integral_constant<LinearFold, kFold> add{};
-            if (parts > 1u) {  // the join adds the residual
-                start(std::integral_constant<LinearFold, LinearFold::kStore>{}, no_types);
-            } else if constexpr (S::kMF == 32u) {
-                switch ((p.e.c.f32 ? 1u : 0u) + (p.e.residual.f32 ? 2u : 0u)) {
-                    case 0: start(add, std::integral_constant<uint32_t, kTyped>{}); break;
-                    case 1: start(add, std::integral_constant<uint32_t, kTyped + 1u>{}); break;
-                    case 2: start(add, std::integral_constant<uint32_t, kTyped + 2u>{}); break;
-                    default: start(add, std::integral_constant<uint32_t, kTyped + 3u>{});
-                }
-            } else {
-                start(add, no_types);
-            }
-        } else {
-            start(std::integral_constant<LinearFold, kFold>{}, no_types);
-        }
+        linear_tile_kernel<S, kOrder, kExperts, kFold>
+            <<<linear_grid<S>(sizes, parts), 64u * S::kWaves, 0, stream>>>(q, each);
         if constexpr (!kExperts) {
             if (parts > 1u) {
                 if (hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
@@ -1782,8 +1717,8 @@ hipError_t launch_linear(const LinearProduct& given, LinearOrder order, LinearFo
     };
     if (!p.offsets) {
         // Where nothing is done to the sums but a residual's addition they go to memory in whole lines: the
-        // input's gradient 8,192 x 512 x 8,192 (rows x outputs x inputs) with a residual 128 us and so 99,
-        // without one 81 and 74; forward 8,192 x 8,192 x 2,048 276 and 240, 240 and 226.
+        // input's gradient 8,192 x 512 x 8,192 (rows x outputs x inputs) with a residual 128 us and so 103,
+        // without one 81 and 74; forward 8,192 x 8,192 x 2,048 276 and 246, 240 and 226.
         const bool as_they_are = p.e.activation == Q38M_ACT_NONE && !p.e.bias.data;
         if (order == LinearOrder::kNT && as_they_are && !p.e.pre.data) return added(NT{}, std::false_type{});
         if (order == LinearOrder::kNT) return launch(NT{}, std::false_type{}, Forward{});
