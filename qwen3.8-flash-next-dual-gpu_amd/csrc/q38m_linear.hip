@@ -845,19 +845,21 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     };
     // gathered stored rows along K: the stage's sources, looked up a stage ahead
     const auto look_ahead = [&](uint32_t first, uint32_t stage, uint32_t count) MX_INLINE {
+        const uint32_t own_lane = fresh_lane();
 #pragma unroll
         for (uint32_t t = 0; t < kDataLoads; ++t) {
             const uint32_t i = wave + t * S::kWaves;
             if (data_live(t) && !of_a(t))
-                source[t] = p.packed[first + min(stage * 64u + B::row(i - kDataA, lane), count - 1u)];
+                source[t] = p.packed[first + min(stage * 64u + B::row(i - kDataA, own_lane), count - 1u)];
         }
     };
     const auto take_sources = [&]() MX_INLINE {
+        const uint32_t own_lane = fresh_lane();
 #pragma unroll
         for (uint32_t t = 0; t < kDataLoads; ++t) {
             const uint32_t i = wave + t * S::kWaves;
             if (data_live(t) && !of_a(t))
-                data[t] = min(source[t] / p.top_k, p.source_rows - 1u) * b_bytes + 16u * min(B::piece(i - kDataA, lane), b_last);
+                data[t] = min(source[t] / p.top_k, p.source_rows - 1u) * b_bytes + 16u * min(B::piece(i - kDataA, own_lane), b_last);
         }
         if (from + 1u < stages) look_ahead(k_from, from + 1u, depth);
         else look_ahead(next_from, 0u, next_depth);
@@ -866,18 +868,19 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     const auto hold_back = [&]() MX_INLINE {
         const uint32_t valid = depth - from * 64u;
         if (valid >= 64u) return;
+        const uint32_t own_lane = fresh_lane();
 #pragma unroll
         for (uint32_t t = 0; t < kDataLoads; ++t) {
             if (!data_live(t)) continue;
             const uint32_t i = wave + t * S::kWaves;
             const auto behind = [&](uint32_t at, uint32_t last) MX_INLINE { return at > last ? at - last : 0u; };
             if (of_a(t)) {
-                if constexpr (kAcrossA) data[t] -= behind(A::row(i, lane), valid - 1u) * a_bytes;
-                else data[t] -= behind(A::piece(i, lane), (valid - 1u) / 8u) * 16u;
+                if constexpr (kAcrossA) data[t] -= behind(A::row(i, own_lane), valid - 1u) * a_bytes;
+                else data[t] -= behind(A::piece(i, own_lane), (valid - 1u) / 8u) * 16u;
             } else if constexpr (kAcrossB) {
-                if (!(kRagged && gather)) data[t] -= behind(B::row(i - kDataA, lane), valid - 1u) * b_bytes;
+                if (!(kRagged && gather)) data[t] -= behind(B::row(i - kDataA, own_lane), valid - 1u) * b_bytes;
             } else {
-                data[t] -= behind(B::piece(i - kDataA, lane), (valid - 1u) / 8u) * 16u;
+                data[t] -= behind(B::piece(i - kDataA, own_lane), (valid - 1u) / 8u) * 16u;
             }
         }
     };
