@@ -526,11 +526,14 @@ __device__ MX_INLINE v4u transpose_quad(v4u r, uint32_t lane) {
 
 // 64 columns of the 32 rows that two of a wave's 32 x 32 tiles side by side have: lane l has of row
 // n = l % 32 the columns 16 k + 8 q .. + 7, q = l / 32, k = 0 .. 3.  Memory is read and written in
-// whole lines, past the caches: four lanes' pieces of 16 bytes change places, so that a lane has
-// its neighbours' rows in turn and a piece of each, and eight lanes a line.  Each lane its own
-// row's pieces, 32 bytes of a line at a time, past the caches or not: 16,384 tokens' gate/up weight
-// gradient in fp32 2,650 us, in whole lines 2,270, past the caches too 2,090; part lines past
-// the caches cost the rows' products more than a fifth.
+// whole lines: four lanes' pieces of 16 bytes change places, so that a lane has its neighbours'
+// rows in turn and a piece of each, and eight lanes a line.  Each lane its own row's pieces, 32
+// bytes of a line at a time, past the caches or not: 16,384 tokens' gate/up weight gradient in
+// fp32 2,650 us, in whole lines 2,270, past the caches too 2,090; part lines past the caches
+// cost the rows' products more than a fifth.
+//
+// kPast: past the caches (linear_past).
+template <bool kPast>
 struct Span {
     uint64_t row;           // of C: the tile's first
     uint32_t first, count;  // the lane's row of the tile, the tile's rows
@@ -551,6 +554,15 @@ struct Span {
     __device__ MX_INLINE uint16_t* piece(LinearMatrix m, uint32_t k) const {
         return static_cast<uint16_t*>(m.data) + place(m, row_of(k)) + column_of();
     }
+    static __device__ MX_INLINE void put(v4u_any v, void* to) {
+        if constexpr (kPast) __builtin_nontemporal_store(v, static_cast<v4u_any*>(to));
+        else *static_cast<v4u_any*>(to) = v;
+    }
+    static __device__ MX_INLINE v4u_any get(const void* from) {
+        if constexpr (kPast) return __builtin_nontemporal_load(static_cast<const v4u_any*>(from));
+        else return *static_cast<const v4u_any*>(from);
+    }
+
     __device__ MX_INLINE void store(LinearMatrix m, const float (&v)[32]) const {
         v4u d[4];
         if (m.f32) {
@@ -567,8 +579,7 @@ struct Span {
                 each_of<4>([&](auto kc) MX_INLINE {
                     constexpr uint32_t k = decltype(kc)::value;
                     if (row_of(k) >= count) return;
-                    __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]},
-                                                reinterpret_cast<v4u_any*>(wide_piece(m, half, k)));
+                    put(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]}, wide_piece(m, half, k));
                 });
             });
             return;
@@ -581,7 +592,7 @@ struct Span {
         each_of<4>([&](auto kc) MX_INLINE {
             constexpr uint32_t k = decltype(kc)::value;
             if (row_of(k) >= count) return;
-            __builtin_nontemporal_store(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]}, reinterpret_cast<v4u_any*>(piece(m, k)));
+            put(v4u_any{d[0][k], d[1][k], d[2][k], d[3][k]}, piece(m, k));
         });
     }
 
@@ -593,7 +604,7 @@ struct Span {
         const auto load = [&](auto piece_of) MX_INLINE {
             each_of<4>([&](auto kc) MX_INLINE {
                 constexpr uint32_t k = decltype(kc)::value;
-                const v4u_any w = __builtin_nontemporal_load(reinterpret_cast<const v4u_any*>(piece_of(k)));
+                const v4u_any w = get(piece_of(k));
                 d[0][k] = w.x, d[1][k] = w.y, d[2][k] = w.z, d[3][k] = w.w;
             });
             each_of<4>([&](auto e) MX_INLINE { d[decltype(e)::value] = transpose_quad(d[decltype(e)::value], lane); });
@@ -642,7 +653,7 @@ struct Span {
 //   2,090 us, 5.4 TB/s read and written): memory.
 // - few tiles (509 x 2,048 x 8,192 31 us and a join of 4): one stage's latency after another, so K
 //   is cut until the card is full, and the parts' sums are joined by a second launch in their order.
-template <typename S, LinearOrder kOrder, bool kExperts, LinearFold kFold>
+template <typename S, LinearOrder kOrder, bool kExperts, LinearFold kFold, bool kPast>
 __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 4u) void linear_tile_kernel(
     LinearProduct p, uint32_t each) {
     constexpr uint32_t kMF = S::kMF, kTM = S::kTM, kTN = S::kTN, kBM = S::kBM, kBN = S::kBN;
@@ -952,7 +963,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
     constexpr bool kSpans = kMF == 32u && kOut % 2u == 0u && (kFold == LinearFold::kStore || kFold == LinearFold::kAdd);
     [[maybe_unused]] const auto span = [&](uint32_t t, uint32_t i, uint32_t place) MX_INLINE {
         const uint32_t own_lane = fresh_lane();
-        return Span{first_row(t), (wm * kTM + i) * kMF + (own_lane & 31u), count_of(t), first_column(t) + 64u * place, own_lane};
+        return Span<kPast>{first_row(t), (wm * kTM + i) * kMF + (own_lane & 31u), count_of(t), first_column(t) + 64u * place, own_lane};
     };
     const auto begin = [&]() MX_INLINE {
 #pragma unroll
@@ -1531,12 +1542,26 @@ bool linear_on_tiles(const LinearProduct& p, LinearOrder order, LinearFold fold)
            std::max<uint64_t>(b_rows, 256u) * p.b_stride < limit;
 }
 
+constexpr uint64_t kLinearStayBytes = 1u << 27;
+
 // 256 x 256 tiles leave the SwiGLU's gradient too few registers.
 bool linear_wide(LinearFold fold) { return fold != LinearFold::kSwigluGrad; }
 
 size_t part_bytes(const LinearSizes& p, const LinearPlan& plan) {
     const uint32_t parts = p.experts != 0u ? 1u : linear_parts(p.depth, plan.splits);
     return parts > 1u ? static_cast<size_t>(parts) * p.rows * p.columns * sizeof(float) : 0u;
+}
+
+// Whether whole lines of C go past the caches, and the residual's come so: weights' gradients and
+// experts' rows always, dense rows, which the next layer reads, where they are more than stays in
+// the memory-side cache beside the operands until then.  us past the caches and through them: four layers
+// of 2,048 x 2,048 over 2,048 rows 131 and 115, the same with residuals 139 and 122, of 512 and 8,192
+// by turns over 8,192 rows 366 and 340; forward 8,192 x 8,192 x 512 into 268 MB of fp32 94 and 88, with an
+// fp32 residual 143 and 170, 16,384 x 8,192 x 2,048 in bf16 with a residual 485 and 528.
+bool linear_past(const LinearProduct& p, uint32_t parts) {
+    const uint64_t values = static_cast<uint64_t>(p.rows) * p.columns;
+    const uint64_t residual = !p.e.residual.data ? 0u : p.e.residual.f32 ? 4u : 2u;
+    return values * (parts * (p.e.c.f32 ? 4u : 2u) + residual) > kLinearStayBytes;
 }
 
 template <typename S, LinearOrder kOrder, bool kExperts, LinearFold kFold>
@@ -1553,8 +1578,16 @@ hipError_t launch_tiles(const LinearProduct& p, const LinearSizes& sizes, uint32
             q.e = LinearEpilogue{};
             q.e.c = LinearMatrix{scratch, p.columns, true};
         }
-        linear_tile_kernel<S, kOrder, kExperts, kFold>
-            <<<linear_grid<S>(sizes, parts), 64u * S::kWaves, 0, stream>>>(q, each);
+        const auto start = [&](auto past) {
+            linear_tile_kernel<S, kOrder, kExperts, kFold, decltype(past)::value>
+                <<<linear_grid<S>(sizes, parts), 64u * S::kWaves, 0, stream>>>(q, each);
+        };
+        // other tiles have stores of one kind
+        constexpr bool kEither = !kExperts && kOrder != LinearOrder::kTN && S::kMF == 32u &&
+                                 (kFold == LinearFold::kStore || kFold == LinearFold::kAdd);
+        if constexpr (!kEither) start(std::true_type{});
+        else if (linear_past(q, parts)) start(std::true_type{});
+        else start(std::false_type{});
         if constexpr (!kExperts) {
             if (parts > 1u) {
                 if (hipError_t rc = hipGetLastError(); rc != hipSuccess) return rc;
