@@ -30,8 +30,8 @@ __device__ MX_INLINE void each_of(F f) {
 
 // Phi(-|z|), with a = |z|, t = 1 / (1 + 0.3 a): exp(-a^2 / 2) times a polynomial in t,
 // fitted here by least squares over 0 <= a <= 14, weights raised where the relative error
-// was largest: 5.8e-8, and in fp32 4.9e-7 near 0 growing with the exponential's argument
-// (6.6e-7 at 3, 1.9e-6 at 6).  `density` gets exp(-a^2 / 2).
+// was largest: with the coefficients as they stand 7.8e-8, at 0, and in fp32 4.9e-7 near 0
+// growing with the exponential's argument (6.6e-7 at 3, 1.9e-6 at 6).  `density` gets exp(-a^2 / 2).
 __device__ __forceinline__ float normal_tail(float z, float* density) {
     const float a = fminf(__builtin_fabsf(z), 14.0f);
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(a, 0.3f, 1.0f));
@@ -642,15 +642,15 @@ struct Span {
 //
 // What bounds it, by counters:
 // - large products (8,192^3 819 us without an epilogue, 1,343 TFLOP/s; across K of one or both
-//   operands 808 and 800): the card's clock, 1.7 GHz of 2.4 under this load, and matrix pipes busy
-//   for 72 % of the rest, the L1s' answers under way for most of what is left; no LDS conflicts.
+//   operands 818 and 798): the card's clock, 1.7 GHz of 2.4 under this load, and matrix pipes busy
+//   for 59 to 68 % of it, the L1s' answers under way for 25 to 45 %; no LDS conflicts.
 //   128 x 128 tiles move twice as much through LDS for the same products (with GELU 1,159 us, 942).
 // - many experts' products with much to store (gate/up of 32,768 tokens 1,600 us, 859 TFLOP/s of
 //   rows that are there): row tiles that an expert's last rows fill partly, a sixth of the products,
 //   and the stores, during which this workgroup multiplies nothing: a second set of sums does not fit
 //   the registers.
-// - experts of few rows (512 tokens 355 us, 6.1 TB/s) and weights' gradients in fp32 (16,384 tokens
-//   2,090 us, 5.4 TB/s read and written): memory.
+// - experts of few rows (512 tokens 355 us, 6.1 TB/s) and weights' gradients in fp32 (16,384 tokens'
+//   gate/up 1,960 to 2,120 us, 4.5 to 4.9 TB/s read and written): memory.
 // - few tiles (509 x 2,048 x 8,192 31 us and a join of 4): one stage's latency after another, so K
 //   is cut until the card is full, and the parts' sums are joined by a second launch in their order.
 template <typename S, LinearOrder kOrder, bool kExperts, LinearFold kFold, bool kPast>
@@ -1325,7 +1325,8 @@ __global__ __launch_bounds__(64u * S::kWaves) void linear_few_kernel(LinearProdu
     });
     uint32_t slot = 0;
     for (uint32_t s = 0; s < count; ++s) {
-        // the stages behind this one may be under way; this one's fragments were read two stages ago
+        // The stages behind this one may be under way.  The slot that is loaded held the stage in front of
+        // this one, whose fragments have been read: the wait at the end of its turn says so.
         if (s + kFewStages - 1u < count) {
             load(first + s + kFewStages - 1u, slot == 0u ? kFewStages - 1u : slot - 1u);
             if (all_rows) asm volatile("s_waitcnt vmcnt(%0)" ::"i"((kFewStages - 1u) * kLoads) : "memory");
@@ -1358,7 +1359,7 @@ __global__ __launch_bounds__(64u * S::kWaves) void linear_few_kernel(LinearProdu
                 acc[j] = mfma_bf16(at[(kFewRows + 16u * j + n) * 8u + piece], a, acc[j]);
             });
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // its slot is loaded anew a stage on
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the next turn loads its slot anew
         slot = slot + 1u == kFewStages ? 0u : slot + 1u;
     }
     __syncthreads();
@@ -1557,7 +1558,8 @@ size_t part_bytes(const LinearSizes& p, const LinearPlan& plan) {
 // the memory-side cache beside the operands until then.  us past the caches and through them: four layers
 // of 2,048 x 2,048 over 2,048 rows 131 and 115, the same with residuals 139 and 122, of 512 and 8,192
 // by turns over 8,192 rows 366 and 340; forward 8,192 x 8,192 x 512 into 268 MB of fp32 94 and 88, with an
-// fp32 residual 143 and 170, 16,384 x 8,192 x 2,048 in bf16 with a residual 485 and 528.
+// fp32 residual 143 and 170, 16,384 x 8,192 x 2,048 in bf16 with a residual 485 and 528.  Smaller ones by
+// themselves, their rows read by nobody: 4,096 x 8,192 x 512 into fp32 55 and 48, 1,024 x 8,192 x 2,048 36 and 38.
 bool linear_past(const LinearProduct& p, uint32_t parts) {
     const uint64_t values = static_cast<uint64_t>(p.rows) * p.columns;
     const uint64_t residual = !p.e.residual.data ? 0u : p.e.residual.f32 ? 4u : 2u;

@@ -17,11 +17,11 @@ typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 // at any element: rows of odd strides start anywhere
 typedef uint32_t v2u_any __attribute__((ext_vector_type(2), aligned(2)));
 
-// 1 / (1 + exp(-g)) on the base-2 exponential and reciprocal instructions (one
-// unit in the last place each), and the SwiGLU fold h = g / (1 + exp(-g)) u.  The reciprocal gives zero in place of a result below the
-// smallest normal, so it is taken of a quarter of the sum, whose reciprocal never is, and a
-// multiplication takes the quarter back.  An exponential past 2^128 is infinite and h a zero,
-// as in the formula in fp32.  kExact puts the rounding of -g log2 e back (of an argument
+// 1 / (1 + exp(-g)) on the base-2 exponential and reciprocal instructions (one unit in the
+// last place each), and the SwiGLU fold h = g / (1 + exp(-g)) u.  The reciprocal gives zero in
+// place of a result below the smallest normal, so it is taken of a quarter of the sum, whose
+// reciprocal never is, and a multiplication takes the quarter back.  An exponential past 2^128
+// is infinite and h a zero, as in the formula in fp32.  kExact puts the rounding of -g log2 e back (of an argument
 // held to where the exponential is long infinite or zero): within 8 roundings of h; without
 // it, |g| roundings more, 2^-17 of h at most, far below half a step of bf16.  (The contract's
 // exp and an IEEE division take three times the instructions: an earlier form of the
