@@ -529,8 +529,8 @@ __device__ MX_INLINE v4u transpose_quad(v4u r, uint32_t lane) {
 // whole lines: four lanes' pieces of 16 bytes change places, so that a lane has its neighbours'
 // rows in turn and a piece of each, and eight lanes a line.  Each lane its own row's pieces, 32
 // bytes of a line at a time, past the caches or not: 16,384 tokens' gate/up weight gradient in
-// fp32 2,650 us, in whole lines 2,270, past the caches too 2,090; part lines past the caches
-// cost the rows' products more than a fifth.
+// fp32 2,650 us, in whole lines 2,270, past the caches too 2,090 (1,959 with what came later);
+// part lines past the caches cost the rows' products more than a fifth.
 //
 // kPast: past the caches (linear_past).
 template <bool kPast>
@@ -1093,7 +1093,7 @@ __global__ __launch_bounds__(64u * S::kWaves, (S::kResident * S::kWaves + 3u) / 
         const uint32_t column0 = first_column(t);
         // A residual is added to all of a wave's sums in front of their stores.  (A span's values where its
         // stores have them, a kernel for each pair of types, which kept none or 5 to 20 registers in memory:
-        // gate/up weights of 16,384 tokens added up in fp32 1,930 us, so 2,006, but memory that is read and
+        // gate/up weights of 16,384 tokens added up in fp32 1,930 us, so 1,959, but memory that is read and
         // written by turns costs a short batch's: 61 x 8,192 x 2,048 29.4, so 26.2.)
         constexpr uint32_t kPlaces = kOut / 2u;
         if constexpr (kSpans && kFold == LinearFold::kAdd) {
