@@ -8,12 +8,12 @@ bf16 once (2^-8 of it; every fp32 step in front is 2^-20 of its terms at most)."
 import pytest
 
 from helpers import stream, torch
-from linear_cases import Matrix, arg, close, lin, output, scratch_for, sync
+from linear_cases import Matrix, close, lin, output, scratch_for, sync
 
 pytestmark = pytest.mark.gpu
 
 
-def check_chain(q38m, m, k, n, act, behind, check_all=True):
+def check_chain(q38m, m, k, n, act, behind):
     """k inputs, n in the middle and out; behind: the skip leaves behind the activation, from h."""
     t = torch()
     call = q38m.call

@@ -3,11 +3,10 @@ is added to it just below, at and above 128 MB together.  The operands are small
 numbers, so that an output is the exact sum and the residual, rounded: bit for bit."""
 import pytest
 
-from helpers import torch
+from helpers import stream, torch
+from linear_cases import Matrix, arg, output, scratch_for, sync
 from linear_tiles import tiles_of
 from test_gpu_linear_residual import typed, whole
-from linear_cases import Matrix, arg, output, scratch_for, sync
-from helpers import stream
 
 pytestmark = pytest.mark.gpu
 

@@ -7,7 +7,7 @@ import random
 import pytest
 
 from helpers import stream, torch
-from linear_cases import Matrix, Sorted, arg, generator, lin, output, scratch_for, sync
+from linear_cases import Matrix, Sorted, generator, lin, output, scratch_for, sync
 from linear_tiles import tiles_of
 from test_gpu_linear_tiles import KINDS, counts_of, found, spread
 
